@@ -61,7 +61,7 @@ typedef enum {
  * take F32, F16 and BF16; tvk_copy takes every one of them. BOOL is one byte holding 0 or
  * 1. F8E4M3FN and F8E5M2 are torch's float8_e4m3fn and float8_e5m2 (OCP 8-bit
  * floats: e4m3 with no infinities and NaN = S.1111.111, e5m2 IEEE-like);
- * only tvk_copy takes them. */
+ * tvk_copy takes both, the norm's output and the paged cache F8E4M3FN. */
 typedef enum {
     TVK_F32 = 0,
     TVK_F16 = 1,
@@ -438,6 +438,140 @@ typedef struct {
 } tvk_attention_bwd_desc;
 
 tvk_status tvk_attention_bwd(const tvk_attention_bwd_desc* desc);
+
+/* ------------------------------------------------------------------------- */
+/* Root-mean-square norm                                                      */
+/* ------------------------------------------------------------------------- */
+
+/* For every row of `cols` values, with the sums in float32:
+ *   h = x + residual, rounded to `dtype` (h = x without a residual),
+ *   y = h / sqrt(mean(h^2) + eps) * weight      (weight NULL: ones),
+ * y rounded to `out_dtype`: `dtype` itself, or F8E4M3FN with
+ *   scale[row] = max|y| / 448 (1 where the row's y is all zero),
+ *   out = y / scale[row] rounded to nearest even (NaN stays NaN),
+ * the per-row scales that _scaled_mm multiplies back. h goes to residual_out
+ * when that is not NULL. dtype: F32, F16 or BF16; weight_dtype: `dtype` or F32.
+ * Rows are contiguous, `*_stride` elements apart; any alignment. out may be x
+ * or residual, and residual_out may be x or residual (the same rows, same
+ * strides), when the types agree. No scratch. The reference has no fused norm:
+ * it composes the operator from element-wise shaders. */
+typedef struct {
+    int32_t dtype, out_dtype, weight_dtype, reserved;
+    int64_t rows, cols;
+    const void* x; int64_t x_stride;
+    const void* residual; int64_t residual_stride;       /* NULL: none */
+    const void* weight;                                  /* [cols] */
+    void* out; int64_t out_stride;
+    void* residual_out; int64_t residual_out_stride;     /* NULL: not wanted */
+    float* scale;                                        /* [rows], F8E4M3FN only */
+    double eps;
+    void* stream;
+} tvk_rms_norm_desc;
+
+tvk_status tvk_rms_norm_fwd(const tvk_rms_norm_desc* desc);
+
+/* Gradients of tvk_rms_norm_fwd (out_dtype == dtype) from the gradient dy of
+ * out, the forward's h (x without a residual) and, when not NULL, the gradient
+ * dh of residual_out. With n = h / sqrt(mean(h^2) + eps), recomputed from h,
+ * and g = dy * weight, all in float32:
+ *   dx = (g - n * mean(g * n)) / sqrt(mean(h^2) + eps) + dh,
+ *   dweight = sum over rows of dy * n.
+ * dx is the gradient of x and of residual alike. dweight (weight_dtype) NULL:
+ * not wanted. The sums over rows run in an order that depends on the sizes
+ * alone: the same bits every run. dx may be dy, h or dh (same strides). Uses
+ * library scratch when dweight is wanted. */
+typedef struct {
+    int32_t dtype, weight_dtype;
+    int64_t rows, cols;
+    const void* dy; int64_t dy_stride;
+    const void* h; int64_t h_stride;
+    const void* dh; int64_t dh_stride;                   /* NULL: none */
+    const void* weight;                                  /* [cols], NULL: ones */
+    void* dx; int64_t dx_stride;
+    void* dweight;                                       /* [cols] */
+    double eps;
+    void* stream;
+} tvk_rms_norm_bwd_desc;
+
+tvk_status tvk_rms_norm_bwd(const tvk_rms_norm_bwd_desc* desc);
+
+/* ------------------------------------------------------------------------- */
+/* Paged key/value cache: append with rotation, attention                     */
+/* ------------------------------------------------------------------------- */
+
+/* A key/value cache in pages of `page_size` slots. Position p of sequence b is
+ * slot p % page_size of page table[b][p / page_size]; an entry outside
+ * [0, pages) is no page, and nothing is read or written through it.
+ * seq_lens[b] counts the sequence's positions, the call's new tokens among
+ * them (0: no sequence in that slot of the batch): with T new tokens, token t
+ * stands at position seq_lens[b] - T + t, and tokens whose position is
+ * negative are padding (sequences with fewer new tokens are padded in front).
+ * Lengths past the table's reach are taken as table_width * page_size (at most
+ * 2^30).
+ * table and seq_lens are read on the device, so a captured call follows them.
+ * dtype: the call's own, or F8E4M3FN (values are stored divided by their
+ * head's scale, saturating at 448, and multiplied by it when read). Strides
+ * are in elements, any page and slot order; head_dim values are contiguous. */
+typedef struct {
+    int32_t dtype, reserved;
+    int64_t pages, page_size, heads_kv, head_dim;
+    void* k; int64_t k_stride[3];                 /* [page][slot][head] */
+    void* v; int64_t v_stride[3];
+    const float* k_scale; const float* v_scale;   /* [heads_kv], NULL: 1 (F8E4M3FN only) */
+    const int32_t* table; int64_t table_stride, table_width;   /* [batch][table_width] */
+    const int32_t* seq_lens;                      /* [batch] */
+} tvk_paged_cache;
+
+/* Rotates the new tokens' queries and keys by their positions and writes keys
+ * and values to their slots. rotary row p holds cos (rotary_dim / 2 values)
+ * then sin of position p's angles, float32; pair i of a head's first
+ * rotary_dim values is (i, i + rotary_dim / 2), or (2i, 2i + 1) when
+ * `interleaved`: (a, b) -> (a cos - b sin, b cos + a sin), in float32, rounded
+ * once. rotary NULL: no rotation. A token without a place (padding, no page, a
+ * position past rotary_len) is not appended and its q_out row is zeros.
+ * q_out may be q. Two sequences must not share the pages they append to.
+ * dtype F32, F16 or BF16; head dims up to 1024, batch * new_tokens below 2^31.
+ * No scratch. */
+typedef struct {
+    tvk_paged_cache cache;
+    int32_t dtype, interleaved;
+    int64_t batch, new_tokens, heads_q;
+    const void* q; int64_t q_stride[3];           /* [batch][token][head]; NULL with heads_q 0 */
+    const void* k; int64_t k_stride[3];
+    const void* v; int64_t v_stride[3];
+    void* q_out; int64_t q_out_stride[3];
+    const float* rotary; int64_t rotary_len, rotary_dim, rotary_stride;
+    void* stream;
+} tvk_paged_append_desc;
+
+tvk_status tvk_paged_append(const tvk_paged_append_desc* desc);
+
+/* out[b,t,h,:] = sum_j softmax_j(scale * q[b,t,h,:] . k[j, h / group, :]) v[j, h / group, :]
+ * over positions j of sequence b with j <= p and, when window > 0, j > p - window,
+ * p = seq_lens[b] - new_tokens + t the token's own position. A token without
+ * keys gives out = 0 and lse = +inf; lse (NULL: not wanted) otherwise as
+ * tvk_attention_fwd's. Scores and the softmax are float32; in the MFMA kernel
+ * the probabilities are rounded to the dtype before the product with v.
+ * max_len: a bound on seq_lens the host knows (it sizes the launch: how the
+ * keys are split over workgroups), longer sequences are cut to it; 0: the
+ * table's reach. Slots past a sequence's length are never read into a result.
+ * dtype F32, F16 or BF16, head_dim up to 512. float16/bfloat16 queries with
+ * head_dim a multiple of 16 up to 256, 16-byte aligned rows and caches below
+ * 64 GiB run the MFMA kernel, other cases a general one. Partial sums of split
+ * keys use library scratch and are joined in split order (the same bits every
+ * run), in the same launch, or by a second one under graph capture. */
+typedef struct {
+    tvk_paged_cache cache;
+    int32_t dtype, reserved;
+    int64_t batch, new_tokens, heads_q, max_len, window;
+    const void* q; int64_t q_stride[3];           /* [batch][token][head] */
+    void* out; int64_t out_stride[3];
+    float* lse; int64_t lse_stride[3];
+    double scale;
+    void* stream;
+} tvk_paged_attention_desc;
+
+tvk_status tvk_paged_attention(const tvk_paged_attention_desc* desc);
 
 /* ------------------------------------------------------------------------- */
 /* Compute: batched strided GEMM with fused epilogue                          */

@@ -188,6 +188,76 @@ class AttentionBwdDesc(C.Structure):
     ]
 
 
+class RmsNormDesc(C.Structure):
+    _fields_ = [
+        ("dtype", C.c_int32), ("out_dtype", C.c_int32), ("weight_dtype", C.c_int32), ("reserved", C.c_int32),
+        ("rows", C.c_int64), ("cols", C.c_int64),
+        ("x", C.c_void_p), ("x_stride", C.c_int64),
+        ("residual", C.c_void_p), ("residual_stride", C.c_int64),
+        ("weight", C.c_void_p),
+        ("out", C.c_void_p), ("out_stride", C.c_int64),
+        ("residual_out", C.c_void_p), ("residual_out_stride", C.c_int64),
+        ("scale", C.c_void_p),
+        ("eps", C.c_double),
+        ("stream", C.c_void_p),
+    ]
+
+
+class RmsNormBwdDesc(C.Structure):
+    _fields_ = [
+        ("dtype", C.c_int32), ("weight_dtype", C.c_int32),
+        ("rows", C.c_int64), ("cols", C.c_int64),
+        ("dy", C.c_void_p), ("dy_stride", C.c_int64),
+        ("h", C.c_void_p), ("h_stride", C.c_int64),
+        ("dh", C.c_void_p), ("dh_stride", C.c_int64),
+        ("weight", C.c_void_p),
+        ("dx", C.c_void_p), ("dx_stride", C.c_int64),
+        ("dweight", C.c_void_p),
+        ("eps", C.c_double),
+        ("stream", C.c_void_p),
+    ]
+
+
+class PagedCache(C.Structure):
+    _fields_ = [
+        ("dtype", C.c_int32), ("reserved", C.c_int32),
+        ("pages", C.c_int64), ("page_size", C.c_int64), ("heads_kv", C.c_int64), ("head_dim", C.c_int64),
+        ("k", C.c_void_p), ("k_stride", I64x3),
+        ("v", C.c_void_p), ("v_stride", I64x3),
+        ("k_scale", C.c_void_p), ("v_scale", C.c_void_p),
+        ("table", C.c_void_p), ("table_stride", C.c_int64), ("table_width", C.c_int64),
+        ("seq_lens", C.c_void_p),
+    ]
+
+
+class PagedAppendDesc(C.Structure):
+    _fields_ = [
+        ("cache", PagedCache),
+        ("dtype", C.c_int32), ("interleaved", C.c_int32),
+        ("batch", C.c_int64), ("new_tokens", C.c_int64), ("heads_q", C.c_int64),
+        ("q", C.c_void_p), ("q_stride", I64x3),
+        ("k", C.c_void_p), ("k_stride", I64x3),
+        ("v", C.c_void_p), ("v_stride", I64x3),
+        ("q_out", C.c_void_p), ("q_out_stride", I64x3),
+        ("rotary", C.c_void_p), ("rotary_len", C.c_int64), ("rotary_dim", C.c_int64), ("rotary_stride", C.c_int64),
+        ("stream", C.c_void_p),
+    ]
+
+
+class PagedAttentionDesc(C.Structure):
+    _fields_ = [
+        ("cache", PagedCache),
+        ("dtype", C.c_int32), ("reserved", C.c_int32),
+        ("batch", C.c_int64), ("new_tokens", C.c_int64), ("heads_q", C.c_int64), ("max_len", C.c_int64),
+        ("window", C.c_int64),
+        ("q", C.c_void_p), ("q_stride", I64x3),
+        ("out", C.c_void_p), ("out_stride", I64x3),
+        ("lse", C.c_void_p), ("lse_stride", I64x3),
+        ("scale", C.c_double),
+        ("stream", C.c_void_p),
+    ]
+
+
 class DeviceProps(C.Structure):
     _fields_ = [
         ("name", C.c_char * 256),
@@ -258,6 +328,10 @@ def load() -> C.CDLL:
         lib.tvk_binary.argtypes = [C.POINTER(BinaryDesc)]
         lib.tvk_attention_fwd.argtypes = [C.POINTER(AttentionDesc)]
         lib.tvk_attention_bwd.argtypes = [C.POINTER(AttentionBwdDesc)]
+        lib.tvk_rms_norm_fwd.argtypes = [C.POINTER(RmsNormDesc)]
+        lib.tvk_rms_norm_bwd.argtypes = [C.POINTER(RmsNormBwdDesc)]
+        lib.tvk_paged_append.argtypes = [C.POINTER(PagedAppendDesc)]
+        lib.tvk_paged_attention.argtypes = [C.POINTER(PagedAttentionDesc)]
         lib.tvk_calibrate_mfma.argtypes = [C.c_int, C.c_int, C.c_int, C.POINTER(C.c_double), C.POINTER(C.c_double)]
         lib.tvk_calibrate_mfma_operands.argtypes = [C.c_int, C.c_int, C.c_int, C.c_int, C.POINTER(C.c_double),
                                                     C.POINTER(C.c_double)]
@@ -280,7 +354,8 @@ _ALL_ENTRY_POINTS = (
     "tvk_conv_candidates", "tvk_conv_choose", "tvk_conv_tune",
     "tvk_copy", "tvk_copy_plan",
     "tvk_fill", "tvk_reduce_sum", "tvk_binary", "tvk_attention_fwd",
-    "tvk_attention_bwd", "tvk_gemm_noalloc", "tvk_event_create", "tvk_event_destroy", "tvk_event_record",
+    "tvk_attention_bwd", "tvk_rms_norm_fwd", "tvk_rms_norm_bwd", "tvk_paged_append", "tvk_paged_attention",
+    "tvk_gemm_noalloc", "tvk_event_create", "tvk_event_destroy", "tvk_event_record",
     "tvk_event_query", "tvk_event_synchronize", "tvk_event_elapsed", "tvk_stream_wait_event", "tvk_stream_query",
     "tvk_calibrate_mfma", "tvk_calibrate_mfma_operands",
     "tvk_calibrate_hbm",
@@ -509,6 +584,220 @@ def attention_bwd(q, k, v, out, lse, dout, bias=None, causal=False, scale=None, 
         d.dscores, d.dscores_stride = ds.data_ptr(), I64x4(*ds.stride())
     check(load().tvk_attention_bwd(C.byref(d)))
     return (dq, dk, dv, ds) if dscores else (dq, dk, dv)
+
+
+# ---------------------------------------------------------------------------
+# root-mean-square norm, paged key/value cache
+# ---------------------------------------------------------------------------
+
+def _invalid(message: str):
+    return TvkError(TVK_ERR_INVALID, message)
+
+
+def _row_stride(t, rows: int, cols: int, dtype, what: str) -> int:
+    """Stride between the rows of a [rows, cols] tensor of `dtype` whose rows are contiguous."""
+    if tuple(t.shape) != (rows, cols):
+        raise _invalid(f"{what}: shape {tuple(t.shape)}, expected {(rows, cols)}")
+    if t.dtype != dtype:
+        raise _invalid(f"{what}: dtype {t.dtype}, expected {dtype}")
+    if cols > 1 and t.stride(1) != 1:
+        raise TvkUnsupported(TVK_ERR_UNSUPPORTED, f"{what}: rows must be contiguous")
+    return t.stride(0)
+
+
+def _vector(t, n: int, dtypes, what: str) -> int:
+    """Address of a contiguous vector of n values."""
+    if tuple(t.shape) != (n,) or t.dtype not in dtypes or (n > 1 and t.stride(0) != 1):
+        raise _invalid(f"{what}: a contiguous vector of {n} {' or '.join(map(str, dtypes))} values is expected")
+    return t.data_ptr()
+
+
+def make_rms_norm_desc(x, weight, out, residual=None, residual_out=None, scale=None, eps=1e-5, stream=None) -> RmsNormDesc:
+    """Describes tvk_rms_norm_fwd over [rows, cols] device tensors; out of x's dtype, or float8_e4m3fn with the
+    float32 row scales in `scale`."""
+    torch = _torch()
+    if x.dim() != 2:
+        raise _invalid(f"x: {x.dim()} dimensions, expected [rows, cols]")
+    rows, cols = x.shape
+    d = RmsNormDesc()
+    d.dtype = _dtype_code(x.dtype)
+    d.rows, d.cols = rows, cols
+    d.x, d.x_stride = x.data_ptr(), _row_stride(x, rows, cols, x.dtype, "x")
+    d.weight_dtype = d.dtype
+    if weight is not None:
+        d.weight, d.weight_dtype = _vector(weight, cols, (x.dtype, torch.float32), "weight"), _dtype_code(weight.dtype)
+    if residual is not None:
+        d.residual, d.residual_stride = residual.data_ptr(), _row_stride(residual, rows, cols, x.dtype, "residual")
+    if residual_out is not None:
+        d.residual_out, d.residual_out_stride = residual_out.data_ptr(), _row_stride(residual_out, rows, cols, x.dtype,
+                                                                                     "residual_out")
+    in8 = out.dtype == torch.float8_e4m3fn
+    d.out_dtype = TVK_F8E4M3FN if in8 else d.dtype
+    d.out, d.out_stride = out.data_ptr(), _row_stride(out, rows, cols, out.dtype if in8 else x.dtype, "out")
+    if in8 != (scale is not None):
+        raise _invalid("scale: wanted with a float8_e4m3fn output and only then")
+    if in8:
+        d.scale = _vector(scale, rows, (torch.float32,), "scale")
+    d.eps = float(eps)
+    d.stream = stream
+    return d
+
+
+def rms_norm_fwd(x, weight=None, residual=None, eps=1e-5, out_dtype=None, stream=None):
+    """(y, h, scale) of tvk_rms_norm_fwd over a [rows, cols] tensor: h is x where there is no residual; scale is None
+    unless out_dtype is float8_e4m3fn."""
+    torch = _torch()
+    y = torch.empty(x.shape, dtype=out_dtype or x.dtype, device=x.device)
+    h = torch.empty(x.shape, dtype=x.dtype, device=x.device) if residual is not None else None
+    scale = torch.empty(x.shape[0], dtype=torch.float32, device=x.device) if y.dtype == torch.float8_e4m3fn else None
+    d = make_rms_norm_desc(x, weight, y, residual, h, scale, eps, _stream_of(x, stream))
+    check(load().tvk_rms_norm_fwd(C.byref(d)))
+    return y, x if h is None else h, scale
+
+
+def make_rms_norm_bwd_desc(dy, h, weight, dx, dweight=None, dh=None, eps=1e-5, stream=None) -> RmsNormBwdDesc:
+    """Describes tvk_rms_norm_bwd over [rows, cols] device tensors."""
+    torch = _torch()
+    if h.dim() != 2:
+        raise _invalid(f"h: {h.dim()} dimensions, expected [rows, cols]")
+    rows, cols = h.shape
+    d = RmsNormBwdDesc()
+    d.dtype = _dtype_code(h.dtype)
+    d.rows, d.cols = rows, cols
+    d.dy, d.dy_stride = dy.data_ptr(), _row_stride(dy, rows, cols, h.dtype, "dy")
+    d.h, d.h_stride = h.data_ptr(), _row_stride(h, rows, cols, h.dtype, "h")
+    if dh is not None:
+        d.dh, d.dh_stride = dh.data_ptr(), _row_stride(dh, rows, cols, h.dtype, "dh")
+    d.dx, d.dx_stride = dx.data_ptr(), _row_stride(dx, rows, cols, h.dtype, "dx")
+    wdtype = h.dtype
+    if weight is not None:
+        d.weight, wdtype = _vector(weight, cols, (h.dtype, torch.float32), "weight"), weight.dtype
+    if dweight is not None:
+        wdtype = wdtype if weight is not None else dweight.dtype
+        d.dweight = _vector(dweight, cols, (wdtype,), "dweight")
+    d.weight_dtype = _dtype_code(wdtype)
+    d.eps = float(eps)
+    d.stream = stream
+    return d
+
+
+def rms_norm_bwd(dy, h, weight=None, dh=None, eps=1e-5, stream=None):
+    """(dx, dweight) of tvk_rms_norm_bwd; dweight is None without a weight."""
+    torch = _torch()
+    dx = torch.empty(h.shape, dtype=h.dtype, device=h.device)
+    dweight = torch.empty_like(weight) if weight is not None else None
+    d = make_rms_norm_bwd_desc(dy, h, weight, dx, dweight, dh, eps, _stream_of(h, stream))
+    check(load().tvk_rms_norm_bwd(C.byref(d)))
+    return dx, dweight
+
+
+def make_paged_cache(k_cache, v_cache, seq_lens, table, k_scale=None, v_scale=None) -> PagedCache:
+    """A cache of [pages, page_size, heads_kv, head_dim] tensors (any strides, head_dim contiguous), int32 table
+    [batch, entries] and int32 lengths [batch]."""
+    torch = _torch()
+    if k_cache.dim() != 4 or k_cache.shape != v_cache.shape or k_cache.dtype != v_cache.dtype:
+        raise _invalid("k_cache and v_cache: [pages, page_size, heads_kv, head_dim] of one shape and dtype are expected")
+    if k_cache.shape[3] > 1 and (k_cache.stride(3) != 1 or v_cache.stride(3) != 1):
+        raise TvkUnsupported(TVK_ERR_UNSUPPORTED, "k_cache and v_cache: head_dim values must be contiguous")
+    if seq_lens.dim() != 1 or seq_lens.dtype != torch.int32 or table.dim() != 2 or table.dtype != torch.int32:
+        raise _invalid("seq_lens and table: int32 [batch] and [batch, entries] are expected")
+    if table.shape[0] != seq_lens.shape[0] or (seq_lens.numel() > 1 and seq_lens.stride(0) != 1) or \
+            (table.shape[1] > 1 and table.stride(1) != 1):
+        raise _invalid("seq_lens and table: one batch, contiguous rows")
+    c = PagedCache()
+    c.dtype = TVK_F8E4M3FN if k_cache.dtype == torch.float8_e4m3fn else _dtype_code(k_cache.dtype)
+    c.pages, c.page_size, c.heads_kv, c.head_dim = k_cache.shape
+    c.k, c.k_stride = k_cache.data_ptr(), I64x3(*k_cache.stride()[:3])
+    c.v, c.v_stride = v_cache.data_ptr(), I64x3(*v_cache.stride()[:3])
+    if k_scale is not None:
+        c.k_scale = _vector(k_scale, c.heads_kv, (torch.float32,), "k_scale")
+    if v_scale is not None:
+        c.v_scale = _vector(v_scale, c.heads_kv, (torch.float32,), "v_scale")
+    c.table, c.table_stride, c.table_width = table.data_ptr(), table.stride(0), table.shape[1]
+    c.seq_lens = seq_lens.data_ptr()
+    return c
+
+
+def _token_strides(t, shape, dtype, what: str):
+    """(batch, token, head) strides of a [batch, tokens, heads, head_dim] tensor."""
+    if tuple(t.shape) != tuple(shape) or t.dtype != dtype:
+        raise _invalid(f"{what}: {tuple(t.shape)} {t.dtype}, expected {tuple(shape)} {dtype}")
+    if shape[3] > 1 and t.stride(3) != 1:
+        raise TvkUnsupported(TVK_ERR_UNSUPPORTED, f"{what}: head_dim values must be contiguous")
+    return I64x3(*t.stride()[:3])
+
+
+def make_paged_append_desc(q, k, v, q_out, k_cache, v_cache, seq_lens, table, rotary=None, interleaved=False,
+                           k_scale=None, v_scale=None, stream=None) -> PagedAppendDesc:
+    """Describes tvk_paged_append over [batch, tokens, heads, head_dim] tokens (q and q_out None: keys and values
+    alone); rotary float32 [positions, rotary_dim], cos then sin."""
+    torch = _torch()
+    d = PagedAppendDesc()
+    d.cache = make_paged_cache(k_cache, v_cache, seq_lens, table, k_scale, v_scale)
+    d.dtype = _dtype_code(k.dtype)
+    shape = (seq_lens.shape[0], k.shape[1] if k.dim() == 4 else -1, d.cache.heads_kv, d.cache.head_dim)
+    d.k, d.k_stride = k.data_ptr(), _token_strides(k, shape, k.dtype, "k")
+    d.v, d.v_stride = v.data_ptr(), _token_strides(v, shape, k.dtype, "v")
+    d.batch, d.new_tokens = shape[:2]
+    if q is not None:
+        if q.dim() != 4 or q_out is None:
+            raise _invalid("q: [batch, tokens, heads, head_dim] and a q_out are expected")
+        shape = (*shape[:2], q.shape[2], shape[3])
+        d.heads_q = q.shape[2]
+        d.q, d.q_stride = q.data_ptr(), _token_strides(q, shape, k.dtype, "q")
+        d.q_out, d.q_out_stride = q_out.data_ptr(), _token_strides(q_out, shape, k.dtype, "q_out")
+    d.interleaved = 1 if interleaved else 0
+    if rotary is not None:
+        if rotary.dim() != 2 or rotary.dtype != torch.float32 or (rotary.shape[1] > 1 and rotary.stride(1) != 1):
+            raise _invalid("rotary: float32 [positions, rotary_dim] with contiguous rows is expected")
+        d.rotary, d.rotary_stride = rotary.data_ptr(), rotary.stride(0)
+        d.rotary_len, d.rotary_dim = rotary.shape
+    d.stream = stream
+    return d
+
+
+def paged_append(q, k, v, k_cache, v_cache, seq_lens, table, rotary=None, interleaved=False, k_scale=None,
+                 v_scale=None, stream=None):
+    """Appends the new tokens' keys and values to the cache and returns their rotated queries (a new tensor)."""
+    torch = _torch()
+    q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device) if q is not None else None
+    d = make_paged_append_desc(q, k, v, q_out, k_cache, v_cache, seq_lens, table, rotary, interleaved, k_scale, v_scale,
+                               _stream_of(k, stream))
+    check(load().tvk_paged_append(C.byref(d)))
+    return q_out
+
+
+def make_paged_attention_desc(q, k_cache, v_cache, out, seq_lens, table, max_len=0, scale=None, window=0, k_scale=None,
+                              v_scale=None, lse=None, stream=None) -> PagedAttentionDesc:
+    """Describes tvk_paged_attention of [batch, tokens, heads, head_dim] queries; lse float32 [batch, tokens, heads]."""
+    torch = _torch()
+    d = PagedAttentionDesc()
+    d.cache = make_paged_cache(k_cache, v_cache, seq_lens, table, k_scale, v_scale)
+    d.dtype = _dtype_code(q.dtype)
+    shape = (seq_lens.shape[0], *(q.shape[1:3] if q.dim() == 4 else (-1, -1)), d.cache.head_dim)
+    d.q, d.q_stride = q.data_ptr(), _token_strides(q, shape, q.dtype, "q")
+    d.out, d.out_stride = out.data_ptr(), _token_strides(out, shape, q.dtype, "out")
+    d.batch, d.new_tokens, d.heads_q = shape[:3]
+    if lse is not None:
+        if tuple(lse.shape) != shape[:3] or lse.dtype != torch.float32:
+            raise _invalid(f"lse: float32 {shape[:3]} is expected")
+        d.lse, d.lse_stride = lse.data_ptr(), I64x3(*lse.stride())
+    d.max_len, d.window = int(max_len or 0), int(window or 0)
+    d.scale = float(scale if scale is not None else shape[3] ** -0.5)
+    d.stream = stream
+    return d
+
+
+def paged_attention(q, k_cache, v_cache, seq_lens, table, max_len=0, scale=None, window=0, k_scale=None, v_scale=None,
+                    stream=None):
+    """(out, lse) of tvk_paged_attention (new tensors)."""
+    torch = _torch()
+    out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    lse = torch.empty(q.shape[:3], dtype=torch.float32, device=q.device)
+    d = make_paged_attention_desc(q, k_cache, v_cache, out, seq_lens, table, max_len, scale, window, k_scale, v_scale, lse,
+                                  _stream_of(q, stream))
+    check(load().tvk_paged_attention(C.byref(d)))
+    return out, lse
 
 
 def _strides3(t) -> tuple[int, int, int]:

@@ -1,0 +1,198 @@
+// Append to a paged key/value cache (tvk_paged_append): rotation of the new
+// tokens' queries and keys, and their keys and values into their slots.
+//
+// A thread rotates one pair of values (or copies two) of one head of one
+// token; the queries', keys' and values' heads of a token follow each other.
+#include "paged.h"
+
+#include <algorithm>
+
+using namespace tvk;
+
+namespace tvk {
+
+tvk_status check_paged_cache(const char* who, const tvk_paged_cache& c, int32_t dtype, int64_t batch) {
+    auto bad = [&](tvk_status st, const char* m) { return fail(st, std::string(who) + ": " + m); };
+    if (dtype != TVK_F32 && dtype != TVK_F16 && dtype != TVK_BF16)
+        return bad(TVK_ERR_UNSUPPORTED, "dtype must be float32, float16 or bfloat16");
+    if (c.dtype != dtype && c.dtype != TVK_F8E4M3FN)
+        return bad(TVK_ERR_UNSUPPORTED, "the cache's dtype must be the tokens' or float8_e4m3fn");
+    if (c.dtype != TVK_F8E4M3FN && (c.k_scale || c.v_scale))
+        return bad(TVK_ERR_INVALID, "scales belong to a float8_e4m3fn cache");
+    if (batch < 0 || c.pages < 0 || c.page_size <= 0 || c.heads_kv <= 0 || c.head_dim <= 0 || c.table_width < 0)
+        return bad(TVK_ERR_INVALID, "a negative size, or a cache without slots or heads");
+    if (c.pages > 0x7fffffff || c.page_size > 0x7fffffff || c.heads_kv > 65535 || batch > 0x7fffffff)
+        return bad(TVK_ERR_UNSUPPORTED, "pages, page size and batch up to 2^31 - 1, key/value heads up to 65535 only");
+    if (c.table_width > 0x7fffffff)
+        return bad(TVK_ERR_UNSUPPORTED, "table rows up to 2^31 - 1 entries only");
+    for (int i = 0; i < 3; ++i)
+        if (c.k_stride[i] < 0 || c.v_stride[i] < 0) return bad(TVK_ERR_INVALID, "negative cache stride");
+    if (batch > 0 && (!c.seq_lens || (c.table_width > 0 && !c.table))) return bad(TVK_ERR_INVALID, "NULL table or lengths");
+    if (batch > 0 && c.pages > 0 && (!c.k || !c.v)) return bad(TVK_ERR_INVALID, "NULL cache");
+    if (batch > 1 && c.table_stride < 0) return bad(TVK_ERR_INVALID, "negative table stride");
+    return TVK_OK;
+}
+
+PagedCache paged_cache(const tvk_paged_cache& c) {
+    PagedCache p{};
+    p.k = c.k;
+    p.v = c.v;
+    for (int i = 0; i < 3; ++i) {
+        p.sk[i] = c.k_stride[i];
+        p.sv[i] = c.v_stride[i];
+    }
+    p.k_scale = c.k_scale;
+    p.v_scale = c.v_scale;
+    p.table = c.table;
+    p.lens = c.seq_lens;
+    p.table_stride = c.table_stride;
+    p.pages = (uint32_t)c.pages;
+    p.reach = (uint32_t)(c.table_width > kMaxReach / c.page_size ? kMaxReach : c.table_width * c.page_size);
+    p.page = make_div((uint32_t)c.page_size);
+    p.kvh = (int)c.heads_kv;
+    p.hd = (int)c.head_dim;
+    return p;
+}
+
+}  // namespace tvk
+
+namespace {
+
+constexpr int AP_THREADS = 256;
+
+struct AppendArgs {
+    PagedCache c;
+    const void* q;
+    const void* k;
+    const void* v;
+    void* qo;
+    int64_t sq[3], sk[3], sv[3], so[3];   // batch, token, head strides
+    const float* rotary;
+    int64_t srot;
+    uint32_t rot_len;
+    int half;               // rotated pairs of a head
+    int interleaved;
+    int heads_q;
+    int64_t tokens;         // batch * new tokens
+    Div32 per_head, per_token, new_tokens;
+};
+
+template <int DT, bool F8>
+__global__ __launch_bounds__(AP_THREADS) void paged_append_kernel(AppendArgs p) {
+    typedef typename elem<DT>::T T;
+    const uint32_t items = p.per_token.d;
+    for (int64_t token = blockIdx.x; token < p.tokens; token += gridDim.x) {
+        const uint32_t b = div32((uint32_t)token, p.new_tokens), t = (uint32_t)token - b * p.new_tokens.d;
+        const int pos = paged_len(p.c, b) - (int)p.new_tokens.d + (int)t;
+        uint32_t page = 0, slot = 0;
+        bool placed = pos >= 0 && (!p.rotary || (uint32_t)pos < p.rot_len);
+        placed = placed && paged_find(p.c, b, (uint32_t)pos, page, slot);
+        const float* rot = p.rotary + (placed ? pos * p.srot : 0);
+        for (uint32_t i = threadIdx.x; i < items; i += AP_THREADS) {
+            const int head = (int)div32(i, p.per_head), j = (int)(i - head * p.per_head.d);
+            const bool is_q = head < p.heads_q, is_k = !is_q && head < p.heads_q + p.c.kvh;
+            const int h = is_q ? head : is_k ? head - p.heads_q : head - p.heads_q - p.c.kvh;
+            if (!placed && !is_q) continue;
+            const T* src = is_q ? static_cast<const T*>(p.q) + b * p.sq[0] + t * p.sq[1] + h * p.sq[2]
+                         : is_k ? static_cast<const T*>(p.k) + b * p.sk[0] + t * p.sk[1] + h * p.sk[2]
+                                : static_cast<const T*>(p.v) + b * p.sv[0] + t * p.sv[1] + h * p.sv[2];
+            const bool turn = (is_q || is_k) && j < p.half;
+            // the item's two values: a rotated pair, or two neighbours (the last one alone)
+            const int d0 = turn && !p.interleaved ? j : 2 * j, d1 = turn && !p.interleaved ? j + p.half : 2 * j + 1;
+            const bool two = d1 < p.c.hd;
+            const T x0 = src[d0], y0 = two ? src[d1] : T(0);
+            float x = elem<DT>::to_f32(x0), y = elem<DT>::to_f32(y0);
+            if (turn && placed) {
+                const float cs = rot[j], sn = rot[p.half + j];
+                const float a = x, bb = y;
+                x = a * cs - bb * sn;
+                y = bb * cs + a * sn;
+            }
+            if (is_q) {
+                T* o = static_cast<T*>(p.qo) + b * p.so[0] + t * p.so[1] + h * p.so[2];
+                // values that are not rotated keep their bits
+                o[d0] = !placed ? T(0) : turn ? elem<DT>::from_f32(x) : x0;
+                if (two) o[d1] = !placed ? T(0) : turn ? elem<DT>::from_f32(y) : y0;
+                continue;
+            }
+            const int64_t* st = is_k ? p.c.sk : p.c.sv;
+            const int64_t off = (int64_t)page * st[0] + (int64_t)slot * st[1] + (int64_t)h * st[2];
+            if (F8) {
+                uint8_t* o = static_cast<uint8_t*>(is_k ? p.c.k : p.c.v) + off;
+                const float* sc = is_k ? p.c.k_scale : p.c.v_scale;
+                const float s = sc ? sc[h] : 1.0f;
+                auto sat = [&](float f) {
+                    f /= s;
+                    return f32_to_f8(f != f ? f : fminf(fmaxf(f, -448.0f), 448.0f), TVK_F8E4M3FN);
+                };
+                o[d0] = sat(x);
+                if (two) o[d1] = sat(y);
+            } else {
+                T* o = static_cast<T*>(is_k ? p.c.k : p.c.v) + off;
+                o[d0] = turn ? elem<DT>::from_f32(x) : x0;
+                if (two) o[d1] = turn ? elem<DT>::from_f32(y) : y0;
+            }
+        }
+    }
+}
+
+}  // namespace
+
+extern "C" tvk_status tvk_paged_append(const tvk_paged_append_desc* d) {
+    const char* who = "tvk_paged_append";
+    auto bad = [&](tvk_status st, const char* m) { return fail(st, std::string(who) + ": " + m); };
+    if (!d) return bad(TVK_ERR_INVALID, "desc is NULL");
+    const tvk_paged_cache& c = d->cache;
+    tvk_status st = check_paged_cache(who, c, d->dtype, d->batch);
+    if (st != TVK_OK) return st;
+    if (d->new_tokens < 0 || d->heads_q < 0) return bad(TVK_ERR_INVALID, "negative size");
+    if (c.head_dim > 1024 || d->heads_q > 65535) return bad(TVK_ERR_UNSUPPORTED, "head dims up to 1024, heads up to 65535 only");
+    if (d->new_tokens > 0x7fffffff || (d->new_tokens > 0 && d->batch > 0x7fffffff / d->new_tokens))
+        return bad(TVK_ERR_UNSUPPORTED, "batch * new_tokens up to 2^31 - 1 only");
+    if (d->rotary) {
+        if (d->rotary_dim <= 0 || d->rotary_dim % 2 != 0 || d->rotary_dim > c.head_dim)
+            return bad(TVK_ERR_INVALID, "rotary_dim must be even, above zero and at most head_dim");
+        if (d->rotary_len < 0 || d->rotary_stride < 0) return bad(TVK_ERR_INVALID, "negative rotary size or stride");
+    }
+    for (const int64_t* s3 : {d->q_stride, d->k_stride, d->v_stride, d->q_out_stride})
+        for (int i = 0; i < 3; ++i)
+            if (s3[i] < 0) return bad(TVK_ERR_INVALID, "negative stride");
+    if (d->batch == 0 || d->new_tokens == 0) return TVK_OK;
+    if (!d->k || !d->v || (d->heads_q > 0 && (!d->q || !d->q_out))) return bad(TVK_ERR_INVALID, "NULL tensor");
+    AppendArgs p{};
+    p.c = paged_cache(c);
+    p.q = d->q;
+    p.k = d->k;
+    p.v = d->v;
+    p.qo = d->q_out;
+    for (int i = 0; i < 3; ++i) {
+        p.sq[i] = d->q_stride[i];
+        p.sk[i] = d->k_stride[i];
+        p.sv[i] = d->v_stride[i];
+        p.so[i] = d->q_out_stride[i];
+    }
+    p.rotary = d->rotary;
+    p.srot = d->rotary_stride;
+    p.rot_len = d->rotary ? (uint32_t)std::min<int64_t>(d->rotary_len, 0x7fffffff) : 0;
+    p.half = d->rotary ? (int)(d->rotary_dim / 2) : 0;
+    p.interleaved = d->interleaved != 0;
+    p.heads_q = (int)d->heads_q;
+    p.tokens = d->batch * d->new_tokens;
+    const uint32_t per_head = (uint32_t)((c.head_dim + 1) / 2);
+    p.per_head = make_div(per_head);
+    p.per_token = make_div((uint32_t)(d->heads_q + 2 * c.heads_kv) * per_head);
+    p.new_tokens = make_div((uint32_t)d->new_tokens);
+    const hipStream_t s = resolve_stream(d->stream);
+    const dim3 grid((unsigned)std::min<int64_t>(p.tokens, 1 << 20)), block(AP_THREADS);
+    const bool f8 = c.dtype == TVK_F8E4M3FN;
+#define TVK_APPEND(DT)                                                                   \
+    if (f8) hipLaunchKernelGGL((paged_append_kernel<DT, true>), grid, block, 0, s, p);   \
+    else hipLaunchKernelGGL((paged_append_kernel<DT, false>), grid, block, 0, s, p)
+    if (d->dtype == TVK_F32) { TVK_APPEND(TVK_F32); }
+    else if (d->dtype == TVK_F16) { TVK_APPEND(TVK_F16); }
+    else { TVK_APPEND(TVK_BF16); }
+#undef TVK_APPEND
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return fail(TVK_ERR_DEVICE, std::string(who) + ": launch failed: " + hipGetErrorString(e));
+    return TVK_OK;
+}
