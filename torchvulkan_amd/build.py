@@ -66,6 +66,9 @@ FILE_FLAGS = {
     "attention_decode.hip": VGPR_FORM,
     "attention_part.hip": VGPR_FORM,
     "calibrate.hip": VGPR_FORM,
+    "paged_attention_bf16.hip": VGPR_FORM,
+    "paged_attention_f16.hip": VGPR_FORM,
+    "paged_attention_f32.hip": VGPR_FORM,
     "gemm_dma128.hip": VGPR_FORM,
     "gemm_seq_ring.hip": VGPR_FORM,
     "gemm_skinny.hip": VGPR_FORM,

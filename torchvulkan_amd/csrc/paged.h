@@ -23,6 +23,21 @@ struct PagedCache {
     int kvh, hd;
 };
 
+struct PagedAttnArgs {
+    PagedCache c;
+    const void* q;
+    void* out;
+    float* lse;
+    int64_t sq[3], so[3], sl[3];   // batch, token, head strides
+    int heads, group, new_tokens;
+    uint32_t max_len;
+    uint32_t window;               // 0: none
+    float scale;
+};
+
+// Queues the MFMA kernel (paged_attention_mfma.h) when it takes the call; false when it does not.
+bool paged_attn_mfma(const PagedAttnArgs& a, int dtype, bool f8, int64_t batch, hipStream_t s);
+
 // TVK_OK when the cache is one the kernels take and its pointers are there.
 tvk_status check_paged_cache(const char* who, const tvk_paged_cache& c, int32_t dtype, int64_t batch);
 PagedCache paged_cache(const tvk_paged_cache& c);

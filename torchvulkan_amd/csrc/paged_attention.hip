@@ -18,18 +18,6 @@ constexpr int PA_WAVES = 4;
 constexpr int PA_MAX_DIM = 512;
 constexpr int PA_UNROLL = 4;
 
-struct PagedAttnArgs {
-    PagedCache c;
-    const void* q;
-    void* out;
-    float* lse;
-    int64_t sq[3], so[3], sl[3];   // batch, token, head strides
-    int heads, group, new_tokens;
-    uint32_t max_len;
-    uint32_t window;               // 0: none
-    float scale;
-};
-
 template <int DT, bool F8>
 __device__ inline float cached(const void* p, int64_t i) {
     if (F8) return f8_to_f32(static_cast<const uint8_t*>(p)[i], TVK_F8E4M3FN);
@@ -169,6 +157,7 @@ extern "C" tvk_status tvk_paged_attention(const tvk_paged_attention_desc* d) {
     const hipStream_t s = resolve_stream(d->stream);
     const int64_t rows = d->batch * d->new_tokens * d->heads_q;
     const bool f8 = c.dtype == TVK_F8E4M3FN;
+    if (paged_attn_mfma(p, d->dtype, f8, d->batch, s)) return TVK_OK;
     if (d->dtype == TVK_F32) f8 ? launch_any<TVK_F32, true>(p, rows, s) : launch_any<TVK_F32, false>(p, rows, s);
     else if (d->dtype == TVK_F16) f8 ? launch_any<TVK_F16, true>(p, rows, s) : launch_any<TVK_F16, false>(p, rows, s);
     else f8 ? launch_any<TVK_BF16, true>(p, rows, s) : launch_any<TVK_BF16, false>(p, rows, s);
