@@ -1,9 +1,15 @@
 // Append to a paged key/value cache (tvk_paged_append): rotation of the new
 // tokens' queries and keys, and their keys and values into their slots.
 //
-// A thread rotates one pair of values (or copies two) of one head of one
-// token; the queries', keys' and values' heads of a token follow each other.
+// The call moves each value once and is bound by that. The queries', keys' and
+// values' heads of a token follow each other. A thread takes two chunks of VEC
+// values of a head, 16 bytes each: the two that are rotated into each other, or
+// neighbours; rotated values are read and written by one thread, so q_out may be
+// q. A token's chunks are taken by as many waves as it needs for the call to fill
+// the chip, and where a lane meets the same place of every head, it keeps its
+// angles. Rotations that do not split into chunks run one pair a thread.
 #include "paged.h"
+#include "words.h"
 
 #include <algorithm>
 
@@ -74,19 +80,41 @@ struct AppendArgs {
     int interleaved;
     int heads_q;
     int64_t tokens;         // batch * new tokens
+    Div32 split;            // waves a token
+    int same_place;         // a lane's chunks lie in the same place of every head it meets
     Div32 per_head, per_token, new_tokens;
 };
 
+// A product and a sum, each rounded: (a cos - b sin, b cos + a sin) is the same from any kernel.
+__device__ inline void rotate(float& a, float& b, float cs, float sn) {
+#pragma clang fp contract(off)
+    const float x = a * cs - b * sn;
+    b = b * cs + a * sn;
+    a = x;
+}
+
+__device__ inline float saturated(float f, float s) {
+    f /= s;
+    return f != f ? f : fminf(fmaxf(f, -448.0f), 448.0f);
+}
+
+// A token's place; false for padding, a position past the angles and a page that is none.
+__device__ inline bool place(const AppendArgs& p, int64_t token, uint32_t& b, uint32_t& t, int& pos, uint32_t& page, uint32_t& slot) {
+    b = div32((uint32_t)token, p.new_tokens);
+    t = (uint32_t)token - b * p.new_tokens.d;
+    pos = paged_len(p.c, b) - (int)p.new_tokens.d + (int)t;
+    page = slot = 0;
+    return pos >= 0 && (!p.rotary || (uint32_t)pos < p.rot_len) && paged_find(p.c, b, (uint32_t)pos, page, slot);
+}
+
 template <int DT, bool F8>
-__global__ __launch_bounds__(AP_THREADS) void paged_append_kernel(AppendArgs p) {
+__global__ __launch_bounds__(AP_THREADS) void paged_append_any_kernel(AppendArgs p) {
     typedef typename elem<DT>::T T;
     const uint32_t items = p.per_token.d;
     for (int64_t token = blockIdx.x; token < p.tokens; token += gridDim.x) {
-        const uint32_t b = div32((uint32_t)token, p.new_tokens), t = (uint32_t)token - b * p.new_tokens.d;
-        const int pos = paged_len(p.c, b) - (int)p.new_tokens.d + (int)t;
-        uint32_t page = 0, slot = 0;
-        bool placed = pos >= 0 && (!p.rotary || (uint32_t)pos < p.rot_len);
-        placed = placed && paged_find(p.c, b, (uint32_t)pos, page, slot);
+        uint32_t b, t, page, slot;
+        int pos;
+        const bool placed = place(p, token, b, t, pos, page, slot);
         const float* rot = p.rotary + (placed ? pos * p.srot : 0);
         for (uint32_t i = threadIdx.x; i < items; i += AP_THREADS) {
             const int head = (int)div32(i, p.per_head), j = (int)(i - head * p.per_head.d);
@@ -102,12 +130,7 @@ __global__ __launch_bounds__(AP_THREADS) void paged_append_kernel(AppendArgs p) 
             const bool two = d1 < p.c.hd;
             const T x0 = src[d0], y0 = two ? src[d1] : T(0);
             float x = elem<DT>::to_f32(x0), y = elem<DT>::to_f32(y0);
-            if (turn && placed) {
-                const float cs = rot[j], sn = rot[p.half + j];
-                const float a = x, bb = y;
-                x = a * cs - bb * sn;
-                y = bb * cs + a * sn;
-            }
+            if (turn && placed) rotate(x, y, rot[j], rot[p.half + j]);
             if (is_q) {
                 T* o = static_cast<T*>(p.qo) + b * p.so[0] + t * p.so[1] + h * p.so[2];
                 // values that are not rotated keep their bits
@@ -121,12 +144,8 @@ __global__ __launch_bounds__(AP_THREADS) void paged_append_kernel(AppendArgs p) 
                 uint8_t* o = static_cast<uint8_t*>(is_k ? p.c.k : p.c.v) + off;
                 const float* sc = is_k ? p.c.k_scale : p.c.v_scale;
                 const float s = sc ? sc[h] : 1.0f;
-                auto sat = [&](float f) {
-                    f /= s;
-                    return f32_to_f8(f != f ? f : fminf(fmaxf(f, -448.0f), 448.0f), TVK_F8E4M3FN);
-                };
-                o[d0] = sat(x);
-                if (two) o[d1] = sat(y);
+                o[d0] = f32_to_f8(saturated(x, s), TVK_F8E4M3FN);
+                if (two) o[d1] = f32_to_f8(saturated(y, s), TVK_F8E4M3FN);
             } else {
                 T* o = static_cast<T*>(is_k ? p.c.k : p.c.v) + off;
                 o[d0] = turn ? elem<DT>::from_f32(x) : x0;
@@ -134,6 +153,129 @@ __global__ __launch_bounds__(AP_THREADS) void paged_append_kernel(AppendArgs p) 
             }
         }
     }
+}
+
+template <int DT, bool F8, int VEC>
+__global__ __launch_bounds__(AP_THREADS) void paged_append_kernel(AppendArgs p) {
+    typedef typename elem<DT>::T T;
+    constexpr int B = VEC * (int)sizeof(T), A = (int)sizeof(T);
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(blockIdx.x * (AP_THREADS / 64) + threadIdx.x / 64);
+    const uint32_t token = div32(wave, p.split), part = wave - token * p.split.d;
+    if (token >= p.tokens) return;
+    uint32_t b, t, page, slot;
+    int pos;
+    const bool placed = place(p, token, b, t, pos, page, slot);
+    const float* rot = p.rotary + (placed ? pos * p.srot : 0);
+    const uint32_t items = placed ? p.per_token.d : (uint32_t)p.heads_q * p.per_head.d;   // without a place: zeros in q_out
+    const int turned = p.half / VEC;   // chunk pairs that are rotated into each other
+    float cs[VEC], sn[VEC];
+    bool angles = false;
+    for (uint32_t i = part * 64 + threadIdx.x % 64; i < items; i += 64 * p.split.d) {
+        const int head = (int)div32(i, p.per_head), j = (int)(i - head * p.per_head.d);
+        const bool is_q = head < p.heads_q, is_k = !is_q && head < p.heads_q + p.c.kvh;
+        const int h = is_q ? head : is_k ? head - p.heads_q : head - p.heads_q - p.c.kvh;
+        const T* src = is_q ? static_cast<const T*>(p.q) + b * p.sq[0] + t * p.sq[1] + h * p.sq[2]
+                     : is_k ? static_cast<const T*>(p.k) + b * p.sk[0] + t * p.sk[1] + h * p.sk[2]
+                            : static_cast<const T*>(p.v) + b * p.sv[0] + t * p.sv[1] + h * p.sv[2];
+        // chunks of pairs (i, i + half) first; interleaved pairs lie inside a chunk
+        const bool across = !p.interleaved && j < turned;
+        const int d0 = across ? VEC * j : 2 * VEC * j, d1 = across ? d0 + p.half : d0 + VEC;
+        const bool two = d1 < p.c.hd;
+        const bool turn0 = !is_q && !is_k ? false : p.interleaved ? d0 < 2 * p.half : across;
+        const bool turn1 = turn0 && (!p.interleaved || d1 < 2 * p.half);
+        Words<B> w0 = load_words<B, A>(src + d0), w1 = two ? load_words<B, A>(src + d1) : Words<B>{};
+        if (placed && turn0 && (!angles || !p.same_place)) {
+            // across: VEC angles, from d0; interleaved: VEC / 2 for each of the two chunks, from d0 / 2
+            const int from = across ? d0 : d0 / 2, n = p.half - from;
+#pragma unroll
+            for (int k = 0; k < VEC; k += 2) {
+                const bool in = k < n;
+                const Words<8> c2 = load_words<8, 4>(rot + from + (in ? k : 0)), s2 = load_words<8, 4>(rot + p.half + from + (in ? k : 0));
+                cs[k] = __builtin_bit_cast(float, c2.w[0]);
+                cs[k + 1] = __builtin_bit_cast(float, c2.w[1]);
+                sn[k] = __builtin_bit_cast(float, s2.w[0]);
+                sn[k + 1] = __builtin_bit_cast(float, s2.w[1]);
+            }
+            angles = true;
+        }
+        float x[VEC], y[VEC];
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) {
+            x[k] = word_at<DT>(w0, k);
+            y[k] = word_at<DT>(w1, k);
+        }
+        if (placed && turn0) {
+            if (across) {
+#pragma unroll
+                for (int k = 0; k < VEC; ++k) rotate(x[k], y[k], cs[k], sn[k]);
+            } else {
+#pragma unroll
+                for (int k = 0; k < VEC; k += 2) rotate(x[k], x[k + 1], cs[k / 2], sn[k / 2]);
+                if (turn1)
+#pragma unroll
+                    for (int k = 0; k < VEC; k += 2) rotate(y[k], y[k + 1], cs[(VEC + k) / 2], sn[(VEC + k) / 2]);
+            }
+        }
+        // values that are not rotated keep their bits
+        const Words<B> o0 = !placed ? Words<B>{} : turn0 ? pack<DT, VEC>(x) : w0;
+        const Words<B> o1 = !placed ? Words<B>{} : turn1 ? pack<DT, VEC>(y) : w1;
+        if (is_q) {
+            T* o = static_cast<T*>(p.qo) + b * p.so[0] + t * p.so[1] + h * p.so[2];
+            store_words<B, A>(o + d0, o0);
+            if (two) store_words<B, A>(o + d1, o1);
+            continue;
+        }
+        const int64_t* st = is_k ? p.c.sk : p.c.sv;
+        const int64_t off = (int64_t)page * st[0] + (int64_t)slot * st[1] + (int64_t)h * st[2];
+        if constexpr (F8) {
+            uint8_t* o = static_cast<uint8_t*>(is_k ? p.c.k : p.c.v) + off;
+            const float* sc = is_k ? p.c.k_scale : p.c.v_scale;
+            const float s = sc ? sc[h] : 1.0f;
+            Words<VEC> e0, e1;
+#pragma unroll
+            for (int k = 0; k < VEC; k += 4) {
+                e0.w[k / 4] = pack4_f8(saturated(x[k], s), saturated(x[k + 1], s), saturated(x[k + 2], s), saturated(x[k + 3], s));
+                e1.w[k / 4] = pack4_f8(saturated(y[k], s), saturated(y[k + 1], s), saturated(y[k + 2], s), saturated(y[k + 3], s));
+            }
+            store_words<VEC, 1>(o + d0, e0);
+            if (two) store_words<VEC, 1>(o + d1, e1);
+        } else {
+            T* o = static_cast<T*>(is_k ? p.c.k : p.c.v) + off;
+            store_words<B, A>(o + d0, o0);
+            if (two) store_words<B, A>(o + d1, o1);
+        }
+    }
+}
+
+template <int DT, bool F8>
+void append(AppendArgs& p, hipStream_t s) {
+    const uint32_t heads = (uint32_t)(p.heads_q + 2 * p.c.kvh);
+    auto fits = [&](int vec) { return p.c.hd % vec == 0 && (p.interleaved ? 2 * p.half : p.half) % vec == 0; };
+    const int vec = DT != TVK_F32 && fits(8) ? 8 : fits(4) ? 4 : 0;
+    if (!vec) {
+        const uint32_t per_head = (uint32_t)((p.c.hd + 1) / 2);
+        p.per_head = make_div(per_head);
+        p.per_token = make_div(heads * per_head);
+        const dim3 grid((unsigned)std::min<int64_t>(p.tokens, 1 << 20)), block(AP_THREADS);
+        hipLaunchKernelGGL((paged_append_any_kernel<DT, F8>), grid, block, 0, s, p);
+        return;
+    }
+    const uint32_t per_head = (uint32_t)((p.c.hd / vec + 1) / 2), items = heads * per_head;
+    p.per_head = make_div(per_head);
+    p.per_token = make_div(items);
+    // waves a token: all it has work for while the chip is not full (32 waves a CU)
+    const int64_t all = (items + 63) / 64, room = std::max<int64_t>(1, 8192 / p.tokens);
+    const int64_t split = std::min(all, room);
+    p.split = make_div((uint32_t)split);
+    p.same_place = 64 * split % per_head == 0;
+    const dim3 grid((unsigned)((p.tokens * split + 3) / 4)), block(AP_THREADS);
+    if constexpr (DT != TVK_F32) {
+        if (vec == 8) {
+            hipLaunchKernelGGL((paged_append_kernel<DT, F8, 8>), grid, block, 0, s, p);
+            return;
+        }
+    }
+    hipLaunchKernelGGL((paged_append_kernel<DT, F8, 4>), grid, block, 0, s, p);
 }
 
 }  // namespace
@@ -178,20 +320,12 @@ extern "C" tvk_status tvk_paged_append(const tvk_paged_append_desc* d) {
     p.interleaved = d->interleaved != 0;
     p.heads_q = (int)d->heads_q;
     p.tokens = d->batch * d->new_tokens;
-    const uint32_t per_head = (uint32_t)((c.head_dim + 1) / 2);
-    p.per_head = make_div(per_head);
-    p.per_token = make_div((uint32_t)(d->heads_q + 2 * c.heads_kv) * per_head);
     p.new_tokens = make_div((uint32_t)d->new_tokens);
     const hipStream_t s = resolve_stream(d->stream);
-    const dim3 grid((unsigned)std::min<int64_t>(p.tokens, 1 << 20)), block(AP_THREADS);
     const bool f8 = c.dtype == TVK_F8E4M3FN;
-#define TVK_APPEND(DT)                                                                   \
-    if (f8) hipLaunchKernelGGL((paged_append_kernel<DT, true>), grid, block, 0, s, p);   \
-    else hipLaunchKernelGGL((paged_append_kernel<DT, false>), grid, block, 0, s, p)
-    if (d->dtype == TVK_F32) { TVK_APPEND(TVK_F32); }
-    else if (d->dtype == TVK_F16) { TVK_APPEND(TVK_F16); }
-    else { TVK_APPEND(TVK_BF16); }
-#undef TVK_APPEND
+    if (d->dtype == TVK_F32) f8 ? append<TVK_F32, true>(p, s) : append<TVK_F32, false>(p, s);
+    else if (d->dtype == TVK_F16) f8 ? append<TVK_F16, true>(p, s) : append<TVK_F16, false>(p, s);
+    else f8 ? append<TVK_BF16, true>(p, s) : append<TVK_BF16, false>(p, s);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return fail(TVK_ERR_DEVICE, std::string(who) + ": launch failed: " + hipGetErrorString(e));
     return TVK_OK;
