@@ -1,5 +1,16 @@
-// Root-mean-square norm (tvk_rms_norm_fwd, tvk_rms_norm_bwd): a workgroup a row.
-#include "convert.h"
+// Root-mean-square norm (tvk_rms_norm_fwd, tvk_rms_norm_bwd).
+//
+// Both directions read and write each value once and are bound by that. A row
+// is held in the registers of TPR threads (16, 64 or 256: part of a wave, a
+// wave, a workgroup), NC chunks of 16 bytes each, while its sums are taken: one
+// pass forward, for the 8-bit output too (max|h w| and the sum of squares come
+// from the same pass, and scale both), one pass backward for both sums and dx.
+// A workgroup takes rows in turn, so that it loads its weights once and, backward,
+// keeps dweight's sums over its rows in registers; those are added up by a second
+// launch in a fixed order. Rows start at any multiple of a value (16-byte accesses
+// need no more); the values past a row's last whole chunk go one to a thread.
+// Rows of more than 2048 chunks are read again for every pass.
+#include "words.h"
 
 #include <algorithm>
 
@@ -68,7 +79,7 @@ __device__ inline float block_all(float v) {
 }
 
 template <int DT>
-__global__ __launch_bounds__(RN_THREADS) void rms_norm_kernel(NormArgs p) {
+__global__ __launch_bounds__(RN_THREADS) void rms_norm_any_kernel(NormArgs p) {
     typedef typename elem<DT>::T T;
     const int64_t row = blockIdx.x;
     const T* x = static_cast<const T*>(p.x) + row * p.sx;
@@ -117,7 +128,7 @@ __global__ __launch_bounds__(RN_THREADS) void rms_norm_inv_kernel(NormBwdArgs p)
 }
 
 template <int DT>
-__global__ __launch_bounds__(RN_THREADS) void rms_norm_bwd_kernel(NormBwdArgs p) {
+__global__ __launch_bounds__(RN_THREADS) void rms_norm_bwd_any_kernel(NormBwdArgs p) {
     typedef typename elem<DT>::T T;
     const int64_t row = blockIdx.x;
     const T* dy = static_cast<const T*>(p.dy) + row * p.sdy;
@@ -159,40 +170,361 @@ __global__ __launch_bounds__(RN_THREADS) void rms_norm_dweight_kernel(NormBwdArg
     if (wave == 0 && c < p.cols) part[blockIdx.y * p.cols + c] = sum[0][lane] + sum[1][lane] + sum[2][lane] + sum[3][lane];
 }
 
+// ---------------------------------------------------------------------------
+// rows in registers
+// ---------------------------------------------------------------------------
+
+// Sums and maxima over the TPR threads of a row, the same bits in each: pairs of lanes, then the waves in order.
+template <int TPR, class Op>
+__device__ inline float row_all(float v) {
+    if constexpr (TPR == RN_THREADS) return block_all<Op>(v);
+#pragma unroll
+    for (int m = TPR / 2; m > 0; m >>= 1) v = Op::of(v, __shfl_xor(v, m));
+    return v;
+}
+
+// What a thread holds of a row: chunk i is the row's chunk t + TPR * i; then, in t < tail, one of the values past them.
+template <int DT, int NC, int TPR>
+struct Row {
+    typedef typename elem<DT>::T T;
+    static constexpr int VEC = 16 / (int)sizeof(T);
+    Words<16> c[NC];
+    float last = 0.0f;
+
+    __device__ __forceinline__ void load(const void* row, int t, int chunks, int tail) {
+        const T* p = static_cast<const T*>(row);
+#pragma unroll
+        for (int i = 0; i < NC; ++i) c[i] = t + TPR * i < chunks ? load_words<16, sizeof(T)>(p + VEC * (t + TPR * i)) : Words<16>{};
+        if (t < tail) last = elem<DT>::to_f32(p[VEC * chunks + t]);
+    }
+    __device__ __forceinline__ float at(int i, int k) const { return word_at<DT>(c[i], k); }
+    // From here on the values are unpacked anew: kept unpacked across the sums, or from row to row, they take twice the
+    // registers and with them the second workgroup on a CU.
+    __device__ __forceinline__ void packed() {
+        if constexpr (DT != TVK_F32)
+#pragma unroll
+            for (int i = 0; i < NC; ++i) asm volatile("" : "+v"(c[i].w[0]), "+v"(c[i].w[1]), "+v"(c[i].w[2]), "+v"(c[i].w[3]));
+    }
+};
+
+// A row's weights: the row's type in registers, or float32 ones beside a 16-bit row read as they are needed.
+template <int DT, int NC, int TPR>
+struct Weights {
+    typedef Row<DT, NC, TPR> R;
+    R r;
+    const float* w32 = nullptr;
+
+    __device__ __forceinline__ void load(const void* w, int is32, int t, int chunks, int tail) {
+        if (!w || (is32 && DT != TVK_F32)) {
+            float ones[R::VEC];
+#pragma unroll
+            for (int k = 0; k < R::VEC; ++k) ones[k] = 1.0f;
+#pragma unroll
+            for (int i = 0; i < NC; ++i) r.c[i] = pack<DT, R::VEC>(ones);
+            r.last = 1.0f;
+            w32 = static_cast<const float*>(w);
+            if (w32 && t < tail) r.last = w32[R::VEC * chunks + t];
+        } else {
+            r.load(w, t, chunks, tail);
+        }
+    }
+    __device__ __forceinline__ void chunk(int i, int t, int chunks, float (&f)[R::VEC]) const {
+        if (DT != TVK_F32 && w32) {
+#pragma unroll
+            for (int k = 0; k < R::VEC; k += 4) {
+                const Words<16> v = t + TPR * i < chunks ? load_words<16, 4>(w32 + R::VEC * (t + TPR * i) + k) : Words<16>{};
+#pragma unroll
+                for (int j = 0; j < 4; ++j) f[k + j] = __builtin_bit_cast(float, v.w[j]);
+            }
+        } else {
+#pragma unroll
+            for (int k = 0; k < R::VEC; ++k) f[k] = r.at(i, k);
+        }
+    }
+};
+
+template <int DT, bool OUT8, int NC, int TPR>
+__global__ __launch_bounds__(RN_THREADS) void rms_norm_kernel(NormArgs p) {
+    typedef Row<DT, NC, TPR> R;
+    typedef typename R::T T;
+    constexpr int VEC = R::VEC;
+    const int t = threadIdx.x % TPR, chunks = (int)p.cols / VEC, tail = (int)p.cols % VEC;
+    Weights<DT, NC, TPR> w;
+    w.load(p.w, p.w32, t, chunks, tail);
+    for (int64_t row = (int64_t)blockIdx.x * (RN_THREADS / TPR) + threadIdx.x / TPR; row < p.rows;
+         row += (int64_t)gridDim.x * (RN_THREADS / TPR)) {
+        R h, r;
+        h.load(static_cast<const T*>(p.x) + row * p.sx, t, chunks, tail);
+        if (p.r) {
+            r.load(static_cast<const T*>(p.r) + row * p.sr, t, chunks, tail);
+#pragma unroll
+            for (int i = 0; i < NC; ++i) {
+                float s[VEC];
+#pragma unroll
+                for (int k = 0; k < VEC; ++k) s[k] = h.at(i, k) + r.at(i, k);
+                h.c[i] = pack<DT, VEC>(s);
+            }
+            h.last = elem<DT>::to_f32(elem<DT>::from_f32(h.last + r.last));
+        }
+        w.r.packed();
+        float ss = h.last * h.last, top = fabsf(h.last * w.r.last);
+#pragma unroll
+        for (int i = 0; i < NC; ++i) {
+            float f[VEC], part = 0.0f;
+            if (OUT8) w.chunk(i, t, chunks, f);
+#pragma unroll
+            for (int k = 0; k < VEC; ++k) {
+                const float v = h.at(i, k);
+                part = fmaf(v, v, part);
+                if (OUT8) top = fmaxf(top, fabsf(v * f[k]));
+            }
+            ss += part;
+        }
+        ss = row_all<TPR, SumOp>(ss);
+        h.packed();
+        w.r.packed();
+        const float inv = 1.0f / sqrtf(ss / (float)p.cols + p.eps);
+        if (p.h) {
+            T* o = static_cast<T*>(p.h) + row * p.sh;
+#pragma unroll
+            for (int i = 0; i < NC; ++i)
+                if (t + TPR * i < chunks) store_words<16, sizeof(T)>(o + VEC * (t + TPR * i), h.c[i]);
+            if (t < tail) o[VEC * chunks + t] = elem<DT>::from_f32(h.last);
+        }
+        if constexpr (OUT8) {
+            // y = h w inv; its largest magnitude is max|h w| times inv, and y / scale = h w (inv / scale). An inv / scale
+            // that leaves float32's range, for rows of values near its ends, is not taken as one factor.
+            top = row_all<TPR, MaxOp>(top) * inv;
+            const float s = top > 0.0f ? top / kF8Max : 1.0f, f8 = inv / s;
+            const bool plain = f8 < 1e30f && f8 > 1e-30f;
+            if (t == 0) p.scale[row] = s;
+            uint8_t* o = static_cast<uint8_t*>(p.out) + row * p.so;
+            auto value = [&](float v, float wv) { return plain ? v * wv * f8 : v * wv * inv / s; };
+#pragma unroll
+            for (int i = 0; i < NC; ++i) {
+                if (t + TPR * i >= chunks) continue;
+                float f[VEC];
+                w.chunk(i, t, chunks, f);
+                Words<VEC> e;
+#pragma unroll
+                for (int k = 0; k < VEC; k += 4)
+                    e.w[k / 4] = pack4_f8(value(h.at(i, k), f[k]), value(h.at(i, k + 1), f[k + 1]), value(h.at(i, k + 2), f[k + 2]),
+                                          value(h.at(i, k + 3), f[k + 3]));
+                store_words<VEC, 1>(o + VEC * (t + TPR * i), e);
+            }
+            if (t < tail) o[VEC * chunks + t] = f32_to_f8(value(h.last, w.r.last), TVK_F8E4M3FN);
+        } else {
+            T* o = static_cast<T*>(p.out) + row * p.so;
+#pragma unroll
+            for (int i = 0; i < NC; ++i) {
+                if (t + TPR * i >= chunks) continue;
+                float f[VEC], y[VEC];
+                w.chunk(i, t, chunks, f);
+#pragma unroll
+                for (int k = 0; k < VEC; ++k) y[k] = h.at(i, k) * inv * f[k];
+                store_words<16, sizeof(T)>(o + VEC * (t + TPR * i), pack<DT, VEC>(y));
+            }
+            if (t < tail) o[VEC * chunks + t] = elem<DT>::from_f32(h.last * inv * w.r.last);
+        }
+    }
+}
+
+// part: [gridDim.x][cols], the workgroups' sums of dy * n over their rows; NULL: not wanted.
+template <int DT, int NC, int TPR>
+__global__ __launch_bounds__(RN_THREADS) void rms_norm_bwd_kernel(NormBwdArgs p, float* part) {
+    typedef Row<DT, NC, TPR> R;
+    typedef typename R::T T;
+    constexpr int VEC = R::VEC, SUBS = RN_THREADS / TPR;
+    const int t = threadIdx.x % TPR, sub = threadIdx.x / TPR, chunks = (int)p.cols / VEC, tail = (int)p.cols % VEC;
+    Weights<DT, NC, TPR> w;
+    w.load(p.w, p.w32, t, chunks, tail);
+    float acc[NC][VEC], acc_last = 0.0f;
+#pragma unroll
+    for (int i = 0; i < NC; ++i)
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) acc[i][k] = 0.0f;
+    for (int64_t row = (int64_t)blockIdx.x * SUBS + sub; row < p.rows; row += (int64_t)gridDim.x * SUBS) {
+        R dy, h, dh;
+        dy.load(static_cast<const T*>(p.dy) + row * p.sdy, t, chunks, tail);
+        h.load(static_cast<const T*>(p.h) + row * p.sh, t, chunks, tail);
+        if (p.dh) dh.load(static_cast<const T*>(p.dh) + row * p.sdh, t, chunks, tail);
+        w.r.packed();
+        float ss = h.last * h.last, gh = dy.last * w.r.last * h.last;
+#pragma unroll
+        for (int i = 0; i < NC; ++i) {
+            float f[VEC], ps = 0.0f, pg = 0.0f;
+            w.chunk(i, t, chunks, f);
+#pragma unroll
+            for (int k = 0; k < VEC; ++k) {
+                const float v = h.at(i, k);
+                ps = fmaf(v, v, ps);
+                pg = fmaf(dy.at(i, k) * f[k], v, pg);
+            }
+            ss += ps;
+            gh += pg;
+        }
+        ss = row_all<TPR, SumOp>(ss);
+        gh = row_all<TPR, SumOp>(gh);
+        dy.packed();
+        h.packed();
+        w.r.packed();
+        const float inv = 1.0f / sqrtf(ss / (float)p.cols + p.eps);
+        const float mean = gh * inv / (float)p.cols;   // of g * n
+        T* dx = static_cast<T*>(p.dx) + row * p.sdx;
+#pragma unroll
+        for (int i = 0; i < NC; ++i) {
+            float f[VEC], o[VEC];
+            w.chunk(i, t, chunks, f);
+#pragma unroll
+            for (int k = 0; k < VEC; ++k) {
+                const float n = h.at(i, k) * inv, g = dy.at(i, k);
+                acc[i][k] = fmaf(g, n, acc[i][k]);
+                o[k] = inv * (g * f[k] - n * mean);
+                if (p.dh) o[k] += dh.at(i, k);
+            }
+            if (t + TPR * i < chunks) store_words<16, sizeof(T)>(dx + VEC * (t + TPR * i), pack<DT, VEC>(o));
+        }
+        if (t < tail) {
+            const float n = h.last * inv;
+            acc_last = fmaf(dy.last, n, acc_last);
+            float o = inv * (dy.last * w.r.last - n * mean);
+            if (p.dh) o += dh.last;
+            dx[VEC * chunks + t] = elem<DT>::from_f32(o);
+        }
+    }
+    if (!part) return;
+    float* out = part + (int64_t)blockIdx.x * p.cols;
+    if constexpr (SUBS == 1) {
+#pragma unroll
+        for (int i = 0; i < NC; ++i)
+            if (t + TPR * i < chunks)
+#pragma unroll
+                for (int k = 0; k < VEC; ++k) out[VEC * (t + TPR * i) + k] = acc[i][k];
+        if (t < tail) out[VEC * chunks + t] = acc_last;
+    } else {
+        __shared__ float sum[VEC * (NC * TPR + 1)];   // the workgroup's rows added in order
+        for (int s = 0; s < SUBS; ++s) {
+            if (sub == s) {
+#pragma unroll
+                for (int i = 0; i < NC; ++i)
+                    if (t + TPR * i < chunks)
+#pragma unroll
+                        for (int k = 0; k < VEC; ++k) {
+                            float& x = sum[VEC * (t + TPR * i) + k];
+                            x = s ? x + acc[i][k] : acc[i][k];
+                        }
+                if (t < tail) {
+                    float& x = sum[VEC * chunks + t];
+                    x = s ? x + acc_last : acc_last;
+                }
+            }
+            __syncthreads();
+        }
+        for (int c = threadIdx.x; c < (int)p.cols; c += RN_THREADS) out[c] = sum[c];
+    }
+}
+
+// Adds the partials up: a workgroup FOLD_COLS columns, its threads every FOLD_ROWS-th partial, then those in order.
+constexpr int FOLD_COLS = 16, FOLD_ROWS = 64;
+
 template <int DT>
-__global__ __launch_bounds__(RN_THREADS) void rms_norm_fold_kernel(const float* part, int64_t parts, int64_t cols, void* dw,
-                                                                   int w32) {
-    const int64_t c = (int64_t)blockIdx.x * RN_THREADS + threadIdx.x;
-    if (c >= cols) return;
+__global__ __launch_bounds__(FOLD_COLS * FOLD_ROWS) void rms_norm_fold_kernel(const float* part, int64_t parts, int64_t cols,
+                                                                              void* dw, int w32) {
+    __shared__ float sum[FOLD_ROWS][FOLD_COLS + 1];
+    const int x = threadIdx.x % FOLD_COLS, y = threadIdx.x / FOLD_COLS;
+    const int64_t c = (int64_t)blockIdx.x * FOLD_COLS + x;
     float s = 0.0f;
-    for (int64_t i = 0; i < parts; ++i) s += part[i * cols + c];
-    if (w32) static_cast<float*>(dw)[c] = s;
-    else put<DT>(dw, c, s);
+    if (c < cols) {
+        int64_t i = y;
+        for (; i + 7 * FOLD_ROWS < parts; i += 8 * FOLD_ROWS) {
+            float v[8];
+#pragma unroll
+            for (int u = 0; u < 8; ++u) v[u] = part[(i + u * FOLD_ROWS) * cols + c];
+#pragma unroll
+            for (int u = 0; u < 8; ++u) s += v[u];
+        }
+        for (; i < parts; i += FOLD_ROWS) s += part[i * cols + c];
+    }
+    sum[y][x] = s;
+#pragma unroll
+    for (int m = FOLD_ROWS / 2; m > 0; m >>= 1) {
+        __syncthreads();
+        if (y < m) sum[y][x] += sum[y + m][x];
+    }
+    if (y != 0 || c >= cols) return;
+    if (w32) static_cast<float*>(dw)[c] = sum[0][x];
+    else put<DT>(dw, c, sum[0][x]);
+}
+
+// Workgroups that are resident together, by the registers of the widest rows.
+constexpr int64_t RN_GROUPS = 1024;
+
+// Calls f(NC, TPR) for rows of `chunks` whole chunks: few threads for short rows, a wave up to 512 chunks; a workgroup
+// for longer rows, and for few rows, whose waves would not fill the chip. False past what registers hold.
+template <class F>
+bool row_shape(int64_t rows, int64_t chunks, int wave_most, F&& f) {
+#define TVK_ROW(nc, tpr) return f(std::integral_constant<int, nc>{}, std::integral_constant<int, tpr>{}), true
+    if (rows > 1024 || chunks <= 64) {
+        if (chunks <= 16) TVK_ROW(1, 16);
+        if (chunks <= 32) TVK_ROW(2, 16);
+        if (chunks <= 64) TVK_ROW(1, 64);
+        if (chunks <= 128) TVK_ROW(2, 64);
+        if (chunks <= 256) TVK_ROW(4, 64);
+        if (chunks <= 512 && wave_most >= 8) TVK_ROW(8, 64);
+    }
+    if (chunks <= 256) TVK_ROW(1, 256);
+    if (chunks <= 512) TVK_ROW(2, 256);
+    if (chunks <= 1024) TVK_ROW(4, 256);
+    if (chunks <= 2048) TVK_ROW(8, 256);
+#undef TVK_ROW
+    return false;
 }
 
 template <int DT>
 void forward(const NormArgs& p, hipStream_t s) {
-    hipLaunchKernelGGL((rms_norm_kernel<DT>), dim3((unsigned)p.rows), dim3(RN_THREADS), 0, s, p);
+    const bool done = row_shape(p.rows, p.cols * (int64_t)dtype_size(DT) / 16, 8, [&](auto nc, auto tpr) {
+        constexpr int NC = decltype(nc)::value, TPR = decltype(tpr)::value, SUBS = RN_THREADS / TPR;
+        const dim3 grid((unsigned)std::min<int64_t>((p.rows + SUBS - 1) / SUBS, RN_GROUPS)), block(RN_THREADS);
+        if (p.out8) hipLaunchKernelGGL((rms_norm_kernel<DT, true, NC, TPR>), grid, block, 0, s, p);
+        else hipLaunchKernelGGL((rms_norm_kernel<DT, false, NC, TPR>), grid, block, 0, s, p);
+    });
+    if (!done) hipLaunchKernelGGL((rms_norm_any_kernel<DT>), dim3((unsigned)p.rows), dim3(RN_THREADS), 0, s, p);
 }
 
 template <int DT>
 tvk_status backward(NormBwdArgs p, void* dw, hipStream_t s) {
     Scratch scratch;
     float* part = nullptr;
-    const int64_t parts = std::max<int64_t>(1, std::min<int64_t>(64, p.rows / 64));
-    if (dw) {
-        p.inv = static_cast<float*>(scratch.get((size_t)(p.rows + parts * p.cols) * 4, s));
-        if (!p.inv) return fail(TVK_ERR_OOM, "tvk_rms_norm_bwd: workspace allocation failed");
-        part = p.inv + p.rows;
+    int64_t parts = 0;
+    auto partials = [&](int64_t n, int64_t more) {   // n partials and `more` floats before them
+        parts = n;
+        if (!dw) return true;
+        part = static_cast<float*>(scratch.get((size_t)(more + parts * p.cols) * 4 + 4, s));
+        return part != nullptr;
+    };
+    bool have = true;
+    const bool done = row_shape(p.rows, p.cols * (int64_t)dtype_size(DT) / 16, 4, [&](auto nc, auto tpr) {
+        constexpr int NC = decltype(nc)::value, TPR = decltype(tpr)::value, SUBS = RN_THREADS / TPR;
+        const int64_t groups = std::min<int64_t>((p.rows + SUBS - 1) / SUBS, RN_GROUPS);
+        have = partials(groups, 0);
+        if (have && p.rows > 0)
+            hipLaunchKernelGGL((rms_norm_bwd_kernel<DT, NC, TPR>), dim3((unsigned)groups), dim3(RN_THREADS), 0, s, p, part);
+    });
+    if (!done) {   // a workgroup a row, dx last: it may lie over dy or h
+        have = partials(std::max<int64_t>(1, std::min<int64_t>(64, p.rows / 64)), p.rows);
+        if (have && dw) {
+            p.inv = part;
+            part += p.rows;
+            if (p.rows > 0) hipLaunchKernelGGL((rms_norm_inv_kernel<DT>), dim3((unsigned)p.rows), dim3(RN_THREADS), 0, s, p);
+            hipLaunchKernelGGL((rms_norm_dweight_kernel<DT>), dim3((unsigned)((p.cols + 63) / 64), (unsigned)parts),
+                               dim3(RN_THREADS), 0, s, p, part);
+        }
+        if (have && p.rows > 0) hipLaunchKernelGGL((rms_norm_bwd_any_kernel<DT>), dim3((unsigned)p.rows), dim3(RN_THREADS), 0, s, p);
     }
-    if (dw) {
-        if (p.rows > 0) hipLaunchKernelGGL((rms_norm_inv_kernel<DT>), dim3((unsigned)p.rows), dim3(RN_THREADS), 0, s, p);
-        hipLaunchKernelGGL((rms_norm_dweight_kernel<DT>), dim3((unsigned)((p.cols + 63) / 64), (unsigned)parts),
-                           dim3(RN_THREADS), 0, s, p, part);
-        hipLaunchKernelGGL((rms_norm_fold_kernel<DT>), dim3((unsigned)((p.cols + RN_THREADS - 1) / RN_THREADS)),
-                           dim3(RN_THREADS), 0, s, part, parts, p.cols, dw, p.w32);
-    }
-    if (p.rows > 0) hipLaunchKernelGGL((rms_norm_bwd_kernel<DT>), dim3((unsigned)p.rows), dim3(RN_THREADS), 0, s, p);
+    if (!have) return fail(TVK_ERR_OOM, "tvk_rms_norm_bwd: workspace allocation failed");
+    if (dw)
+        hipLaunchKernelGGL((rms_norm_fold_kernel<DT>), dim3((unsigned)((p.cols + FOLD_COLS - 1) / FOLD_COLS)),
+                           dim3(FOLD_COLS * FOLD_ROWS), 0, s, part, parts, p.cols, dw, p.w32);
     return TVK_OK;
 }
 
