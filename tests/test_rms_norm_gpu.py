@@ -236,3 +236,51 @@ def test_streams_and_capture(gpu):
         torch.cuda.synchronize()
         assert torch.equal(y.view(torch.uint8), want[0][0].view(torch.uint8)) and torch.equal(scale, want[0][2])
         assert torch.equal(dx, want[1][0]) and torch.equal(dw, want[1][1])
+
+
+# more rows than a launch has workgroups to give one each: a wave, a part of one or several to a row, with rows left over
+@pytest.mark.parametrize("cols", [96, 129, 250, 513, 640, 1023, 1024, 2050, 4099])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_many_rows(gpu, cols, dtype):
+    rows = 2051
+    x, w, r = rand((rows, cols), dtype, cols), rand((cols,), dtype, 1) + 1, rand((rows, cols), dtype, 2, 3.0)
+    check_fwd(x, w, r, what=f"{cols} {dtype}")
+    check_fwd(x, w.float(), out8=True, what=f"{cols} {dtype} 8 bits, float32 weight")
+    check_bwd(r, x, w, rand((rows, cols), dtype, 3), what=f"{cols} {dtype}")
+    check_bwd(r, x, w.float(), what=f"{cols} {dtype} float32 weight")
+
+
+@pytest.mark.parametrize("cols", [200, 1500])
+def test_many_rows_in_place(gpu, cols):
+    # rows inside wider ones at odd offsets, the output over x, dx over dh, inputs shared by all rows
+    rows, dtype = 2051, torch.float16
+    wide = rand((rows, cols + 3), dtype, 1)
+    w, one = rand((cols,), dtype, 2), rand((1, cols), dtype, 3).expand(rows, cols)
+    h, y = oracle(wide[:, 1:1 + cols], w, one, 1e-5)
+    xd, od = wide.to(DEV), one[:1].to(DEV).expand(rows, cols)
+    lib, stream = _abi.load(), torch.cuda.current_stream().cuda_stream
+    wd, hd = w.to(DEV), torch.empty((rows, cols), dtype=dtype, device=DEV)
+    d = _abi.make_rms_norm_desc(xd[:, 1:1 + cols], wd, xd[:, 1:1 + cols], residual=od, residual_out=hd, stream=stream)
+    _abi.check(lib.tvk_rms_norm_fwd(C.byref(d)))
+    f = factor(cols)
+    assert torch.equal(hd.cpu(), h)
+    close(xd[:, 1:1 + cols], y, f * y.abs() + half_step(y, dtype), "over x")
+    assert torch.equal(xd[:, 0].cpu(), wide[:, 0]) and torch.equal(xd[:, 1 + cols:].cpu(), wide[:, 1 + cols:])
+    dh = rand((rows, cols), dtype, 5)
+    dx, dw, size, wsize = oracle_bwd(one, h, w, dh, 1e-5)
+    t, gw = dh.to(DEV), torch.empty_like(wd)
+    d = _abi.make_rms_norm_bwd_desc(od, hd, wd, t, gw, dh=t, stream=stream)
+    _abi.check(lib.tvk_rms_norm_bwd(C.byref(d)))
+    close(t, dx, f * size + half_step(dx, dtype), "dx over dh")
+    close(gw, dw, (f + rows * U) * wsize + half_step(dw, dtype), "dw")
+
+
+@pytest.mark.parametrize("cols", [64, 300, 2048])
+def test_8bit_rows_near_the_ends_of_float32(gpu, cols):
+    # scales beside which one over the other leaves float32: tiny rows without eps, large ones
+    x = rand((3, cols), torch.float32, 1)
+    x[0] *= 2.0 ** -50
+    x[1] *= 2.0 ** 50
+    w = torch.ones(cols) * 2.0 ** -80
+    check_fwd(x, w, eps=0.0, out8=True, what="tiny weights")
+    check_fwd(x, w * 2.0 ** 140, eps=0.0, out8=True, what="large weights")

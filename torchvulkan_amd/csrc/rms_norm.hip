@@ -1,13 +1,12 @@
 // Root-mean-square norm (tvk_rms_norm_fwd, tvk_rms_norm_bwd).
 //
 // Both directions read and write each value once and are bound by that. A row
-// is held in the registers of TPR threads (16, 64 or 256: part of a wave, a
-// wave, a workgroup), NC chunks of 16 bytes each, while its sums are taken: one
+// is held in the registers of TPR threads (part of a wave, a wave, or a workgroup
+// of 256 to 1024), one or two chunks of 16 bytes each, while its sums are taken: one
 // pass forward, for the 8-bit output too (max|h w| and the sum of squares come
 // from the same pass, and scale both), one pass backward for both sums and dx.
-// A workgroup takes rows in turn, so that it loads its weights once and, backward,
-// keeps dweight's sums over its rows in registers; those are added up by a second
-// launch in a fixed order. Rows start at any multiple of a value (16-byte accesses
+// Backward, a workgroup takes rows in turn and keeps dweight's sums over them in
+// registers; those are added up by a second launch in a fixed order. Rows start at any multiple of a value (16-byte accesses
 // need no more); the values past a row's last whole chunk go one to a thread.
 // Rows of more than 2048 chunks are read again for every pass.
 #include "words.h"
@@ -174,14 +173,68 @@ __global__ __launch_bounds__(RN_THREADS) void rms_norm_dweight_kernel(NormBwdArg
 // rows in registers
 // ---------------------------------------------------------------------------
 
-// Sums and maxima over the TPR threads of a row, the same bits in each: pairs of lanes, then the waves in order.
-template <int TPR, class Op>
-__device__ inline float row_all(float v) {
-    if constexpr (TPR == RN_THREADS) return block_all<Op>(v);
-#pragma unroll
-    for (int m = TPR / 2; m > 0; m >>= 1) v = Op::of(v, __shfl_xor(v, m));
-    return v;
+template <int CTRL>
+__device__ __forceinline__ float moved(float v) {   // a lane's value from another lane of its 16
+    const int i = __builtin_bit_cast(int, v);
+    return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(i, i, CTRL, 0xf, 0xf, false));
 }
+
+// Over 16 lanes, then 64: every lane ends with the same bits. Moves between lanes are DPP and lane swaps, a fifth of the
+// latency of the shuffles through LDS.
+template <class Op>
+__device__ __forceinline__ float lanes16_all(float v) {
+    v = Op::of(v, moved<0xB1>(v));    // lane ^ 1
+    v = Op::of(v, moved<0x4E>(v));    // lane ^ 2
+    v = Op::of(v, moved<0x141>(v));   // mirrored in 8
+    return Op::of(v, moved<0x140>(v));   // mirrored in 16
+}
+template <class Op>
+__device__ __forceinline__ float lanes64_all(float v) {
+    v = lanes16_all<Op>(v);
+    uint32_t u = __builtin_bit_cast(uint32_t, v);
+    const auto a = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+    v = Op::of(__builtin_bit_cast(float, (uint32_t)a[0]), __builtin_bit_cast(float, (uint32_t)a[1]));
+    u = __builtin_bit_cast(uint32_t, v);
+    const auto b = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+    return Op::of(__builtin_bit_cast(float, (uint32_t)b[0]), __builtin_bit_cast(float, (uint32_t)b[1]));
+}
+
+// A row's two sums (or a sum and a maximum) over its TPR threads, the same bits in each: lanes, then the waves in order.
+// `turn` alternates from row to row: with two sets of LDS words one barrier a row is enough.
+template <int TPR, class OpA, class OpB>
+__device__ __forceinline__ void row_all(float& a, float& b, int turn) {
+    if constexpr (TPR == 16) {
+        a = lanes16_all<OpA>(a);
+        b = lanes16_all<OpB>(b);
+    } else {
+        a = lanes64_all<OpA>(a);
+        b = lanes64_all<OpB>(b);
+    }
+    if constexpr (TPR > 64) {
+        __shared__ float part[2][2][1024 / 64];
+        const int wave = threadIdx.x / 64, w0 = threadIdx.x / TPR * (TPR / 64);
+        if (threadIdx.x % 64 == 0) {
+            part[turn][0][wave] = a;
+            part[turn][1][wave] = b;
+        }
+        __syncthreads();
+        a = part[turn][0][w0];
+        b = part[turn][1][w0];
+#pragma unroll
+        for (int w = 1; w < TPR / 64; ++w) {
+            a = OpA::of(a, part[turn][0][w0 + w]);
+            b = OpB::of(b, part[turn][1][w0 + w]);
+        }
+    }
+}
+
+// A thread's row among its workgroup's: the wave's where a row takes whole waves, so that addresses are scalar.
+template <int TPR>
+__device__ __forceinline__ int row_of_thread() {
+    return TPR < 64 ? threadIdx.x / TPR : __builtin_amdgcn_readfirstlane(threadIdx.x / TPR);
+}
+
+constexpr int row_threads(int tpr) { return tpr < RN_THREADS ? RN_THREADS : tpr; }
 
 // What a thread holds of a row: chunk i is the row's chunk t + TPR * i; then, in t < tail, one of the values past them.
 template <int DT, int NC, int TPR>
@@ -194,12 +247,11 @@ struct Row {
     __device__ __forceinline__ void load(const void* row, int t, int chunks, int tail) {
         const T* p = static_cast<const T*>(row);
 #pragma unroll
-        for (int i = 0; i < NC; ++i) c[i] = t + TPR * i < chunks ? load_words<16, sizeof(T)>(p + VEC * (t + TPR * i)) : Words<16>{};
-        if (t < tail) last = elem<DT>::to_f32(p[VEC * chunks + t]);
+        for (int i = 0; i < NC; ++i) c[i] = t + TPR * i < chunks ? load_words<16, sizeof(T)>(p + (uint32_t)(VEC * (t + TPR * i))) : Words<16>{};
+        if (t < tail) last = elem<DT>::to_f32(p[(uint32_t)(VEC * chunks + t)]);
     }
     __device__ __forceinline__ float at(int i, int k) const { return word_at<DT>(c[i], k); }
-    // From here on the values are unpacked anew: kept unpacked across the sums, or from row to row, they take twice the
-    // registers and with them the second workgroup on a CU.
+    // From here on the values are unpacked anew: kept unpacked across a row's sums they take twice the registers.
     __device__ __forceinline__ void packed() {
         if constexpr (DT != TVK_F32)
 #pragma unroll
@@ -244,15 +296,15 @@ struct Weights {
 };
 
 template <int DT, bool OUT8, int NC, int TPR>
-__global__ __launch_bounds__(RN_THREADS) void rms_norm_kernel(NormArgs p) {
+__global__ __launch_bounds__(row_threads(TPR)) void rms_norm_kernel(NormArgs p) {
     typedef Row<DT, NC, TPR> R;
     typedef typename R::T T;
-    constexpr int VEC = R::VEC;
+    constexpr int VEC = R::VEC, SUBS = row_threads(TPR) / TPR;
     const int t = threadIdx.x % TPR, chunks = (int)p.cols / VEC, tail = (int)p.cols % VEC;
     Weights<DT, NC, TPR> w;
     w.load(p.w, p.w32, t, chunks, tail);
-    for (int64_t row = (int64_t)blockIdx.x * (RN_THREADS / TPR) + threadIdx.x / TPR; row < p.rows;
-         row += (int64_t)gridDim.x * (RN_THREADS / TPR)) {
+    int turn = 0;
+    for (int64_t row = (int64_t)blockIdx.x * SUBS + row_of_thread<TPR>(); row < p.rows; row += (int64_t)gridDim.x * SUBS) {
         R h, r;
         h.load(static_cast<const T*>(p.x) + row * p.sx, t, chunks, tail);
         if (p.r) {
@@ -266,76 +318,89 @@ __global__ __launch_bounds__(RN_THREADS) void rms_norm_kernel(NormArgs p) {
             }
             h.last = elem<DT>::to_f32(elem<DT>::from_f32(h.last + r.last));
         }
-        w.r.packed();
-        float ss = h.last * h.last, top = fabsf(h.last * w.r.last);
+        // v: the row's values, for the 8-bit output times the weights
+        float ss = h.last * h.last, last = OUT8 ? h.last * w.r.last : h.last, top = fabsf(last), v[NC][VEC];
 #pragma unroll
         for (int i = 0; i < NC; ++i) {
             float f[VEC], part = 0.0f;
             if (OUT8) w.chunk(i, t, chunks, f);
 #pragma unroll
             for (int k = 0; k < VEC; ++k) {
-                const float v = h.at(i, k);
-                part = fmaf(v, v, part);
-                if (OUT8) top = fmaxf(top, fabsf(v * f[k]));
+                v[i][k] = h.at(i, k);
+                part = fmaf(v[i][k], v[i][k], part);
+                if (OUT8) {
+                    v[i][k] *= f[k];
+                    top = fmaxf(top, fabsf(v[i][k]));
+                }
             }
             ss += part;
         }
-        ss = row_all<TPR, SumOp>(ss);
-        h.packed();
-        w.r.packed();
+        if (OUT8) row_all<TPR, SumOp, MaxOp>(ss, top, turn);
+        else row_all<TPR, SumOp, SumOp>(ss, top, turn);
+        turn ^= 1;
         const float inv = 1.0f / sqrtf(ss / (float)p.cols + p.eps);
         if (p.h) {
             T* o = static_cast<T*>(p.h) + row * p.sh;
 #pragma unroll
             for (int i = 0; i < NC; ++i)
-                if (t + TPR * i < chunks) store_words<16, sizeof(T)>(o + VEC * (t + TPR * i), h.c[i]);
+                if (t + TPR * i < chunks) store_words<16, sizeof(T)>(o + (uint32_t)(VEC * (t + TPR * i)), h.c[i]);
             if (t < tail) o[VEC * chunks + t] = elem<DT>::from_f32(h.last);
         }
         if constexpr (OUT8) {
             // y = h w inv; its largest magnitude is max|h w| times inv, and y / scale = h w (inv / scale). An inv / scale
             // that leaves float32's range, for rows of values near its ends, is not taken as one factor.
-            top = row_all<TPR, MaxOp>(top) * inv;
+            top *= inv;
             const float s = top > 0.0f ? top / kF8Max : 1.0f, f8 = inv / s;
             const bool plain = f8 < 1e30f && f8 > 1e-30f;
+            const float a = plain ? f8 : inv, b = plain ? 1.0f : s;
             if (t == 0) p.scale[row] = s;
             uint8_t* o = static_cast<uint8_t*>(p.out) + row * p.so;
-            auto value = [&](float v, float wv) { return plain ? v * wv * f8 : v * wv * inv / s; };
 #pragma unroll
             for (int i = 0; i < NC; ++i) {
                 if (t + TPR * i >= chunks) continue;
-                float f[VEC];
-                w.chunk(i, t, chunks, f);
+#pragma unroll
+                for (int k = 0; k < VEC; ++k) v[i][k] *= a;
+                if (!plain)
+#pragma unroll
+                    for (int k = 0; k < VEC; ++k) v[i][k] /= b;
                 Words<VEC> e;
 #pragma unroll
-                for (int k = 0; k < VEC; k += 4)
-                    e.w[k / 4] = pack4_f8(value(h.at(i, k), f[k]), value(h.at(i, k + 1), f[k + 1]), value(h.at(i, k + 2), f[k + 2]),
-                                          value(h.at(i, k + 3), f[k + 3]));
-                store_words<VEC, 1>(o + VEC * (t + TPR * i), e);
+                for (int k = 0; k < VEC; k += 4) e.w[k / 4] = pack4_f8(v[i][k], v[i][k + 1], v[i][k + 2], v[i][k + 3]);
+                store_words<VEC, 1>(o + (uint32_t)(VEC * (t + TPR * i)), e);
             }
-            if (t < tail) o[VEC * chunks + t] = f32_to_f8(value(h.last, w.r.last), TVK_F8E4M3FN);
+            if (t < tail) o[VEC * chunks + t] = f32_to_f8(last * a / b, TVK_F8E4M3FN);
         } else {
             T* o = static_cast<T*>(p.out) + row * p.so;
 #pragma unroll
             for (int i = 0; i < NC; ++i) {
                 if (t + TPR * i >= chunks) continue;
-                float f[VEC], y[VEC];
+                float f[VEC];
                 w.chunk(i, t, chunks, f);
 #pragma unroll
-                for (int k = 0; k < VEC; ++k) y[k] = h.at(i, k) * inv * f[k];
-                store_words<16, sizeof(T)>(o + VEC * (t + TPR * i), pack<DT, VEC>(y));
+                for (int k = 0; k < VEC; ++k) v[i][k] = v[i][k] * inv * f[k];
+                store_words<16, sizeof(T)>(o + (uint32_t)(VEC * (t + TPR * i)), pack<DT, VEC>(v[i]));
             }
-            if (t < tail) o[VEC * chunks + t] = elem<DT>::from_f32(h.last * inv * w.r.last);
+            if (t < tail) o[VEC * chunks + t] = elem<DT>::from_f32(last * inv * w.r.last);
         }
     }
 }
 
+// Backward, a workgroup keeps dweight's sums over all of its rows: as many workgroups as are resident together (16 waves a
+// CU). Forward takes a row each: loading the next row's weights again costs less than waiting for it (bfloat16
+// 16384 x 4096 to 8 bits: 82 us, 90 with 1024 workgroups that keep their weights).
+constexpr int64_t RN_BWD_THREADS = 1024 * 256;
+
+// Threads of a backward workgroup: two rows of 256 threads at a time halve the partials that are folded
+// (bfloat16 16384 x 4096: 105.7 us, 110.7 with one row), four make the waves wait for each other.
+constexpr int bwd_threads(int tpr) { return tpr < 512 ? 512 : tpr; }
+
 // part: [gridDim.x][cols], the workgroups' sums of dy * n over their rows; NULL: not wanted.
-template <int DT, int NC, int TPR>
-__global__ __launch_bounds__(RN_THREADS) void rms_norm_bwd_kernel(NormBwdArgs p, float* part) {
+template <int DT, int NC, int TPR, int THREADS>
+__global__ __launch_bounds__(THREADS) void rms_norm_bwd_kernel(NormBwdArgs p, float* part) {
     typedef Row<DT, NC, TPR> R;
     typedef typename R::T T;
-    constexpr int VEC = R::VEC, SUBS = RN_THREADS / TPR;
-    const int t = threadIdx.x % TPR, sub = threadIdx.x / TPR, chunks = (int)p.cols / VEC, tail = (int)p.cols % VEC;
+    constexpr int VEC = R::VEC, SUBS = THREADS / TPR;
+    const int t = threadIdx.x % TPR, sub = row_of_thread<TPR>(), chunks = (int)p.cols / VEC, tail = (int)p.cols % VEC;
     Weights<DT, NC, TPR> w;
     w.load(p.w, p.w32, t, chunks, tail);
     float acc[NC][VEC], acc_last = 0.0f;
@@ -343,52 +408,64 @@ __global__ __launch_bounds__(RN_THREADS) void rms_norm_bwd_kernel(NormBwdArgs p,
     for (int i = 0; i < NC; ++i)
 #pragma unroll
         for (int k = 0; k < VEC; ++k) acc[i][k] = 0.0f;
-    for (int64_t row = (int64_t)blockIdx.x * SUBS + sub; row < p.rows; row += (int64_t)gridDim.x * SUBS) {
-        R dy, h, dh;
+    int64_t row = (int64_t)blockIdx.x * SUBS + sub;
+    const int64_t step = (int64_t)gridDim.x * SUBS;
+    int turn = 0;
+    R dy, h, dh;   // of the next row, on their way while one is computed
+    auto load = [&]() {
         dy.load(static_cast<const T*>(p.dy) + row * p.sdy, t, chunks, tail);
         h.load(static_cast<const T*>(p.h) + row * p.sh, t, chunks, tail);
         if (p.dh) dh.load(static_cast<const T*>(p.dh) + row * p.sdh, t, chunks, tail);
-        w.r.packed();
-        float ss = h.last * h.last, gh = dy.last * w.r.last * h.last;
+    };
+    if (row < p.rows) load();
+    // a workgroup's rows keep step: their sums meet at barriers
+    for (int64_t first = (int64_t)blockIdx.x * SUBS; first < p.rows; first += step) {
+        R g = dy, x = h, add = dh;
+        const bool live = row < p.rows;
+        T* dx = static_cast<T*>(p.dx) + row * p.sdx;
+        row += step;
+        if (row < p.rows) load();
+        float ss = x.last * x.last, gh = g.last * w.r.last * x.last;
 #pragma unroll
         for (int i = 0; i < NC; ++i) {
             float f[VEC], ps = 0.0f, pg = 0.0f;
             w.chunk(i, t, chunks, f);
 #pragma unroll
             for (int k = 0; k < VEC; ++k) {
-                const float v = h.at(i, k);
+                const float v = x.at(i, k);
                 ps = fmaf(v, v, ps);
-                pg = fmaf(dy.at(i, k) * f[k], v, pg);
+                pg = fmaf(g.at(i, k) * f[k], v, pg);
             }
             ss += ps;
             gh += pg;
         }
-        ss = row_all<TPR, SumOp>(ss);
-        gh = row_all<TPR, SumOp>(gh);
-        dy.packed();
-        h.packed();
+        row_all<TPR, SumOp, SumOp>(ss, gh, turn);
+        turn ^= 1;
+        if (!live) continue;
+        g.packed();
+        x.packed();
+        add.packed();
         w.r.packed();
         const float inv = 1.0f / sqrtf(ss / (float)p.cols + p.eps);
         const float mean = gh * inv / (float)p.cols;   // of g * n
-        T* dx = static_cast<T*>(p.dx) + row * p.sdx;
 #pragma unroll
         for (int i = 0; i < NC; ++i) {
             float f[VEC], o[VEC];
             w.chunk(i, t, chunks, f);
 #pragma unroll
             for (int k = 0; k < VEC; ++k) {
-                const float n = h.at(i, k) * inv, g = dy.at(i, k);
-                acc[i][k] = fmaf(g, n, acc[i][k]);
-                o[k] = inv * (g * f[k] - n * mean);
-                if (p.dh) o[k] += dh.at(i, k);
+                const float n = x.at(i, k) * inv, d = g.at(i, k);
+                acc[i][k] = fmaf(d, n, acc[i][k]);
+                o[k] = inv * (d * f[k] - n * mean);
+                if (p.dh) o[k] += add.at(i, k);
             }
-            if (t + TPR * i < chunks) store_words<16, sizeof(T)>(dx + VEC * (t + TPR * i), pack<DT, VEC>(o));
+            if (t + TPR * i < chunks) store_words<16, sizeof(T)>(dx + (uint32_t)(VEC * (t + TPR * i)), pack<DT, VEC>(o));
         }
         if (t < tail) {
-            const float n = h.last * inv;
-            acc_last = fmaf(dy.last, n, acc_last);
-            float o = inv * (dy.last * w.r.last - n * mean);
-            if (p.dh) o += dh.last;
+            const float n = x.last * inv;
+            acc_last = fmaf(g.last, n, acc_last);
+            float o = inv * (g.last * w.r.last - n * mean);
+            if (p.dh) o += add.last;
             dx[VEC * chunks + t] = elem<DT>::from_f32(o);
         }
     }
@@ -402,25 +479,20 @@ __global__ __launch_bounds__(RN_THREADS) void rms_norm_bwd_kernel(NormBwdArgs p,
                 for (int k = 0; k < VEC; ++k) out[VEC * (t + TPR * i) + k] = acc[i][k];
         if (t < tail) out[VEC * chunks + t] = acc_last;
     } else {
-        __shared__ float sum[VEC * (NC * TPR + 1)];   // the workgroup's rows added in order
-        for (int s = 0; s < SUBS; ++s) {
-            if (sub == s) {
+        __shared__ float sum[SUBS][VEC * (NC * TPR + 1)];
 #pragma unroll
-                for (int i = 0; i < NC; ++i)
-                    if (t + TPR * i < chunks)
+        for (int i = 0; i < NC; ++i)
+            if (t + TPR * i < chunks)
 #pragma unroll
-                        for (int k = 0; k < VEC; ++k) {
-                            float& x = sum[VEC * (t + TPR * i) + k];
-                            x = s ? x + acc[i][k] : acc[i][k];
-                        }
-                if (t < tail) {
-                    float& x = sum[VEC * chunks + t];
-                    x = s ? x + acc_last : acc_last;
-                }
-            }
-            __syncthreads();
+                for (int k = 0; k < VEC; ++k) sum[sub][VEC * (t + TPR * i) + k] = acc[i][k];
+        if (t < tail) sum[sub][VEC * chunks + t] = acc_last;
+        __syncthreads();
+        for (int c = threadIdx.x; c < (int)p.cols; c += THREADS) {
+            float v = sum[0][c];
+#pragma unroll
+            for (int i = 1; i < SUBS; ++i) v += sum[i][c];
+            out[c] = v;
         }
-        for (int c = threadIdx.x; c < (int)p.cols; c += RN_THREADS) out[c] = sum[c];
     }
 }
 
@@ -435,15 +507,13 @@ __global__ __launch_bounds__(FOLD_COLS * FOLD_ROWS) void rms_norm_fold_kernel(co
     const int64_t c = (int64_t)blockIdx.x * FOLD_COLS + x;
     float s = 0.0f;
     if (c < cols) {
-        int64_t i = y;
-        for (; i + 7 * FOLD_ROWS < parts; i += 8 * FOLD_ROWS) {
+        for (int64_t i = y; i < parts; i += 8 * FOLD_ROWS) {   // eight loads on their way together
             float v[8];
 #pragma unroll
-            for (int u = 0; u < 8; ++u) v[u] = part[(i + u * FOLD_ROWS) * cols + c];
+            for (int u = 0; u < 8; ++u) v[u] = part[min(i + u * FOLD_ROWS, parts - 1) * cols + c];
 #pragma unroll
-            for (int u = 0; u < 8; ++u) s += v[u];
+            for (int u = 0; u < 8; ++u) s += i + u * FOLD_ROWS < parts ? v[u] : 0.0f;
         }
-        for (; i < parts; i += FOLD_ROWS) s += part[i * cols + c];
     }
     sum[y][x] = s;
 #pragma unroll
@@ -456,35 +526,30 @@ __global__ __launch_bounds__(FOLD_COLS * FOLD_ROWS) void rms_norm_fold_kernel(co
     else put<DT>(dw, c, sum[0][x]);
 }
 
-// Workgroups that are resident together, by the registers of the widest rows.
-constexpr int64_t RN_GROUPS = 1024;
-
-// Calls f(NC, TPR) for rows of `chunks` whole chunks: few threads for short rows, a wave up to 512 chunks; a workgroup
-// for longer rows, and for few rows, whose waves would not fill the chip. False past what registers hold.
+// Calls f(NC, TPR) for rows of `chunks` whole chunks; false past what registers hold. At most two chunks a thread: more
+// take the registers of the waves that hide the row's latency (bfloat16 16384 x 4096 to 8 bits: 82 us with two chunks in
+// 256 threads, 197 with eight in a wave). A wave with two chunks beats four waves with half of one each where rows are many
+// (float16 2000 x 1024: 4.5 us, 5.4), and loses where they are few.
 template <class F>
-bool row_shape(int64_t rows, int64_t chunks, int wave_most, F&& f) {
+bool row_shape(int64_t rows, int64_t chunks, F&& f) {
 #define TVK_ROW(nc, tpr) return f(std::integral_constant<int, nc>{}, std::integral_constant<int, tpr>{}), true
-    if (rows > 1024 || chunks <= 64) {
-        if (chunks <= 16) TVK_ROW(1, 16);
-        if (chunks <= 32) TVK_ROW(2, 16);
-        if (chunks <= 64) TVK_ROW(1, 64);
-        if (chunks <= 128) TVK_ROW(2, 64);
-        if (chunks <= 256) TVK_ROW(4, 64);
-        if (chunks <= 512 && wave_most >= 8) TVK_ROW(8, 64);
-    }
+    if (chunks <= 16) TVK_ROW(1, 16);
+    if (chunks <= 32) TVK_ROW(2, 16);
+    if (chunks <= 64) TVK_ROW(1, 64);
+    if (chunks <= 128 && rows > 1024) TVK_ROW(2, 64);
     if (chunks <= 256) TVK_ROW(1, 256);
     if (chunks <= 512) TVK_ROW(2, 256);
-    if (chunks <= 1024) TVK_ROW(4, 256);
-    if (chunks <= 2048) TVK_ROW(8, 256);
+    if (chunks <= 1024) TVK_ROW(2, 512);
+    if (chunks <= 2048) TVK_ROW(2, 1024);
 #undef TVK_ROW
     return false;
 }
 
 template <int DT>
 void forward(const NormArgs& p, hipStream_t s) {
-    const bool done = row_shape(p.rows, p.cols * (int64_t)dtype_size(DT) / 16, 8, [&](auto nc, auto tpr) {
-        constexpr int NC = decltype(nc)::value, TPR = decltype(tpr)::value, SUBS = RN_THREADS / TPR;
-        const dim3 grid((unsigned)std::min<int64_t>((p.rows + SUBS - 1) / SUBS, RN_GROUPS)), block(RN_THREADS);
+    const bool done = row_shape(p.rows, p.cols * (int64_t)dtype_size(DT) / 16, [&](auto nc, auto tpr) {
+        constexpr int NC = decltype(nc)::value, TPR = decltype(tpr)::value, SUBS = row_threads(TPR) / TPR;
+        const dim3 grid((unsigned)std::min<int64_t>((p.rows + SUBS - 1) / SUBS, 1 << 20)), block(row_threads(TPR));
         if (p.out8) hipLaunchKernelGGL((rms_norm_kernel<DT, true, NC, TPR>), grid, block, 0, s, p);
         else hipLaunchKernelGGL((rms_norm_kernel<DT, false, NC, TPR>), grid, block, 0, s, p);
     });
@@ -503,12 +568,12 @@ tvk_status backward(NormBwdArgs p, void* dw, hipStream_t s) {
         return part != nullptr;
     };
     bool have = true;
-    const bool done = row_shape(p.rows, p.cols * (int64_t)dtype_size(DT) / 16, 4, [&](auto nc, auto tpr) {
-        constexpr int NC = decltype(nc)::value, TPR = decltype(tpr)::value, SUBS = RN_THREADS / TPR;
-        const int64_t groups = std::min<int64_t>((p.rows + SUBS - 1) / SUBS, RN_GROUPS);
+    const bool done = row_shape(p.rows, p.cols * (int64_t)dtype_size(DT) / 16, [&](auto nc, auto tpr) {
+        constexpr int NC = decltype(nc)::value, TPR = decltype(tpr)::value, THREADS = bwd_threads(TPR), SUBS = THREADS / TPR;
+        const int64_t groups = std::min<int64_t>((p.rows + SUBS - 1) / SUBS, RN_BWD_THREADS / THREADS);
         have = partials(groups, 0);
         if (have && p.rows > 0)
-            hipLaunchKernelGGL((rms_norm_bwd_kernel<DT, NC, TPR>), dim3((unsigned)groups), dim3(RN_THREADS), 0, s, p, part);
+            hipLaunchKernelGGL((rms_norm_bwd_kernel<DT, NC, TPR, THREADS>), dim3((unsigned)groups), dim3(THREADS), 0, s, p, part);
     });
     if (!done) {   // a workgroup a row, dx last: it may lie over dy or h
         have = partials(std::max<int64_t>(1, std::min<int64_t>(64, p.rows / 64)), p.rows);
