@@ -555,11 +555,12 @@ tvk_status tvk_paged_append(const tvk_paged_append_desc* desc);
  * max_len: a bound on seq_lens the host knows (it sizes the launch: how the
  * keys are split over workgroups), longer sequences are cut to it; 0: the
  * table's reach. Slots past a sequence's length are never read into a result.
- * dtype F32, F16 or BF16, head_dim up to 512. float16/bfloat16 queries with
- * head_dim a multiple of 16 up to 256, 16-byte aligned rows and caches below
- * 64 GiB run the MFMA kernel, other cases a general one. Partial sums of split
- * keys use library scratch and are joined in split order (the same bits every
- * run), in the same launch, or by a second one under graph capture. */
+ * dtype F32, F16 or BF16, head_dim up to 512. Head dims in 16s up to 256 with
+ * 16-byte aligned rows, caches below 64 GiB and any cache type but F8E4M3FN
+ * beside F32 run the MFMA kernel, other cases a general one. Table entries past a
+ * sequence's pages may be read, and what they name, but not into a result. Partial
+ * sums of split keys use library scratch and are joined in an order that depends
+ * on sizes and lengths alone (the same bits every run). */
 typedef struct {
     tvk_paged_cache cache;
     int32_t dtype, reserved;

@@ -496,3 +496,71 @@ def test_append_in_place_and_strides(gpu, dim, offset):
             close(args[0].cpu()[at], y, 2.0 ** -8 * y.abs() + 4 * U * size + TINY[BF16], "k")
             assert torch.equal(args[1].cpu()[at], v[b, t])
     assert torch.equal(dk.cpu(), k) and torch.equal(dv.cpu(), v)
+
+
+# ---------------------------------------------------------------------------
+# attention: masked places, how work is dealt
+# ---------------------------------------------------------------------------
+
+@pytest.mark.parametrize("dim", [32, 64, 80, 128, 256, 40])
+@pytest.mark.parametrize("dtype,cache_dtype", [(HALF, HALF), (BF16, BF16), (torch.float32, torch.float32), (BF16, F8)])
+def test_masked_places(gpu, dim, dtype, cache_dtype):
+    # keys and values that are no numbers where only some of the new tokens see them: the others' rows stay finite
+    for lens, window in (([40, 90, 64, 3], 0), ([300, 33, 128, 700], 30), ([4000, 2], 0)):
+        cache = Cache(lens, 16, 2, dim, cache_dtype, seed=dim)
+        for b, n in enumerate(lens):
+            at = lambda p: (cache.table[b, p // 16], p % 16)   # noqa: E731
+            cache.v[at(n - 1)][0, 1] = float("nan")
+            cache.k[at(n - 2)][1, 0] = float("nan")
+            if cache_dtype != F8:
+                cache.v[at(n - 1)][1, 3] = float("inf")
+                cache.v[at(n - 2)][1, 3] = float("-inf")
+                cache.v[at(n - 1)][1, 5] = float("-inf")
+            if window and n > window + 4:
+                cache.v[at(n - window - 2)][:, 2] = float("nan")   # left behind by the later tokens' windows
+        q = rand((len(lens), 4, 12, dim), dtype, 1)
+        want, _, tol = attention_oracle(q, cache, dim ** -0.5, window)
+        args, scales = cache.dev()
+        got, _ = _abi.paged_attention(q.to(DEV), *args, window=window, **scales)
+        close(got, want, tol, f"D {dim} {dtype} {cache_dtype} window {window}")
+        inf = want.isinf()
+        assert torch.equal(got.double().cpu()[inf], want[inf])
+        assert got[0, 0].isfinite().all() or window   # its token sees none of them
+
+
+@pytest.mark.parametrize("lens,hq,hkv,new,dim", [
+    ([700 - 9 * i for i in range(70)], 8, 8, 1, 64),                # more segments than run together, whole
+    ([1500 - 20 * i for i in range(70)], 8, 4, 1, 64),              # many, in chunks
+    ([3000 + i for i in range(40)], 8, 8, 1, 32),                   # many, in stretches
+    ([40, 0, 61, 1] * 40, 8, 8, 1, 128), ([128, 100] * 65, 16, 8, 2, 64),   # a wave each
+    ([30000] + [5] * 31, 8, 2, 1, 128),                             # one sequence has nearly all the keys
+    ([30000] + [5] * 31, 8, 2, 4, 64),
+    ([9000, 20], 8, 1, 4, 128), ([5000], 16, 1, 3, 80),             # joined by a second launch
+])
+@pytest.mark.parametrize("page", [16, 20])
+def test_dealing(gpu, lens, hq, hkv, new, dim, page):
+    cache = Cache(lens, page, hkv, dim, BF16, seed=len(lens), stale=float("nan"))
+    q = rand((len(lens), new, hq, dim), BF16, 3)
+    args, _ = cache.dev()
+    for max_len in (0, max(lens)):
+        got = check_attention(cache, q, max_len=max_len, what=f"{len(lens)} sequences, max_len {max_len}")
+        # a captured call joins in a launch of its own, with the same bits
+        qd, out = q.to(DEV), torch.empty_like(got)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=torch.cuda.Stream()):
+            d = _abi.make_paged_attention_desc(qd, args[0], args[1], out, args[2], args[3], max_len=max_len,
+                                               stream=torch.cuda.current_stream().cuda_stream)
+            _abi.check(_abi.load().tvk_paged_attention(C.byref(d)))
+        for _ in range(3):
+            out.fill_(float("nan"))
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(out, got)
+
+
+def test_prompt_chunk(gpu):
+    # tokens of a prompt after a cached prefix: many row blocks, each up to its own last key
+    cache = Cache([400, 130, 300], 16, 2, 64, BF16, seed=3, stale=float("nan"))
+    q = rand((3, 200, 8, 64), BF16, 2)
+    check_attention(cache, q, what="prompt")
+    check_attention(cache, q, window=50, what="prompt with a window")

@@ -44,7 +44,8 @@ PagedCache paged_cache(const tvk_paged_cache& c);
 
 // Positions of sequence b: never below zero nor past its table row.
 __device__ inline int paged_len(const PagedCache& c, int b) {
-    const int n = c.lens[b];
+    // not written while a kernel reads it: a scalar load where b is a wave's
+    const int n = ((const __attribute__((address_space(4))) int32_t*)(uintptr_t)c.lens)[b];
     return n < 0 ? 0 : (uint32_t)n > c.reach ? (int)c.reach : n;
 }
 

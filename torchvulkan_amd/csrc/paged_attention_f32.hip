@@ -9,7 +9,7 @@ void paged_attn_f32(PagedMfmaArgs& p, int64_t batch, hipStream_t s) { paged_disp
 bool paged_attn_mfma(const PagedAttnArgs& a, int dtype, bool f8, int64_t batch, hipStream_t s) {
     const PagedCache& c = a.c;
     const bool f32 = dtype == TVK_F32;
-    if (c.hd % 16 != 0 || c.hd > 256 || (f32 && f8) || c.pages == 0) return false;
+    if (c.hd % 16 != 0 || c.hd > 256 || (f32 && f8) || c.pages == 0 || c.reach == 0) return false;
     const int64_t es = f8 ? 1 : f32 ? 4 : 2, qes = f32 ? 4 : 2;
     // strides of a dimension of one entry do not matter
     auto even = [](const void* p, const int64_t* st, std::initializer_list<int64_t> sizes, int64_t es, int64_t by) {
@@ -31,10 +31,9 @@ bool paged_attn_mfma(const PagedAttnArgs& a, int dtype, bool f8, int64_t batch, 
     }
     PagedMfmaArgs p{};
     p.a = a;
-    p.out_vec = even(a.out, a.so, rows, qes, 4 * qes);
     const int64_t nr = (int64_t)a.new_tokens * a.group;
     // every sum of tiles, pieces and segments below 2^31
-    const double tiles = (a.max_len + 31) / 32 + 1.0;
+    const double tiles = (a.max_len + 15.0) / 16 + 1.0;
     if (nr > 0x7fffffff || (double)batch * ((nr + 15) / 16) * c.kvh * tiles >= 0x1p31) return false;
     p.rows = (int)nr;
     if (f32) paged_attn_f32(p, batch, s);

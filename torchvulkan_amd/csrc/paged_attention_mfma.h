@@ -18,19 +18,25 @@
 //      the product for value e is column EV * m + e of the output. float32
 //      values and probabilities are operands of the 16x16x4 product as they are.
 //
-// Work is dealt to a fixed number of workgroups by every workgroup itself, from
-// the lengths on the device: a batch's lengths are not on the host, and a launch
-// sized by the longest would leave the others' workgroups idle. A segment is a
-// row block of a sequence and a key/value head. Where every segment can be cut
-// into chunks of at least 4 (8, 16) tiles without exceeding the workgroups, each
-// takes one chunk; else all tiles of the call, in segment order, are cut into
-// equal stretches, and a workgroup's stretch may end one segment and begin
-// others. Its 4 waves take a stretch's tiles in turn and are merged through LDS
-// in wave order. A segment that lies in one workgroup is written out; the pieces
-// of another go to scratch as float32 (max, sum, O), written through to memory
-// as the skinny GEMM's split_fixup does, and the last workgroup to finish merges
-// them in order; without counters for the stream a second launch does. Both
-// give the same bits every run.
+// Work is dealt by every workgroup itself, from the lengths on the device: a
+// batch's lengths are not on the host, and a launch sized by the longest would
+// leave the others' workgroups idle. A segment is a row block of a sequence and a
+// key/value head. Short ones take a wave or a workgroup each, as max_len tells the
+// host. Else segments are cut into chunks of at least 4 (8, 16) tiles where those
+// do not exceed the workgroups that run together; where they do, all tiles of the
+// call, in segment order, are cut into equal stretches, and a workgroup's stretch
+// may end one segment and begin others. Its 4 waves take a stretch's tiles in turn
+// and are merged through LDS in wave order. A segment that lies in one workgroup is
+// written out; the pieces of another go to scratch as float32 (max, sum, O), written
+// through to memory as the skinny GEMM's split_fixup does. They are joined in runs,
+// and the runs' results in order, by the last workgroup to finish; where that is
+// more than one workgroup reads in a few microseconds, by the last of each run and
+// then the last of all, or by a second launch, which a stream without counters takes
+// too. All give the same bits every run.
+//
+// Measured: one sequence of 100001 keys (32/8 heads of 128, bfloat16) 81 us, 5.0
+// TB/s; 32 of up to 8000 keys 110 us, 4.9 TB/s; 24 of up to 6001 in 8 bits with 4
+// tokens each 52 us, 3.4 TB/s, where stretches that cross segments end late.
 #pragma once
 
 #include "attention_kernels.h"
@@ -40,32 +46,41 @@ namespace tvk {
 
 struct PagedMfmaArgs {
     PagedAttnArgs a;
+    uint32_t kp, ks, vp, vs;   // page and slot strides of keys and values, in 16 bytes
     int rows;              // new_tokens * group
-    int nrb;               // row blocks of a key/value head
-    int items;             // batch * nrb
+    int items;             // batch * row blocks of a key/value head
     int wgs;               // workgroups the tiles are dealt to; 0: one a segment
-    int out_vec;           // output rows take vector stores
+    int resident;          // workgroups that run together
+    int many;              // segments enough to fill the chip: chunks only
+    Div32 nrb, kvh, group;
     float* part_o;         // [2 * wgs][16 * CT][hd]
-    float* part_ml;        // [2 * wgs][16 * CT][2]: max, sum
+    float* part_ml;        // [2][2 * wgs][16 * CT][2]: max, sum; again where a run's result is kept
     unsigned part_bytes;   // of both
-    unsigned* count;       // a segment's finished pieces, zero before and after the launch; NULL: a second launch merges
+    // finished pieces (or runs) of every segment, then finished pieces of the run that begins in every slot; zero before
+    // and after the launch. NULL: a second launch joins, one of `slices` workgroups some of a segment's rows, and
+    // `seg` [items * kvh][2] tells it a segment's first workgroup and its pieces
+    unsigned* count;
+    uint32_t* seg;
+    int slices;
 };
 
 namespace {
 
 constexpr int PM_WAVES = 4;
-constexpr int PM_BN = 32;   // keys per tile
 
 template <int DT, bool F8, int D>
 struct PagedTile {
+    static constexpr int NB = DT == TVK_F32 ? 1 : 2;            // blocks of 16 keys in a tile
+    static constexpr int BN = 16 * NB;
     static constexpr int ES = F8 ? 1 : DT == TVK_F32 ? 4 : 2;   // bytes of a cached value
     static constexpr int KL = (D * ES + 63) / 64;               // 16-byte K chunks a lane holds of a row
     static constexpr int QS = F8 ? 2 * KL : KL;                 // Q fragments of 16 bytes
     static constexpr int EV = D == 96 ? 8 : D / 16;             // V values a lane holds of a row
     static constexpr int DV = 16 * EV;
     static constexpr int VW = EV * ES / 4;                      // the same in 32-bit words
-    // workgroups a CU by the registers: K and V tiles, Q and O, and some 100 more
-    static constexpr int regs(int ct) { return 8 * KL + 8 * VW + ct * (4 * QS + 4 * EV + 8) + 100; }
+    // Workgroups a CU by the registers: K and V tiles, Q, O and S, and 90 beside them. Three of bfloat16 and 128 columns
+    // would fit their loop, but 12 waves with a tile each on its way read slower than 8 (32 x 8000 keys: 124 us, 112).
+    static constexpr int regs(int ct) { return 4 * NB * (KL + VW) + ct * (4 * QS + 4 * EV + 4 * NB) + 90; }
     static constexpr int occ(int ct) { return regs(ct) <= 128 ? 4 : regs(ct) <= 168 ? 3 : regs(ct) <= 256 ? 2 : 1; }
 };
 
@@ -80,79 +95,95 @@ struct PagedSpan {
     int tiles;    // at least one: a segment without keys writes its zeros
 };
 
-template <int CT>
+// Keys below it are seen by token t of a sequence; of those, the ones from window_lo on.
+__device__ __forceinline__ int window_lo(int hi, uint32_t window) { return window && hi > (int)window ? hi - (int)window : 0; }
+
+template <int BN, int CT>
 __device__ __forceinline__ PagedSpan paged_span(const PagedMfmaArgs& p, int e) {
     PagedSpan s;
-    s.b = e / p.nrb;
-    const int r0 = (e - s.b * p.nrb) * 16 * CT, r1 = min(p.rows, r0 + 16 * CT) - 1;
+    s.b = (int)div32((uint32_t)e, p.nrb);
+    const int r0 = (e - s.b * (int)p.nrb.d) * 16 * CT, r1 = min(p.rows, r0 + 16 * CT) - 1;
     s.len = (int)min((uint32_t)paged_len(p.a.c, s.b), p.a.max_len);
-    s.t0 = r0 / p.a.group;
-    s.t1 = r1 / p.a.group;
+    s.t0 = (int)div32((uint32_t)r0, p.group);
+    s.t1 = (int)div32((uint32_t)r1, p.group);
     s.hi = max(0, s.len - p.a.new_tokens + s.t1 + 1);
-    const int64_t first = (int64_t)s.len - p.a.new_tokens + s.t0 + 1 - (int64_t)p.a.window;
-    s.lo = p.a.window ? (int)min((int64_t)s.hi, max((int64_t)0, first)) : 0;
-    s.tiles = s.hi > s.lo ? (s.hi + PM_BN - 1) / PM_BN - s.lo / PM_BN : 1;
+    s.lo = min(s.hi, window_lo(s.len - p.a.new_tokens + s.t0 + 1, p.a.window));
+    s.tiles = s.hi > s.lo ? (s.hi + BN - 1) / BN - s.lo / BN : 1;
     return s;
 }
 
-struct PagedDeal {
-    uint32_t chunk;   // tiles a segment's chunks have at least; 0: stretches
-    uint32_t per;     // tiles a workgroup's stretch has
-    uint32_t total;   // tiles of the call
-    __device__ uint32_t units(uint32_t tiles) const { return chunk ? max(1u, tiles / chunk) : tiles; }
-};
-
-__device__ __forceinline__ uint32_t wave_sum(uint32_t v) {
-#pragma unroll
-    for (int m = 32; m > 0; m >>= 1) v += __shfl_xor(v, m);
-    return __builtin_amdgcn_readfirstlane(v);
+// n / d for a quotient below 2^22: a float estimate that is at most one off.
+__device__ __forceinline__ uint32_t small_div(uint32_t n, uint32_t d) {
+    uint32_t q = (uint32_t)((float)n * __builtin_amdgcn_rcpf((float)d));
+    const int r = (int)(n - q * d);
+    if (r < 0) --q;
+    else if (r >= (int)d) ++q;
+    return q;
 }
 
-// Sums stay below 2^31 (paged_attn_mfma).
-template <int CT>
-__device__ __forceinline__ PagedDeal paged_deal(const PagedMfmaArgs& p, int lane) {
-    PagedDeal d{0x7fffffff, 0, 0};
-    if (!p.wgs) return d;
-    uint32_t n = 0, n4 = 0, n8 = 0, n16 = 0;
-    for (int e = lane; e < p.items; e += 64) {
-        const uint32_t t = (uint32_t)paged_span<CT>(p, e).tiles;
-        n += t;
-        n4 += max(1u, t / 4);
-        n8 += max(1u, t / 8);
-        n16 += max(1u, t / 16);
+struct PagedDeal {
+    int shift;        // segments are cut into chunks of at least 2^shift tiles; -1: stretches
+    uint32_t per;     // tiles a workgroup's stretch has
+    uint32_t snap;    // an end of a stretch this near to a segment's moves there: a short piece costs more than its tiles
+    uint32_t total;   // tiles of the call
+    __device__ __forceinline__ uint32_t units(uint32_t tiles) const { return shift >= 0 ? max(1u, tiles >> shift) : tiles; }
+};
+
+// v + the lane's value from lanes below it by a DPP move (0 where there is none), in the rows of 16 lanes that MASK names.
+template <int CTRL, int MASK>
+__device__ __forceinline__ uint32_t plus_moved(uint32_t v) {
+    return v + (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, MASK, 0xf, false);
+}
+// Inclusive sums over a wave's lanes.
+__device__ __forceinline__ uint32_t wave_scan(uint32_t v) {
+    v = plus_moved<0x111, 0xf>(v);   // row_shr 1, 2, 4, 8
+    v = plus_moved<0x112, 0xf>(v);
+    v = plus_moved<0x114, 0xf>(v);
+    v = plus_moved<0x118, 0xf>(v);
+    v = plus_moved<0x142, 0xa>(v);   // row_bcast 15 into rows 1 and 3
+    return plus_moved<0x143, 0xc>(v);   // row_bcast 31 into rows 2 and 3
+}
+__device__ __forceinline__ uint32_t wave_sum(uint32_t v) { return (uint32_t)__builtin_amdgcn_readlane((int)wave_scan(v), 63); }
+
+// Sums stay below 2^31 (paged_attn_mfma). mine: the tiles of item `lane`.
+template <int BN, int CT>
+__device__ __forceinline__ PagedDeal paged_deal(const PagedMfmaArgs& p, int lane, uint32_t mine) {
+    PagedDeal d;
+    uint32_t n = mine;
+    for (int e = lane + 64; e < p.items; e += 64) n += (uint32_t)paged_span<BN, CT>(p, e).tiles;
+    d.total = wave_sum(n) * p.kvh.d;
+    const uint32_t resident = (uint32_t)min(p.wgs, p.resident);
+    // at least total / resident: the float product is off by less than one in 2^22
+    d.per = (uint32_t)((float)d.total * __builtin_amdgcn_rcpf((float)resident) * 1.000001f) + 1;
+    d.snap = min(128u / BN, d.per / 4);
+    // Many segments and short stretches: a piece's start and end would cost more than its tiles (float32 20 x 16/16 heads x
+    // 1442 keys of 64: 44 us in chunks, 56 in stretches). At most a chunk a segment and two for each of the resident
+    // workgroups: they fit the launch.
+    if (p.many && d.per < 1536 / BN) {
+        d.shift = BN == 32 ? 3 : 4;
+        while ((uint64_t)p.resident << (d.shift + 1) < d.total) ++d.shift;
+        return d;
     }
-    const uint32_t most = (uint32_t)p.wgs / (uint32_t)p.a.c.kvh;
-    n4 = wave_sum(n4);
-    n8 = wave_sum(n8);
-    n16 = wave_sum(n16);
-    d.total = wave_sum(n) * (uint32_t)p.a.c.kvh;
-    d.chunk = n4 <= most ? 4 : n8 <= most ? 8 : n16 <= most ? 16 : 0;
-    d.per = (d.total + (uint32_t)p.wgs - 1) / (uint32_t)p.wgs;
+    if (!p.many) {
+#pragma unroll 1
+        for (d.shift = 2; d.shift <= 4; ++d.shift) {
+            uint32_t u = mine ? d.units(mine) : 0;
+            for (int e = lane + 64; e < p.items; e += 64) u += d.units((uint32_t)paged_span<BN, CT>(p, e).tiles);
+            if (wave_sum(u) * p.kvh.d <= (uint32_t)p.wgs) return d;
+        }
+    }
+    d.shift = -1;
     return d;
 }
 
-// Units of the items before `stop` (all of a wave's lanes take part).
-template <int CT>
-__device__ __forceinline__ uint32_t paged_before(const PagedMfmaArgs& p, const PagedDeal& d, int stop, int lane) {
-    uint32_t n = 0;
-    for (int e = lane; e < stop; e += 64) n += d.units((uint32_t)paged_span<CT>(p, e).tiles);
-    return wave_sum(n);
-}
-
 // The item that holds unit x of the call, and the unit's place among the item's; false past the last.
-template <int CT>
-__device__ __forceinline__ bool paged_locate(const PagedMfmaArgs& p, const PagedDeal& d, uint32_t x, int lane, int& item, uint32_t& at) {
+template <int BN, int CT>
+__device__ __forceinline__ bool paged_locate(const PagedMfmaArgs& p, const PagedDeal& d, uint32_t x, int lane, uint32_t mine, int& item,
+                                             uint32_t& at) {
     uint32_t base = 0;
-    for (int e0 = 0; e0 < p.items; e0 += 64) {
-        const int e = e0 + lane;
-        const uint32_t n = e < p.items ? d.units((uint32_t)paged_span<CT>(p, e).tiles) * (uint32_t)p.a.c.kvh : 0;
-        uint32_t s = n;
-#pragma unroll
-        for (int m = 1; m < 64; m <<= 1) {
-            const uint32_t o = __shfl_up(s, m);
-            s += lane >= m ? o : 0;
-        }
-        s += base;
+    for (int e0 = 0;;) {
+        const uint32_t n = mine ? d.units(mine) * p.kvh.d : 0;
+        const uint32_t s = base + wave_scan(n);
         const uint64_t past = __ballot(s > x);
         if (past) {
             const int l = __ffsll((unsigned long long)past) - 1;
@@ -160,9 +191,11 @@ __device__ __forceinline__ bool paged_locate(const PagedMfmaArgs& p, const Paged
             at = x - (uint32_t)__builtin_amdgcn_readlane((int)(s - n), l);
             return true;
         }
+        e0 += 64;
+        if (e0 >= p.items) return false;
         base = (uint32_t)__builtin_amdgcn_readlane((int)s, 63);
+        mine = e0 + lane < p.items ? (uint32_t)paged_span<BN, CT>(p, e0 + lane).tiles : 0;
     }
-    return false;
 }
 
 // A stretch of a segment's tiles, [c0, c1), and the workgroups whose pieces make up the segment.
@@ -172,9 +205,17 @@ struct PagedPiece {
     uint32_t first, pieces;
 };
 
+// Of the segment of `tiles` tiles from tile `begin` of the call, when stretches are dealt: ends of stretches inside it that
+// do not move to its ends cut it.
 __device__ __forceinline__ void paged_pieces(const PagedDeal& d, uint32_t begin, uint32_t tiles, PagedPiece& pc) {
-    pc.first = begin / d.per;
-    pc.pieces = (begin + tiles - 1) / d.per - pc.first + 1;
+    pc.first = small_div(begin + d.snap, d.per);
+    const uint32_t last = tiles > 2 * d.snap ? small_div(begin + tiles - d.snap - 1, d.per) : 0;
+    pc.pieces = last > pc.first ? last - pc.first + 1 : 1;
+}
+
+// Where the end of a stretch at tile x of a segment's tiles lies.
+__device__ __forceinline__ uint32_t paged_cut(const PagedDeal& d, uint32_t x, uint32_t tiles) {
+    return x <= d.snap ? 0 : tiles - x <= d.snap ? tiles : x;
 }
 
 // Where a segment's piece i is kept: a workgroup has at most one piece that does not begin its segment and one that does
@@ -185,45 +226,34 @@ __device__ __forceinline__ uint32_t paged_slot(uint32_t first, uint32_t i) { ret
 // partials and outputs
 // ---------------------------------------------------------------------------
 
-template <int DT>
-__device__ __forceinline__ void paged_store(const PagedMfmaArgs& p, int64_t off, f32x4 o) {
-    if constexpr (DT == TVK_F32) {
-        float* op = static_cast<float*>(p.a.out) + off;
-        if (p.out_vec) *reinterpret_cast<f32x4*>(op) = o;
-        else
-#pragma unroll
-            for (int i = 0; i < 4; ++i) op[i] = o[i];
-    } else {
-        uint16_t* op = static_cast<uint16_t*>(p.a.out) + off;
-        if (p.out_vec) *reinterpret_cast<u32x2*>(op) = u32x2{pack2<DT>(o[0], o[1]), pack2<DT>(o[2], o[3])};
-        else
-#pragma unroll
-            for (int i = 0; i < 4; ++i) op[i] = __builtin_bit_cast(uint16_t, elem<DT>::from_f32(o[i]));
+// Query row r of (b, hk), its softmax's max and sum known: where it goes, and the factor of its products.
+struct PagedRow {
+    int64_t o, lse;
+    float f, l;
+    __device__ __forceinline__ PagedRow(const PagedMfmaArgs& p, int b, int hk, int r, float m, float sum) {
+        const int t = (int)div32((uint32_t)r, p.group), h = hk * (int)p.group.d + (r - t * (int)p.group.d);
+        o = (int64_t)b * p.a.so[0] + (int64_t)t * p.a.so[1] + (int64_t)h * p.a.so[2];
+        lse = (int64_t)b * p.a.sl[0] + (int64_t)t * p.a.sl[1] + (int64_t)h * p.a.sl[2];
+        // a NaN sum is a NaN row; only a row without keys is zeros, as its products are
+        const bool none = sum == 0.0f;
+        f = none ? 0.0f : (p.a.c.v_scale ? p.a.c.v_scale[hk] : 1.0f) * __builtin_amdgcn_rcpf(sum);   // sum >= 1, or no number
+        l = none ? INFINITY : (m + __builtin_amdgcn_logf(sum)) * AT_LN2;
     }
-}
-
-// Columns dv .. dv + 3 of query row r of (b, hk), from its softmax's max, sum and products.
-template <int DT>
-__device__ __forceinline__ void paged_finish(const PagedMfmaArgs& p, int b, int hk, int r, int dv, float m, float l, f32x4 o) {
-    const int t = r / p.a.group, h = hk * p.a.group + (r - t * p.a.group);
-    // a NaN sum is a NaN row; only a row without keys is zeros
-    const bool none = l == 0.0f;
-    const float f = p.a.c.v_scale ? p.a.c.v_scale[hk] / l : 1.0f / l;
-    paged_store<DT>(p, (int64_t)b * p.a.so[0] + (int64_t)t * p.a.so[1] + (int64_t)h * p.a.so[2] + dv,
-                    none ? f32x4{0, 0, 0, 0} : f32x4{o[0] * f, o[1] * f, o[2] * f, o[3] * f});
-    if (dv == 0 && p.a.lse)
-        p.a.lse[(int64_t)b * p.a.sl[0] + (int64_t)t * p.a.sl[1] + (int64_t)h * p.a.sl[2]] =
-            none ? INFINITY : m * AT_LN2 + logf(l);
-}
-
-__device__ __forceinline__ __amdgpu_buffer_rsrc_t paged_rsrc(const PagedMfmaArgs& p) {
-    return __builtin_amdgcn_make_buffer_rsrc((void*)p.part_o, 0, (int)p.part_bytes, 0x00020000);
-}
-// Byte offsets of the partials: below 2 GiB (paged_attn_mfma).
-__device__ __forceinline__ int paged_o_at(const PagedMfmaArgs& p, uint32_t row, int dv) { return (int)((row * (uint32_t)p.a.c.hd + dv) * 4); }
-__device__ __forceinline__ int paged_ml_at(const PagedMfmaArgs& p, uint32_t row) {
-    return (int)((const char*)(p.part_ml + (int64_t)row * 2) - (const char*)p.part_o);
-}
+    // columns dv .. dv + 3
+    template <int DT>
+    __device__ __forceinline__ void store(const PagedMfmaArgs& p, int dv, f32x4 v) const {
+        if (dv == 0 && p.a.lse) p.a.lse[lse] = l;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] *= f;
+        if constexpr (DT == TVK_F32) {
+            typedef float V __attribute__((ext_vector_type(4), aligned(4)));
+            *reinterpret_cast<V*>(static_cast<float*>(p.a.out) + o + dv) = v;
+        } else {
+            *reinterpret_cast<u32x2u*>(static_cast<uint16_t*>(p.a.out) + o + dv) =
+                u32x2u{pack2<DT>(v[0], v[1]), pack2<DT>(v[2], v[3])};
+        }
+    }
+};
 
 // A running (max, sum, O) takes in another.
 struct PagedSum {
@@ -244,72 +274,177 @@ struct PagedSum {
     }
 };
 
-constexpr int PM_MERGE_BYTES = 64 * PM_WAVES * 24;   // of LDS that paged_merge uses
+// The runs that a segment's pieces are joined in: run r is the pieces [at(r), at(r + 1)).
+struct PagedRuns {
+    uint32_t pieces, n;
+    bool apart;   // by several workgroups
+    __device__ __forceinline__ uint32_t at(uint32_t r) const { return pieces * r / n; }
+    __device__ __forceinline__ uint32_t of(uint32_t i) const { return ((i + 1) * n - 1) / pieces; }
+};
 
-// Merges a segment's pieces in order and writes its rows. Where the rows' quads of columns are few, each is shared by
-// several threads, a run of pieces to each, whose sums are then joined through LDS in order.
-template <int DT, int CT>
-__device__ __forceinline__ void paged_merge(const PagedMfmaArgs& p, int item, int hk, uint32_t first, uint32_t pieces, char* lds) {
-    const __amdgpu_buffer_rsrc_t rs = paged_rsrc(p);
-    const int tid = threadIdx.x, b = item / p.nrb, r0 = (item - b * p.nrb) * 16 * CT;
-    const int nr = min(16 * CT, p.rows - r0), quads = p.a.c.hd / 4, all = nr * quads;
-    const int share = all <= 128 && pieces >= 8 ? (int)min(64u * PM_WAVES / (uint32_t)all, pieces / 4) : 1;
-    auto sum = [&](int row, int dv, uint32_t i0, uint32_t i1) __attribute__((always_inline)) {
+__device__ __forceinline__ PagedRuns paged_runs(uint32_t pieces, uint32_t quads) {   // quads of columns in all of the rows
+    PagedRuns r{pieces, 1, pieces * quads > 8192};   // 128 KB
+    if (r.apart) r.n = min(32u, (pieces + 7) / 8);
+    else if (quads <= 128 && pieces >= 8)
+        r.n = min(min(32u, 256u / quads), pieces / 4);   // threads that would be idle take one each
+    return r;
+}
+
+// Partials in memory. SHARED: other workgroups of the launch write and read them, through the L2 (an XCD's lines may be
+// older than another's stores); else an earlier launch wrote them.
+template <int CT, bool SHARED>
+struct PagedParts {
+    const PagedMfmaArgs& p;
+    __amdgpu_buffer_rsrc_t rs;
+    __device__ __forceinline__ PagedParts(const PagedMfmaArgs& a)
+        : p(a), rs(__builtin_amdgcn_make_buffer_rsrc((void*)a.part_o, 0, (int)a.part_bytes, 0x00020000)) {}
+    // byte offsets: below 2 GiB; of a run's result in the place of its first piece, whose max and sum others still read
+    __device__ __forceinline__ int run_ml_at(uint32_t slot, int lr) const { return ml_at(slot + 2 * p.wgs, lr); }
+    __device__ __forceinline__ int o_at(uint32_t slot, int lr, int dv) const {
+        return (int)(((slot * 16 * CT + lr) * (uint32_t)p.a.c.hd + dv) * 4);
+    }
+    __device__ __forceinline__ int ml_at(uint32_t slot, int lr) const {
+        return (int)((const char*)p.part_ml - (const char*)p.part_o) + (int)(slot * 16 * CT + lr) * 8;
+    }
+    __device__ __forceinline__ f32x2v ml(int at) const {
+        return __builtin_bit_cast(f32x2v, __builtin_amdgcn_raw_buffer_load_b64(rs, at, 0, SHARED ? kCoherent : 0));
+    }
+    __device__ __forceinline__ f32x4 o(uint32_t slot, int lr, int dv) const {
+        return __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(rs, o_at(slot, lr, dv), 0, SHARED ? kCoherent : 0));
+    }
+    __device__ __forceinline__ void store(uint32_t slot, int lr, int dv, const PagedSum& s, bool piece) const {
+        const u32x2 w = __builtin_bit_cast(u32x2, f32x2v{s.m, s.l});
+        __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, s.o), rs, o_at(slot, lr, dv), 0, kCoherent);
+        if (dv == 0) __builtin_amdgcn_raw_buffer_store_b64(w, rs, run_ml_at(slot, lr), 0, kCoherent);   // a run of one piece
+        if (dv == 0 && piece) __builtin_amdgcn_raw_buffer_store_b64(w, rs, ml_at(slot, lr), 0, kCoherent);
+    }
+    // Joins pieces i0 .. i1 - 1 in order, eight on their way together. Past the last piece it is read again, and masked: a
+    // weight of 0 would make NaN of an infinite sum, and a branch lets the loads sink to their uses.
+    __device__ __forceinline__ PagedSum run(uint32_t first, uint32_t i0, uint32_t i1, int lr, int dv) const {
         PagedSum s;
         constexpr uint32_t U = 8;
         for (uint32_t i = i0; i < i1; i += U) {
-            u32x2 w[U];
-            u32x4 os[U];
-            // past the last piece it is read again, and its max and sums masked: a weight of 0 would make NaN of an
-            // infinite sum, and a branch lets the loads sink to their uses
-            auto at = [&](uint32_t u) { return paged_slot(first, min(i + u, i1 - 1)) * 16 * CT + row; };
+            f32x2v w[U];
+            f32x4 os[U];
 #pragma unroll
-            for (uint32_t u = 0; u < U; ++u)
-                w[u] = __builtin_bit_cast(u32x2, __builtin_amdgcn_raw_buffer_load_b64(rs, paged_ml_at(p, at(u)), 0, kCoherent));
+            for (uint32_t u = 0; u < U; ++u) w[u] = ml(ml_at(paged_slot(first, min(i + u, i1 - 1)), lr));
 #pragma unroll
-            for (uint32_t u = 0; u < U; ++u)
-                os[u] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(rs, paged_o_at(p, at(u), dv), 0, kCoherent));
+            for (uint32_t u = 0; u < U; ++u) os[u] = o(paged_slot(first, min(i + u, i1 - 1)), lr, dv);
             __builtin_amdgcn_sched_barrier(0);
             float mn = s.m;
 #pragma unroll
             for (uint32_t u = 0; u < U; ++u) {
-                if (i + u >= i1) w[u][0] = 0xff800000u;
-                mn = fmaxf(mn, __builtin_bit_cast(float, (uint32_t)w[u][0]));
+                if (i + u >= i1) w[u][0] = -INFINITY;
+                mn = fmaxf(mn, w[u][0]);
             }
             s.raise(mn);
 #pragma unroll
             for (uint32_t u = 0; u < U; ++u) {
-                os[u] = os[u] & (i + u < i1 ? ~0u : 0u);
-                s.add(__builtin_bit_cast(float, (uint32_t)w[u][0]), __builtin_bit_cast(float, (uint32_t)w[u][1]),
-                      __builtin_bit_cast(f32x4, os[u]));
+                const u32x4 kept = __builtin_bit_cast(u32x4, os[u]) & (i + u < i1 ? ~0u : 0u);
+                s.add(w[u][0], w[u][1], __builtin_bit_cast(f32x4, kept));
             }
         }
         return s;
-    };
-    if (share == 1) {
-        for (int c = tid; c < all; c += 64 * PM_WAVES) {
-            const int row = c / quads, dv = (c - row * quads) * 4;
-            const PagedSum s = sum(row, dv, 0, pieces);
-            paged_finish<DT>(p, b, hk, r0 + row, dv, s.m, s.l, s.o);
+    }
+    // Joins the results of runs, kept where each run's first piece was.
+    __device__ __forceinline__ PagedSum runs(uint32_t first, const PagedRuns& r, int lr, int dv) const {
+        PagedSum s;
+        constexpr uint32_t U = 8;
+        for (uint32_t i = 0; i < r.n; i += U) {
+            f32x2v w[U];
+#pragma unroll
+            for (uint32_t u = 0; u < U; ++u) w[u] = ml(run_ml_at(paged_slot(first, r.at(min(i + u, r.n - 1))), lr));
+#pragma unroll
+            for (uint32_t u = 0; u < U; ++u) s.m = fmaxf(s.m, w[u][0]);
+        }
+        for (uint32_t i = 0; i < r.n; i += U) {
+            f32x2v w[U];
+            f32x4 os[U];
+#pragma unroll
+            for (uint32_t u = 0; u < U; ++u) {
+                const uint32_t slot = paged_slot(first, r.at(min(i + u, r.n - 1)));
+                w[u] = ml(run_ml_at(slot, lr));
+                os[u] = o(slot, lr, dv);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (uint32_t u = 0; u < U; ++u)
+                if (i + u < r.n) s.add(w[u][0], w[u][1], os[u]);
+        }
+        return s;
+    }
+};
+
+// Joins `n` runs whose results lie in LDS, `step` apart.
+__device__ __forceinline__ PagedSum paged_runs_lds(const f32x4* o, const f32x2v* ml, uint32_t n, uint32_t step) {
+    PagedSum s;
+    for (uint32_t i = 0; i < n; ++i) s.m = fmaxf(s.m, ml[i * step][0]);
+    for (uint32_t i = 0; i < n; ++i) s.add(ml[i * step][0], ml[i * step][1], o[i * step]);
+    return s;
+}
+
+// This workgroup has stored a piece: whether it is the last of the `n` that count on cnt, which is then zero again.
+__device__ __forceinline__ bool paged_last(unsigned* cnt, uint32_t n, int* flag) {
+    __builtin_amdgcn_s_waitcnt(0x0F70);   // vmcnt(0): this wave's partials are in memory
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        *flag = atomicAdd_system(cnt, 1u) + 1 == n;
+        if (*flag) atomicExch_system(cnt, 0u);
+    }
+    __syncthreads();
+    return *flag;
+}
+
+constexpr int PM_JOIN_BYTES = 256 * 24;   // of LDS that paged_join uses
+
+// After a workgroup of 256 threads has stored its piece i of a segment: the last one joins.
+template <int DT, int CT>
+__device__ __forceinline__ void paged_join(const PagedMfmaArgs& p, int item, int hk, uint32_t first, uint32_t pieces, uint32_t i,
+                                           char* lds, int* flag) {
+    const PagedParts<CT, true> parts(p);
+    const int tid = threadIdx.x, b = (int)div32((uint32_t)item, p.nrb), r0 = (item - b * (int)p.nrb.d) * 16 * CT;
+    const int quads = p.a.c.hd / 4, all = min(16 * CT, p.rows - r0) * quads;
+    const PagedRuns r = paged_runs(pieces, all);
+    unsigned* cnt = p.count + (int64_t)item * p.a.c.kvh + hk;
+    if (r.apart) {
+        const uint32_t run = r.of(i), i0 = r.at(run), i1 = r.at(run + 1), slot = paged_slot(first, i0);
+        if (i1 - i0 > 1) {
+            if (!paged_last(p.count + (int64_t)p.items * p.a.c.kvh + slot, i1 - i0, flag)) return;
+            for (int c = tid; c < all; c += 256) {
+                const int lr = c / quads, dv = (c - lr * quads) * 4;
+                parts.store(slot, lr, dv, parts.run(first, i0, i1, lr, dv), false);
+            }
+        }
+        if (!paged_last(cnt, r.n, flag)) return;
+        for (int c = tid; c < all; c += 256) {
+            const int lr = c / quads, dv = (c - lr * quads) * 4;
+            const PagedSum s = parts.runs(first, r, lr, dv);
+            PagedRow(p, b, hk, r0 + lr, s.m, s.l).template store<DT>(p, dv, s.o);
         }
         return;
     }
-    f32x4* po = reinterpret_cast<f32x4*>(lds);
-    float* pm = reinterpret_cast<float*>(lds + 64 * PM_WAVES * 16);
-    float* pl = pm + 64 * PM_WAVES;
-    const int part = tid / all, c = tid - part * all, row = c / quads, dv = (c - row * quads) * 4;
-    if (part < share) {
-        const PagedSum s = sum(row, dv, pieces * part / share, pieces * (part + 1) / share);
-        po[tid] = s.o;
-        pm[tid] = s.m;
-        pl[tid] = s.l;
+    if (!paged_last(cnt, pieces, flag)) return;
+    if (r.n == 1) {
+        for (int c = tid; c < all; c += 256) {
+            const int lr = c / quads, dv = (c - lr * quads) * 4;
+            const PagedSum s = parts.run(first, 0, pieces, lr, dv);
+            PagedRow(p, b, hk, r0 + lr, s.m, s.l).template store<DT>(p, dv, s.o);
+        }
+        return;
+    }
+    f32x4* o = reinterpret_cast<f32x4*>(lds);
+    f32x2v* ml = reinterpret_cast<f32x2v*>(lds + 256 * 16);
+    const uint32_t run = tid / all, c = tid - run * all;
+    const int lr = c / quads, dv = (c - lr * quads) * 4;
+    if (run < r.n) {
+        const PagedSum s = parts.run(first, r.at(run), r.at(run + 1), lr, dv);
+        o[tid] = s.o;
+        ml[tid] = f32x2v{s.m, s.l};
     }
     __syncthreads();
-    if (part) return;
-    PagedSum s;
-    for (int i = 0; i < share; ++i) s.m = fmaxf(s.m, pm[i * all + c]);
-    for (int i = 0; i < share; ++i) s.add(pm[i * all + c], pl[i * all + c], po[i * all + c]);
-    paged_finish<DT>(p, b, hk, r0 + row, dv, s.m, s.l, s.o);
+    if (run) return;
+    const PagedSum s = paged_runs_lds(o + c, ml + c, r.n, all);
+    PagedRow(p, b, hk, r0 + lr, s.m, s.l).template store<DT>(p, dv, s.o);
 }
 
 // ---------------------------------------------------------------------------
@@ -353,11 +488,6 @@ __device__ __forceinline__ uint32_t widen8(uint32_t w, bool hi) {
                                                : __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.0f, false));
 }
 
-// Bits i of a mask spread over the halves of a word.
-__device__ __forceinline__ uint32_t half_bits(uint32_t m, int lo, int hi) {
-    return ((m >> lo) & 1 ? 0xffffu : 0u) | ((m >> hi) & 1 ? 0xffff0000u : 0u);
-}
-
 // Bits of the keys k0 .. k0 + 31 that lie in [lo, hi).
 __device__ __forceinline__ uint32_t key_bits(int k0, int lo, int hi) {
     const int n = min(max(hi - k0, 0), 32), f = min(max(lo - k0, 0), 32);
@@ -365,68 +495,98 @@ __device__ __forceinline__ uint32_t key_bits(int k0, int lo, int hi) {
 }
 
 // FAST: the page size is a multiple of 16, so that a half tile lies in one page and its address is the wave's, not a
-// lane's, and rows fill their KL chunks of 64 bytes.
-template <int DT, bool F8, int D, int CT, bool FAST>
-__global__ __launch_bounds__(64 * PM_WAVES, (PagedTile<DT, F8, D>::occ(CT))) void paged_attn_mfma_kernel(PagedMfmaArgs) {
+// lane's, and rows fill their KL chunks of 64 bytes. WAVES 1: a wave a segment, for short sequences.
+template <int DT, bool F8, int D, int CT, bool FAST, int WAVES>
+__global__ __launch_bounds__(64 * WAVES, (PagedTile<DT, F8, D>::occ(CT))) void paged_attn_mfma_kernel(PagedMfmaArgs) {
     typedef PagedTile<DT, F8, D> G;
     constexpr bool F32 = DT == TVK_F32;
-    constexpr int KL = G::KL, QS = G::QS, EV = G::EV, DV = G::DV, VW = G::VW, ES = G::ES;
-    constexpr int LDO = DV + 4;
-    __shared__ __attribute__((aligned(16))) float red[PM_WAVES * 16 * LDO];
-    __shared__ float ml[2][PM_WAVES][16 * CT];
-    __shared__ int last;
-    static_assert(sizeof(red) >= PM_MERGE_BYTES, "the merge of pieces reuses the waves'");
-
+    constexpr int NB = G::NB, BN = G::BN, KL = G::KL, QS = G::QS, EV = G::EV, DV = G::DV, VW = G::VW, ES = G::ES;
+    constexpr int COLS = 16 * CT, LDO = DV + 4;
+    constexpr int RED = WAVES == 1 ? 16 * DV : WAVES * COLS * LDO;
+    __shared__ __attribute__((aligned(16))) float red[RED];
+    __shared__ float ml[2][WAVES][COLS];
+    __shared__ int flag;
+    static_assert(WAVES == 1 || (sizeof(red) >= PM_JOIN_BYTES && WAVES == 4), "the join of pieces reuses the waves'");
+    __shared__ int has_marks;
     __shared__ uint32_t marks[CT * DV];   // two bits for each row and column: the infinities (1, 2) it takes in, both for NaN
-    const int tid = threadIdx.x, lane = tid % 64, wave = __builtin_amdgcn_readfirstlane(tid / 64);
+    const int tid = threadIdx.x, lane = tid % 64, wave = WAVES == 1 ? 0 : __builtin_amdgcn_readfirstlane(tid / 64);
     const int g = lane / 16, c16 = lane % 16;
     const uint32_t wg = blockIdx.x;
-    const PagedDeal deal = paged_deal<CT>(paged_args(), lane);
-    PagedPiece pc;
-    uint32_t at;
-    uint32_t x = deal.chunk ? wg : wg * deal.per;
-    if (!paged_locate<CT>(paged_args(), deal, x, lane, pc.item, at)) return;
-    const uint32_t stop = deal.chunk ? x + 1 : min(deal.total, x + deal.per);
+    PagedDeal deal{31, 0, 0, 0};
+    PagedPiece pc, part[2];   // part: pieces of segments that others share, the one that begins its segment second
+    int parts = 0;
+    uint32_t at = 0, x = wg, stop = 0;
+    const bool dealt = WAVES > 1 && paged_args().wgs;
+    if (!dealt) {
+        const PagedMfmaArgs& p = paged_args();
+        pc.item = (int)div32(wg, p.kvh);
+        pc.hk = (int)(wg - pc.item * p.kvh.d);
+    } else {
+        const PagedMfmaArgs& p = paged_args();
+        const uint32_t mine = lane < p.items ? (uint32_t)paged_span<BN, CT>(p, lane).tiles : 0;
+        deal = paged_deal<BN, CT>(p, lane, mine);
+        if (deal.shift < 0) {
+            x = wg * deal.per;
+            stop = min(deal.total, x + deal.per);
+        }
+        if (!paged_locate<BN, CT>(p, deal, x, lane, mine, pc.item, at)) return;
+    }
 
     for (bool more_pieces = true; more_pieces;) {
-        __syncthreads();   // the piece before has been merged
+        if (WAVES > 1) __syncthreads();   // the piece before has been merged
         const PagedMfmaArgs& p = paged_args();
         const PagedAttnArgs& a = p.a;
         const bool several = a.new_tokens > 1;
         if (several) {
-            for (int i = tid; i < CT * DV; i += 64 * PM_WAVES) marks[i] = 0;
-            __syncthreads();
+            for (int i = tid; i < CT * DV; i += 64 * WAVES) marks[i] = 0;
+            if (tid == 0) has_marks = 0;
+            if (WAVES > 1) __syncthreads();
         }
-        const PagedSpan sp = paged_span<CT>(p, pc.item);
-        const uint32_t units = deal.units((uint32_t)sp.tiles);
-        pc.hk = (int)(at / units);
-        at -= (uint32_t)pc.hk * units;
-        if (deal.chunk) {
-            pc.c0 = (uint32_t)((uint64_t)at * (uint32_t)sp.tiles / units);
-            pc.c1 = (uint32_t)((uint64_t)(at + 1) * (uint32_t)sp.tiles / units);
-            pc.first = x - at;
-            pc.pieces = units;
-            more_pieces = false;
-        } else {
-            pc.c0 = at;
-            pc.c1 = min((uint32_t)sp.tiles, at + (stop - x));
-            paged_pieces(deal, x - at, (uint32_t)sp.tiles, pc);
+        const PagedSpan sp = paged_span<BN, CT>(p, pc.item);
+        const uint32_t tiles = (uint32_t)sp.tiles;
+        more_pieces = false;
+        pc.c0 = 0;
+        pc.c1 = tiles;
+        pc.pieces = 1;
+        if (dealt) {
+            const uint32_t units = deal.units(tiles);
+            pc.hk = (int)small_div(at, units);
+            at -= (uint32_t)pc.hk * units;   // of the segment
+            if (deal.shift >= 0) {
+                const uint32_t q = small_div(tiles, units), r = tiles - q * units;
+                pc.c0 = at * q + min(at, r);
+                pc.c1 = pc.c0 + q + (at < r);
+                pc.first = x - at;
+                pc.pieces = units;
+            } else {
+                const uint32_t rest = tiles - at;   // of the stretch
+                paged_pieces(deal, x - at, tiles, pc);
+                pc.c0 = paged_cut(deal, at, tiles);
+                pc.c1 = stop - x < rest ? paged_cut(deal, at + (stop - x), tiles) : tiles;
+                // the next segment: the item's next head, or the next item's first
+                x += rest;
+                more_pieces = x < stop;
+                at = (uint32_t)(pc.hk + 1) * tiles;
+            }
         }
-        const int b = sp.b, hk = pc.hk, r0 = (pc.item - b * p.nrb) * 16 * CT;
+        const int item = pc.item;
+        if (more_pieces && pc.hk + 1 == (int)p.kvh.d) {
+            ++pc.item;
+            at = 0;
+        }
+        if (pc.c0 >= pc.c1) continue;
+        const int b = sp.b, hk = pc.hk, r0 = (item - b * (int)p.nrb.d) * COLS;
 
         // ---- queries: scores in log2 units are c2 * q.k, with q's signs turned where c2 would be negative
         const float cs = a.scale * (F8 && a.c.k_scale ? a.c.k_scale[hk] : 1.0f) * AT_LOG2E;
         const float c2 = cs < 0.0f ? -cs : cs;
-        const uint32_t flip = cs < 0.0f ? (F32 ? 0x80000000u : 0x80008000u) : 0u;
         u32x4 qf[CT][QS];
-        int first_c[CT], last_c[CT];
+        int last_c[CT];   // keys below it are seen by the column's row
 #pragma unroll
         for (int ct = 0; ct < CT; ++ct) {
             const int r = min(r0 + 16 * ct + c16, p.rows - 1);   // columns past the rows repeat the last one, unused
-            const int t = r / a.group, h = hk * a.group + (r - t * a.group);
-            
+            const int t = (int)div32((uint32_t)r, p.group), h = hk * (int)p.group.d + (r - t * (int)p.group.d);
             last_c[ct] = sp.len - a.new_tokens + t + 1;
-            first_c[ct] = a.window ? (int)max((int64_t)0, (int64_t)last_c[ct] - (int64_t)a.window) : 0;
             constexpr int QES = F32 ? 4 : 2;
             const char* Q = static_cast<const char*>(a.q) +
                             ((int64_t)b * a.sq[0] + (int64_t)t * a.sq[1] + (int64_t)h * a.sq[2]) * QES;
@@ -434,10 +594,14 @@ __global__ __launch_bounds__(64 * PM_WAVES, (PagedTile<DT, F8, D>::occ(CT))) voi
             for (int s = 0; s < QS; ++s) {
                 // the first value of the fragment that K's chunk s (8-bit: half a chunk) meets
                 const int d = F8 ? 64 * (s / 2) + 16 * g + 8 * (s % 2) : (64 * s + 16 * g) / ES;
-                u32x4 v = d < a.c.hd ? *reinterpret_cast<const u32x4*>(Q + d * QES) : u32x4{0, 0, 0, 0};
-                v ^= flip;
-                qf[ct][s] = v;
+                qf[ct][s] = FAST || d < a.c.hd ? *reinterpret_cast<const u32x4*>(Q + d * QES) : u32x4{0, 0, 0, 0};
             }
+        }
+        if (__builtin_expect(cs < 0.0f, 0)) {
+#pragma unroll
+            for (int ct = 0; ct < CT; ++ct)
+#pragma unroll
+                for (int s = 0; s < QS; ++s) qf[ct][s] ^= F32 ? 0x80000000u : 0x80008000u;
         }
 
         f32x4 oacc[EV][CT];
@@ -452,7 +616,7 @@ __global__ __launch_bounds__(64 * PM_WAVES, (PagedTile<DT, F8, D>::occ(CT))) voi
 
         // ---- where a tile's keys are
         // lane offsets, in bytes, of a row's chunks and values
-        const uint32_t krow = (uint32_t)a.c.sk[1] * ES, vrow = (uint32_t)a.c.sv[1] * ES;
+        const uint32_t krow = p.ks * 16, vrow = p.vs * 16;
         const uint32_t kbytes = (uint32_t)a.c.hd * ES;
         uint32_t kcol[FAST ? 1 : KL];   // chunks past the row are its last one, and zeros when it comes to the product
         if constexpr (FAST) kcol[0] = c16 * krow + 16 * g;
@@ -469,16 +633,19 @@ __global__ __launch_bounds__(64 * PM_WAVES, (PagedTile<DT, F8, D>::occ(CT))) voi
         const int32_t* trow = a.c.table + (int64_t)b * a.c.table_stride;
         const char* Kh = static_cast<const char*>(a.c.k) + (int64_t)hk * a.c.sk[2] * ES;
         const char* Vh = static_cast<const char*>(a.c.v) + (int64_t)hk * a.c.sv[2] * ES;
-        constexpr int NE = FAST ? 2 : 1;
+        constexpr uint32_t ALL = BN == 32 ? ~0u : (1u << BN) - 1;
+        constexpr int NE = FAST ? NB : 1;
         uint32_t entry[NE], slot[NE];      // of the tile after next: table entries on their way
-        const char* kbase[2];              // FAST: a half's first row
-        const char* vbase[2];
-        uint32_t koff = 0, voff = 0;       // else: lane j's for key j % 32, in 16 bytes
+        const char* kbase[NB];             // FAST: a block's first row
+        const char* vbase[NB];
+        uint32_t koff = 0, voff = 0;       // else: lane j's for key j % BN, in 16 bytes
         uint32_t ok = 0;                   // keys that have a page
-        auto fetch = [&](int t) {          // hi > 0; past the last key its own entry is read again
+        const uint32_t kp = p.kp, ks = p.ks, vp = p.vp, vs = p.vs;
+        const int reach = (int)a.c.reach - 1;
+        auto fetch = [&](int t) {          // past the table its last entry is read again
 #pragma unroll
             for (int i = 0; i < NE; ++i) {
-                const uint32_t pos = FAST ? min(t * PM_BN + 16 * i, (sp.hi - 1) & ~15) : min(t * PM_BN + lane % 32, sp.hi - 1);
+                const uint32_t pos = FAST ? min(t * BN + 16 * i, reach & ~15) : min(t * BN + lane % BN, reach);
                 const uint32_t n = div32(pos, a.c.page);
                 slot[i] = pos - n * a.c.page.d;
                 if constexpr (FAST) entry[i] = (uint32_t)((table_ptr)(uintptr_t)trow)[n];
@@ -486,29 +653,28 @@ __global__ __launch_bounds__(64 * PM_WAVES, (PagedTile<DT, F8, D>::occ(CT))) voi
             }
         };
         auto resolve = [&]() {   // keys without a page read page 0 and are masked
+            uint32_t page[NE];
+#pragma unroll
+            for (int i = 0; i < NE; ++i) page[i] = entry[i] < a.c.pages ? entry[i] : 0;
             if constexpr (FAST) {
                 ok = 0;
 #pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    const bool in = entry[i] < a.c.pages;
-                    const int64_t page = in ? entry[i] : 0;
-                    ok |= in ? 0xffffu << (16 * i) : 0u;
-                    kbase[i] = Kh + (page * a.c.sk[0] + (int64_t)slot[i] * a.c.sk[1]) * ES;
-                    vbase[i] = Vh + (page * a.c.sv[0] + (int64_t)slot[i] * a.c.sv[1]) * ES;
+                for (int i = 0; i < NB; ++i) {
+                    ok |= entry[i] < a.c.pages ? 0xffffu << (16 * i) : 0u;
+                    kbase[i] = Kh + (uint64_t)(page[i] * kp + slot[i] * ks) * 16;
+                    vbase[i] = Vh + (uint64_t)(page[i] * vp + slot[i] * vs) * 16;
                 }
             } else {
-                const bool in = entry[0] < a.c.pages;
-                const int64_t page = in ? entry[0] : 0;
-                ok = (uint32_t)__ballot(in);
-                koff = (uint32_t)((uint64_t)((page * a.c.sk[0] + (int64_t)slot[0] * a.c.sk[1]) * ES) / 16);
-                voff = (uint32_t)((uint64_t)((page * a.c.sv[0] + (int64_t)slot[0] * a.c.sv[1]) * ES) / 16);
+                ok = (uint32_t)__ballot(entry[0] < a.c.pages) & ALL;
+                koff = page[0] * kp + slot[0] * ks;
+                voff = page[0] * vp + slot[0] * vs;
             }
         };
-        u32x4 kr[2][KL];
-        uint32_t vr[8][VW];
+        u32x4 kr[NB][KL];
+        uint32_t vr[4 * NB][VW];
         auto load_k = [&]() {
 #pragma unroll
-            for (int kb = 0; kb < 2; ++kb) {
+            for (int kb = 0; kb < NB; ++kb) {
                 const char* row = Kh;
                 if constexpr (!FAST) row += (uint64_t)__shfl(koff, 16 * kb + c16) * 16;
 #pragma unroll
@@ -518,7 +684,7 @@ __global__ __launch_bounds__(64 * PM_WAVES, (PagedTile<DT, F8, D>::occ(CT))) voi
         };
         auto load_v = [&]() {
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
+            for (int j = 0; j < 4 * NB; ++j) {
                 if constexpr (FAST) load_words<VW>(vbase[j / 4] + vfast[j % 4], vr[j]);
                 else load_words<VW>(Vh + (uint64_t)__shfl(voff, 16 * (j / 4) + 4 * g + j % 4) * 16 + vcol, vr[j]);
             }
@@ -527,14 +693,14 @@ __global__ __launch_bounds__(64 * PM_WAVES, (PagedTile<DT, F8, D>::occ(CT))) voi
         int t = 0;
         auto next_k = [&]() {
             resolve();
-            fetch(t + 2 * PM_WAVES);
+            fetch(t + 2 * WAVES);
             load_k();
         };
 
-        const int tile0 = sp.lo / PM_BN;
+        const int tile0 = sp.lo / BN;
         const int end = sp.hi > sp.lo ? tile0 + (int)pc.c1 : 0;
         // keys that every row of the block sees
-        const int all_lo = a.window ? (int)max((int64_t)0, (int64_t)sp.hi - (int64_t)a.window) : 0;
+        const int all_lo = window_lo(sp.hi, a.window);
         const int all_hi = sp.len - a.new_tokens + sp.t0 + 1;
         t = tile0 + (int)pc.c0 + wave;
         if (t < end) {
@@ -542,30 +708,30 @@ __global__ __launch_bounds__(64 * PM_WAVES, (PagedTile<DT, F8, D>::occ(CT))) voi
             resolve();
             load_k();
             load_v();
-            fetch(t + PM_WAVES);
+            fetch(t + WAVES);
         }
-        for (; t < end; t += PM_WAVES) {
-            const int k0 = t * PM_BN;
+        for (; t < end; t += WAVES) {
+            const int k0 = t * BN;
             const uint32_t keys = ok & key_bits(k0, sp.lo, sp.hi);
-            const bool plain = keys == ~0u && k0 >= all_lo && k0 + PM_BN <= all_hi;
-            const bool more = t + PM_WAVES < end;
+            const bool plain = keys == ALL && k0 >= all_lo && k0 + BN <= all_hi;
+            const bool more = t + WAVES < end;
             // ---- S^T = K Q^T
             if constexpr (!FAST) {
 #pragma unroll
                 for (int s = 0; s < KL; ++s)
 #pragma unroll
-                    for (int kb = 0; kb < 2; ++kb)
+                    for (int kb = 0; kb < NB; ++kb)
                         if (16 * g + 64 * s >= (int)kbytes) kr[kb][s] = u32x4{0, 0, 0, 0};
             }
-            f32x4 sacc[2][CT];
+            f32x4 sacc[NB][CT];
 #pragma unroll
-            for (int kb = 0; kb < 2; ++kb)
+            for (int kb = 0; kb < NB; ++kb)
 #pragma unroll
                 for (int ct = 0; ct < CT; ++ct) sacc[kb][ct] = f32x4{0, 0, 0, 0};
 #pragma unroll
             for (int s = 0; s < KL; ++s)
 #pragma unroll
-                for (int kb = 0; kb < 2; ++kb) {
+                for (int kb = 0; kb < NB; ++kb) {
                     const u32x4 kv = kr[kb][s];
                     if constexpr (F32) {
 #pragma unroll
@@ -597,15 +763,15 @@ __global__ __launch_bounds__(64 * PM_WAVES, (PagedTile<DT, F8, D>::occ(CT))) voi
             for (int ct = 0; ct < CT; ++ct) {
                 float tmax = -INFINITY;
                 if (!plain) {
-                    const uint32_t mine = (keys & key_bits(k0, first_c[ct], last_c[ct])) >> (4 * g);
+                    const uint32_t mine = (keys & key_bits(k0, window_lo(last_c[ct], a.window), last_c[ct])) >> (4 * g);
 #pragma unroll
-                    for (int kb = 0; kb < 2; ++kb)
+                    for (int kb = 0; kb < NB; ++kb)
 #pragma unroll
                         for (int r = 0; r < 4; ++r)
                             sacc[kb][ct][r] = (mine >> (16 * kb + r)) & 1 ? sacc[kb][ct][r] * c2 : -INFINITY;
                 }
 #pragma unroll
-                for (int kb = 0; kb < 2; ++kb)
+                for (int kb = 0; kb < NB; ++kb)
 #pragma unroll
                     for (int r = 0; r < 4; ++r) tmax = fmaxf(tmax, sacc[kb][ct][r]);
                 tmax = lanes4_max(tmax);
@@ -616,7 +782,7 @@ __global__ __launch_bounds__(64 * PM_WAVES, (PagedTile<DT, F8, D>::occ(CT))) voi
                 rescale = rescale || alpha[ct] != 1.0f;
                 float rsum = 0.0f;
 #pragma unroll
-                for (int kb = 0; kb < 2; ++kb)
+                for (int kb = 0; kb < NB; ++kb)
 #pragma unroll
                     for (int r = 0; r < 4; ++r) {
                         const float e = __builtin_amdgcn_exp2f(plain ? __builtin_fmaf(sacc[kb][ct][r], c2, -m_use) : sacc[kb][ct][r] - m_use);
@@ -638,56 +804,67 @@ __global__ __launch_bounds__(64 * PM_WAVES, (PagedTile<DT, F8, D>::occ(CT))) voi
             // values of keys that no row sees may be anything: zeros
             if (!plain) {
 #pragma unroll
-                for (int j = 0; j < 8; ++j)
+                for (int j = 0; j < 4 * NB; ++j)
 #pragma unroll
                     for (int w = 0; w < VW; ++w) vr[j][w] = (keys >> (4 * g + 16 * (j / 4) + j % 4)) & 1 ? vr[j][w] : 0u;
             }
-            constexpr int RW = EV * (F32 ? 4 : 2) / 4;
-            uint32_t vw[8][RW];   // 8-bit values widened
-#pragma unroll
-            for (int j = 0; j < 8; ++j)
-#pragma unroll
-                for (int w = 0; w < RW; ++w) {
-                    if constexpr (F8) vw[j][w] = widen8<DT>(vr[j][w / 2], w % 2);
-                    else vw[j][w] = vr[j][w];
-                }
             // Keys that some rows see and others do not, with values that are not finite: a probability of zero must not
             // meet them. They are marked for the rows that see them, and zeros in the product.
             if (__builtin_expect(!plain && several, 0)) {
-                constexpr uint32_t top = F32 ? 0x7f800000u : DT == TVK_F16 ? 0x7c00u : 0x7f80u;
-                int odd = 0;
+                typedef typename std::conditional<F8, uint8_t, typename std::conditional<F32, uint32_t, uint16_t>::type>::type U;
+                // a value's bits that are all set in infinities and NaN (8 bits: in NaN alone)
+                constexpr uint32_t top = F8 ? 0x7fu : F32 ? 0x7f800000u : DT == TVK_F16 ? 0x7c00u : 0x7f80u;
+                constexpr uint32_t sign = F8 ? 0x80u : F32 ? 0x80000000u : 0x8000u;
+                constexpr int PER = 4 / ES;   // values in a word
+                // any value's such bits all set, a word's values together
+                bool odd;
+                if constexpr (F8) {
+                    uint32_t any = 0;
 #pragma unroll
-                for (int j = 0; j < 8; ++j)
+                    for (int j = 0; j < 4 * NB; ++j)
 #pragma unroll
-                    for (int w = 0; w < RW; ++w)
-                        odd |= (int)((vw[j][w] & top) == top) | (F32 ? 0 : (int)((vw[j][w] >> 16 & top) == top));
+                        for (int w = 0; w < VW; ++w) any |= (vr[j][w] & 0x7f7f7f7fu) + 0x01010101u;
+                    odd = any & 0x80808080u;
+                } else {
+                    typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
+                    u16x2 most = {0, 0};
+                    uint32_t most32 = 0;
+#pragma unroll
+                    for (int j = 0; j < 4 * NB; ++j)
+#pragma unroll
+                        for (int w = 0; w < VW; ++w) {
+                            if constexpr (F32) most32 = max(most32, vr[j][w] & top);
+                            else most = __builtin_elementwise_max(most, __builtin_bit_cast(u16x2, vr[j][w] & (top | top << 16)));
+                        }
+                    odd = F32 ? most32 == top : most[0] == top || most[1] == top;
+                }
                 if (__any(odd)) {
-                    uint32_t* tile = reinterpret_cast<uint32_t*>(red + wave * 16 * LDO);   // the wave's own: a half's values
+                    if (lane == 0) has_marks = 1;
+                    U* tile = reinterpret_cast<U*>(red + wave * (WAVES == 1 ? 0 : COLS * LDO));   // the wave's own: a block's values
 #pragma unroll
-                    for (int kb = 0; kb < 2; ++kb) {
+                    for (int kb = 0; kb < NB; ++kb) {
                         __builtin_amdgcn_wave_barrier();
 #pragma unroll
                         for (int j = 0; j < 4; ++j)
 #pragma unroll
-                            for (int w = 0; w < RW; ++w) {
-                                uint32_t& v = vw[4 * kb + j][w];
-                                tile[((4 * g + j) * 16 + c16) * RW + w] = v;
-                                if constexpr (F32) v = (v & top) == top ? 0u : v;
-                                else v &= ((v & top) == top ? 0u : 0xffffu) | ((v >> 16 & top) == top ? 0u : 0xffff0000u);
+                            for (int w = 0; w < VW; ++w) {
+                                uint32_t& v = vr[4 * kb + j][w];
+                                reinterpret_cast<uint32_t*>(tile)[((4 * g + j) * 16 + c16) * VW + w] = v;
+#pragma unroll
+                                for (int i = 0; i < PER; ++i)
+                                    if ((v >> (8 * ES * i) & top) == top) v &= ~((top | sign) << (8 * ES * i));
                             }
                         __builtin_amdgcn_wave_barrier();
 #pragma unroll 1
                         for (int i = lane; i < 16 * DV; i += 64) {
                             const int key = 16 * kb + i / DV, dv = i % DV;
-                            const uint32_t v = F32 ? tile[i] : reinterpret_cast<const uint16_t*>(tile)[i];
+                            const uint32_t v = tile[i];
                             if ((v & top) != top) continue;
-                            const uint32_t sign = F32 ? 0x80000000u : 0x8000u;
-                            const uint32_t mark = (v & ~sign) != top ? 3u : v & sign ? 2u : 1u;
+                            const uint32_t mark = F8 || (v & ~sign) != top ? 3u : v & sign ? 2u : 1u;
 #pragma unroll 1
-                            for (int col = 0; col < 16 * CT; ++col) {
-                                const int hi = sp.len - a.new_tokens + min(r0 + col, p.rows - 1) / a.group + 1;
-                                const int lo = a.window ? (int)max((int64_t)0, (int64_t)hi - (int64_t)a.window) : 0;
-                                if ((keys & key_bits(k0, lo, hi)) >> key & 1) atomicOr(&marks[(col * DV + dv) / 16], mark << 2 * (dv % 16));
+                            for (int col = 0; col < COLS; ++col) {
+                                const int hi = sp.len - a.new_tokens + (int)div32((uint32_t)min(r0 + col, p.rows - 1), p.group) + 1;
+                                if ((keys & key_bits(k0, window_lo(hi, a.window), hi)) >> key & 1) atomicOr(&marks[(col * DV + dv) / 16], mark << 2 * (dv % 16));
                             }
                         }
                     }
@@ -695,29 +872,36 @@ __global__ __launch_bounds__(64 * PM_WAVES, (PagedTile<DT, F8, D>::occ(CT))) voi
             }
             if constexpr (F32) {
 #pragma unroll
-                for (int j = 0; j < 8; ++j)
+                for (int j = 0; j < 4 * NB; ++j)
 #pragma unroll
                     for (int i = 0; i < EV; ++i)
 #pragma unroll
                         for (int ct = 0; ct < CT; ++ct)
-                            oacc[i][ct] = __builtin_amdgcn_mfma_f32_16x16x4f32(__builtin_bit_cast(float, vw[j][i]),
+                            oacc[i][ct] = __builtin_amdgcn_mfma_f32_16x16x4f32(__builtin_bit_cast(float, vr[j][i]),
                                                                                sacc[j / 4][ct][j % 4], oacc[i][ct], 0, 0, 0);
             } else {
                 u32x4 pf[CT];
 #pragma unroll
                 for (int ct = 0; ct < CT; ++ct) {
-                    const f32x4 y = sacc[0][ct], z = sacc[1][ct];
+                    const f32x4 y = sacc[0][ct], z = sacc[NB - 1][ct];
                     pf[ct] = u32x4{pack2<DT>(y[0], y[1]), pack2<DT>(y[2], y[3]), pack2<DT>(z[0], z[1]), pack2<DT>(z[2], z[3])};
                 }
 #pragma unroll
-                for (int i = 0; i < EV; ++i) {   // value i of the lane's eight keys
-                    const uint32_t sel = i % 2 ? 0x07060302u : 0x05040100u;
-                    const u32x4 vf = u32x4{__builtin_amdgcn_perm(vw[1][i / 2], vw[0][i / 2], sel),
-                                           __builtin_amdgcn_perm(vw[3][i / 2], vw[2][i / 2], sel),
-                                           __builtin_amdgcn_perm(vw[5][i / 2], vw[4][i / 2], sel),
-                                           __builtin_amdgcn_perm(vw[7][i / 2], vw[6][i / 2], sel)};
+                for (int w = 0; w < EV / 2; ++w) {
+                    uint32_t two[8];   // values 2w, 2w + 1 of the lane's eight keys
 #pragma unroll
-                    for (int ct = 0; ct < CT; ++ct) oacc[i][ct] = mfma16<DT>(vf, pf[ct], oacc[i][ct]);
+                    for (int j = 0; j < 8; ++j) {
+                        if constexpr (F8) two[j] = widen8<DT>(vr[j % (4 * NB)][w / 2], w % 2);
+                        else two[j] = vr[j % (4 * NB)][w % VW];
+                    }
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        const uint32_t sel = i ? 0x07060302u : 0x05040100u;
+                        const u32x4 vf = u32x4{__builtin_amdgcn_perm(two[1], two[0], sel), __builtin_amdgcn_perm(two[3], two[2], sel),
+                                               __builtin_amdgcn_perm(two[5], two[4], sel), __builtin_amdgcn_perm(two[7], two[6], sel)};
+#pragma unroll
+                        for (int ct = 0; ct < CT; ++ct) oacc[2 * w + i][ct] = mfma16<DT>(vf, pf[ct], oacc[2 * w + i][ct]);
+                    }
                 }
             }
             if (more) {
@@ -726,127 +910,184 @@ __global__ __launch_bounds__(64 * PM_WAVES, (PagedTile<DT, F8, D>::occ(CT))) voi
             }
         }
 
-        // ---- merge the waves, one 16-column block at a time
         const PagedMfmaArgs& pe = paged_args();
-        const bool whole = pc.pieces == 1;
+        auto marked = [&](int lr, int dv, f32x4 o) {   // with the infinities and NaN that were kept out of the products
+            const uint32_t mark = marks[(lr * DV + dv) / 16] >> 2 * (dv % 16);
 #pragma unroll
-        for (int ct = 0; ct < CT; ++ct) {
-            const float l_tot = lanes4_sum(l_run[ct]);
-            __syncthreads();   // the block (piece) before has been read
-            if (g == 0) {
-                ml[0][wave][16 * ct + c16] = m_run[ct];
-                ml[1][wave][16 * ct + c16] = l_tot;
+            for (int i = 0; i < 4; ++i) {
+                const uint32_t two = mark >> 2 * i & 3;
+                if (two) o[i] += two == 1 ? INFINITY : two == 2 ? -INFINITY : NAN;
             }
+            return o;
+        };
+        if constexpr (WAVES == 1) {
+            // ---- a lane's values are columns EV * 4g .. of its rows
+            const bool mark = several && has_marks;
 #pragma unroll
-            for (int r = 0; r < 4; ++r)
+            for (int ct = 0; ct < CT; ++ct) {
+                const float l = lanes4_sum(l_run[ct]);
+                const int lr = 16 * ct + c16;
+                if (r0 + lr >= pe.rows) continue;
+                const PagedRow row(pe, b, hk, r0 + lr, m_run[ct], l);
 #pragma unroll
-                for (int i = 0; i < EV; i += 4)
-                    *reinterpret_cast<f32x4*>(&red[(wave * 16 + c16) * LDO + EV * (4 * g + r) + i]) =
-                        f32x4{oacc[i][ct][r], oacc[i + 1][ct][r], oacc[i + 2][ct][r], oacc[i + 3][ct][r]};
+                for (int r = 0; r < 4; ++r)
+#pragma unroll
+                    for (int i = 0; i < EV; i += 4) {
+                        const int dv = EV * (4 * g + r) + i;
+                        f32x4 o = f32x4{oacc[i][ct][r], oacc[i + 1][ct][r], oacc[i + 2][ct][r], oacc[i + 3][ct][r]};
+                        if (!FAST && dv >= pe.a.c.hd) continue;
+                        if (__builtin_expect(mark, 0)) o = marked(lr, dv, o);
+                        row.template store<DT>(pe, dv, o);
+                    }
+            }
+        } else {
+            // ---- merge the waves
+            const bool whole = pc.pieces == 1;
+#pragma unroll
+            for (int ct = 0; ct < CT; ++ct) {
+                const float l_tot = lanes4_sum(l_run[ct]);
+                if (g == 0) {
+                    ml[0][wave][16 * ct + c16] = m_run[ct];
+                    ml[1][wave][16 * ct + c16] = l_tot;
+                }
+#pragma unroll
+                for (int r = 0; r < 4; ++r)
+#pragma unroll
+                    for (int i = 0; i < EV; i += 4)
+                        *reinterpret_cast<f32x4*>(&red[(wave * COLS + 16 * ct + c16) * LDO + EV * (4 * g + r) + i]) =
+                            f32x4{oacc[i][ct][r], oacc[i + 1][ct][r], oacc[i + 2][ct][r], oacc[i + 3][ct][r]};
+            }
             __syncthreads();
-            for (int c = tid; c < 16 * (DV / 4); c += 64 * PM_WAVES) {
-                const int col = c / (DV / 4), dv = (c % (DV / 4)) * 4;
-                const int lr = 16 * ct + col, r = r0 + lr;
-                if (r >= pe.rows || dv >= pe.a.c.hd) continue;
+            for (int c = tid; c < min(COLS, pe.rows - r0) * (DV / 4); c += 64 * WAVES) {
+                const int lr = c / (DV / 4), dv = (c % (DV / 4)) * 4;
+                if (!FAST && dv >= pe.a.c.hd) continue;
                 PagedSum s;
 #pragma unroll
-                for (int w = 0; w < PM_WAVES; ++w) s.m = fmaxf(s.m, ml[0][w][lr]);
+                for (int w = 0; w < WAVES; ++w) s.m = fmaxf(s.m, ml[0][w][lr]);
 #pragma unroll
-                for (int w = 0; w < PM_WAVES; ++w)
-                    s.add(ml[0][w][lr], ml[1][w][lr], *reinterpret_cast<const f32x4*>(&red[(w * 16 + col) * LDO + dv]));
-                if (several) {
-                    const uint32_t mark = marks[(lr * DV + dv) / 16] >> 2 * (dv % 16);
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const uint32_t two = mark >> 2 * i & 3;
-                        if (two) s.o[i] += two == 1 ? INFINITY : two == 2 ? -INFINITY : NAN;
-                    }
-                }
-                if (whole) {
-                    paged_finish<DT>(pe, b, hk, r, dv, s.m, s.l, s.o);
-                } else {
-                    const __amdgpu_buffer_rsrc_t rs = paged_rsrc(pe);
-                    const uint32_t row = (2 * wg + (pc.c0 == 0)) * 16 * CT + lr;
-                    __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, s.o), rs, paged_o_at(pe, row, dv), 0, kCoherent);
-                    if (dv == 0)
-                        __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(u32x2, f32x2v{s.m, s.l}), rs, paged_ml_at(pe, row), 0, kCoherent);
-                }
+                for (int w = 0; w < WAVES; ++w)
+                    s.add(ml[0][w][lr], ml[1][w][lr], *reinterpret_cast<const f32x4*>(&red[(w * COLS + lr) * LDO + dv]));
+                if (__builtin_expect(several && has_marks, 0)) s.o = marked(lr, dv, s.o);
+                if (whole) PagedRow(pe, b, hk, r0 + lr, s.m, s.l).template store<DT>(pe, dv, s.o);
+                else PagedParts<CT, true>(pe).store(2 * wg + (pc.c0 == 0), lr, dv, s, true);
+            }
+            if (!whole && pe.count) {
+                const int second = pc.c0 == 0;
+                part[second] = pc;
+                part[second].item = item;
+                parts |= 1 << second;
+            } else if (dealt && !pe.count && pc.c0 == 0 && tid == 0) {
+                *reinterpret_cast<u32x2*>(pe.seg + 2 * ((int64_t)item * pe.kvh.d + hk)) = u32x2{pc.first, pc.pieces};
             }
         }
-        if (!whole && pe.count) {
-            // ---- the last workgroup of the segment merges its pieces; none waits for another
-            __builtin_amdgcn_s_waitcnt(0x0F70);   // vmcnt(0): this wave's partials are in memory
-            __syncthreads();
-            if (tid == 0) {
-                unsigned* cnt = pe.count + (pc.item * pe.a.c.kvh + hk);
-                last = atomicAdd_system(cnt, 1u) + 1 == pc.pieces;
-                if (last) atomicExch_system(cnt, 0u);
-            }
-            __syncthreads();
-            if (last) paged_merge<DT, CT>(pe, pc.item, hk, pc.first, pc.pieces, reinterpret_cast<char*>(red));
-        }
-        if (more_pieces) {
-            x += pc.c1 - pc.c0;
-            more_pieces = x < stop;
-            // the next segment: the item's next head, or the next item's first
-            at = (uint32_t)(hk + 1) * (uint32_t)sp.tiles;
-            if (hk + 1 == pe.a.c.kvh) {
-                ++pc.item;
-                at = 0;
-            }
+    }
+    if constexpr (WAVES > 1) {
+#pragma unroll 1
+        for (int i = 0; i < 2; ++i) {
+            if (!(parts >> i & 1)) continue;
+            const PagedPiece& q = part[0];
+            const int item = i ? part[1].item : q.item, hk = i ? part[1].hk : q.hk;
+            const uint32_t first = i ? part[1].first : q.first, pieces = i ? part[1].pieces : q.pieces;
+            paged_join<DT, CT>(paged_args(), item, hk, first, pieces, wg - first, reinterpret_cast<char*>(red), &flag);
         }
     }
 }
 
-// The merge as a launch of its own: a workgroup a segment.
+// The join as a launch of its own: a workgroup a segment, or one of `slices` that take its rows in turn. A row's quads of
+// columns are shared by as many threads as there are, every so-manieth run to each.
+constexpr int PM_JOIN_THREADS = 512;
 template <int DT, int CT>
-__global__ __launch_bounds__(64 * PM_WAVES) void paged_attn_merge_kernel(PagedMfmaArgs p) {
-    __shared__ __attribute__((aligned(16))) char lds[PM_MERGE_BYTES];
-    const int item = blockIdx.x / p.a.c.kvh, hk = blockIdx.x % p.a.c.kvh, lane = threadIdx.x % 64;
-    const PagedDeal deal = paged_deal<CT>(p, lane);
-    const uint32_t tiles = (uint32_t)paged_span<CT>(p, item).tiles, units = deal.units(tiles);
-    PagedPiece pc;
-    const uint32_t begin = paged_before<CT>(p, deal, item, lane) * (uint32_t)p.a.c.kvh + (uint32_t)hk * units;
-    if (deal.chunk) {
-        pc.first = begin;
-        pc.pieces = units;
-    } else {
-        paged_pieces(deal, begin, tiles, pc);
+__global__ __launch_bounds__(PM_JOIN_THREADS) void paged_attn_join_kernel(PagedMfmaArgs p) {
+    constexpr int RUNS = 32;   // paged_runs
+    __shared__ f32x4 o[RUNS * 64];
+    __shared__ f32x2v ml[RUNS * 64];
+    const uint32_t slice = blockIdx.x % (uint32_t)p.slices, id = blockIdx.x / (uint32_t)p.slices;
+    const uint32_t first = p.seg[2 * (int64_t)id], pieces = p.seg[2 * (int64_t)id + 1];
+    if (pieces == 1) return;
+    const PagedParts<CT, false> parts(p);
+    const int item = (int)div32(id, p.kvh), hk = (int)(id - item * p.kvh.d);
+    const int b = (int)div32((uint32_t)item, p.nrb), r0 = (item - b * (int)p.nrb.d) * 16 * CT;
+    const int nr = min(16 * CT, p.rows - r0), quads = p.a.c.hd / 4, share = PM_JOIN_THREADS / quads;
+    const int part = threadIdx.x / quads, c = threadIdx.x - part * quads;
+    const PagedRuns r = paged_runs(pieces, nr * quads);
+    for (int lr = slice; lr < nr; lr += p.slices) {
+        __syncthreads();   // the row before has been read
+        PagedSum s;
+        for (uint32_t run = part; part < share && run < r.n; run += share) {
+            s = parts.run(first, r.at(run), r.at(run + 1), lr, 4 * c);
+            o[run * quads + c] = s.o;
+            ml[run * quads + c] = f32x2v{s.m, s.l};
+        }
+        __syncthreads();
+        if (part) continue;
+        if (r.n > 1) s = paged_runs_lds(o + c, ml + c, r.n, quads);
+        PagedRow(p, b, hk, r0 + lr, s.m, s.l).template store<DT>(p, 4 * c, s.o);
     }
-    if (pc.pieces > 1) paged_merge<DT, CT>(p, item, hk, pc.first, pc.pieces, lds);
 }
 
 constexpr int PM_CUS = 256;
+// Keys of a segment, in tiles of 32, up to which it takes one wave and one workgroup. A wave spares the merge of four
+// (float16 98 x 64/8 heads x 16 keys of 128: 6.0 us, 10.9 with four) and takes the tiles one after another. More segments
+// than run together wait less for shorter workgroups; segments that fill a third of the chip have no use for being cut
+// (bfloat16 52 x 64/16 heads x 743 keys of 64: 20.9 us whole, 24.3 in pieces), few long ones do (float32 6 x 32/8 heads x
+// 640 keys of 256: 16 us in pieces, 35 whole).
+constexpr int PM_WAVE = 2, PM_WAVE_MANY = 4, PM_WHOLE = 17, PM_WHOLE_MANY = 33;
+constexpr double PM_MANY = 0.35;
+// Quads of columns and pieces of an average segment up to which its last workgroup joins it: beyond, the second launch's
+// many workgroups are faster (float16 1 x 16/4 heads, 4 tokens, 32576 keys of 128: 22 us, 28 joined by the last ones).
+constexpr double PM_JOIN_ALONE = 4096;
 
 template <int DT, bool F8, int D, int CT>
 void paged_launch(PagedMfmaArgs& p, int64_t batch, hipStream_t s) {
     typedef PagedTile<DT, F8, D> G;
-    p.nrb = (p.rows + 16 * CT - 1) / (16 * CT);
-    p.items = (int)(batch * p.nrb);
+    const int nrb = (p.rows + 16 * CT - 1) / (16 * CT);
+    p.nrb = make_div((uint32_t)nrb);
+    p.kp = (uint32_t)(p.a.c.sk[0] * G::ES / 16);
+    p.ks = (uint32_t)(p.a.c.sk[1] * G::ES / 16);
+    p.vp = (uint32_t)(p.a.c.sv[0] * G::ES / 16);
+    p.vs = (uint32_t)(p.a.c.sv[1] * G::ES / 16);
+    p.kvh = make_div((uint32_t)p.a.c.kvh);
+    p.group = make_div((uint32_t)p.a.group);
+    p.items = (int)(batch * nrb);
     const int64_t segments = (int64_t)p.items * p.a.c.kvh;
-    // a workgroup for every 4 tiles the sequences may have, as many as are resident together
-    const int64_t tiles = ((int64_t)p.a.max_len + PM_BN - 1) / PM_BN + 1;
-    const int64_t most = (int64_t)PM_CUS * G::occ(CT);
-    int64_t wgs = tiles / PM_WAVES > most ? most : std::min<int64_t>(most, segments * (tiles / PM_WAVES));
+    const bool fast = p.a.c.page.d % 16 == 0 && p.a.c.hd * G::ES == G::KL * 64;
+    const int64_t keys = p.a.window ? std::min<int64_t>(p.a.max_len, (int64_t)p.a.window + p.a.new_tokens + G::BN) : p.a.max_len;
+    const int64_t tiles = (keys + G::BN - 1) / G::BN;   // at most, of a segment
+    p.resident = PM_CUS * G::occ(CT);
+    if (tiles * G::BN <= 32 * (segments > p.resident ? PM_WAVE_MANY : PM_WAVE)) {
+        const dim3 grid((unsigned)segments), block(64);
+        if (fast) hipLaunchKernelGGL((paged_attn_mfma_kernel<DT, F8, D, CT, true, 1>), grid, block, 0, s, p);
+        else hipLaunchKernelGGL((paged_attn_mfma_kernel<DT, F8, D, CT, false, 1>), grid, block, 0, s, p);
+        return;
+    }
     Scratch scratch;
-    if (wgs > 0 && (tiles / PM_WAVES > 1)) {
-        const size_t rows = (size_t)2 * wgs * 16 * CT, bytes = rows * (p.a.c.hd + 2) * 4;
-        float* part = s == hipStreamPerThread ? nullptr : static_cast<float*>(scratch.get(bytes, s));
+    p.many = segments > p.resident * PM_MANY;
+    if (tiles * G::BN > 32 * (p.many ? PM_WHOLE_MANY : PM_WHOLE)) {
+        // a workgroup for every 4 tiles the sequences may have, as many as are resident together, or what paged_deal's
+        // chunks may come to
+        const int64_t wgs = p.many ? segments + 2 * p.resident : std::min<int64_t>(p.resident, segments * (tiles / PM_WAVES));
+        const size_t rows = (size_t)2 * wgs * 16 * CT, bytes = rows * (p.a.c.hd + 4) * 4;
+        float* part = s == hipStreamPerThread || bytes >= (size_t)1 << 31
+                          ? nullptr : static_cast<float*>(scratch.get(bytes + (size_t)segments * 8, s));
         if (part) {
             p.wgs = (int)wgs;
             p.part_o = part;
             p.part_ml = part + rows * p.a.c.hd;
             p.part_bytes = (unsigned)bytes;
-            p.count = split_counters(s, segments);
+            p.seg = reinterpret_cast<uint32_t*>(p.part_ml + rows * 4);
+            const double wide = std::max(1.0, (double)p.resident / segments) * std::min(p.rows, 16 * CT) * p.a.c.hd / 4;
+            p.count = wide > PM_JOIN_ALONE ? nullptr : split_counters(s, segments + 2 * wgs);
         } else {
             clear_error();
         }
     }
     const dim3 grid((unsigned)(p.wgs ? p.wgs : segments)), block(64 * PM_WAVES);
-    if (p.a.c.page.d % 16 == 0 && p.a.c.hd * G::ES == G::KL * 64) hipLaunchKernelGGL((paged_attn_mfma_kernel<DT, F8, D, CT, true>), grid, block, 0, s, p);
-    else hipLaunchKernelGGL((paged_attn_mfma_kernel<DT, F8, D, CT, false>), grid, block, 0, s, p);
-    if (p.wgs && !p.count)
-        hipLaunchKernelGGL((paged_attn_merge_kernel<DT, CT>), dim3((unsigned)segments), block, 0, s, p);
+    if (fast) hipLaunchKernelGGL((paged_attn_mfma_kernel<DT, F8, D, CT, true, PM_WAVES>), grid, block, 0, s, p);
+    else hipLaunchKernelGGL((paged_attn_mfma_kernel<DT, F8, D, CT, false, PM_WAVES>), grid, block, 0, s, p);
+    if (p.wgs && !p.count) {
+        p.slices = (int)std::min<int64_t>(std::min(p.rows, 16 * CT), std::max<int64_t>(1, 2048 / segments));
+        hipLaunchKernelGGL((paged_attn_join_kernel<DT, CT>), dim3((unsigned)(segments * p.slices)), dim3(PM_JOIN_THREADS), 0, s, p);
+    }
 }
 
 template <int DT, bool F8>
