@@ -181,3 +181,30 @@ def test_norm_backward_formula_is_the_forwards_derivative(with_dh):
             down.view(-1)[i] -= step
             diff = (loss(up, w) - loss(down, w)) if t is x else (loss(x, up) - loss(x, down))
             assert abs(diff / (2 * step) - grad.reshape(-1)[i]) < 1e-8
+
+
+def test_cache_bookkeeping_on_the_host():
+    from torchvulkan_amd import decoder
+
+    cache = decoder.PagedKVCache(2, 5, 4, 1, 8, torch.float32, "cpu", max_len=16)
+    cache.extend([5, 1])
+    assert cache.lens.tolist() == [5, 1] and (cache.table >= 0).sum(1).tolist() == [2, 1]
+    for bad in ([1], [-1, 0], [12, 0]):
+        with pytest.raises(_abi.TvkError) as e:
+            cache.extend(bad)
+        assert e.value.status == _abi.TVK_ERR_INVALID
+    with pytest.raises(_abi.TvkError) as e:
+        cache.extend([8, 4])   # a page more than there are
+    assert e.value.status == _abi.TVK_ERR_OOM
+    assert cache.lens.tolist() == [5, 1] and (cache.table >= 0).sum() == 3
+    cache.release(0)
+    cache.extend([0, 15])
+    assert cache.lens.tolist() == [0, 16] and sorted(cache.table[1].tolist()) == sorted(set(cache.table[1].tolist()))
+    assert (cache.table[0] == -1).all()
+    with pytest.raises(_abi.TvkError):
+        decoder.PagedKVCache(0, 5, 4, 1, 8)
+    x = torch.zeros((2, 4))
+    with pytest.raises(_abi.TvkError):
+        decoder.rms_norm(x)   # not on a device
+    with pytest.raises(_abi.TvkError):
+        decoder.rms_norm(x, residual=torch.zeros((2, 5)))

@@ -11,7 +11,9 @@ The module also provides the reference's device API subset: is_available,
 device_count, current_device, set_device, synchronize, empty_cache,
 memory_allocated, max_memory_allocated, memory_reserved, mem_get_info,
 reset_peak_memory_stats, memory_stats, get_device_properties, get_device_name,
-manual_seed (torchvulkan/__init__.py:32-166).
+manual_seed (torchvulkan/__init__.py:32-166). torchvulkan_amd.decoder has the
+operators of a decoder's block that the reference composes or lacks: the
+root-mean-square norm and a paged key/value cache with its attention.
 """
 from __future__ import annotations
 
@@ -174,3 +176,5 @@ def _tensor_to_vulkan(self, device=None, non_blocking=False, **kwargs) -> torch.
 torch.Tensor.vulkan = _tensor_to_vulkan
 torch.Tensor.is_vulkan = property(lambda self: self.device.type == "vulkan")
 torch.utils.generate_methods_for_privateuse1_backend(for_tensor=False)
+
+from . import decoder  # noqa: E402,F401  (the norm and the paged key/value cache)

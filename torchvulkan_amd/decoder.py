@@ -1,0 +1,174 @@
+"""The decoder block's operators as a program uses them: the root-mean-square
+norm with its gradients, and a paged key/value cache that prompts and new tokens
+are appended to and attended over. Tensors of the vulkan device or of "cuda"; the
+calls are queued on the tensors' device's current stream. The reference composes
+these operators from element-wise shaders and keeps dense caches."""
+from __future__ import annotations
+
+import ctypes as C
+
+import torch
+
+from . import _abi
+
+__all__ = ["rms_norm", "rms_norm_fp8", "rotary_table", "PagedKVCache"]
+
+
+def _stream(t: torch.Tensor):
+    if t.device.type == "cuda":
+        return torch.cuda.current_stream(t.device).cuda_stream
+    if t.device.type != "vulkan":
+        raise _abi.TvkError(_abi.TVK_ERR_INVALID, f"a tensor on {t.device}: the decoder's operators run on vulkan or cuda devices")
+    s = C.c_void_p()
+    _abi.check(_abi.load().tvk_get_stream(t.device.index or 0, C.byref(s)))
+    return s.value
+
+
+def _rows(t: torch.Tensor) -> torch.Tensor:
+    """[..., cols] as [rows, cols] with contiguous rows (a copy only where the strides allow no view)."""
+    t = t.reshape(-1, t.shape[-1])
+    return t if t.shape[-1] <= 1 or t.stride(1) == 1 else t.contiguous()
+
+
+class _RmsNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, residual, eps):
+        shape, x2 = x.shape, _rows(x)
+        r2 = None if residual is None else _rows(residual)
+        y = torch.empty(x2.shape, dtype=x.dtype, device=x.device)
+        h = x2 if r2 is None else torch.empty(x2.shape, dtype=x.dtype, device=x.device)
+        d = _abi.make_rms_norm_desc(x2, weight, y, r2, None if r2 is None else h, None, eps, _stream(x))
+        _abi.check(_abi.load().tvk_rms_norm_fwd(C.byref(d)))
+        ctx.save_for_backward(h, weight)
+        ctx.eps, ctx.shape, ctx.added = eps, shape, r2 is not None
+        if r2 is None:
+            return y.view(shape), None
+        return y.view(shape), h.view(shape)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy, dh):
+        h, weight = ctx.saved_tensors
+        dy2 = torch.zeros(h.shape, dtype=h.dtype, device=h.device) if dy is None else _rows(dy)
+        dh2 = None if dh is None else _rows(dh)
+        dx = torch.empty(h.shape, dtype=h.dtype, device=h.device)
+        dw = torch.empty(weight.shape, dtype=weight.dtype, device=weight.device) \
+            if weight is not None and ctx.needs_input_grad[1] else None
+        d = _abi.make_rms_norm_bwd_desc(dy2, h, weight, dx, dw, dh2, ctx.eps, _stream(h))
+        _abi.check(_abi.load().tvk_rms_norm_bwd(C.byref(d)))
+        dx = dx.view(ctx.shape)
+        return dx, dw, dx if ctx.added else None, None
+
+
+def _check_norm(x, weight, residual) -> None:
+    if x.dim() == 0 or (residual is not None and (residual.shape != x.shape or residual.dtype != x.dtype)):
+        raise _abi.TvkError(_abi.TVK_ERR_INVALID, "x: [..., cols], and a residual of its shape and dtype, are expected")
+    for t in (weight, residual):
+        if t is not None and t.device != x.device:
+            raise _abi.TvkError(_abi.TVK_ERR_INVALID, f"tensors on {x.device} and {t.device}")
+
+
+def rms_norm(x, weight=None, residual=None, eps: float = 1e-5):
+    """x / sqrt(mean(x^2) + eps) * weight over the last dimension; with a residual (y, h) of h = x + residual.
+    Differentiable in x, weight and residual (tvk_rms_norm_fwd, tvk_rms_norm_bwd)."""
+    _check_norm(x, weight, residual)
+    y, h = _RmsNorm.apply(x, weight, residual, float(eps))
+    return y if residual is None else (y, h)
+
+
+def rms_norm_fp8(x, weight=None, residual=None, eps: float = 1e-5):
+    """(y, scale, h): the norm in float8_e4m3fn with a float32 scale for each row, y * scale[..., None] being the norm;
+    h is x without a residual. No gradient."""
+    _check_norm(x, weight, residual)
+    x2 = _rows(x.detach())
+    y = torch.empty(x2.shape, dtype=torch.float8_e4m3fn, device=x.device)
+    scale = torch.empty(x2.shape[0], dtype=torch.float32, device=x.device)
+    r2 = None if residual is None else _rows(residual.detach())
+    h = None if r2 is None else torch.empty(x2.shape, dtype=x.dtype, device=x.device)
+    d = _abi.make_rms_norm_desc(x2, weight, y, r2, h, scale, eps, _stream(x))
+    _abi.check(_abi.load().tvk_rms_norm_fwd(C.byref(d)))
+    return y.view(x.shape), scale.view(x.shape[:-1]), x if h is None else h.view(x.shape)
+
+
+def rotary_table(positions: int, rotary_dim: int, base: float = 10000.0, device="cpu") -> torch.Tensor:
+    """The angles of positions 0 .. positions - 1: float32 [positions, rotary_dim], cosines then sines, from 64 bits."""
+    angle = torch.arange(positions, dtype=torch.float64)[:, None] * torch.pow(
+        torch.tensor(base, dtype=torch.float64), -torch.arange(0, rotary_dim, 2, dtype=torch.float64) / rotary_dim)
+    return torch.cat([angle.cos(), angle.sin()], 1).float().to(device)
+
+
+class PagedKVCache:
+    """Keys and values of up to `batch` sequences in `pages` pages of `page_size` slots, in each of a model's layers: the
+    layers share the lengths and the pages' places.
+
+    The host keeps the sequences' lengths and free pages; extend() gives sequences new positions, release() ends one.
+    Both only write the device's `table` and `lens`, which the calls read there, so a captured step (append, attend)
+    replays for other lengths. dtype float8_e4m3fn keeps 8 bits, divided by k_scale and v_scale of each head."""
+
+    def __init__(self, batch: int, pages: int, page_size: int, heads_kv: int, head_dim: int, dtype=torch.bfloat16, device="cuda",
+                 max_len: int | None = None, layers: int = 1, k_scale=None, v_scale=None):
+        if min(batch, pages, page_size, heads_kv, head_dim, layers) <= 0:
+            raise _abi.TvkError(_abi.TVK_ERR_INVALID, "PagedKVCache: sizes must be above zero")
+        self.page_size, self.max_len = page_size, int(max_len or pages * page_size)
+        self.k, self.v = (torch.empty((layers, pages, page_size, heads_kv, head_dim), dtype=dtype, device=device)
+                          for _ in range(2))
+        self.k_scale, self.v_scale = k_scale, v_scale
+        width = -(-self.max_len // page_size)
+        self._table = torch.full((batch, width), -1, dtype=torch.int32)
+        self._lens = torch.zeros(batch, dtype=torch.int32)
+        self._free = list(range(pages - 1, -1, -1))
+        self.table, self.lens = self._table.to(device), self._lens.to(device)
+
+    def length(self, b: int) -> int:
+        return int(self._lens[b])
+
+    def extend(self, new) -> None:
+        """Adds new[b] positions (an int: the same for all) to every sequence, with pages for them; raises and changes
+        nothing where a sequence would pass max_len or the pages run out."""
+        counts = [int(new)] * len(self._lens) if isinstance(new, int) else [int(n) for n in new]
+        if len(counts) != len(self._lens) or min(counts) < 0:
+            raise _abi.TvkError(_abi.TVK_ERR_INVALID, "extend: a count of at least zero for each sequence is expected")
+        ends = [self.length(b) + n for b, n in enumerate(counts)]
+        if max(ends) > self.max_len:
+            raise _abi.TvkError(_abi.TVK_ERR_INVALID, f"extend: a sequence of {max(ends)} positions, the cache's longest are {self.max_len}")
+        have = [-(-self.length(b) // self.page_size) for b in range(len(ends))]
+        need = [-(-end // self.page_size) for end in ends]
+        if sum(need) - sum(have) > len(self._free):
+            raise _abi.TvkOutOfMemory(_abi.TVK_ERR_OOM, f"extend: {sum(need) - sum(have)} pages are wanted, {len(self._free)} are free")
+        for b, end in enumerate(ends):
+            for i in range(have[b], need[b]):
+                self._table[b, i] = self._free.pop()
+            self._lens[b] = end
+        self._sync(sum(need) != sum(have))
+
+    def release(self, b: int) -> None:
+        """Ends sequence b: its pages are free again and its slot of the batch is empty."""
+        for i in range(-(-self.length(b) // self.page_size)):
+            self._free.append(int(self._table[b, i]))
+            self._table[b, i] = -1
+        self._lens[b] = 0
+        self._sync(True)
+
+    def _sync(self, table: bool) -> None:
+        if table:
+            self.table.copy_(self._table)
+        self.lens.copy_(self._lens)
+
+    def append(self, q, k, v, rotary=None, interleaved: bool = False, out=None, layer: int = 0):
+        """Writes the newest positions' keys and values, rotated as `rotary` says, and returns their rotated queries
+        (tokens [batch, new, heads, head_dim]; sequences with fewer new positions are padded in front). out may be q."""
+        out = torch.empty(q.shape, dtype=q.dtype, device=q.device) if out is None and q is not None else out
+        d = _abi.make_paged_append_desc(q, k, v, out, self.k[layer], self.v[layer], self.lens, self.table, rotary, interleaved,
+                                        self.k_scale, self.v_scale, _stream(k))
+        _abi.check(_abi.load().tvk_paged_append(C.byref(d)))
+        return out
+
+    def attend(self, q, scale: float | None = None, window: int = 0, out=None, max_len: int | None = None, layer: int = 0):
+        """Attention of the newest positions' queries over their sequences. max_len: a bound on the lengths, for a call
+        that is captured and replayed; else the longest sequence's."""
+        out = torch.empty(q.shape, dtype=q.dtype, device=q.device) if out is None else out
+        d = _abi.make_paged_attention_desc(q, self.k[layer], self.v[layer], out, self.lens, self.table,
+                                           max_len or max(1, int(self._lens.max())), scale, window, self.k_scale, self.v_scale,
+                                           stream=_stream(q))
+        _abi.check(_abi.load().tvk_paged_attention(C.byref(d)))
+        return out
