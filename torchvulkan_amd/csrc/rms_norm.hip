@@ -29,7 +29,7 @@ struct NormArgs {
     float* scale;
     int64_t sx, sr, so, sh;   // row strides, elements
     int64_t rows, cols;
-    float eps;
+    float eps, rcols;
     int w32, out8;
 };
 
@@ -39,10 +39,11 @@ struct NormBwdArgs {
     const void* dh;
     const void* w;
     void* dx;
+    void* dw;      // of a single workgroup, which needs no partials; or NULL
     float* inv;    // [rows], or NULL
     int64_t sdy, sh, sdh, sdx;
     int64_t rows, cols;
-    float eps;
+    float eps, rcols;
     int w32;
 };
 
@@ -234,6 +235,13 @@ __device__ __forceinline__ int row_of_thread() {
     return TPR < 64 ? threadIdx.x / TPR : __builtin_amdgcn_readfirstlane(threadIdx.x / TPR);
 }
 
+// 1 / sqrt(ss / cols + eps), rcols being 1 / cols: the reciprocal square root instruction is within a step of float32 where
+// its argument is not near float32's ends.
+__device__ __forceinline__ float inv_rms(float ss, float rcols, float eps) {
+    const float x = fmaf(ss, rcols, eps);
+    return x > 1e-30f && x < 1e30f ? __builtin_amdgcn_rsqf(x) : 1.0f / sqrtf(x);
+}
+
 constexpr int row_threads(int tpr) { return tpr < RN_THREADS ? RN_THREADS : tpr; }
 
 // What a thread holds of a row: chunk i is the row's chunk t + TPR * i; then, in t < tail, one of the values past them.
@@ -338,7 +346,7 @@ __global__ __launch_bounds__(row_threads(TPR)) void rms_norm_kernel(NormArgs p) 
         if (OUT8) row_all<TPR, SumOp, MaxOp>(ss, top, turn);
         else row_all<TPR, SumOp, SumOp>(ss, top, turn);
         turn ^= 1;
-        const float inv = 1.0f / sqrtf(ss / (float)p.cols + p.eps);
+        const float inv = inv_rms(ss, p.rcols, p.eps);
         if (p.h) {
             T* o = static_cast<T*>(p.h) + row * p.sh;
 #pragma unroll
@@ -350,7 +358,7 @@ __global__ __launch_bounds__(row_threads(TPR)) void rms_norm_kernel(NormArgs p) 
             // y = h w inv; its largest magnitude is max|h w| times inv, and y / scale = h w (inv / scale). An inv / scale
             // that leaves float32's range, for rows of values near its ends, is not taken as one factor.
             top *= inv;
-            const float s = top > 0.0f ? top / kF8Max : 1.0f, f8 = inv / s;
+            const float s = top > 0.0f ? top / kF8Max : 1.0f, f8 = inv * __builtin_amdgcn_rcpf(s);
             const bool plain = f8 < 1e30f && f8 > 1e-30f;
             const float a = plain ? f8 : inv, b = plain ? 1.0f : s;
             if (t == 0) p.scale[row] = s;
@@ -446,8 +454,8 @@ __global__ __launch_bounds__(THREADS) void rms_norm_bwd_kernel(NormBwdArgs p, fl
         x.packed();
         add.packed();
         w.r.packed();
-        const float inv = 1.0f / sqrtf(ss / (float)p.cols + p.eps);
-        const float mean = gh * inv / (float)p.cols;   // of g * n
+        const float inv = inv_rms(ss, p.rcols, p.eps);
+        const float mean = gh * inv * p.rcols;   // of g * n
 #pragma unroll
         for (int i = 0; i < NC; ++i) {
             float f[VEC], o[VEC];
@@ -469,30 +477,37 @@ __global__ __launch_bounds__(THREADS) void rms_norm_bwd_kernel(NormBwdArgs p, fl
             dx[VEC * chunks + t] = elem<DT>::from_f32(o);
         }
     }
-    if (!part) return;
+    if (!part && !p.dw) return;
     float* out = part + (int64_t)blockIdx.x * p.cols;
-    if constexpr (SUBS == 1) {
+    // chunks of floats, to a partial or LDS; a single workgroup's sums to dweight itself
+    auto put_sum = [&](int c, float v) {
+        if (!p.dw) out[c] = v;
+        else if (p.w32) static_cast<float*>(p.dw)[c] = v;
+        else put<DT>(p.dw, c, v);
+    };
+    auto put_chunks = [&](float* to) {
 #pragma unroll
         for (int i = 0; i < NC; ++i)
             if (t + TPR * i < chunks)
 #pragma unroll
-                for (int k = 0; k < VEC; ++k) out[VEC * (t + TPR * i) + k] = acc[i][k];
-        if (t < tail) out[VEC * chunks + t] = acc_last;
-    } else {
-        __shared__ float sum[SUBS][VEC * (NC * TPR + 1)];
+                for (int k = 0; k < VEC; k += 4) {
+                    const float four[4] = {acc[i][k], acc[i][k + 1], acc[i][k + 2], acc[i][k + 3]};
+                    store_words<16, 4>(to + (uint32_t)(VEC * (t + TPR * i) + k), pack<TVK_F32, 4>(four));
+                }
+        if (t < tail) to[VEC * chunks + t] = acc_last;
+    };
+    if (SUBS == 1 && !p.dw) {
+        put_chunks(out);
+        return;
+    }
+    __shared__ __attribute__((aligned(16))) float sum[SUBS][VEC * (NC * TPR + 1)];
+    put_chunks(sum[sub]);
+    __syncthreads();
+    for (int c = threadIdx.x; c < (int)p.cols; c += THREADS) {
+        float v = sum[0][c];
 #pragma unroll
-        for (int i = 0; i < NC; ++i)
-            if (t + TPR * i < chunks)
-#pragma unroll
-                for (int k = 0; k < VEC; ++k) sum[sub][VEC * (t + TPR * i) + k] = acc[i][k];
-        if (t < tail) sum[sub][VEC * chunks + t] = acc_last;
-        __syncthreads();
-        for (int c = threadIdx.x; c < (int)p.cols; c += THREADS) {
-            float v = sum[0][c];
-#pragma unroll
-            for (int i = 1; i < SUBS; ++i) v += sum[i][c];
-            out[c] = v;
-        }
+        for (int i = 1; i < SUBS; ++i) v += sum[i][c];
+        put_sum(c, v);
     }
 }
 
@@ -529,14 +544,15 @@ __global__ __launch_bounds__(FOLD_COLS * FOLD_ROWS) void rms_norm_fold_kernel(co
 // Calls f(NC, TPR) for rows of `chunks` whole chunks; false past what registers hold. At most two chunks a thread: more
 // take the registers of the waves that hide the row's latency (bfloat16 16384 x 4096 to 8 bits: 82 us with two chunks in
 // 256 threads, 197 with eight in a wave). A wave with two chunks beats four waves with half of one each where rows are many
-// (float16 2000 x 1024: 4.5 us, 5.4), and loses where they are few.
+// (float16 2000 x 1024: 4.5 us, 5.4), and loses where they are few; backward, where it halves the partials too, from fewer rows
+// on (1000 x 777: 8.5 us, 9.1).
 template <class F>
-bool row_shape(int64_t rows, int64_t chunks, F&& f) {
+bool row_shape(int64_t rows, int64_t few, int64_t chunks, F&& f) {
 #define TVK_ROW(nc, tpr) return f(std::integral_constant<int, nc>{}, std::integral_constant<int, tpr>{}), true
     if (chunks <= 16) TVK_ROW(1, 16);
     if (chunks <= 32) TVK_ROW(2, 16);
     if (chunks <= 64) TVK_ROW(1, 64);
-    if (chunks <= 128 && rows > 1024) TVK_ROW(2, 64);
+    if (chunks <= 128 && rows > few) TVK_ROW(2, 64);
     if (chunks <= 256) TVK_ROW(1, 256);
     if (chunks <= 512) TVK_ROW(2, 256);
     if (chunks <= 1024) TVK_ROW(2, 512);
@@ -547,7 +563,7 @@ bool row_shape(int64_t rows, int64_t chunks, F&& f) {
 
 template <int DT>
 void forward(const NormArgs& p, hipStream_t s) {
-    const bool done = row_shape(p.rows, p.cols * (int64_t)dtype_size(DT) / 16, [&](auto nc, auto tpr) {
+    const bool done = row_shape(p.rows, 1024, p.cols * (int64_t)dtype_size(DT) / 16, [&](auto nc, auto tpr) {
         constexpr int NC = decltype(nc)::value, TPR = decltype(tpr)::value, SUBS = row_threads(TPR) / TPR;
         const dim3 grid((unsigned)std::min<int64_t>((p.rows + SUBS - 1) / SUBS, 1 << 20)), block(row_threads(TPR));
         if (p.out8) hipLaunchKernelGGL((rms_norm_kernel<DT, true, NC, TPR>), grid, block, 0, s, p);
@@ -568,10 +584,11 @@ tvk_status backward(NormBwdArgs p, void* dw, hipStream_t s) {
         return part != nullptr;
     };
     bool have = true;
-    const bool done = row_shape(p.rows, p.cols * (int64_t)dtype_size(DT) / 16, [&](auto nc, auto tpr) {
+    const bool done = row_shape(p.rows, 256, p.cols * (int64_t)dtype_size(DT) / 16, [&](auto nc, auto tpr) {
         constexpr int NC = decltype(nc)::value, TPR = decltype(tpr)::value, THREADS = bwd_threads(TPR), SUBS = THREADS / TPR;
         const int64_t groups = std::min<int64_t>((p.rows + SUBS - 1) / SUBS, RN_BWD_THREADS / THREADS);
-        have = partials(groups, 0);
+        if (dw && groups == 1) p.dw = dw;
+        else have = partials(groups, 0);
         if (have && p.rows > 0)
             hipLaunchKernelGGL((rms_norm_bwd_kernel<DT, NC, TPR, THREADS>), dim3((unsigned)groups), dim3(THREADS), 0, s, p, part);
     });
@@ -587,7 +604,7 @@ tvk_status backward(NormBwdArgs p, void* dw, hipStream_t s) {
         if (have && p.rows > 0) hipLaunchKernelGGL((rms_norm_bwd_any_kernel<DT>), dim3((unsigned)p.rows), dim3(RN_THREADS), 0, s, p);
     }
     if (!have) return fail(TVK_ERR_OOM, "tvk_rms_norm_bwd: workspace allocation failed");
-    if (dw)
+    if (dw && !p.dw)
         hipLaunchKernelGGL((rms_norm_fold_kernel<DT>), dim3((unsigned)((p.cols + FOLD_COLS - 1) / FOLD_COLS)),
                            dim3(FOLD_COLS * FOLD_ROWS), 0, s, part, parts, p.cols, dw, p.w32);
     return TVK_OK;
@@ -638,6 +655,7 @@ extern "C" tvk_status tvk_rms_norm_fwd(const tvk_rms_norm_desc* d) {
     p.rows = d->rows;
     p.cols = d->cols;
     p.eps = (float)d->eps;
+    p.rcols = 1.0f / (float)d->cols;
     p.w32 = d->weight_dtype == TVK_F32;
     p.out8 = out8;
     const hipStream_t s = resolve_stream(d->stream);
@@ -672,6 +690,7 @@ extern "C" tvk_status tvk_rms_norm_bwd(const tvk_rms_norm_bwd_desc* d) {
     p.rows = d->rows;
     p.cols = d->cols;
     p.eps = (float)d->eps;
+    p.rcols = 1.0f / (float)d->cols;
     p.w32 = d->weight_dtype == TVK_F32;
     const hipStream_t s = resolve_stream(d->stream);
     if (d->dtype == TVK_F32) st = backward<TVK_F32>(p, d->dweight, s);
