@@ -168,6 +168,30 @@ def test_dims(gpu, dim, dtype):
     check_attention(cache, rand((4, 2, 6, dim), dtype, 1), what=f"D {dim} {dtype} 8 bits")
 
 
+# pages of whole 16-key blocks, whose rows are read by other code, in each way of dealing: a wave a sequence, a workgroup, and
+# pieces that are joined. What lies around the output's rows is not the call's.
+@pytest.mark.parametrize("dim", [1, 16, 32, 48, 64, 80, 96, 112, 128, 160, 192, 224, 256, 264])
+@pytest.mark.parametrize("lens,hkv", [([60, 5, 0, 33], 2), ([300, 70, 0, 400], 2), ([3000, 40], 1)])
+@pytest.mark.parametrize("dtype", [HALF, BF16, torch.float32])
+def test_dims_in_whole_pages(gpu, dim, lens, hkv, dtype):
+    for new, cache_dtype in ((1, dtype), (3, dtype), (1, F8)):
+        what = f"D {dim} {dtype} {cache_dtype} {lens} {new}"
+        cache = Cache(lens, 16, hkv, dim, cache_dtype, seed=dim, stale=float("nan"))
+        q = rand((len(lens), new, 3 * hkv, dim), dtype, 1)
+        want, _, tol = attention_oracle(q, cache, dim ** -0.5)
+        args, scales = cache.dev()
+        qd = q.to(DEV)
+        around = torch.full((len(lens), new, 3 * hkv + 2, dim + 16), 7.0, dtype=dtype, device=DEV)
+        out = around[:, :, 1:-1, 8:8 + dim]
+        d = _abi.make_paged_attention_desc(qd, args[0], args[1], out, args[2], args[3],
+                                           stream=torch.cuda.current_stream().cuda_stream, **scales)
+        _abi.check(_abi.load().tvk_paged_attention(C.byref(d)))
+        torch.cuda.synchronize()
+        close(out, want, tol, what)
+        out.fill_(7.0)
+        assert around.eq(7.0).all(), what + ": values around the output's rows were written"
+
+
 # rows of one key/value head: 1 to several row blocks; tokens in front of a sequence's start see nothing
 @pytest.mark.parametrize("hq,hkv,new", [(1, 1, 1), (3, 1, 5), (8, 8, 1), (16, 1, 1), (17, 1, 1), (33, 1, 1), (8, 2, 7),
                                         (4, 2, 16), (64, 2, 2), (6, 3, 40)])

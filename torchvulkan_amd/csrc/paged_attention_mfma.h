@@ -935,7 +935,7 @@ __global__ __launch_bounds__(64 * WAVES, (PagedTile<DT, F8, D>::occ(CT))) void p
                     for (int i = 0; i < EV; i += 4) {
                         const int dv = EV * (4 * g + r) + i;
                         f32x4 o = f32x4{oacc[i][ct][r], oacc[i + 1][ct][r], oacc[i + 2][ct][r], oacc[i + 3][ct][r]};
-                        if (!FAST && dv >= pe.a.c.hd) continue;
+                        if ((!FAST || DV != D) && dv >= pe.a.c.hd) continue;
                         if (__builtin_expect(mark, 0)) o = marked(lr, dv, o);
                         row.template store<DT>(pe, dv, o);
                     }
@@ -960,7 +960,7 @@ __global__ __launch_bounds__(64 * WAVES, (PagedTile<DT, F8, D>::occ(CT))) void p
             __syncthreads();
             for (int c = tid; c < min(COLS, pe.rows - r0) * (DV / 4); c += 64 * WAVES) {
                 const int lr = c / (DV / 4), dv = (c % (DV / 4)) * 4;
-                if (!FAST && dv >= pe.a.c.hd) continue;
+                if ((!FAST || DV != D) && dv >= pe.a.c.hd) continue;
                 PagedSum s;
 #pragma unroll
                 for (int w = 0; w < WAVES; ++w) s.m = fmaxf(s.m, ml[0][w][lr]);
