@@ -60,6 +60,7 @@ struct PagedMfmaArgs {
     // and after the launch. NULL: a second launch joins, one of `slices` workgroups some of a segment's rows, and
     // `seg` [items * kvh][2] tells it a segment's first workgroup and its pieces
     unsigned* count;
+    int spread;            // log2 of the words from a segment's counter to the next
     uint32_t* seg;
     int slices;
 };
@@ -378,8 +379,24 @@ struct PagedParts {
 // Joins `n` runs whose results lie in LDS, `step` apart.
 __device__ __forceinline__ PagedSum paged_runs_lds(const f32x4* o, const f32x2v* ml, uint32_t n, uint32_t step) {
     PagedSum s;
-    for (uint32_t i = 0; i < n; ++i) s.m = fmaxf(s.m, ml[i * step][0]);
-    for (uint32_t i = 0; i < n; ++i) s.add(ml[i * step][0], ml[i * step][1], o[i * step]);
+    constexpr uint32_t U = 8;   // read together
+    for (uint32_t i = 0; i < n; i += U) {
+        f32x2v w[U];
+        f32x4 os[U];
+#pragma unroll
+        for (uint32_t u = 0; u < U; ++u) {
+            const uint32_t k = min(i + u, n - 1) * step;
+            w[u] = ml[k];
+            os[u] = o[k];
+        }
+        float mn = s.m;
+#pragma unroll
+        for (uint32_t u = 0; u < U; ++u) mn = fmaxf(mn, w[u][0]);
+        s.raise(mn);
+#pragma unroll
+        for (uint32_t u = 0; u < U; ++u)
+            if (i + u < n) s.add(w[u][0], w[u][1], os[u]);
+    }
     return s;
 }
 
@@ -405,11 +422,11 @@ __device__ __forceinline__ void paged_join(const PagedMfmaArgs& p, int item, int
     const int tid = threadIdx.x, b = (int)div32((uint32_t)item, p.nrb), r0 = (item - b * (int)p.nrb.d) * 16 * CT;
     const int quads = p.a.c.hd / 4, all = min(16 * CT, p.rows - r0) * quads;
     const PagedRuns r = paged_runs(pieces, all);
-    unsigned* cnt = p.count + (int64_t)item * p.a.c.kvh + hk;
+    unsigned* cnt = p.count + (((int64_t)item * p.a.c.kvh + hk) << p.spread);
     if (r.apart) {
         const uint32_t run = r.of(i), i0 = r.at(run), i1 = r.at(run + 1), slot = paged_slot(first, i0);
         if (i1 - i0 > 1) {
-            if (!paged_last(p.count + (int64_t)p.items * p.a.c.kvh + slot, i1 - i0, flag)) return;
+            if (!paged_last(p.count + ((int64_t)p.items * p.a.c.kvh << p.spread) + slot, i1 - i0, flag)) return;
             for (int c = tid; c < all; c += 256) {
                 const int lr = c / quads, dv = (c - lr * quads) * 4;
                 parts.store(slot, lr, dv, parts.run(first, i0, i1, lr, dv), false);
@@ -920,8 +937,14 @@ __global__ __launch_bounds__(64 * WAVES, (PagedTile<DT, F8, D>::occ(CT))) void p
             }
             return o;
         };
+        // a lane's values are the 4 EV columns of its row from EV * 4g on
+        auto quad = [&](int ct, int j) {
+            f32x4 o;
+#pragma unroll
+            for (int u = 0; u < 4; ++u) o[u] = oacc[(4 * j + u) % EV][ct][(4 * j + u) / EV];
+            return o;
+        };
         if constexpr (WAVES == 1) {
-            // ---- a lane's values are columns EV * 4g .. of its rows
             const bool mark = several && has_marks;
 #pragma unroll
             for (int ct = 0; ct < CT; ++ct) {
@@ -930,15 +953,13 @@ __global__ __launch_bounds__(64 * WAVES, (PagedTile<DT, F8, D>::occ(CT))) void p
                 if (r0 + lr >= pe.rows) continue;
                 const PagedRow row(pe, b, hk, r0 + lr, m_run[ct], l);
 #pragma unroll
-                for (int r = 0; r < 4; ++r)
-#pragma unroll
-                    for (int i = 0; i < EV; i += 4) {
-                        const int dv = EV * (4 * g + r) + i;
-                        f32x4 o = f32x4{oacc[i][ct][r], oacc[i + 1][ct][r], oacc[i + 2][ct][r], oacc[i + 3][ct][r]};
-                        if ((!FAST || DV != D) && dv >= pe.a.c.hd) continue;
-                        if (__builtin_expect(mark, 0)) o = marked(lr, dv, o);
-                        row.template store<DT>(pe, dv, o);
-                    }
+                for (int j = 0; j < EV; ++j) {
+                    const int dv = 4 * (EV * g + j);
+                    f32x4 o = quad(ct, j);
+                    if ((!FAST || DV != D) && dv >= pe.a.c.hd) continue;
+                    if (__builtin_expect(mark, 0)) o = marked(lr, dv, o);
+                    row.template store<DT>(pe, dv, o);
+                }
             }
         } else {
             // ---- merge the waves
@@ -951,11 +972,8 @@ __global__ __launch_bounds__(64 * WAVES, (PagedTile<DT, F8, D>::occ(CT))) void p
                     ml[1][wave][16 * ct + c16] = l_tot;
                 }
 #pragma unroll
-                for (int r = 0; r < 4; ++r)
-#pragma unroll
-                    for (int i = 0; i < EV; i += 4)
-                        *reinterpret_cast<f32x4*>(&red[(wave * COLS + 16 * ct + c16) * LDO + EV * (4 * g + r) + i]) =
-                            f32x4{oacc[i][ct][r], oacc[i + 1][ct][r], oacc[i + 2][ct][r], oacc[i + 3][ct][r]};
+                for (int j = 0; j < EV; ++j)
+                    *reinterpret_cast<f32x4*>(&red[(wave * COLS + 16 * ct + c16) * LDO + 4 * (EV * g + j)]) = quad(ct, j);
             }
             __syncthreads();
             for (int c = tid; c < min(COLS, pe.rows - r0) * (DV / 4); c += 64 * WAVES) {
@@ -1031,11 +1049,12 @@ constexpr int PM_CUS = 256;
 // than run together wait less for shorter workgroups; segments that fill a third of the chip have no use for being cut
 // (bfloat16 52 x 64/16 heads x 743 keys of 64: 20.9 us whole, 24.3 in pieces), few long ones do (float32 6 x 32/8 heads x
 // 640 keys of 256: 16 us in pieces, 35 whole).
-constexpr int PM_WAVE = 2, PM_WAVE_MANY = 4, PM_WHOLE = 17, PM_WHOLE_MANY = 33;
+constexpr int PM_WAVE = 2, PM_WAVE_MANY = 4, PM_WHOLE = 17, PM_WHOLE_MANY = 49;
 constexpr double PM_MANY = 0.35;
 // Quads of columns and pieces of an average segment up to which its last workgroup joins it: beyond, the second launch's
 // many workgroups are faster (float16 1 x 16/4 heads, 4 tokens, 32576 keys of 128: 22 us, 28 joined by the last ones).
 constexpr double PM_JOIN_ALONE = 4096;
+constexpr int PM_SPREAD = 5, PM_COUNTERS = 16384;
 
 template <int DT, bool F8, int D, int CT>
 void paged_launch(PagedMfmaArgs& p, int64_t batch, hipStream_t s) {
@@ -1075,8 +1094,11 @@ void paged_launch(PagedMfmaArgs& p, int64_t batch, hipStream_t s) {
             p.part_ml = part + rows * p.a.c.hd;
             p.part_bytes = (unsigned)bytes;
             p.seg = reinterpret_cast<uint32_t*>(p.part_ml + rows * 4);
-            const double wide = std::max(1.0, (double)p.resident / segments) * std::min(p.rows, 16 * CT) * p.a.c.hd / 4;
-            p.count = wide > PM_JOIN_ALONE ? nullptr : split_counters(s, segments + 2 * wgs);
+            const double pieces = std::min((double)p.resident / segments, (double)tiles / PM_WAVES);
+            const double wide = std::max(1.0, pieces) * std::min(p.rows, 16 * CT) * p.a.c.hd / 4;
+            p.spread = PM_SPREAD;
+            while (p.spread > 0 && (segments << p.spread) + 2 * wgs > PM_COUNTERS) --p.spread;
+            p.count = wide > PM_JOIN_ALONE ? nullptr : split_counters(s, (segments << p.spread) + 2 * wgs);
         } else {
             clear_error();
         }
@@ -1095,6 +1117,9 @@ void paged_dispatch(PagedMfmaArgs& p, int64_t batch, hipStream_t s) {
     const bool two = p.rows > 16;
     const int hd = p.a.c.hd;
 #define TVK_PAGED(D) (two ? paged_launch<DT, F8, D, 2>(p, batch, s) : paged_launch<DT, F8, D, 1>(p, batch, s))
+    if constexpr (!F8) {   // 8-bit rows of 32 bytes would be values of half a word a lane
+        if (hd <= 32) return TVK_PAGED(32);
+    }
     if (hd <= 64) TVK_PAGED(64);
     else if (hd <= 96) TVK_PAGED(96);
     else if (hd <= 128) TVK_PAGED(128);
