@@ -32,7 +32,15 @@
 // and the runs' results in order, by the last workgroup to finish; where that is
 // more than one workgroup reads in a few microseconds, by the last of each run and
 // then the last of all, or by a second launch, which a stream without counters takes
-// too. All give the same bits every run.
+// too. All give the same bits every run. Segments count 128 bytes apart: those that
+// count on one line wait for each other, 13 ns each (6 x 15334 keys of one head of 32,
+// 120 pieces each: 16.7 us on one line, 12.5 apart).
+//
+// Slots with rows of less than whole 128-byte lines share lines between heads, and an
+// XCD that reads one head fetches its neighbours' values too. Workgroups go to the XCDs
+// in turn, so the heads of a sequence are numbered to meet on one (bfloat16 73 x 64/16
+// heads x 1149 keys of 32: 42 us, 61 in the order of the heads; 128-byte rows keep
+// that order, which spreads long sequences better: 65 us, 69 for 110 x 1149 keys of 128).
 //
 // Measured: one sequence of 100001 keys (32/8 heads of 128, bfloat16) 81 us, 5.0
 // TB/s; 32 of up to 8000 keys 110 us, 4.9 TB/s; 24 of up to 6001 in 8 bits with 4
@@ -52,6 +60,7 @@ struct PagedMfmaArgs {
     int wgs;               // workgroups the tiles are dealt to; 0: one a segment
     int resident;          // workgroups that run together
     int many;              // segments enough to fill the chip: chunks only
+    int shared;            // rows of neighbouring heads share 128-byte lines
     Div32 nrb, kvh, group;
     float* part_o;         // [2 * wgs][16 * CT][hd]
     float* part_ml;        // [2][2 * wgs][16 * CT][2]: max, sum; again where a run's result is kept
@@ -127,6 +136,7 @@ struct PagedDeal {
     uint32_t per;     // tiles a workgroup's stretch has
     uint32_t snap;    // an end of a stretch this near to a segment's moves there: a short piece costs more than its tiles
     uint32_t total;   // tiles of the call
+    uint32_t used;    // workgroups that get any, if heads share lines
     __device__ __forceinline__ uint32_t units(uint32_t tiles) const { return shift >= 0 ? max(1u, tiles >> shift) : tiles; }
 };
 
@@ -160,20 +170,25 @@ __device__ __forceinline__ PagedDeal paged_deal(const PagedMfmaArgs& p, int lane
     // Many segments and short stretches: a piece's start and end would cost more than its tiles (float32 20 x 16/16 heads x
     // 1442 keys of 64: 44 us in chunks, 56 in stretches). At most a chunk a segment and two for each of the resident
     // workgroups: they fit the launch.
-    if (p.many && d.per < 1536 / BN) {
+    const bool chunks = p.many && d.per < 1536 / BN;
+    d.shift = 2;
+    if (chunks) {
         d.shift = BN == 32 ? 3 : 4;
         while ((uint64_t)p.resident << (d.shift + 1) < d.total) ++d.shift;
-        return d;
+        if (!p.shared) return d;
     }
-    if (!p.many) {
+    if (chunks || !p.many) {
 #pragma unroll 1
-        for (d.shift = 2; d.shift <= 4; ++d.shift) {
+        for (;; ++d.shift) {
             uint32_t u = mine ? d.units(mine) : 0;
             for (int e = lane + 64; e < p.items; e += 64) u += d.units((uint32_t)paged_span<BN, CT>(p, e).tiles);
-            if (wave_sum(u) * p.kvh.d <= (uint32_t)p.wgs) return d;
+            d.used = wave_sum(u) * p.kvh.d;
+            if (chunks || d.used <= (uint32_t)p.wgs) return d;
+            if (d.shift == 4) break;
         }
     }
     d.shift = -1;
+    d.used = small_div(d.total + d.per - 1, d.per);
     return d;
 }
 
@@ -528,20 +543,26 @@ __global__ __launch_bounds__(64 * WAVES, (PagedTile<DT, F8, D>::occ(CT))) void p
     __shared__ uint32_t marks[CT * DV];   // two bits for each row and column: the infinities (1, 2) it takes in, both for NaN
     const int tid = threadIdx.x, lane = tid % 64, wave = WAVES == 1 ? 0 : __builtin_amdgcn_readfirstlane(tid / 64);
     const int g = lane / 16, c16 = lane % 16;
-    const uint32_t wg = blockIdx.x;
-    PagedDeal deal{31, 0, 0, 0};
+    uint32_t wg = blockIdx.x;
+    PagedDeal deal{31, 0, 0, 0, 0};
     PagedPiece pc, part[2];   // part: pieces of segments that others share, the one that begins its segment second
     int parts = 0;
     uint32_t at = 0, x = wg, stop = 0;
     const bool dealt = WAVES > 1 && paged_args().wgs;
     if (!dealt) {
         const PagedMfmaArgs& p = paged_args();
-        pc.item = (int)div32(wg, p.kvh);
-        pc.hk = (int)(wg - pc.item * p.kvh.d);
+        // the heads of an item on one XCD, as long as there are items for all of them
+        const uint32_t grouped = p.shared ? (uint32_t)p.items / 8 * 8 * p.kvh.d : 0;
+        const uint32_t of = wg < grouped ? wg / 8 : wg, n = div32(of, p.kvh);
+        pc.item = (int)(wg < grouped ? 8 * n + wg % 8 : n);
+        pc.hk = (int)(of - n * p.kvh.d);
     } else {
         const PagedMfmaArgs& p = paged_args();
         const uint32_t mine = lane < p.items ? (uint32_t)paged_span<BN, CT>(p, lane).tiles : 0;
         deal = paged_deal<BN, CT>(p, lane, mine);
+        // a stretch of neighbours' work for each XCD
+        if (p.shared && wg < deal.used / 8 * 8) wg = wg % 8 * (deal.used / 8) + wg / 8;
+        x = wg;
         if (deal.shift < 0) {
             x = wg * deal.per;
             stop = min(deal.total, x + deal.per);
@@ -1069,6 +1090,9 @@ void paged_launch(PagedMfmaArgs& p, int64_t batch, hipStream_t s) {
     p.group = make_div((uint32_t)p.a.group);
     p.items = (int)(batch * nrb);
     const int64_t segments = (int64_t)p.items * p.a.c.kvh;
+    // Workgroups go to the XCDs in turn, and each XCD reads for itself a line that its heads share with another's.
+    const auto partial = [&](const int64_t* stride) { return stride[2] * G::ES % 128 != 0; };
+    p.shared = p.a.c.kvh > 1 && (partial(p.a.c.sk) || partial(p.a.c.sv));
     const bool fast = p.a.c.page.d % 16 == 0 && p.a.c.hd * G::ES == G::KL * 64;
     const int64_t keys = p.a.window ? std::min<int64_t>(p.a.max_len, (int64_t)p.a.window + p.a.new_tokens + G::BN) : p.a.max_len;
     const int64_t tiles = (keys + G::BN - 1) / G::BN;   // at most, of a segment
