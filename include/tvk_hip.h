@@ -17,9 +17,10 @@
  *     waits for and the caching allocator's blocks are ordered on.
  *   - strides are in ELEMENTS, not bytes, and may be zero (broadcast) or any
  *     positive value; element offsets must fit in int64.
- *   - scratch memory: tvk_gemm, tvk_conv2d_*, tvk_conv_*, tvk_reduce_sum and
- *     tvk_attention_bwd lease library scratch (split-K partials, repacked
- *     operands, convolution partials, the attention delta) from a per-device
+ *   - scratch memory: tvk_gemm, tvk_conv2d_*, tvk_conv_*, tvk_reduce_sum,
+ *     tvk_attention_bwd, tvk_rms_norm_bwd and tvk_paged_attention lease library
+ *     scratch (split-K partials, repacked operands, convolution partials, the
+ *     attention delta, partial sums of rows and of split keys) from a per-device
  *     pool for the kernels they queue on their `stream`. A buffer is leased
  *     again only for the stream its first lease named, so stream order puts
  *     each call's kernels after the previous holder's; concurrent calls (other
@@ -478,8 +479,8 @@ tvk_status tvk_rms_norm_fwd(const tvk_rms_norm_desc* desc);
  *   dweight = sum over rows of dy * n.
  * dx is the gradient of x and of residual alike. dweight (weight_dtype) NULL:
  * not wanted. The sums over rows run in an order that depends on the sizes
- * alone: the same bits every run. dx may be dy, h or dh (same strides). Uses
- * library scratch when dweight is wanted. */
+ * alone: the same bits every run. dx may be dy, h or dh (same strides). May
+ * use library scratch when dweight is wanted. */
 typedef struct {
     int32_t dtype, weight_dtype;
     int64_t rows, cols;

@@ -42,9 +42,10 @@
 // heads x 1149 keys of 32: 42 us, 61 in the order of the heads; 128-byte rows keep
 // that order, which spreads long sequences better: 65 us, 69 for 110 x 1149 keys of 128).
 //
-// Measured: one sequence of 100001 keys (32/8 heads of 128, bfloat16) 81 us, 5.0
-// TB/s; 32 of up to 8000 keys 110 us, 4.9 TB/s; 24 of up to 6001 in 8 bits with 4
-// tokens each 52 us, 3.4 TB/s, where stretches that cross segments end late.
+// Measured: one sequence of 100001 keys (32/8 heads of 128, bfloat16) 82 us, 5.0
+// TB/s; 32 of up to 8000 keys 111 us, 4.9 TB/s; 24 of up to 6001 in 8 bits with 4
+// tokens each 52 us, 3.4 TB/s, where stretches that cross segments end late; 16 with
+// windows of 1000 keys, 12 heads of 80 in float16 16.5 us, 3.1 TB/s.
 #pragma once
 
 #include "attention_kernels.h"

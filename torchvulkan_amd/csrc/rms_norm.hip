@@ -6,9 +6,14 @@
 // pass forward, for the 8-bit output too (max|h w| and the sum of squares come
 // from the same pass, and scale both), one pass backward for both sums and dx.
 // Backward, a workgroup takes rows in turn and keeps dweight's sums over them in
-// registers; those are added up by a second launch in a fixed order. Rows start at any multiple of a value (16-byte accesses
-// need no more); the values past a row's last whole chunk go one to a thread.
+// registers; those are added up by a second launch in a fixed order, or stored as they
+// are where one workgroup takes all rows. Rows start at any multiple of a value (16-byte
+// accesses need no more); the values past a row's last whole chunk go one to a thread.
 // Rows of more than 2048 chunks are read again for every pass.
+//
+// Measured (a 2 GiB copy moves 4.9 TB/s): residual, norm and 8 bits of 16384 x 4096 in
+// bfloat16 81 us, 5.8 TB/s; its gradients at 16384 x 2048 56 us, 4.8 TB/s, 5 of them
+// the second launch; 7 x 4096 3.9 us and gradients of 1000 x 777 8.1 us, the launches.
 #include "words.h"
 
 #include <algorithm>
