@@ -50,6 +50,7 @@
 
 #include "attention_kernels.h"
 #include "paged.h"
+#include "paged_deal.h"
 
 namespace tvk {
 
@@ -58,10 +59,7 @@ struct PagedMfmaArgs {
     uint32_t kp, ks, vp, vs;   // page and slot strides of keys and values, in 16 bytes
     int rows;              // new_tokens * group
     int items;             // batch * row blocks of a key/value head
-    int wgs;               // workgroups the tiles are dealt to; 0: one a segment
-    int resident;          // workgroups that run together
-    int many;              // segments enough to fill the chip: chunks only
-    int shared;            // rows of neighbouring heads share 128-byte lines
+    PagedPlan plan;        // wgs 0: a workgroup a segment
     Div32 nrb, kvh, group;
     float* part_o;         // [2 * wgs][16 * CT][hd]
     float* part_ml;        // [2][2 * wgs][16 * CT][2]: max, sum; again where a run's result is kept
@@ -77,7 +75,7 @@ struct PagedMfmaArgs {
 
 namespace {
 
-constexpr int PM_WAVES = 4;
+constexpr int PM_WAVES = 4;   // paged_wgs: a tile for each
 
 template <int DT, bool F8, int D>
 struct PagedTile {
@@ -123,23 +121,8 @@ __device__ __forceinline__ PagedSpan paged_span(const PagedMfmaArgs& p, int e) {
     return s;
 }
 
-// n / d for a quotient below 2^22: a float estimate that is at most one off.
-__device__ __forceinline__ uint32_t small_div(uint32_t n, uint32_t d) {
-    uint32_t q = (uint32_t)((float)n * __builtin_amdgcn_rcpf((float)d));
-    const int r = (int)(n - q * d);
-    if (r < 0) --q;
-    else if (r >= (int)d) ++q;
-    return q;
-}
-
-struct PagedDeal {
-    int shift;        // segments are cut into chunks of at least 2^shift tiles; -1: stretches
-    uint32_t per;     // tiles a workgroup's stretch has
-    uint32_t snap;    // an end of a stretch this near to a segment's moves there: a short piece costs more than its tiles
-    uint32_t total;   // tiles of the call
-    uint32_t used;    // workgroups that get any, if heads share lines
-    __device__ __forceinline__ uint32_t units(uint32_t tiles) const { return shift >= 0 ? max(1u, tiles >> shift) : tiles; }
-};
+__device__ __forceinline__ float wave_rcp(float x) { return __builtin_amdgcn_rcpf(x); }
+__device__ __forceinline__ uint32_t wave_div(uint32_t n, uint32_t d) { return small_div(n, d, wave_rcp((float)d)); }
 
 // v + the lane's value from lanes below it by a DPP move (0 where there is none), in the rows of 16 lanes that MASK names.
 template <int CTRL, int MASK>
@@ -157,40 +140,17 @@ __device__ __forceinline__ uint32_t wave_scan(uint32_t v) {
 }
 __device__ __forceinline__ uint32_t wave_sum(uint32_t v) { return (uint32_t)__builtin_amdgcn_readlane((int)wave_scan(v), 63); }
 
-// Sums stay below 2^31 (paged_attn_mfma). mine: the tiles of item `lane`.
+// mine: the tiles of item `lane`.
 template <int BN, int CT>
-__device__ __forceinline__ PagedDeal paged_deal(const PagedMfmaArgs& p, int lane, uint32_t mine) {
-    PagedDeal d;
+__device__ __forceinline__ PagedDeal paged_deal_of(const PagedMfmaArgs& p, int lane, uint32_t mine) {
     uint32_t n = mine;
     for (int e = lane + 64; e < p.items; e += 64) n += (uint32_t)paged_span<BN, CT>(p, e).tiles;
-    d.total = wave_sum(n) * p.kvh.d;
-    const uint32_t resident = (uint32_t)min(p.wgs, p.resident);
-    // at least total / resident: the float product is off by less than one in 2^22
-    d.per = (uint32_t)((float)d.total * __builtin_amdgcn_rcpf((float)resident) * 1.000001f) + 1;
-    d.snap = min(128u / BN, d.per / 4);
-    // Many segments and short stretches: a piece's start and end would cost more than its tiles (float32 20 x 16/16 heads x
-    // 1442 keys of 64: 44 us in chunks, 56 in stretches). At most a chunk a segment and two for each of the resident
-    // workgroups: they fit the launch.
-    const bool chunks = p.many && d.per < 1536 / BN;
-    d.shift = 2;
-    if (chunks) {
-        d.shift = BN == 32 ? 3 : 4;
-        while ((uint64_t)p.resident << (d.shift + 1) < d.total) ++d.shift;
-        if (!p.shared) return d;
-    }
-    if (chunks || !p.many) {
-#pragma unroll 1
-        for (;; ++d.shift) {
-            uint32_t u = mine ? d.units(mine) : 0;
-            for (int e = lane + 64; e < p.items; e += 64) u += d.units((uint32_t)paged_span<BN, CT>(p, e).tiles);
-            d.used = wave_sum(u) * p.kvh.d;
-            if (chunks || d.used <= (uint32_t)p.wgs) return d;
-            if (d.shift == 4) break;
-        }
-    }
-    d.shift = -1;
-    d.used = small_div(d.total + d.per - 1, d.per);
-    return d;
+    auto count = [&](const PagedDeal& d) {
+        uint32_t u = mine ? d.units(mine) : 0;
+        for (int e = lane + 64; e < p.items; e += 64) u += d.units((uint32_t)paged_span<BN, CT>(p, e).tiles);
+        return wave_sum(u) * p.kvh.d;
+    };
+    return paged_deal<BN>(p.plan, wave_sum(n) * p.kvh.d, count, [](float x) { return wave_rcp(x); });
 }
 
 // The item that holds unit x of the call, and the unit's place among the item's; false past the last.
@@ -214,30 +174,6 @@ __device__ __forceinline__ bool paged_locate(const PagedMfmaArgs& p, const Paged
         mine = e0 + lane < p.items ? (uint32_t)paged_span<BN, CT>(p, e0 + lane).tiles : 0;
     }
 }
-
-// A stretch of a segment's tiles, [c0, c1), and the workgroups whose pieces make up the segment.
-struct PagedPiece {
-    int item, hk;
-    uint32_t c0, c1;
-    uint32_t first, pieces;
-};
-
-// Of the segment of `tiles` tiles from tile `begin` of the call, when stretches are dealt: ends of stretches inside it that
-// do not move to its ends cut it.
-__device__ __forceinline__ void paged_pieces(const PagedDeal& d, uint32_t begin, uint32_t tiles, PagedPiece& pc) {
-    pc.first = small_div(begin + d.snap, d.per);
-    const uint32_t last = tiles > 2 * d.snap ? small_div(begin + tiles - d.snap - 1, d.per) : 0;
-    pc.pieces = last > pc.first ? last - pc.first + 1 : 1;
-}
-
-// Where the end of a stretch at tile x of a segment's tiles lies.
-__device__ __forceinline__ uint32_t paged_cut(const PagedDeal& d, uint32_t x, uint32_t tiles) {
-    return x <= d.snap ? 0 : tiles - x <= d.snap ? tiles : x;
-}
-
-// Where a segment's piece i is kept: a workgroup has at most one piece that does not begin its segment and one that does
-// and does not end it.
-__device__ __forceinline__ uint32_t paged_slot(uint32_t first, uint32_t i) { return 2 * (first + i) + (i == 0); }
 
 // ---------------------------------------------------------------------------
 // partials and outputs
@@ -316,7 +252,7 @@ struct PagedParts {
     __device__ __forceinline__ PagedParts(const PagedMfmaArgs& a)
         : p(a), rs(__builtin_amdgcn_make_buffer_rsrc((void*)a.part_o, 0, (int)a.part_bytes, 0x00020000)) {}
     // byte offsets: below 2 GiB; of a run's result in the place of its first piece, whose max and sum others still read
-    __device__ __forceinline__ int run_ml_at(uint32_t slot, int lr) const { return ml_at(slot + 2 * p.wgs, lr); }
+    __device__ __forceinline__ int run_ml_at(uint32_t slot, int lr) const { return ml_at(slot + 2 * p.plan.wgs, lr); }
     __device__ __forceinline__ int o_at(uint32_t slot, int lr, int dv) const {
         return (int)(((slot * 16 * CT + lr) * (uint32_t)p.a.c.hd + dv) * 4);
     }
@@ -549,26 +485,21 @@ __global__ __launch_bounds__(64 * WAVES, (PagedTile<DT, F8, D>::occ(CT))) void p
     PagedPiece pc, part[2];   // part: pieces of segments that others share, the one that begins its segment second
     int parts = 0;
     uint32_t at = 0, x = wg, stop = 0;
-    const bool dealt = WAVES > 1 && paged_args().wgs;
+    const bool dealt = WAVES > 1 && paged_args().plan.wgs;
     if (!dealt) {
         const PagedMfmaArgs& p = paged_args();
         // the heads of an item on one XCD, as long as there are items for all of them
-        const uint32_t grouped = p.shared ? (uint32_t)p.items / 8 * 8 * p.kvh.d : 0;
+        const uint32_t grouped = p.plan.shared ? (uint32_t)p.items / 8 * 8 * p.kvh.d : 0;
         const uint32_t of = wg < grouped ? wg / 8 : wg, n = div32(of, p.kvh);
         pc.item = (int)(wg < grouped ? 8 * n + wg % 8 : n);
         pc.hk = (int)(of - n * p.kvh.d);
     } else {
         const PagedMfmaArgs& p = paged_args();
         const uint32_t mine = lane < p.items ? (uint32_t)paged_span<BN, CT>(p, lane).tiles : 0;
-        deal = paged_deal<BN, CT>(p, lane, mine);
+        deal = paged_deal_of<BN, CT>(p, lane, mine);
         // a stretch of neighbours' work for each XCD
-        if (p.shared && wg < deal.used / 8 * 8) wg = wg % 8 * (deal.used / 8) + wg / 8;
-        x = wg;
-        if (deal.shift < 0) {
-            x = wg * deal.per;
-            stop = min(deal.total, x + deal.per);
-        }
-        if (!paged_locate<BN, CT>(p, deal, x, lane, mine, pc.item, at)) return;
+        if (p.plan.shared && wg < deal.used / 8 * 8) wg = wg % 8 * (deal.used / 8) + wg / 8;
+        if (!paged_start(deal, wg, x, stop) || !paged_locate<BN, CT>(p, deal, x, lane, mine, pc.item, at)) return;
     }
 
     for (bool more_pieces = true; more_pieces;) {
@@ -589,21 +520,14 @@ __global__ __launch_bounds__(64 * WAVES, (PagedTile<DT, F8, D>::occ(CT))) void p
         pc.pieces = 1;
         if (dealt) {
             const uint32_t units = deal.units(tiles);
-            pc.hk = (int)small_div(at, units);
+            pc.hk = (int)wave_div(at, units);
             at -= (uint32_t)pc.hk * units;   // of the segment
             if (deal.shift >= 0) {
-                const uint32_t q = small_div(tiles, units), r = tiles - q * units;
-                pc.c0 = at * q + min(at, r);
-                pc.c1 = pc.c0 + q + (at < r);
-                pc.first = x - at;
-                pc.pieces = units;
+                paged_chunk(x, at, tiles, units, wave_rcp((float)units), pc);
             } else {
-                const uint32_t rest = tiles - at;   // of the stretch
-                paged_pieces(deal, x - at, tiles, pc);
-                pc.c0 = paged_cut(deal, at, tiles);
-                pc.c1 = stop - x < rest ? paged_cut(deal, at + (stop - x), tiles) : tiles;
+                paged_stretch(deal, x, at, tiles, stop, wave_rcp((float)deal.per), pc);
                 // the next segment: the item's next head, or the next item's first
-                x += rest;
+                x += tiles - at;
                 more_pieces = x < stop;
                 at = (uint32_t)(pc.hk + 1) * tiles;
             }
@@ -1066,13 +990,6 @@ __global__ __launch_bounds__(PM_JOIN_THREADS) void paged_attn_join_kernel(PagedM
 }
 
 constexpr int PM_CUS = 256;
-// Keys of a segment, in tiles of 32, up to which it takes one wave and one workgroup. A wave spares the merge of four
-// (float16 98 x 64/8 heads x 16 keys of 128: 6.0 us, 10.9 with four) and takes the tiles one after another. More segments
-// than run together wait less for shorter workgroups; segments that fill a third of the chip have no use for being cut
-// (bfloat16 52 x 64/16 heads x 743 keys of 64: 20.9 us whole, 24.3 in pieces), few long ones do (float32 6 x 32/8 heads x
-// 640 keys of 256: 16 us in pieces, 35 whole).
-constexpr int PM_WAVE = 2, PM_WAVE_MANY = 4, PM_WHOLE = 17, PM_WHOLE_MANY = 49;
-constexpr double PM_MANY = 0.35;
 // Quads of columns and pieces of an average segment up to which its last workgroup joins it: beyond, the second launch's
 // many workgroups are faster (float16 1 x 16/4 heads, 4 tokens, 32576 keys of 128: 22 us, 28 joined by the last ones).
 constexpr double PM_JOIN_ALONE = 4096;
@@ -1093,33 +1010,31 @@ void paged_launch(PagedMfmaArgs& p, int64_t batch, hipStream_t s) {
     const int64_t segments = (int64_t)p.items * p.a.c.kvh;
     // Workgroups go to the XCDs in turn, and each XCD reads for itself a line that its heads share with another's.
     const auto partial = [&](const int64_t* stride) { return stride[2] * G::ES % 128 != 0; };
-    p.shared = p.a.c.kvh > 1 && (partial(p.a.c.sk) || partial(p.a.c.sv));
+    p.plan.shared = p.a.c.kvh > 1 && (partial(p.a.c.sk) || partial(p.a.c.sv));
     const bool fast = p.a.c.page.d % 16 == 0 && p.a.c.hd * G::ES == G::KL * 64;
     const int64_t keys = p.a.window ? std::min<int64_t>(p.a.max_len, (int64_t)p.a.window + p.a.new_tokens + G::BN) : p.a.max_len;
     const int64_t tiles = (keys + G::BN - 1) / G::BN;   // at most, of a segment
-    p.resident = PM_CUS * G::occ(CT);
-    if (tiles * G::BN <= 32 * (segments > p.resident ? PM_WAVE_MANY : PM_WAVE)) {
+    p.plan.resident = PM_CUS * G::occ(CT);
+    if (tiles * G::BN <= 32 * (segments > p.plan.resident ? PM_WAVE_MANY : PM_WAVE)) {
         const dim3 grid((unsigned)segments), block(64);
         if (fast) hipLaunchKernelGGL((paged_attn_mfma_kernel<DT, F8, D, CT, true, 1>), grid, block, 0, s, p);
         else hipLaunchKernelGGL((paged_attn_mfma_kernel<DT, F8, D, CT, false, 1>), grid, block, 0, s, p);
         return;
     }
     Scratch scratch;
-    p.many = segments > p.resident * PM_MANY;
-    if (tiles * G::BN > 32 * (p.many ? PM_WHOLE_MANY : PM_WHOLE)) {
-        // a workgroup for every 4 tiles the sequences may have, as many as are resident together, or what paged_deal's
-        // chunks may come to
-        const int64_t wgs = p.many ? segments + 2 * p.resident : std::min<int64_t>(p.resident, segments * (tiles / PM_WAVES));
+    p.plan.many = paged_many(segments, p.plan.resident);
+    if (paged_is_dealt(p.plan.many, tiles * G::BN)) {
+        const int64_t wgs = paged_wgs(p.plan.many, segments, tiles, p.plan.resident);
         const size_t rows = (size_t)2 * wgs * 16 * CT, bytes = rows * (p.a.c.hd + 4) * 4;
         float* part = s == hipStreamPerThread || bytes >= (size_t)1 << 31
                           ? nullptr : static_cast<float*>(scratch.get(bytes + (size_t)segments * 8, s));
         if (part) {
-            p.wgs = (int)wgs;
+            p.plan.wgs = (int)wgs;
             p.part_o = part;
             p.part_ml = part + rows * p.a.c.hd;
             p.part_bytes = (unsigned)bytes;
             p.seg = reinterpret_cast<uint32_t*>(p.part_ml + rows * 4);
-            const double pieces = std::min((double)p.resident / segments, (double)tiles / PM_WAVES);
+            const double pieces = std::min((double)p.plan.resident / segments, (double)tiles / PM_WAVES);
             const double wide = std::max(1.0, pieces) * std::min(p.rows, 16 * CT) * p.a.c.hd / 4;
             p.spread = PM_SPREAD;
             while (p.spread > 0 && (segments << p.spread) + 2 * wgs > PM_COUNTERS) --p.spread;
@@ -1128,10 +1043,10 @@ void paged_launch(PagedMfmaArgs& p, int64_t batch, hipStream_t s) {
             clear_error();
         }
     }
-    const dim3 grid((unsigned)(p.wgs ? p.wgs : segments)), block(64 * PM_WAVES);
+    const dim3 grid((unsigned)(p.plan.wgs ? p.plan.wgs : segments)), block(64 * PM_WAVES);
     if (fast) hipLaunchKernelGGL((paged_attn_mfma_kernel<DT, F8, D, CT, true, PM_WAVES>), grid, block, 0, s, p);
     else hipLaunchKernelGGL((paged_attn_mfma_kernel<DT, F8, D, CT, false, PM_WAVES>), grid, block, 0, s, p);
-    if (p.wgs && !p.count) {
+    if (p.plan.wgs && !p.count) {
         p.slices = (int)std::min<int64_t>(std::min(p.rows, 16 * CT), std::max<int64_t>(1, 2048 / segments));
         hipLaunchKernelGGL((paged_attn_join_kernel<DT, CT>), dim3((unsigned)(segments * p.slices)), dim3(PM_JOIN_THREADS), 0, s, p);
     }
