@@ -506,10 +506,14 @@ tvk_status tvk_rms_norm_bwd(const tvk_rms_norm_bwd_desc* desc);
  * seq_lens[b] counts the sequence's positions, the call's new tokens among
  * them (0: no sequence in that slot of the batch): with T new tokens, token t
  * stands at position seq_lens[b] - T + t, and tokens whose position is
- * negative are padding (sequences with fewer new tokens are padded in front).
+ * negative are padding. Sequences with fewer new tokens are padded in front:
+ * new_lens[b] counts sequence b's own, the last of the call's (NULL: all of
+ * them; above T: T), and the tokens before those are padding, whatever their
+ * position. Padding is not appended and sees no key.
  * Lengths past the table's reach are taken as table_width * page_size (at most
  * 2^30).
- * table and seq_lens are read on the device, so a captured call follows them.
+ * table, seq_lens and new_lens are read on the device, so a captured call
+ * follows them.
  * dtype: the call's own, or F8E4M3FN (values are stored divided by their
  * head's scale, saturating at 448, and multiplied by it when read). Strides
  * are in elements, any page and slot order; head_dim values are contiguous. */
@@ -521,6 +525,7 @@ typedef struct {
     const float* k_scale; const float* v_scale;   /* [heads_kv], NULL: 1 (F8E4M3FN only) */
     const int32_t* table; int64_t table_stride, table_width;   /* [batch][table_width] */
     const int32_t* seq_lens;                      /* [batch] */
+    const int32_t* new_lens;                      /* [batch], NULL: the call's tokens each */
 } tvk_paged_cache;
 
 /* Rotates the new tokens' queries and keys by their positions and writes keys

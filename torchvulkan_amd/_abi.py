@@ -226,7 +226,7 @@ class PagedCache(C.Structure):
         ("v", C.c_void_p), ("v_stride", I64x3),
         ("k_scale", C.c_void_p), ("v_scale", C.c_void_p),
         ("table", C.c_void_p), ("table_stride", C.c_int64), ("table_width", C.c_int64),
-        ("seq_lens", C.c_void_p),
+        ("seq_lens", C.c_void_p), ("new_lens", C.c_void_p),
     ]
 
 
@@ -691,9 +691,9 @@ def rms_norm_bwd(dy, h, weight=None, dh=None, eps=1e-5, stream=None):
     return dx, dweight
 
 
-def make_paged_cache(k_cache, v_cache, seq_lens, table, k_scale=None, v_scale=None) -> PagedCache:
+def make_paged_cache(k_cache, v_cache, seq_lens, table, k_scale=None, v_scale=None, new_lens=None) -> PagedCache:
     """A cache of [pages, page_size, heads_kv, head_dim] tensors (any strides, head_dim contiguous), int32 table
-    [batch, entries] and int32 lengths [batch]."""
+    [batch, entries], int32 lengths [batch] and, where sequences have new tokens of their own number, those [batch]."""
     torch = _torch()
     if k_cache.dim() != 4 or k_cache.shape != v_cache.shape or k_cache.dtype != v_cache.dtype:
         raise _invalid("k_cache and v_cache: [pages, page_size, heads_kv, head_dim] of one shape and dtype are expected")
@@ -715,6 +715,8 @@ def make_paged_cache(k_cache, v_cache, seq_lens, table, k_scale=None, v_scale=No
         c.v_scale = _vector(v_scale, c.heads_kv, (torch.float32,), "v_scale")
     c.table, c.table_stride, c.table_width = table.data_ptr(), table.stride(0), table.shape[1]
     c.seq_lens = seq_lens.data_ptr()
+    if new_lens is not None:
+        c.new_lens = _vector(new_lens, seq_lens.shape[0], (torch.int32,), "new_lens")
     return c
 
 
@@ -728,12 +730,12 @@ def _token_strides(t, shape, dtype, what: str):
 
 
 def make_paged_append_desc(q, k, v, q_out, k_cache, v_cache, seq_lens, table, rotary=None, interleaved=False,
-                           k_scale=None, v_scale=None, stream=None) -> PagedAppendDesc:
+                           k_scale=None, v_scale=None, stream=None, new_lens=None) -> PagedAppendDesc:
     """Describes tvk_paged_append over [batch, tokens, heads, head_dim] tokens (q and q_out None: keys and values
     alone); rotary float32 [positions, rotary_dim], cos then sin."""
     torch = _torch()
     d = PagedAppendDesc()
-    d.cache = make_paged_cache(k_cache, v_cache, seq_lens, table, k_scale, v_scale)
+    d.cache = make_paged_cache(k_cache, v_cache, seq_lens, table, k_scale, v_scale, new_lens)
     d.dtype = _dtype_code(k.dtype)
     shape = (seq_lens.shape[0], k.shape[1] if k.dim() == 4 else -1, d.cache.heads_kv, d.cache.head_dim)
     d.k, d.k_stride = k.data_ptr(), _token_strides(k, shape, k.dtype, "k")
@@ -757,22 +759,22 @@ def make_paged_append_desc(q, k, v, q_out, k_cache, v_cache, seq_lens, table, ro
 
 
 def paged_append(q, k, v, k_cache, v_cache, seq_lens, table, rotary=None, interleaved=False, k_scale=None,
-                 v_scale=None, stream=None):
+                 v_scale=None, stream=None, new_lens=None):
     """Appends the new tokens' keys and values to the cache and returns their rotated queries (a new tensor)."""
     torch = _torch()
     q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device) if q is not None else None
     d = make_paged_append_desc(q, k, v, q_out, k_cache, v_cache, seq_lens, table, rotary, interleaved, k_scale, v_scale,
-                               _stream_of(k, stream))
+                               _stream_of(k, stream), new_lens)
     check(load().tvk_paged_append(C.byref(d)))
     return q_out
 
 
 def make_paged_attention_desc(q, k_cache, v_cache, out, seq_lens, table, max_len=0, scale=None, window=0, k_scale=None,
-                              v_scale=None, lse=None, stream=None) -> PagedAttentionDesc:
+                              v_scale=None, lse=None, stream=None, new_lens=None) -> PagedAttentionDesc:
     """Describes tvk_paged_attention of [batch, tokens, heads, head_dim] queries; lse float32 [batch, tokens, heads]."""
     torch = _torch()
     d = PagedAttentionDesc()
-    d.cache = make_paged_cache(k_cache, v_cache, seq_lens, table, k_scale, v_scale)
+    d.cache = make_paged_cache(k_cache, v_cache, seq_lens, table, k_scale, v_scale, new_lens)
     d.dtype = _dtype_code(q.dtype)
     shape = (seq_lens.shape[0], *(q.shape[1:3] if q.dim() == 4 else (-1, -1)), d.cache.head_dim)
     d.q, d.q_stride = q.data_ptr(), _token_strides(q, shape, q.dtype, "q")
@@ -789,13 +791,13 @@ def make_paged_attention_desc(q, k_cache, v_cache, out, seq_lens, table, max_len
 
 
 def paged_attention(q, k_cache, v_cache, seq_lens, table, max_len=0, scale=None, window=0, k_scale=None, v_scale=None,
-                    stream=None):
+                    stream=None, new_lens=None):
     """(out, lse) of tvk_paged_attention (new tensors)."""
     torch = _torch()
     out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
     lse = torch.empty(q.shape[:3], dtype=torch.float32, device=q.device)
     d = make_paged_attention_desc(q, k_cache, v_cache, out, seq_lens, table, max_len, scale, window, k_scale, v_scale, lse,
-                                  _stream_of(q, stream))
+                                  _stream_of(q, stream), new_lens)
     check(load().tvk_paged_attention(C.byref(d)))
     return out, lse
 

@@ -16,6 +16,7 @@ struct PagedCache {
     const float* v_scale;
     const int32_t* table;
     const int32_t* lens;
+    const int32_t* news;    // or NULL
     int64_t table_stride;
     uint32_t pages;
     uint32_t reach;         // positions a table row spans (at most kMaxReach)
@@ -47,6 +48,13 @@ __device__ inline int paged_len(const PagedCache& c, int b) {
     // not written while a kernel reads it: a scalar load where b is a wave's
     const int n = ((const __attribute__((address_space(4))) int32_t*)(uintptr_t)c.lens)[b];
     return n < 0 ? 0 : (uint32_t)n > c.reach ? (int)c.reach : n;
+}
+
+// Of a call's `new_tokens` tokens, those in front of sequence b's own.
+__device__ inline int paged_padding(const PagedCache& c, int b, int new_tokens) {
+    if (!c.news) return 0;
+    const int n = ((const __attribute__((address_space(4))) int32_t*)(uintptr_t)c.news)[b];
+    return new_tokens - min(max(n, 0), new_tokens);
 }
 
 // The page and slot of position p (0 <= p < c.reach) of sequence b; false where its entry is no page.

@@ -55,6 +55,7 @@ PagedCache paged_cache(const tvk_paged_cache& c) {
     p.v_scale = c.v_scale;
     p.table = c.table;
     p.lens = c.seq_lens;
+    p.news = c.new_lens;
     p.table_stride = c.table_stride;
     p.pages = (uint32_t)c.pages;
     p.reach = (uint32_t)(c.table_width > kMaxReach / c.page_size ? kMaxReach : c.table_width * c.page_size);
@@ -108,7 +109,7 @@ __device__ inline bool place(const AppendArgs& p, int64_t token, uint32_t& b, ui
     t = (uint32_t)token - b * p.new_tokens.d;
     pos = paged_len(p.c, b) - (int)p.new_tokens.d + (int)t;
     page = slot = 0;
-    return pos >= 0 && (!p.rotary || (uint32_t)pos < p.rot_len) && paged_find(p.c, b, (uint32_t)pos, page, slot);
+    return (int)t >= paged_padding(p.c, b, (int)p.new_tokens.d) && pos >= 0 && (!p.rotary || (uint32_t)pos < p.rot_len) && paged_find(p.c, b, (uint32_t)pos, page, slot);
 }
 
 template <int DT, bool F8>

@@ -34,7 +34,7 @@ __global__ __launch_bounds__(64 * PA_WAVES) void paged_attn_any_kernel(PagedAttn
     const int t = bt % p.new_tokens, b = bt / p.new_tokens, hk = h / p.group;
     const int hd = p.c.hd;
     const int len = (int)min((uint32_t)paged_len(p.c, b), p.max_len);
-    const int last = len - p.new_tokens + t + 1;   // keys below it are seen
+    const int last = t < paged_padding(p.c, b, p.new_tokens) ? 0 : len - p.new_tokens + t + 1;   // keys below it are seen
     const int first = p.window ? (int)max((int64_t)0, (int64_t)last - (int64_t)p.window) : 0;
     const T* q = static_cast<const T*>(p.q) + b * p.sq[0] + t * p.sq[1] + h * p.sq[2];
     const float ks = F8 && p.c.k_scale ? p.c.k_scale[hk] : 1.0f, vs = F8 && p.c.v_scale ? p.c.v_scale[hk] : 1.0f;

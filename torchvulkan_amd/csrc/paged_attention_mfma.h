@@ -100,6 +100,7 @@ struct PagedTile {
 struct PagedSpan {
     int b, len;
     int t0, t1;   // the row block's first and last token
+    int pad;      // tokens in front that are padding
     int lo, hi;   // keys that some row of the block sees
     int tiles;    // at least one: a segment without keys writes its zeros
 };
@@ -115,8 +116,9 @@ __device__ __forceinline__ PagedSpan paged_span(const PagedMfmaArgs& p, int e) {
     s.len = (int)min((uint32_t)paged_len(p.a.c, s.b), p.a.max_len);
     s.t0 = (int)div32((uint32_t)r0, p.group);
     s.t1 = (int)div32((uint32_t)r1, p.group);
-    s.hi = max(0, s.len - p.a.new_tokens + s.t1 + 1);
-    s.lo = min(s.hi, window_lo(s.len - p.a.new_tokens + s.t0 + 1, p.a.window));
+    s.pad = paged_padding(p.a.c, s.b, p.a.new_tokens);
+    s.hi = s.t1 < s.pad ? 0 : max(0, s.len - p.a.new_tokens + s.t1 + 1);
+    s.lo = min(s.hi, window_lo(s.len - p.a.new_tokens + max(s.t0, s.pad) + 1, p.a.window));
     s.tiles = s.hi > s.lo ? (s.hi + BN - 1) / BN - s.lo / BN : 1;
     return s;
 }
@@ -549,7 +551,7 @@ __global__ __launch_bounds__(64 * WAVES, (PagedTile<DT, F8, D>::occ(CT))) void p
         for (int ct = 0; ct < CT; ++ct) {
             const int r = min(r0 + 16 * ct + c16, p.rows - 1);   // columns past the rows repeat the last one, unused
             const int t = (int)div32((uint32_t)r, p.group), h = hk * (int)p.group.d + (r - t * (int)p.group.d);
-            last_c[ct] = sp.len - a.new_tokens + t + 1;
+            last_c[ct] = t < sp.pad ? 0 : sp.len - a.new_tokens + t + 1;
             constexpr int QES = F32 ? 4 : 2;
             const char* Q = static_cast<const char*>(a.q) +
                             ((int64_t)b * a.sq[0] + (int64_t)t * a.sq[1] + (int64_t)h * a.sq[2]) * QES;
@@ -664,7 +666,7 @@ __global__ __launch_bounds__(64 * WAVES, (PagedTile<DT, F8, D>::occ(CT))) void p
         const int end = sp.hi > sp.lo ? tile0 + (int)pc.c1 : 0;
         // keys that every row of the block sees
         const int all_lo = window_lo(sp.hi, a.window);
-        const int all_hi = sp.len - a.new_tokens + sp.t0 + 1;
+        const int all_hi = sp.t0 < sp.pad ? 0 : sp.len - a.new_tokens + sp.t0 + 1;
         t = tile0 + (int)pc.c0 + wave;
         if (t < end) {
             fetch(t);
@@ -826,7 +828,8 @@ __global__ __launch_bounds__(64 * WAVES, (PagedTile<DT, F8, D>::occ(CT))) void p
                             const uint32_t mark = F8 || (v & ~sign) != top ? 3u : v & sign ? 2u : 1u;
 #pragma unroll 1
                             for (int col = 0; col < COLS; ++col) {
-                                const int hi = sp.len - a.new_tokens + (int)div32((uint32_t)min(r0 + col, p.rows - 1), p.group) + 1;
+                                const int tok = (int)div32((uint32_t)min(r0 + col, p.rows - 1), p.group);
+                                const int hi = tok < sp.pad ? 0 : sp.len - a.new_tokens + tok + 1;
                                 if ((keys & key_bits(k0, window_lo(hi, a.window), hi)) >> key & 1) atomicOr(&marks[(col * DV + dv) / 16], mark << 2 * (dv % 16));
                             }
                         }

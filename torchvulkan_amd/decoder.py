@@ -24,6 +24,10 @@ def _stream(t: torch.Tensor):
     return s.value
 
 
+def _capturing(t: torch.Tensor) -> bool:
+    return t.device.type == "cuda" and torch.cuda.is_current_stream_capturing()
+
+
 def _rows(t: torch.Tensor) -> torch.Tensor:
     """[..., cols] as [rows, cols] with contiguous rows (a copy only where the strides allow no view)."""
     t = t.reshape(-1, t.shape[-1])
@@ -102,8 +106,8 @@ class PagedKVCache:
     layers share the lengths and the pages' places.
 
     The host keeps the sequences' lengths and free pages; extend() gives sequences new positions, release() ends one.
-    Both only write the device's `table` and `lens`, which the calls read there, so a captured step (append, attend)
-    replays for other lengths. dtype float8_e4m3fn keeps 8 bits, divided by k_scale and v_scale of each head."""
+    Both only write the device's `table`, `lens` and `new` (how many of each sequence's positions are new), which the calls
+    read there, so a captured step (append, attend) replays for other lengths. dtype float8_e4m3fn keeps 8 bits, divided by k_scale and v_scale of each head."""
 
     def __init__(self, batch: int, pages: int, page_size: int, heads_kv: int, head_dim: int, dtype=torch.bfloat16, device="cuda",
                  max_len: int | None = None, layers: int = 1, k_scale=None, v_scale=None):
@@ -115,30 +119,39 @@ class PagedKVCache:
         self.k_scale, self.v_scale = k_scale, v_scale
         width = -(-self.max_len // page_size)
         self._table = torch.full((batch, width), -1, dtype=torch.int32)
-        self._lens = torch.zeros(batch, dtype=torch.int32)
+        self._state = torch.zeros((2, batch), dtype=torch.int32)
+        self._lens, self._new = self._state[0], self._state[1]
+        self._appended, self._captured = False, False
         self._free = list(range(pages - 1, -1, -1))
-        self.table, self.lens = self._table.to(device), self._lens.to(device)
+        self.table, self._device_state = self._table.to(device), self._state.to(device)
+        self.lens, self.new = self._device_state[0], self._device_state[1]
 
     def length(self, b: int) -> int:
         return int(self._lens[b])
 
     def extend(self, new) -> None:
         """Adds new[b] positions (an int: the same for all) to every sequence, with pages for them; raises and changes
-        nothing where a sequence would pass max_len or the pages run out."""
+        nothing where a sequence would pass max_len or the pages run out. They are the sequence's new positions until the
+        extend() after the next append(), or, once an append() has been captured and may be replayed, until the next."""
         counts = [int(new)] * len(self._lens) if isinstance(new, int) else [int(n) for n in new]
         if len(counts) != len(self._lens) or min(counts) < 0:
             raise _abi.TvkError(_abi.TVK_ERR_INVALID, "extend: a count of at least zero for each sequence is expected")
-        ends = [self.length(b) + n for b, n in enumerate(counts)]
+        lens = self._lens.tolist()
+        ends = [n + more for n, more in zip(lens, counts)]
         if max(ends) > self.max_len:
             raise _abi.TvkError(_abi.TVK_ERR_INVALID, f"extend: a sequence of {max(ends)} positions, the cache's longest are {self.max_len}")
-        have = [-(-self.length(b) // self.page_size) for b in range(len(ends))]
+        have = [-(-n // self.page_size) for n in lens]
         need = [-(-end // self.page_size) for end in ends]
         if sum(need) - sum(have) > len(self._free):
             raise _abi.TvkOutOfMemory(_abi.TVK_ERR_OOM, f"extend: {sum(need) - sum(have)} pages are wanted, {len(self._free)} are free")
-        for b, end in enumerate(ends):
+        for b in range(len(ends)):
             for i in range(have[b], need[b]):
                 self._table[b, i] = self._free.pop()
-            self._lens[b] = end
+        if self._appended or self._captured:
+            self._new.zero_()
+            self._appended = False
+        self._new += torch.tensor(counts, dtype=torch.int32)
+        self._lens.copy_(torch.tensor(ends, dtype=torch.int32))
         self._sync(sum(need) != sum(have))
 
     def release(self, b: int) -> None:
@@ -146,29 +159,31 @@ class PagedKVCache:
         for i in range(-(-self.length(b) // self.page_size)):
             self._free.append(int(self._table[b, i]))
             self._table[b, i] = -1
-        self._lens[b] = 0
+        self._lens[b] = self._new[b] = 0
         self._sync(True)
 
     def _sync(self, table: bool) -> None:
         if table:
             self.table.copy_(self._table)
-        self.lens.copy_(self._lens)
+        self._device_state.copy_(self._state)
 
     def append(self, q, k, v, rotary=None, interleaved: bool = False, out=None, layer: int = 0):
         """Writes the newest positions' keys and values, rotated as `rotary` says, and returns their rotated queries
-        (tokens [batch, new, heads, head_dim]; sequences with fewer new positions are padded in front). out may be q."""
+        (tokens [batch, new, heads, head_dim]; sequences with fewer new positions are padded in front, and that padding is
+        not written and gives zeros). out may be q."""
         out = torch.empty(q.shape, dtype=q.dtype, device=q.device) if out is None and q is not None else out
         d = _abi.make_paged_append_desc(q, k, v, out, self.k[layer], self.v[layer], self.lens, self.table, rotary, interleaved,
-                                        self.k_scale, self.v_scale, _stream(k))
+                                        self.k_scale, self.v_scale, _stream(k), self.new)
         _abi.check(_abi.load().tvk_paged_append(C.byref(d)))
+        self._appended, self._captured = True, self._captured or _capturing(k)
         return out
 
     def attend(self, q, scale: float | None = None, window: int = 0, out=None, max_len: int | None = None, layer: int = 0):
-        """Attention of the newest positions' queries over their sequences. max_len: a bound on the lengths, for a call
-        that is captured and replayed; else the longest sequence's."""
+        """Attention of the new positions' queries over their sequences (zeros for padding in front of them). max_len: a
+        bound on the lengths, for a call that is captured and replayed; else the longest sequence's."""
         out = torch.empty(q.shape, dtype=q.dtype, device=q.device) if out is None else out
         d = _abi.make_paged_attention_desc(q, self.k[layer], self.v[layer], out, self.lens, self.table,
                                            max_len or max(1, int(self._lens.max())), scale, window, self.k_scale, self.v_scale,
-                                           stream=_stream(q))
+                                           stream=_stream(q), new_lens=self.new)
         _abi.check(_abi.load().tvk_paged_attention(C.byref(d)))
         return out
