@@ -1,4 +1,5 @@
-"""The paged cache's count of each sequence's new positions, on the host."""
+"""The paged cache of torchvulkan_amd.decoder on the host: the count of each sequence's new positions, and which calls it
+makes of the library."""
 import pytest
 import torch
 
@@ -59,3 +60,28 @@ def test_binding_refuses_other_counts():
             _abi.make_paged_attention_desc(q, k, k, q, lens, table, new_lens=bad)
         with pytest.raises(_abi.TvkError):
             _abi.make_paged_append_desc(q, kv, kv, q, k, k, lens, table, new_lens=bad)
+
+
+@pytest.mark.parametrize("other", ["q", "k", "v", "rotary", "out", "k_scale", "v_scale"])
+def test_tensors_of_another_device_are_refused(calls, other):
+    # "meta" stands for a device that the cache's kernels cannot read
+    dtype = torch.float8_e4m3fn if "scale" in other else torch.float32
+    cache = decoder.PagedKVCache(2, 40, 4, 1, 8, dtype, "cpu", k_scale=torch.ones(1), v_scale=torch.ones(1)) \
+        if "scale" in other else decoder.PagedKVCache(2, 40, 4, 1, 8, dtype, "cpu")
+    cache.extend(1)
+    t = {n: torch.zeros((2, 1, 1, 8)) for n in ("q", "k", "v", "out")}
+    t["rotary"] = decoder.rotary_table(9, 8)
+    cache.append(**t)
+    cache.attend(t["q"], out=t["out"])
+    assert len(calls) == 2
+    if "scale" in other:
+        setattr(cache, other, getattr(cache, other).to("meta"))
+    else:
+        t[other] = t[other].to("meta")
+    with pytest.raises(_abi.TvkError) as e:
+        cache.append(**t)
+    assert e.value.status == _abi.TVK_ERR_INVALID
+    if other not in ("k", "v", "rotary"):
+        with pytest.raises(_abi.TvkError):
+            cache.attend(t["q"], out=t["out"])
+    assert len(calls) == 2

@@ -64,12 +64,17 @@ class _RmsNorm(torch.autograd.Function):
         return dx, dw, dx if ctx.added else None, None
 
 
+def _check_devices(device, *tensors) -> None:
+    """Kernels follow every address they are given: none may be another device's, or the host's."""
+    for t in tensors:
+        if t is not None and t.device != device:
+            raise _abi.TvkError(_abi.TVK_ERR_INVALID, f"tensors on {device} and {t.device}")
+
+
 def _check_norm(x, weight, residual) -> None:
     if x.dim() == 0 or (residual is not None and (residual.shape != x.shape or residual.dtype != x.dtype)):
         raise _abi.TvkError(_abi.TVK_ERR_INVALID, "x: [..., cols], and a residual of its shape and dtype, are expected")
-    for t in (weight, residual):
-        if t is not None and t.device != x.device:
-            raise _abi.TvkError(_abi.TVK_ERR_INVALID, f"tensors on {x.device} and {t.device}")
+    _check_devices(x.device, weight, residual)
 
 
 def rms_norm(x, weight=None, residual=None, eps: float = 1e-5):
@@ -95,7 +100,8 @@ def rms_norm_fp8(x, weight=None, residual=None, eps: float = 1e-5):
 
 
 def rotary_table(positions: int, rotary_dim: int, base: float = 10000.0, device="cpu") -> torch.Tensor:
-    """The angles of positions 0 .. positions - 1: float32 [positions, rotary_dim], cosines then sines, from 64 bits."""
+    """The angles of positions 0 .. positions - 1: float32 [positions, rotary_dim], cosines then sines, from 64 bits.
+    append() takes one on its cache's device."""
     angle = torch.arange(positions, dtype=torch.float64)[:, None] * torch.pow(
         torch.tensor(base, dtype=torch.float64), -torch.arange(0, rotary_dim, 2, dtype=torch.float64) / rotary_dim)
     return torch.cat([angle.cos(), angle.sin()], 1).float().to(device)
@@ -171,6 +177,7 @@ class PagedKVCache:
         """Writes the newest positions' keys and values, rotated as `rotary` says, and returns their rotated queries
         (tokens [batch, new, heads, head_dim]; sequences with fewer new positions are padded in front, and that padding is
         not written and gives zeros). out may be q."""
+        _check_devices(self.k.device, q, k, v, rotary, out, self.k_scale, self.v_scale)
         out = torch.empty(q.shape, dtype=q.dtype, device=q.device) if out is None and q is not None else out
         d = _abi.make_paged_append_desc(q, k, v, out, self.k[layer], self.v[layer], self.lens, self.table, rotary, interleaved,
                                         self.k_scale, self.v_scale, _stream(k), self.new)
@@ -181,6 +188,7 @@ class PagedKVCache:
     def attend(self, q, scale: float | None = None, window: int = 0, out=None, max_len: int | None = None, layer: int = 0):
         """Attention of the new positions' queries over their sequences (zeros for padding in front of them). max_len: a
         bound on the lengths, for a call that is captured and replayed; else the longest sequence's."""
+        _check_devices(self.k.device, q, out, self.k_scale, self.v_scale)
         out = torch.empty(q.shape, dtype=q.dtype, device=q.device) if out is None else out
         d = _abi.make_paged_attention_desc(q, self.k[layer], self.v[layer], out, self.lens, self.table,
                                            max_len or max(1, int(self._lens.max())), scale, window, self.k_scale, self.v_scale,
