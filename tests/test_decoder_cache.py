@@ -85,3 +85,15 @@ def test_tensors_of_another_device_are_refused(calls, other):
         with pytest.raises(_abi.TvkError):
             cache.attend(t["q"], out=t["out"])
     assert len(calls) == 2
+
+
+def test_a_captured_call_is_bounded_by_the_cache(calls, monkeypatch):
+    cache = decoder.PagedKVCache(2, 40, 4, 1, 8, torch.float32, "cpu", max_len=60)
+    q = torch.zeros((2, 1, 1, 8))
+    cache.extend([7, 3])
+    cache.attend(q)
+    cache.attend(q, max_len=20)
+    monkeypatch.setattr(decoder, "_capturing", lambda t: True)
+    cache.attend(q)
+    cache.attend(q, max_len=20)
+    assert [d.max_len for _, d in calls] == [7, 20, 60, 20]

@@ -157,3 +157,28 @@ def test_tokens_of_two_extends_in_one_append(gpu):
     cache.append(None, k, k)
     for b, n in enumerate((5, 4)):
         assert torch.equal(cache.k[0, cache.table[b, 0], :n], k[b, 5 - n:])
+
+
+def test_replays_past_the_captured_length(gpu):
+    # a step captured without a bound follows sequences that grow past what they were at capture
+    hq, hkv, dim = 4, 2, 64
+    cache = decoder.PagedKVCache(2, 120, 16, hkv, dim, BF16, "cuda", max_len=900)
+    rotary = decoder.rotary_table(900, dim, device="cuda")
+    q, k, v = (rand((2, 1, h, dim), BF16, 1).cuda() for h in (hq, hkv, hkv))
+    cache.extend([5, 30])
+    prompt = rand((2, 30, hkv, dim), BF16, 2).cuda()
+    cache.append(None, prompt, prompt, rotary)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = cache.attend(cache.append(q, k, v, rotary))
+    for step in range(3):
+        if step:   # many positions at once, then a token at a time again
+            more = rand((2, 300, hkv, dim), BF16, 3 + step).cuda()
+            cache.extend(300)
+            cache.append(None, more, more, rotary)
+        for t, seed in ((q, 10), (k, 20), (v, 30)):
+            t.copy_(rand(t.shape, BF16, seed + step))
+        cache.extend(1)
+        graph.replay()
+        captured = out.clone()
+        assert torch.equal(captured, cache.attend(cache.append(q, k, v, rotary), max_len=900))

@@ -187,11 +187,13 @@ class PagedKVCache:
 
     def attend(self, q, scale: float | None = None, window: int = 0, out=None, max_len: int | None = None, layer: int = 0):
         """Attention of the new positions' queries over their sequences (zeros for padding in front of them). max_len: a
-        bound on the lengths, for a call that is captured and replayed; else the longest sequence's."""
+        bound on the lengths, past which keys are cut off; without it the longest sequence's, or, in a call that is captured
+        and replayed for other lengths, the cache's."""
         _check_devices(self.k.device, q, out, self.k_scale, self.v_scale)
         out = torch.empty(q.shape, dtype=q.dtype, device=q.device) if out is None else out
+        max_len = max_len or (self.max_len if _capturing(q) else max(1, int(self._lens.max())))
         d = _abi.make_paged_attention_desc(q, self.k[layer], self.v[layer], out, self.lens, self.table,
-                                           max_len or max(1, int(self._lens.max())), scale, window, self.k_scale, self.v_scale,
-                                           stream=_stream(q), new_lens=self.new)
+                                           max_len, scale, window, self.k_scale, self.v_scale, stream=_stream(q),
+                                           new_lens=self.new)
         _abi.check(_abi.load().tvk_paged_attention(C.byref(d)))
         return out
