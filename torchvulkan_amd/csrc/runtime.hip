@@ -96,7 +96,7 @@ void release_cached_locked(int device) {
 // device-wide drain before any free (every call makes the device current for
 // its duration).
 struct HipScratchBackend {
-    typedef hipStream_t Stream;
+    typedef ThreadStream<hipStream_t> Stream;
     int device = 0;
 
     struct On {
@@ -188,8 +188,17 @@ void* Scratch::get(size_t bytes, hipStream_t stream) {
     int dev = 0;
     if (hipGetDevice(&dev) != hipSuccess || dev < 0 || dev >= kMaxDevices) return nullptr;
     auto& pool = device_scratch(dev)->pool;
+    const HipScratchBackend::Stream key(stream, stream == hipStreamPerThread);
     HipScratchBackend::Capture c;
-    auto* buf = capture_of(stream, c) ? pool.acquire_captured(bytes, stream, c) : pool.acquire(bytes, stream);
+    const bool captured = capture_of(stream, c);
+    if (key.thread && !captured) {
+        // once a thread and device: the buffers of threads that have ended
+        static thread_local uint64_t trimmed = 0;
+        static_assert(kMaxDevices <= 64, "a bit for each device");
+        if (!(trimmed >> dev & 1)) pool.trim_gone();
+        trimmed |= (uint64_t)1 << dev;
+    }
+    auto* buf = captured ? pool.acquire_captured(bytes, key, c) : pool.acquire(bytes, key);
     if (!buf) return nullptr;
     lease_ = buf;
     device_ = dev;

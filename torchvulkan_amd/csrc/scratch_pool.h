@@ -20,6 +20,8 @@
 //     on the same stream (which the graph orders behind it), and neither leased
 //     to any other call nor freed before the graph and everything instantiated
 //     from it are gone, which the backend reports through `returned`.
+//   - a handle that stands for a stream of each thread (hipStreamPerThread) is no
+//     one stream: its buffers are kept by ThreadStream, the handle and the thread.
 // The logic is independent of HIP: the backend supplies allocation and the
 // device-wide wait, so the ownership rules can be exercised on the CPU with a
 // model backend.
@@ -33,6 +35,37 @@
 #include <vector>
 
 namespace tvk {
+
+// Of the calling thread, and of no other that was or will be.
+struct ThreadMark {
+    uint64_t id;
+    std::shared_ptr<std::atomic<bool>> ended;
+    static const ThreadMark& mine() {
+        struct Mark : ThreadMark {
+            ~Mark() { ended->store(true); }
+        };
+        static std::atomic<uint64_t> next{1};
+        thread_local Mark m{{next.fetch_add(1), std::make_shared<std::atomic<bool>>(false)}};
+        return m;
+    }
+};
+
+// A stream as the pool tells them apart: a handle, with the thread where the handle means another stream in each.
+template <class Handle>
+struct ThreadStream {
+    Handle handle{};
+    uint64_t thread = 0;
+    std::shared_ptr<std::atomic<bool>> ended;   // the thread has
+
+    ThreadStream() = default;
+    ThreadStream(Handle h, bool of_thread) : handle(h) {
+        if (!of_thread) return;
+        thread = ThreadMark::mine().id;
+        ended = ThreadMark::mine().ended;
+    }
+    bool operator==(const ThreadStream& o) const { return handle == o.handle && thread == o.thread; }
+    bool gone() const { return ended && *ended; }
+};
 
 // Backend B provides:
 //   typedef ... Stream;
@@ -152,6 +185,12 @@ public:
     void trim() {
         std::lock_guard<std::mutex> lk(mu_);
         retire_idle_locked([](const Buffer&) { return true; });
+    }
+
+    // Frees the idle buffers of streams that are gone with their threads.
+    void trim_gone() {
+        std::lock_guard<std::mutex> lk(mu_);
+        retire_idle_locked([](const Buffer& b) { return b.stream.gone(); });
     }
 
     size_t buffer_count() {
