@@ -66,3 +66,31 @@ def test_norm_gradients_from_threads(gpu, cols):
         assert torch.equal(dx, want[0]) and torch.equal(dw, want[1])
 
     in_threads(work)
+
+
+@pytest.mark.gpu
+def test_paged_attention_from_threads(gpu):
+    # long sequences are cut there as on any stream (joined by a second launch, with the same bits)
+    lens, page, hkv, dim, lib = [20000, 700], 16, 2, 128, _abi.load()
+    table = torch.arange(2 * 1250, dtype=torch.int32).view(2, 1250).cuda()
+    seq = torch.tensor(lens, dtype=torch.int32).cuda()
+    calls = []
+    for i in range(4):
+        g = torch.Generator(device="cuda").manual_seed(i)
+        k, v = (torch.randn((2500, page, hkv, dim), generator=g, device="cuda").to(torch.bfloat16) for _ in range(2))
+        q = torch.randn((2, 1, 8, dim), generator=g, device="cuda").to(torch.bfloat16)
+        want, _ = _abi.paged_attention(q, k, v, seq, table)
+        out = torch.empty_like(q)
+        calls.append((_abi.make_paged_attention_desc(q, k, v, out, seq, table, stream=PER_THREAD), out, want, (q, k, v)))
+    torch.cuda.synchronize()
+
+    def work(i):
+        d, out, want, _ = calls[i]
+        for _ in range(20):
+            out.fill_(float("nan"))
+            torch.cuda.synchronize()
+            _abi.check(lib.tvk_paged_attention(C.byref(d)))
+            torch.cuda.synchronize()
+            assert torch.equal(out, want)
+
+    in_threads(work)

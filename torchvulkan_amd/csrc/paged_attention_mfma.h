@@ -1029,7 +1029,7 @@ void paged_launch(PagedMfmaArgs& p, int64_t batch, hipStream_t s) {
     if (paged_is_dealt(p.plan.many, tiles * G::BN)) {
         const int64_t wgs = paged_wgs(p.plan.many, segments, tiles, p.plan.resident);
         const size_t rows = (size_t)2 * wgs * 16 * CT, bytes = rows * (p.a.c.hd + 4) * 4;
-        float* part = s == hipStreamPerThread || bytes >= (size_t)1 << 31
+        float* part = bytes >= (size_t)1 << 31
                           ? nullptr : static_cast<float*>(scratch.get(bytes + (size_t)segments * 8, s));
         if (part) {
             p.plan.wgs = (int)wgs;
