@@ -157,10 +157,11 @@ extern "C" tvk_status tvk_paged_attention(const tvk_paged_attention_desc* d) {
     const hipStream_t s = resolve_stream(d->stream);
     const int64_t rows = d->batch * d->new_tokens * d->heads_q;
     const bool f8 = c.dtype == TVK_F8E4M3FN;
-    if (paged_attn_mfma(p, d->dtype, f8, d->batch, s)) return TVK_OK;
-    if (d->dtype == TVK_F32) f8 ? launch_any<TVK_F32, true>(p, rows, s) : launch_any<TVK_F32, false>(p, rows, s);
-    else if (d->dtype == TVK_F16) f8 ? launch_any<TVK_F16, true>(p, rows, s) : launch_any<TVK_F16, false>(p, rows, s);
-    else f8 ? launch_any<TVK_BF16, true>(p, rows, s) : launch_any<TVK_BF16, false>(p, rows, s);
+    if (!paged_attn_mfma(p, d->dtype, f8, d->batch, s)) {
+        if (d->dtype == TVK_F32) f8 ? launch_any<TVK_F32, true>(p, rows, s) : launch_any<TVK_F32, false>(p, rows, s);
+        else if (d->dtype == TVK_F16) f8 ? launch_any<TVK_F16, true>(p, rows, s) : launch_any<TVK_F16, false>(p, rows, s);
+        else f8 ? launch_any<TVK_BF16, true>(p, rows, s) : launch_any<TVK_BF16, false>(p, rows, s);
+    }
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return fail(TVK_ERR_DEVICE, std::string(who) + ": launch failed: " + hipGetErrorString(e));
     return TVK_OK;
