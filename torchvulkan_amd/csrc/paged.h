@@ -6,6 +6,7 @@
 
 namespace tvk {
 
+constexpr int64_t kGridThreads = 0xffffffff;     // of a launch in one dimension of its grid
 constexpr int64_t kMaxReach = (int64_t)1 << 30;   // positions: index sums stay in 32 bits
 
 struct PagedCache {
@@ -36,7 +37,8 @@ struct PagedAttnArgs {
     float scale;
 };
 
-// Queues the MFMA kernel (paged_attention_mfma.h) when it takes the call; false when it does not.
+// Queues the MFMA kernel (paged_attention_mfma.h) when it takes the call; false when it does not, its launch having too
+// many workgroups among the reasons.
 bool paged_attn_mfma(const PagedAttnArgs& a, int dtype, bool f8, int64_t batch, hipStream_t s);
 
 // TVK_OK when the cache is one the kernels take and its pointers are there.

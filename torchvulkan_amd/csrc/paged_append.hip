@@ -86,6 +86,7 @@ struct AppendArgs {
     int heads_q;
     int64_t tokens;         // batch * new tokens
     Div32 split;            // waves a token
+    uint32_t width;         // workgroups in the grid's first dimension, which does not hold those of 2^26 tokens
     int same_place;         // a lane's chunks lie in the same place of every head it meets
     Div32 per_head, per_token, new_tokens;
 };
@@ -164,7 +165,7 @@ template <int DT, bool F8, int VEC>
 __global__ __launch_bounds__(AP_THREADS) void paged_append_kernel(AppendArgs p) {
     typedef typename elem<DT>::T T;
     constexpr int B = VEC * (int)sizeof(T), A = (int)sizeof(T);
-    const uint32_t wave = __builtin_amdgcn_readfirstlane(blockIdx.x * (AP_THREADS / 64) + threadIdx.x / 64);
+    const uint32_t wave = __builtin_amdgcn_readfirstlane((blockIdx.y * p.width + blockIdx.x) * (AP_THREADS / 64) + threadIdx.x / 64);
     const uint32_t token = div32(wave, p.split), part = wave - token * p.split.d;
     if (token >= p.tokens) return;
     uint32_t b, t, page, slot;
@@ -273,7 +274,9 @@ void append(AppendArgs& p, hipStream_t s) {
     const int64_t split = std::min(all, room);
     p.split = make_div((uint32_t)split);
     p.same_place = 64 * split % per_head == 0;
-    const dim3 grid((unsigned)((p.tokens * split + 3) / 4)), block(AP_THREADS);
+    const int64_t wgs = (p.tokens * split + 3) / 4;   // below 2^30: more than 8192 tokens take a wave each
+    p.width = (uint32_t)std::min<int64_t>(wgs, 1 << 23);
+    const dim3 grid(p.width, (unsigned)((wgs + p.width - 1) / p.width)), block(AP_THREADS);
     if constexpr (DT != TVK_F32) {
         if (vec == 8) {
             hipLaunchKernelGGL((paged_append_kernel<DT, F8, 8>), grid, block, 0, s, p);

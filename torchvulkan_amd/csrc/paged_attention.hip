@@ -25,12 +25,14 @@ __device__ inline float cached(const void* p, int64_t i) {
 }
 
 template <int DT, bool F8, int ND>
-__global__ __launch_bounds__(64 * PA_WAVES) void paged_attn_any_kernel(PagedAttnArgs p) {
+__global__ __launch_bounds__(64 * PA_WAVES) void paged_attn_any_kernel(PagedAttnArgs p, int64_t rows) {
     typedef typename elem<DT>::T T;
     __shared__ float red[PA_WAVES][64 * ND];
     __shared__ float ml[PA_WAVES][2];
     const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
-    const int h = blockIdx.x % p.heads, bt = blockIdx.x / p.heads;
+    const int64_t row = (int64_t)blockIdx.y * gridDim.x + blockIdx.x;   // a dimension of the grid does not hold them all
+    if (row >= rows) return;
+    const int h = (int)(row % p.heads), bt = (int)(row / p.heads);
     const int t = bt % p.new_tokens, b = bt / p.new_tokens, hk = h / p.group;
     const int hd = p.c.hd;
     const int len = (int)min((uint32_t)paged_len(p.c, b), p.max_len);
@@ -111,11 +113,12 @@ __global__ __launch_bounds__(64 * PA_WAVES) void paged_attn_any_kernel(PagedAttn
 
 template <int DT, bool F8>
 void launch_any(const PagedAttnArgs& p, int64_t rows, hipStream_t s) {
-    const dim3 grid((unsigned)rows), block(64 * PA_WAVES);
-    if (p.c.hd <= 64) hipLaunchKernelGGL((paged_attn_any_kernel<DT, F8, 1>), grid, block, 0, s, p);
-    else if (p.c.hd <= 128) hipLaunchKernelGGL((paged_attn_any_kernel<DT, F8, 2>), grid, block, 0, s, p);
-    else if (p.c.hd <= 256) hipLaunchKernelGGL((paged_attn_any_kernel<DT, F8, 4>), grid, block, 0, s, p);
-    else hipLaunchKernelGGL((paged_attn_any_kernel<DT, F8, 8>), grid, block, 0, s, p);
+    const int64_t x = std::min<int64_t>(rows, 1 << 23);
+    const dim3 grid((unsigned)x, (unsigned)((rows + x - 1) / x)), block(64 * PA_WAVES);
+    if (p.c.hd <= 64) hipLaunchKernelGGL((paged_attn_any_kernel<DT, F8, 1>), grid, block, 0, s, p, rows);
+    else if (p.c.hd <= 128) hipLaunchKernelGGL((paged_attn_any_kernel<DT, F8, 2>), grid, block, 0, s, p, rows);
+    else if (p.c.hd <= 256) hipLaunchKernelGGL((paged_attn_any_kernel<DT, F8, 4>), grid, block, 0, s, p, rows);
+    else hipLaunchKernelGGL((paged_attn_any_kernel<DT, F8, 8>), grid, block, 0, s, p, rows);
 }
 
 }  // namespace

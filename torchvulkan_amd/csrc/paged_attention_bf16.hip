@@ -3,8 +3,8 @@
 
 namespace tvk {
 
-void paged_attn_bf16(PagedMfmaArgs& p, bool f8, int64_t batch, hipStream_t s) {
-    f8 ? paged_dispatch<TVK_BF16, true>(p, batch, s) : paged_dispatch<TVK_BF16, false>(p, batch, s);
+bool paged_attn_bf16(PagedMfmaArgs& p, bool f8, int64_t batch, hipStream_t s) {
+    return f8 ? paged_dispatch<TVK_BF16, true>(p, batch, s) : paged_dispatch<TVK_BF16, false>(p, batch, s);
 }
 
 }  // namespace tvk

@@ -3,7 +3,7 @@
 
 namespace tvk {
 
-void paged_attn_f32(PagedMfmaArgs& p, int64_t batch, hipStream_t s) { paged_dispatch<TVK_F32, false>(p, batch, s); }
+bool paged_attn_f32(PagedMfmaArgs& p, int64_t batch, hipStream_t s) { return paged_dispatch<TVK_F32, false>(p, batch, s); }
 
 // Head dims in 16s up to 256, rows whose 16-byte chunks are aligned, cache offsets that fit 32 bits in units of 16 bytes.
 bool paged_attn_mfma(const PagedAttnArgs& a, int dtype, bool f8, int64_t batch, hipStream_t s) {
@@ -36,10 +36,7 @@ bool paged_attn_mfma(const PagedAttnArgs& a, int dtype, bool f8, int64_t batch, 
     const double tiles = (a.max_len + 15.0) / 16 + 1.0;
     if (nr > 0x7fffffff || (double)batch * ((nr + 15) / 16) * c.kvh * tiles >= 0x1p31) return false;
     p.rows = (int)nr;
-    if (f32) paged_attn_f32(p, batch, s);
-    else if (dtype == TVK_F16) paged_attn_f16(p, f8, batch, s);
-    else paged_attn_bf16(p, f8, batch, s);
-    return true;
+    return f32 ? paged_attn_f32(p, batch, s) : dtype == TVK_F16 ? paged_attn_f16(p, f8, batch, s) : paged_attn_bf16(p, f8, batch, s);
 }
 
 }  // namespace tvk

@@ -998,8 +998,9 @@ constexpr int PM_CUS = 256;
 constexpr double PM_JOIN_ALONE = 4096;
 constexpr int PM_SPREAD = 5, PM_COUNTERS = 16384;
 
+// False, and nothing queued, where the launch would have too many threads.
 template <int DT, bool F8, int D, int CT>
-void paged_launch(PagedMfmaArgs& p, int64_t batch, hipStream_t s) {
+bool paged_launch(PagedMfmaArgs& p, int64_t batch, hipStream_t s) {
     typedef PagedTile<DT, F8, D> G;
     const int nrb = (p.rows + 16 * CT - 1) / (16 * CT);
     p.nrb = make_div((uint32_t)nrb);
@@ -1019,14 +1020,16 @@ void paged_launch(PagedMfmaArgs& p, int64_t batch, hipStream_t s) {
     const int64_t tiles = (keys + G::BN - 1) / G::BN;   // at most, of a segment
     p.plan.resident = PM_CUS * G::occ(CT);
     if (tiles * G::BN <= 32 * (segments > p.plan.resident ? PM_WAVE_MANY : PM_WAVE)) {
+        if (segments * 64 > kGridThreads) return false;
         const dim3 grid((unsigned)segments), block(64);
         if (fast) hipLaunchKernelGGL((paged_attn_mfma_kernel<DT, F8, D, CT, true, 1>), grid, block, 0, s, p);
         else hipLaunchKernelGGL((paged_attn_mfma_kernel<DT, F8, D, CT, false, 1>), grid, block, 0, s, p);
-        return;
+        return true;
     }
+    if (segments * 64 * PM_WAVES > kGridThreads) return false;
     Scratch scratch;
     p.plan.many = paged_many(segments, p.plan.resident);
-    if (paged_is_dealt(p.plan.many, tiles * G::BN)) {
+    if (paged_is_dealt(p.plan.many, tiles * G::BN) && segments * PM_JOIN_THREADS <= kGridThreads) {
         const int64_t wgs = paged_wgs(p.plan.many, segments, tiles, p.plan.resident);
         const size_t rows = (size_t)2 * wgs * 16 * CT, bytes = rows * (p.a.c.hd + 4) * 4;
         float* part = bytes >= (size_t)1 << 31
@@ -1053,29 +1056,30 @@ void paged_launch(PagedMfmaArgs& p, int64_t batch, hipStream_t s) {
         p.slices = (int)std::min<int64_t>(std::min(p.rows, 16 * CT), std::max<int64_t>(1, 2048 / segments));
         hipLaunchKernelGGL((paged_attn_join_kernel<DT, CT>), dim3((unsigned)(segments * p.slices)), dim3(PM_JOIN_THREADS), 0, s, p);
     }
+    return true;
 }
 
 template <int DT, bool F8>
-void paged_dispatch(PagedMfmaArgs& p, int64_t batch, hipStream_t s) {
+bool paged_dispatch(PagedMfmaArgs& p, int64_t batch, hipStream_t s) {
     const bool two = p.rows > 16;
     const int hd = p.a.c.hd;
 #define TVK_PAGED(D) (two ? paged_launch<DT, F8, D, 2>(p, batch, s) : paged_launch<DT, F8, D, 1>(p, batch, s))
     if constexpr (!F8) {   // 8-bit rows of 32 bytes would be values of half a word a lane
         if (hd <= 32) return TVK_PAGED(32);
     }
-    if (hd <= 64) TVK_PAGED(64);
-    else if (hd <= 96) TVK_PAGED(96);
-    else if (hd <= 128) TVK_PAGED(128);
-    else if constexpr (DT == TVK_F32) paged_launch<DT, F8, 256, 1>(p, batch, s);   // two row blocks' registers would spill
-    else TVK_PAGED(256);
+    if (hd <= 64) return TVK_PAGED(64);
+    if (hd <= 96) return TVK_PAGED(96);
+    if (hd <= 128) return TVK_PAGED(128);
+    if constexpr (DT == TVK_F32) return paged_launch<DT, F8, 256, 1>(p, batch, s);   // two row blocks' registers would spill
+    else return TVK_PAGED(256);
 #undef TVK_PAGED
 }
 
 }  // namespace
 
 // One translation unit each (paged_attention_f16.hip and its neighbours).
-void paged_attn_f16(PagedMfmaArgs& p, bool f8, int64_t batch, hipStream_t s);
-void paged_attn_bf16(PagedMfmaArgs& p, bool f8, int64_t batch, hipStream_t s);
-void paged_attn_f32(PagedMfmaArgs& p, int64_t batch, hipStream_t s);
+bool paged_attn_f16(PagedMfmaArgs& p, bool f8, int64_t batch, hipStream_t s);
+bool paged_attn_bf16(PagedMfmaArgs& p, bool f8, int64_t batch, hipStream_t s);
+bool paged_attn_f32(PagedMfmaArgs& p, int64_t batch, hipStream_t s);
 
 }  // namespace tvk
