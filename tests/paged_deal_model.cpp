@@ -5,7 +5,8 @@
 //   2. a segment's pieces agree on their number and on the first, and come once;
 //   3. a segment in one piece is whole;
 //   4. pieces that are kept for a join lie in places of their own, inside the buffer.
-// Arguments: BN CT resident kvh group new window shared batch longest shortest.
+// Arguments: BN CT resident kvh group new window shared batch longest shortest power: lengths rise to the longest as the power of a
+// line.
 // Prints "ok", the launch's workgroups (0: segments of so few keys are not cut) and the kept pieces' places; a violation
 // ends it with a message.
 #include "paged_deal.h"
@@ -78,7 +79,9 @@ void run(const Call& c, int64_t& launch, uint32_t& places) {
 
     std::vector<std::vector<Kept>> of((size_t)segments);
     places = 0;
-    std::vector<char> taken((size_t)2 * p.wgs, 0);
+    std::vector<char> taken((size_t)2 * paged_places(p.many, p.wgs, p.resident), 0);
+    std::vector<uint64_t> tile0((size_t)items + 1, 0);   // tiles before an item
+    for (int64_t e = 0; e < items; ++e) tile0[(size_t)e + 1] = tile0[(size_t)e] + (uint64_t)tiles[(size_t)e] * c.kvh;
     for (uint32_t launched = 0; launched < (uint32_t)p.wgs; ++launched) {
         uint32_t wg = launched, x, stop = 0;
         if (p.shared && wg < d.used / 8 * 8) wg = wg % 8 * (d.used / 8) + wg / 8;
@@ -94,9 +97,9 @@ void run(const Call& c, int64_t& launch, uint32_t& places) {
             const int64_t segment = (int64_t)pc.item * c.kvh + pc.hk;
             if (pc.hk >= c.kvh) die("a head past the last", pc.item, pc.hk);
             if (d.shift >= 0) {
-                paged_chunk(x, at, n, units, rcp((float)units), pc);
+                paged_chunk(p, d, x, (uint32_t)tile0[(size_t)pc.item] + (uint32_t)pc.hk * n, at, n, units, rcp((float)units), pc);
             } else {
-                paged_stretch(d, x, at, n, stop, rcp((float)d.per), pc);
+                paged_stretch(d, wg, x, at, n, stop, rcp((float)d.per), pc);
                 x += n - at;
                 more = x < stop;
                 at = (uint32_t)(pc.hk + 1) * n;
@@ -107,11 +110,10 @@ void run(const Call& c, int64_t& launch, uint32_t& places) {
             }
             if (pc.c0 >= pc.c1) continue;
             if (pc.c1 > n) die("tiles past a segment's last", (long long)segment, pc.c1);
-            const uint32_t i = wg - pc.first;
-            of[(size_t)segment].push_back(Kept{pc.c0, pc.c1, pc.first, pc.pieces, i});
+            of[(size_t)segment].push_back(Kept{pc.c0, pc.c1, pc.first, pc.pieces, pc.i});
             if (pc.pieces == 1) continue;
-            if (i >= pc.pieces || (i == 0) != (pc.c0 == 0)) die("a piece that is not one of its segment's", (long long)segment, i);
-            const uint32_t slot = paged_slot(pc.first, i);
+            if (pc.i >= pc.pieces || (pc.i == 0) != (pc.c0 == 0)) die("a piece that is not one of its segment's", (long long)segment, pc.i);
+            const uint32_t slot = paged_slot(pc.first, pc.i);
             if (slot >= taken.size()) die("a place past the buffer", (long long)segment, slot);
             if (taken[slot]++) die("a place that is kept twice", (long long)segment, slot);
             places = std::max(places, slot + 1);
@@ -124,6 +126,7 @@ void run(const Call& c, int64_t& launch, uint32_t& places) {
         for (const Kept& k : v) {
             if (k.c0 != at) die("a tile that none or two pieces have", (long long)s, k.c0);
             if (k.first != v[0].first || k.pieces != v.size()) die("pieces that disagree", (long long)s, k.pieces);
+            if (v.size() > 1 && k.i != (uint32_t)(&k - v.data())) die("pieces out of order", (long long)s, k.i);
             at = k.c1;
         }
         if (at != tiles[(size_t)(s / c.kvh)]) die("tiles that no piece has", (long long)s, at);
@@ -133,11 +136,11 @@ void run(const Call& c, int64_t& launch, uint32_t& places) {
 }  // namespace
 
 int main(int argc, char** argv) {
-    if (argc != 12) return 2;
-    long long a[11];
-    for (int i = 0; i < 11; ++i) a[i] = std::atoll(argv[i + 1]);
+    if (argc != 13) return 2;
+    long long a[12];
+    for (int i = 0; i < 12; ++i) a[i] = std::atoll(argv[i + 1]);
     Call c{(int)a[0], (int)a[1], (int)a[2], (int)a[3], (int)a[4], a[5], a[6], (int)a[7], {}};
-    for (long long i = 0; i < a[8]; ++i) c.lens.push_back(a[9] - (a[9] - a[10]) * i / std::max(1LL, a[8] - 1));
+    for (long long i = 0; i < a[8]; ++i) c.lens.push_back(a[10] + (int64_t)((double)(a[9] - a[10]) * std::pow((double)(i + 1) / (double)a[8], (double)a[11])));
     int64_t launch = 0;
     uint32_t places = 0;
     for (g_off = -1; g_off <= 1; ++g_off) {

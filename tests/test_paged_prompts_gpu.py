@@ -6,6 +6,8 @@ their magnitudes' sum and its exponential by that and 2 u of the score, twice; t
 probability-weighted |v|; a probability rounded to a 16-bit type is off by eps / 2, and so is the output."""
 from __future__ import annotations
 
+import ctypes as C
+
 import pytest
 import torch
 
@@ -98,3 +100,32 @@ def test_prompt_of_more_workgroups_than_stretches(gpu):
     q = rand((1, 42000, 32, 128), BF16, 1)
     got, lse = _abi.paged_attention(q, *cache.args(), max_len=42000)
     check(got, lse, q, cache, 128 ** -0.5, step=2000)
+
+
+def reserved():
+    v = C.c_size_t()
+    _abi.check(_abi.load().tvk_memory_reserved(0, C.byref(v)))
+    return v.value
+
+
+def test_scratch_of_a_prompt(gpu):
+    # partials go by the workgroups that run together: a prompt of 8192 segments takes no more than the pool's smallest buffers
+    cache = Prompts([8192], 8, 128, BF16, page=64)
+    q = rand((1, 8192, 32, 128), BF16, 1)
+    torch.cuda.synchronize()
+    _abi.check(_abi.load().tvk_empty_cache(0))
+    before = reserved()
+    eager, _ = _abi.paged_attention(q, *cache.args(), max_len=8192)
+    assert reserved() - before <= 32 << 20
+    out, graph = torch.empty_like(q), torch.cuda.CUDAGraph()
+    before = reserved()
+    with torch.cuda.graph(graph, stream=torch.cuda.Stream()):
+        d = _abi.make_paged_attention_desc(q, cache.k, cache.v, out, cache.lens, cache.table, max_len=8192,
+                                           stream=torch.cuda.current_stream().cuda_stream)
+        _abi.check(_abi.load().tvk_paged_attention(C.byref(d)))
+    assert reserved() - before <= 32 << 20
+    for _ in range(2):
+        out.fill_(float("nan"))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, eager)

@@ -61,8 +61,9 @@ struct PagedMfmaArgs {
     int items;             // batch * row blocks of a key/value head
     PagedPlan plan;        // wgs 0: a workgroup a segment
     Div32 nrb, kvh, group;
-    float* part_o;         // [2 * wgs][16 * CT][hd]
-    float* part_ml;        // [2][2 * wgs][16 * CT][2]: max, sum; again where a run's result is kept
+    int places;            // workgroups whose pieces are kept
+    float* part_o;         // [2 * places][16 * CT][hd]
+    float* part_ml;        // [2][2 * places][16 * CT][2]: max, sum; again where a run's result is kept
     unsigned part_bytes;   // of both
     // finished pieces (or runs) of every segment, then finished pieces of the run that begins in every slot; zero before
     // and after the launch. NULL: a second launch joins, one of `slices` workgroups some of a segment's rows, and
@@ -155,24 +156,29 @@ __device__ __forceinline__ PagedDeal paged_deal_of(const PagedMfmaArgs& p, int l
     return paged_deal<BN>(p.plan, wave_sum(n) * p.kvh.d, count, [](float x) { return wave_rcp(x); });
 }
 
-// The item that holds unit x of the call, and the unit's place among the item's; false past the last.
+// The item that holds unit x of the call, the unit's place among the item's, and, where many segments are cut into chunks,
+// the item's first tile of the call; false past the last.
 template <int BN, int CT>
 __device__ __forceinline__ bool paged_locate(const PagedMfmaArgs& p, const PagedDeal& d, uint32_t x, int lane, uint32_t mine, int& item,
-                                             uint32_t& at) {
-    uint32_t base = 0;
+                                             uint32_t& at, uint32_t& begin) {
+    uint32_t base = 0, tiles = 0;
+    const bool begins = p.plan.many && d.shift >= 0;
     for (int e0 = 0;;) {
         const uint32_t n = mine ? d.units(mine) * p.kvh.d : 0;
         const uint32_t s = base + wave_scan(n);
+        const uint32_t ts = begins ? tiles + wave_scan(mine * p.kvh.d) : 0;
         const uint64_t past = __ballot(s > x);
         if (past) {
             const int l = __ffsll((unsigned long long)past) - 1;
             item = e0 + l;
             at = x - (uint32_t)__builtin_amdgcn_readlane((int)(s - n), l);
+            begin = (uint32_t)__builtin_amdgcn_readlane((int)(ts - mine * p.kvh.d), l);
             return true;
         }
         e0 += 64;
         if (e0 >= p.items) return false;
         base = (uint32_t)__builtin_amdgcn_readlane((int)s, 63);
+        tiles = (uint32_t)__builtin_amdgcn_readlane((int)ts, 63);
         mine = e0 + lane < p.items ? (uint32_t)paged_span<BN, CT>(p, e0 + lane).tiles : 0;
     }
 }
@@ -254,7 +260,7 @@ struct PagedParts {
     __device__ __forceinline__ PagedParts(const PagedMfmaArgs& a)
         : p(a), rs(__builtin_amdgcn_make_buffer_rsrc((void*)a.part_o, 0, (int)a.part_bytes, 0x00020000)) {}
     // byte offsets: below 2 GiB; of a run's result in the place of its first piece, whose max and sum others still read
-    __device__ __forceinline__ int run_ml_at(uint32_t slot, int lr) const { return ml_at(slot + 2 * p.plan.wgs, lr); }
+    __device__ __forceinline__ int run_ml_at(uint32_t slot, int lr) const { return ml_at(slot + 2 * p.places, lr); }
     __device__ __forceinline__ int o_at(uint32_t slot, int lr, int dv) const {
         return (int)(((slot * 16 * CT + lr) * (uint32_t)p.a.c.hd + dv) * 4);
     }
@@ -486,7 +492,7 @@ __global__ __launch_bounds__(64 * WAVES, (PagedTile<DT, F8, D>::occ(CT))) void p
     PagedDeal deal{31, 0, 0, 0, 0};
     PagedPiece pc, part[2];   // part: pieces of segments that others share, the one that begins its segment second
     int parts = 0;
-    uint32_t at = 0, x = wg, stop = 0;
+    uint32_t at = 0, x = wg, stop = 0, begin = 0;
     const bool dealt = WAVES > 1 && paged_args().plan.wgs;
     if (!dealt) {
         const PagedMfmaArgs& p = paged_args();
@@ -501,7 +507,7 @@ __global__ __launch_bounds__(64 * WAVES, (PagedTile<DT, F8, D>::occ(CT))) void p
         deal = paged_deal_of<BN, CT>(p, lane, mine);
         // a stretch of neighbours' work for each XCD
         if (p.plan.shared && wg < deal.used / 8 * 8) wg = wg % 8 * (deal.used / 8) + wg / 8;
-        if (!paged_start(deal, wg, x, stop) || !paged_locate<BN, CT>(p, deal, x, lane, mine, pc.item, at)) return;
+        if (!paged_start(deal, wg, x, stop) || !paged_locate<BN, CT>(p, deal, x, lane, mine, pc.item, at, begin)) return;
     }
 
     for (bool more_pieces = true; more_pieces;) {
@@ -525,9 +531,9 @@ __global__ __launch_bounds__(64 * WAVES, (PagedTile<DT, F8, D>::occ(CT))) void p
             pc.hk = (int)wave_div(at, units);
             at -= (uint32_t)pc.hk * units;   // of the segment
             if (deal.shift >= 0) {
-                paged_chunk(x, at, tiles, units, wave_rcp((float)units), pc);
+                paged_chunk(p.plan, deal, x, begin + (uint32_t)pc.hk * tiles, at, tiles, units, wave_rcp((float)units), pc);
             } else {
-                paged_stretch(deal, x, at, tiles, stop, wave_rcp((float)deal.per), pc);
+                paged_stretch(deal, wg, x, at, tiles, stop, wave_rcp((float)deal.per), pc);
                 // the next segment: the item's next head, or the next item's first
                 x += tiles - at;
                 more_pieces = x < stop;
@@ -936,7 +942,7 @@ __global__ __launch_bounds__(64 * WAVES, (PagedTile<DT, F8, D>::occ(CT))) void p
                     s.add(ml[0][w][lr], ml[1][w][lr], *reinterpret_cast<const f32x4*>(&red[(w * COLS + lr) * LDO + dv]));
                 if (__builtin_expect(several && has_marks, 0)) s.o = marked(lr, dv, s.o);
                 if (whole) PagedRow(pe, b, hk, r0 + lr, s.m, s.l).template store<DT>(pe, dv, s.o);
-                else PagedParts<CT, true>(pe).store(2 * wg + (pc.c0 == 0), lr, dv, s, true);
+                else PagedParts<CT, true>(pe).store(paged_slot(pc.first, pc.i), lr, dv, s, true);
             }
             if (!whole && pe.count) {
                 const int second = pc.c0 == 0;
@@ -955,7 +961,7 @@ __global__ __launch_bounds__(64 * WAVES, (PagedTile<DT, F8, D>::occ(CT))) void p
             const PagedPiece& q = part[0];
             const int item = i ? part[1].item : q.item, hk = i ? part[1].hk : q.hk;
             const uint32_t first = i ? part[1].first : q.first, pieces = i ? part[1].pieces : q.pieces;
-            paged_join<DT, CT>(paged_args(), item, hk, first, pieces, wg - first, reinterpret_cast<char*>(red), &flag);
+            paged_join<DT, CT>(paged_args(), item, hk, first, pieces, i ? part[1].i : q.i, reinterpret_cast<char*>(red), &flag);
         }
     }
 }
@@ -996,6 +1002,9 @@ constexpr int PM_CUS = 256;
 // Quads of columns and pieces of an average segment up to which its last workgroup joins it: beyond, the second launch's
 // many workgroups are faster (float16 1 x 16/4 heads, 4 tokens, 32576 keys of 128: 22 us, 28 joined by the last ones).
 constexpr double PM_JOIN_ALONE = 4096;
+// Values of the row blocks from which segments are whole whatever their keys (bfloat16 32/8 heads of 128, 512 new tokens of
+// 4000 for 128 sequences: 9.3 ms whole, 18.4 in stretches).
+constexpr double PM_WHOLE_VALUES = 0x1p28;
 constexpr int PM_SPREAD = 5, PM_COUNTERS = 16384;
 
 // False, and nothing queued, where the launch would have too many threads.
@@ -1029,13 +1038,15 @@ bool paged_launch(PagedMfmaArgs& p, int64_t batch, hipStream_t s) {
     if (segments * 64 * PM_WAVES > kGridThreads) return false;
     Scratch scratch;
     p.plan.many = paged_many(segments, p.plan.resident);
-    if (paged_is_dealt(p.plan.many, tiles * G::BN) && segments * PM_JOIN_THREADS <= kGridThreads) {
-        const int64_t wgs = paged_wgs(p.plan.many, segments, tiles, p.plan.resident);
-        const size_t rows = (size_t)2 * wgs * 16 * CT, bytes = rows * (p.a.c.hd + 4) * 4;
-        float* part = bytes >= (size_t)1 << 31
-                          ? nullptr : static_cast<float*>(scratch.get(bytes + (size_t)segments * 8, s));
+    const int64_t wgs = paged_wgs(p.plan.many, segments, tiles, p.plan.resident);
+    const bool most = (double)wgs * 16 * CT * (p.a.c.hd + 4) >= PM_WHOLE_VALUES;
+    if (paged_is_dealt(p.plan.many, tiles * G::BN) && !most && segments * PM_JOIN_THREADS <= kGridThreads) {
+        const int64_t places = paged_places(p.plan.many, wgs, p.plan.resident);
+        const size_t rows = (size_t)2 * places * 16 * CT, bytes = rows * (p.a.c.hd + 4) * 4;
+        float* part = static_cast<float*>(scratch.get(bytes + (size_t)segments * 8, s));   // (at most 2^28 bytes of partials)
         if (part) {
             p.plan.wgs = (int)wgs;
+            p.places = (int)places;
             p.part_o = part;
             p.part_ml = part + rows * p.a.c.hd;
             p.part_bytes = (unsigned)bytes;
@@ -1043,8 +1054,8 @@ bool paged_launch(PagedMfmaArgs& p, int64_t batch, hipStream_t s) {
             const double pieces = std::min((double)p.plan.resident / segments, (double)tiles / PM_WAVES);
             const double wide = std::max(1.0, pieces) * std::min(p.rows, 16 * CT) * p.a.c.hd / 4;
             p.spread = PM_SPREAD;
-            while (p.spread > 0 && (segments << p.spread) + 2 * wgs > PM_COUNTERS) --p.spread;
-            p.count = wide > PM_JOIN_ALONE ? nullptr : split_counters(s, (segments << p.spread) + 2 * wgs);
+            while (p.spread > 0 && (segments << p.spread) + 2 * places > PM_COUNTERS) --p.spread;
+            p.count = wide > PM_JOIN_ALONE ? nullptr : split_counters(s, (segments << p.spread) + 2 * places);
         } else {
             clear_error();
         }

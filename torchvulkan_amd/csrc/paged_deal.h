@@ -48,6 +48,10 @@ TVK_DEAL int64_t paged_wgs(bool many, int64_t segments, int64_t tiles, int64_t r
     return many ? segments + 2 * resident : some < resident ? some : resident;
 }
 
+// Workgroups whose pieces have a place in the scratch: those that share a segment with others. Many segments are cut into
+// at most 2 * resident chunks beside the whole ones, or into a stretch for each resident workgroup.
+TVK_DEAL int64_t paged_places(bool many, int64_t wgs, int64_t resident) { return many ? 2 * resident : wgs; }
+
 struct PagedDeal {
     int shift;        // segments are cut into chunks of at least 2^shift tiles; -1: stretches
     uint32_t per;     // tiles a workgroup's stretch has
@@ -96,11 +100,11 @@ TVK_DEAL bool paged_start(const PagedDeal& d, uint32_t wg, uint32_t& x, uint32_t
     return true;
 }
 
-// A stretch of a segment's tiles, [c0, c1), and the workgroups whose pieces make up the segment.
+// Piece i of a segment: a stretch of its tiles, [c0, c1); how many there are, and the place of the first.
 struct PagedPiece {
     int item, hk;
     uint32_t c0, c1;
-    uint32_t first, pieces;
+    uint32_t first, pieces, i;
 };
 
 // Where the end of a stretch at tile x of a segment's tiles lies.
@@ -108,22 +112,27 @@ TVK_DEAL uint32_t paged_cut(const PagedDeal& d, uint32_t x, uint32_t tiles) {
     return x <= d.snap ? 0 : tiles - x <= d.snap ? tiles : x;
 }
 
-// The chunk `at` of a segment that is cut into `units`; it is workgroup x's.
-TVK_DEAL void paged_chunk(uint32_t x, uint32_t at, uint32_t tiles, uint32_t units, float r_units, PagedPiece& pc) {
+// The chunk `at` of a segment that is cut into `units`; it is workgroup x's. `begin`: the segment's first tile of the call,
+// which says where its pieces are kept where many segments are whole: k chunks have 2^shift * k tiles and more, and floor(a)
+// + floor(b) <= floor(a + b).
+TVK_DEAL void paged_chunk(const PagedPlan& p, const PagedDeal& d, uint32_t x, uint32_t begin, uint32_t at, uint32_t tiles,
+                          uint32_t units, float r_units, PagedPiece& pc) {
     const uint32_t q = small_div(tiles, units, r_units), r = tiles - q * units;
     pc.c0 = at * q + (at < r ? at : r);
     pc.c1 = pc.c0 + q + (at < r);
-    pc.first = x - at;
+    pc.first = p.many ? begin >> d.shift : x - at;
     pc.pieces = units;
+    pc.i = at;
 }
 
-// The piece of a segment from its tile `at`, tile x of the call, on, of a stretch that ends at `stop`. Ends of stretches
-// inside a segment that do not move to its ends cut it.
-TVK_DEAL void paged_stretch(const PagedDeal& d, uint32_t x, uint32_t at, uint32_t tiles, uint32_t stop, float r_per, PagedPiece& pc) {
+// The piece of a segment from its tile `at`, tile x of the call, on, of workgroup wg's stretch that ends at `stop`. Ends of
+// stretches inside a segment that do not move to its ends cut it.
+TVK_DEAL void paged_stretch(const PagedDeal& d, uint32_t wg, uint32_t x, uint32_t at, uint32_t tiles, uint32_t stop, float r_per, PagedPiece& pc) {
     const uint32_t begin = x - at;
     pc.first = small_div(begin + d.snap, d.per, r_per);
     const uint32_t last = tiles > 2 * d.snap ? small_div(begin + tiles - d.snap - 1, d.per, r_per) : 0;
     pc.pieces = last > pc.first ? last - pc.first + 1 : 1;
+    pc.i = wg - pc.first;
     pc.c0 = paged_cut(d, at, tiles);
     pc.c1 = stop - x < tiles - at ? paged_cut(d, at + (stop - x), tiles) : tiles;
 }
