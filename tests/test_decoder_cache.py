@@ -97,3 +97,38 @@ def test_a_captured_call_is_bounded_by_the_cache(calls, monkeypatch):
     cache.attend(q)
     cache.attend(q, max_len=20)
     assert [d.max_len for _, d in calls] == [7, 20, 60, 20]
+
+
+def test_a_backward_pass_ends_at_calls_without_a_gradient(calls):
+    cache = decoder.PagedKVCache(2, 40, 4, 1, 8, torch.float32, "cpu")
+    x = torch.zeros((2, 1, 1, 8))
+    leaf = torch.ones((2, 1, 1, 8), requires_grad=True)
+    cache.extend(1)
+    for result in (lambda: cache.append(leaf * 2, x, x), lambda: cache.append(x, leaf * 2, x), lambda: cache.append(x, x, leaf * 2),
+                   lambda: cache.attend(leaf * 2), lambda: decoder.rms_norm_fp8(leaf * 2)[1],
+                   lambda: decoder.rms_norm_fp8(x, residual=leaf * 2)[2],
+                   lambda: decoder.rms_norm_fp8(x, leaf.view(-1)[:8])[0].float()):
+        with pytest.raises(_abi.TvkUnsupported):
+            (result() + leaf.view(-1)[0]).sum().backward()
+        with torch.no_grad():
+            assert not result().requires_grad
+    assert not cache.attend(cache.append(x, x, x)).requires_grad
+    assert decoder.rms_norm_fp8(leaf)[2] is leaf
+    out = torch.empty_like(x)
+    assert cache.attend(x, out=out) is out and cache.append(out, x, x, out=out) is out
+
+
+def test_a_tensor_that_is_written_is_known_to_autograd(calls):
+    # what was kept for a backward pass may not be written behind its back
+    cache = decoder.PagedKVCache(2, 40, 4, 1, 8, torch.float32, "cpu")
+    x = torch.zeros((2, 1, 1, 8))
+    cache.extend(1)
+    for write in (lambda q: cache.append(q, x, x, out=q), lambda q: cache.attend(x, out=q)):
+        q = torch.rand((2, 1, 1, 8))
+        w = torch.ones((), requires_grad=True)
+        y = q * w
+        write(q)
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            y.sum().backward()
+        with torch.inference_mode():
+            write(torch.rand((2, 1, 1, 8)))

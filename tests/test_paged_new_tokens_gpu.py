@@ -182,3 +182,16 @@ def test_replays_past_the_captured_length(gpu):
         graph.replay()
         captured = out.clone()
         assert torch.equal(captured, cache.attend(cache.append(q, k, v, rotary), max_len=900))
+
+
+def test_backward_passes_end_at_the_cache(gpu):
+    # (the device whose autograd the package serves)
+    cache = decoder.PagedKVCache(2, 8, 16, 1, 16, torch.float32, "vulkan")
+    x = rand((2, 1, 1, 16), torch.float32, 1).to("vulkan")
+    leaf = x.clone().requires_grad_()
+    cache.extend(1)
+    for result in (lambda: cache.append(leaf * 2, x, x), lambda: cache.attend(leaf * 2), lambda: decoder.rms_norm_fp8(leaf * 2)[1]):
+        with pytest.raises(_abi.TvkUnsupported):
+            result().sum().backward()
+    out = torch.empty_like(x)
+    assert torch.equal(cache.attend(leaf).detach().cpu(), cache.attend(x, out=out).cpu())

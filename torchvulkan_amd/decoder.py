@@ -28,6 +28,35 @@ def _capturing(t: torch.Tensor) -> bool:
     return t.device.type == "cuda" and torch.cuda.is_current_stream_capturing()
 
 
+class _WithoutGradient(torch.autograd.Function):
+    """The results of a call that has no gradient: a backward pass that reaches them ends there with an error, where it
+    would go past tensors that know of no inputs."""
+
+    @staticmethod
+    def forward(ctx, name, count, *tensors):
+        ctx.name = name
+        ctx.set_materialize_grads(False)
+        results = tuple(t.detach() for t in tensors[:count])
+        return results if count > 1 else results[0]
+
+    @staticmethod
+    def backward(ctx, *grads):
+        raise _abi.TvkUnsupported(_abi.TVK_ERR_UNSUPPORTED, f"{ctx.name} has no gradient")
+
+
+def _without_gradient(name: str, results, *inputs):
+    if not torch.is_grad_enabled() or not any(t is not None and t.requires_grad for t in inputs):
+        return results
+    many = results if isinstance(results, tuple) else (results,)
+    return _WithoutGradient.apply(name, len(many), *many, *(t for t in inputs if t is not None))
+
+
+def _written(t: torch.Tensor) -> None:
+    """Autograd learns of a caller's tensor that a kernel wrote."""
+    if not t.is_inference():
+        torch.autograd.graph.increment_version(t)
+
+
 def _rows(t: torch.Tensor) -> torch.Tensor:
     """[..., cols] as [rows, cols] with contiguous rows (a copy only where the strides allow no view)."""
     t = t.reshape(-1, t.shape[-1])
@@ -78,8 +107,9 @@ def _check_norm(x, weight, residual) -> None:
 
 
 def rms_norm(x, weight=None, residual=None, eps: float = 1e-5):
-    """x / sqrt(mean(x^2) + eps) * weight over the last dimension; with a residual (y, h) of h = x + residual.
-    Differentiable in x, weight and residual (tvk_rms_norm_fwd, tvk_rms_norm_bwd)."""
+    """x / sqrt(mean(x^2) + eps) * weight over the last dimension; with a residual (y, h) of h = x + residual
+    (tvk_rms_norm_fwd, tvk_rms_norm_bwd). Differentiable in x, weight and residual on the vulkan device; torch's engine
+    follows one accelerator's streams, and refuses a backward pass of cuda tensors once the vulkan device is registered."""
     _check_norm(x, weight, residual)
     y, h = _RmsNorm.apply(x, weight, residual, float(eps))
     return y if residual is None else (y, h)
@@ -87,7 +117,7 @@ def rms_norm(x, weight=None, residual=None, eps: float = 1e-5):
 
 def rms_norm_fp8(x, weight=None, residual=None, eps: float = 1e-5):
     """(y, scale, h): the norm in float8_e4m3fn with a float32 scale for each row, y * scale[..., None] being the norm;
-    h is x without a residual. No gradient."""
+    h is x without a residual. No gradient: a backward pass that reaches the results raises."""
     _check_norm(x, weight, residual)
     x2 = _rows(x.detach())
     y = torch.empty(x2.shape, dtype=torch.float8_e4m3fn, device=x.device)
@@ -96,7 +126,10 @@ def rms_norm_fp8(x, weight=None, residual=None, eps: float = 1e-5):
     h = None if r2 is None else torch.empty(x2.shape, dtype=x.dtype, device=x.device)
     d = _abi.make_rms_norm_desc(x2, weight, y, r2, h, scale, eps, _stream(x))
     _abi.check(_abi.load().tvk_rms_norm_fwd(C.byref(d)))
-    return y.view(x.shape), scale.view(x.shape[:-1]), x if h is None else h.view(x.shape)
+    out = y.view(x.shape), scale.view(x.shape[:-1])
+    if h is None:
+        return *_without_gradient("rms_norm_fp8", out, x, weight), x
+    return _without_gradient("rms_norm_fp8", (*out, h.view(x.shape)), x, weight, residual)
 
 
 def rotary_table(positions: int, rotary_dim: int, base: float = 10000.0, device="cpu") -> torch.Tensor:
@@ -113,7 +146,8 @@ class PagedKVCache:
 
     The host keeps the sequences' lengths and free pages; extend() gives sequences new positions, release() ends one.
     Both only write the device's `table`, `lens` and `new` (how many of each sequence's positions are new), which the calls
-    read there, so a captured step (append, attend) replays for other lengths. dtype float8_e4m3fn keeps 8 bits, divided by k_scale and v_scale of each head."""
+    read there, so a captured step (append, attend) replays for other lengths. append and attend have no gradient: a
+    backward pass that reaches their results raises. dtype float8_e4m3fn keeps 8 bits, divided by k_scale and v_scale of each head."""
 
     def __init__(self, batch: int, pages: int, page_size: int, heads_kv: int, head_dim: int, dtype=torch.bfloat16, device="cuda",
                  max_len: int | None = None, layers: int = 1, k_scale=None, v_scale=None):
@@ -178,22 +212,28 @@ class PagedKVCache:
         (tokens [batch, new, heads, head_dim]; sequences with fewer new positions are padded in front, and that padding is
         not written and gives zeros). out may be q."""
         _check_devices(self.k.device, q, k, v, rotary, out, self.k_scale, self.v_scale)
+        given = out is not None
         out = torch.empty(q.shape, dtype=q.dtype, device=q.device) if out is None and q is not None else out
         d = _abi.make_paged_append_desc(q, k, v, out, self.k[layer], self.v[layer], self.lens, self.table, rotary, interleaved,
                                         self.k_scale, self.v_scale, _stream(k), self.new)
         _abi.check(_abi.load().tvk_paged_append(C.byref(d)))
         self._appended, self._captured = True, self._captured or _capturing(k)
-        return out
+        if given:
+            _written(out)
+        return out if out is None else _without_gradient("PagedKVCache.append", out, q, k, v)
 
     def attend(self, q, scale: float | None = None, window: int = 0, out=None, max_len: int | None = None, layer: int = 0):
         """Attention of the new positions' queries over their sequences (zeros for padding in front of them). max_len: a
         bound on the lengths, past which keys are cut off; without it the longest sequence's, or, in a call that is captured
         and replayed for other lengths, the cache's."""
         _check_devices(self.k.device, q, out, self.k_scale, self.v_scale)
+        given = out is not None
         out = torch.empty(q.shape, dtype=q.dtype, device=q.device) if out is None else out
         max_len = max_len or (self.max_len if _capturing(q) else max(1, int(self._lens.max())))
         d = _abi.make_paged_attention_desc(q, self.k[layer], self.v[layer], out, self.lens, self.table,
                                            max_len, scale, window, self.k_scale, self.v_scale, stream=_stream(q),
                                            new_lens=self.new)
         _abi.check(_abi.load().tvk_paged_attention(C.byref(d)))
-        return out
+        if given:
+            _written(out)
+        return _without_gradient("PagedKVCache.attend", out, q)
