@@ -132,3 +132,13 @@ def test_a_tensor_that_is_written_is_known_to_autograd(calls):
             y.sum().backward()
         with torch.inference_mode():
             write(torch.rand((2, 1, 1, 8)))
+
+
+def test_norm_of_rows_without_values(calls):
+    for x in (torch.zeros((3, 5, 0)), torch.zeros((0, 0)), torch.zeros((0, 8)), torch.zeros(0)):
+        w = torch.ones(x.shape[-1])
+        y, h = decoder.rms_norm(x, w, x)
+        assert y.shape == h.shape == x.shape
+        y, scale, _ = decoder.rms_norm_fp8(x, w)
+        assert y.shape == x.shape and scale.shape == x.shape[:-1]
+    assert [(d.rows, d.cols) for _, d in calls[::2]] == [(15, 0), (0, 0), (0, 8), (1, 0)]

@@ -641,8 +641,8 @@ extern "C" tvk_status tvk_rms_norm_fwd(const tvk_rms_norm_desc* d) {
     const bool out8 = d->out_dtype == TVK_F8E4M3FN;
     if (!out8 && d->out_dtype != d->dtype)
         return fail(TVK_ERR_UNSUPPORTED, "tvk_rms_norm_fwd: the output's dtype must be the input's or float8_e4m3fn");
-    if (d->rows == 0 || d->cols == 0) return TVK_OK;
-    if (!d->x || !d->out || (out8 && !d->scale)) return fail(TVK_ERR_INVALID, "tvk_rms_norm_fwd: NULL tensor");
+    if (d->rows == 0 || (d->cols == 0 && !out8)) return TVK_OK;   // rows without values have a scale all the same
+    if ((d->cols > 0 && (!d->x || !d->out)) || (out8 && !d->scale)) return fail(TVK_ERR_INVALID, "tvk_rms_norm_fwd: NULL tensor");
     if (d->x_stride < 0 || (d->residual && d->residual_stride < 0) || !rows_apart(d->out_stride, d->rows, d->cols) ||
         (d->residual_out && !rows_apart(d->residual_out_stride, d->rows, d->cols)))
         return fail(TVK_ERR_INVALID, "tvk_rms_norm_fwd: negative strides, or output rows that overlap");

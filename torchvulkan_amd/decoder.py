@@ -6,6 +6,7 @@ these operators from element-wise shaders and keeps dense caches."""
 from __future__ import annotations
 
 import ctypes as C
+import math
 
 import torch
 
@@ -59,7 +60,7 @@ def _written(t: torch.Tensor) -> None:
 
 def _rows(t: torch.Tensor) -> torch.Tensor:
     """[..., cols] as [rows, cols] with contiguous rows (a copy only where the strides allow no view)."""
-    t = t.reshape(-1, t.shape[-1])
+    t = t.reshape(math.prod(t.shape[:-1]), t.shape[-1])
     return t if t.shape[-1] <= 1 or t.stride(1) == 1 else t.contiguous()
 
 
