@@ -83,78 +83,84 @@ __device__ inline float block_all(float v) {
     return v;
 }
 
+// Workgroups that take rows in turn, 2^32 threads in a dimension of a grid being too many.
+dim3 rows_grid(int64_t rows) { return dim3((unsigned)std::min<int64_t>(rows, 1 << 16)); }
+
 template <int DT>
 __global__ __launch_bounds__(RN_THREADS) void rms_norm_any_kernel(NormArgs p) {
     typedef typename elem<DT>::T T;
-    const int64_t row = blockIdx.x;
-    const T* x = static_cast<const T*>(p.x) + row * p.sx;
-    const T* r = p.r ? static_cast<const T*>(p.r) + row * p.sr : nullptr;
-    T* h = p.h ? static_cast<T*>(p.h) + row * p.sh : nullptr;
-    auto value = [&](int64_t c) {
-        float v = at<DT>(x, c);
-        if (r) v = elem<DT>::to_f32(elem<DT>::from_f32(v + at<DT>(r, c)));
-        return v;
-    };
-    float ss = 0.0f;
-    for (int64_t c = threadIdx.x; c < p.cols; c += RN_THREADS) {
-        const float v = value(c);
-        ss += v * v;
-        if (h) put<DT>(h, c, v);
-    }
-    const float inv = 1.0f / sqrtf(block_all<SumOp>(ss) / (float)p.cols + p.eps);
-    // residual_out may lie over x or residual: from here on h is read back
-    auto norm = [&](int64_t c) { return (h ? at<DT>(h, c) : value(c)) * inv * weight_at<DT>(p.w, p.w32, c); };
-    if (p.out8) {
-        float top = 0.0f;
-        for (int64_t c = threadIdx.x; c < p.cols; c += RN_THREADS) top = fmaxf(top, fabsf(norm(c)));
-        top = block_all<MaxOp>(top);
-        const float s = top > 0.0f ? top / kF8Max : 1.0f;
-        if (threadIdx.x == 0) p.scale[row] = s;
-        uint8_t* o = static_cast<uint8_t*>(p.out) + row * p.so;
-        for (int64_t c = threadIdx.x; c < p.cols; c += RN_THREADS) o[c] = f32_to_f8(norm(c) / s, TVK_F8E4M3FN);
-    } else {
-        T* o = static_cast<T*>(p.out) + row * p.so;
-        for (int64_t c = threadIdx.x; c < p.cols; c += RN_THREADS) put<DT>(o, c, norm(c));
+    for (int64_t row = blockIdx.x; row < p.rows; row += gridDim.x) {
+        const T* x = static_cast<const T*>(p.x) + row * p.sx;
+        const T* r = p.r ? static_cast<const T*>(p.r) + row * p.sr : nullptr;
+        T* h = p.h ? static_cast<T*>(p.h) + row * p.sh : nullptr;
+        auto value = [&](int64_t c) {
+            float v = at<DT>(x, c);
+            if (r) v = elem<DT>::to_f32(elem<DT>::from_f32(v + at<DT>(r, c)));
+            return v;
+        };
+        float ss = 0.0f;
+        for (int64_t c = threadIdx.x; c < p.cols; c += RN_THREADS) {
+            const float v = value(c);
+            ss += v * v;
+            if (h) put<DT>(h, c, v);
+        }
+        const float inv = 1.0f / sqrtf(block_all<SumOp>(ss) / (float)p.cols + p.eps);
+        // residual_out may lie over x or residual: from here on h is read back
+        auto norm = [&](int64_t c) { return (h ? at<DT>(h, c) : value(c)) * inv * weight_at<DT>(p.w, p.w32, c); };
+        if (p.out8) {
+            float top = 0.0f;
+            for (int64_t c = threadIdx.x; c < p.cols; c += RN_THREADS) top = fmaxf(top, fabsf(norm(c)));
+            top = block_all<MaxOp>(top);
+            const float s = top > 0.0f ? top / kF8Max : 1.0f;
+            if (threadIdx.x == 0) p.scale[row] = s;
+            uint8_t* o = static_cast<uint8_t*>(p.out) + row * p.so;
+            for (int64_t c = threadIdx.x; c < p.cols; c += RN_THREADS) o[c] = f32_to_f8(norm(c) / s, TVK_F8E4M3FN);
+        } else {
+            T* o = static_cast<T*>(p.out) + row * p.so;
+            for (int64_t c = threadIdx.x; c < p.cols; c += RN_THREADS) put<DT>(o, c, norm(c));
+        }
     }
 }
 
 // 1 / sqrt(mean(h^2) + eps) of every row, for dweight's sums. dx comes after those: it may lie over dy or h.
 template <int DT>
 __global__ __launch_bounds__(RN_THREADS) void rms_norm_inv_kernel(NormBwdArgs p) {
-    const int64_t row = blockIdx.x;
-    const void* h = static_cast<const typename elem<DT>::T*>(p.h) + row * p.sh;
-    float ss = 0.0f;
-    for (int64_t c = threadIdx.x; c < p.cols; c += RN_THREADS) {
-        const float v = at<DT>(h, c);
-        ss += v * v;
+    for (int64_t row = blockIdx.x; row < p.rows; row += gridDim.x) {
+        const void* h = static_cast<const typename elem<DT>::T*>(p.h) + row * p.sh;
+        float ss = 0.0f;
+        for (int64_t c = threadIdx.x; c < p.cols; c += RN_THREADS) {
+            const float v = at<DT>(h, c);
+            ss += v * v;
+        }
+        ss = block_all<SumOp>(ss);
+        if (threadIdx.x == 0) p.inv[row] = 1.0f / sqrtf(ss / (float)p.cols + p.eps);
     }
-    ss = block_all<SumOp>(ss);
-    if (threadIdx.x == 0) p.inv[row] = 1.0f / sqrtf(ss / (float)p.cols + p.eps);
 }
 
 template <int DT>
 __global__ __launch_bounds__(RN_THREADS) void rms_norm_bwd_any_kernel(NormBwdArgs p) {
     typedef typename elem<DT>::T T;
-    const int64_t row = blockIdx.x;
-    const T* dy = static_cast<const T*>(p.dy) + row * p.sdy;
-    const T* h = static_cast<const T*>(p.h) + row * p.sh;
-    const T* dh = p.dh ? static_cast<const T*>(p.dh) + row * p.sdh : nullptr;
-    float ss = 0.0f, gh = 0.0f;
-    for (int64_t c = threadIdx.x; c < p.cols; c += RN_THREADS) {
-        const float v = at<DT>(h, c);
-        ss += v * v;
-        gh += at<DT>(dy, c) * weight_at<DT>(p.w, p.w32, c) * v;
-    }
-    ss = block_all<SumOp>(ss);
-    gh = block_all<SumOp>(gh);
-    const float inv = 1.0f / sqrtf(ss / (float)p.cols + p.eps);
-    const float mean = gh * inv / (float)p.cols;   // of g * n
-    T* dx = static_cast<T*>(p.dx) + row * p.sdx;
-    for (int64_t c = threadIdx.x; c < p.cols; c += RN_THREADS) {
-        const float g = at<DT>(dy, c) * weight_at<DT>(p.w, p.w32, c);
-        float v = inv * (g - at<DT>(h, c) * inv * mean);
-        if (dh) v += at<DT>(dh, c);
-        put<DT>(dx, c, v);
+    for (int64_t row = blockIdx.x; row < p.rows; row += gridDim.x) {
+        const T* dy = static_cast<const T*>(p.dy) + row * p.sdy;
+        const T* h = static_cast<const T*>(p.h) + row * p.sh;
+        const T* dh = p.dh ? static_cast<const T*>(p.dh) + row * p.sdh : nullptr;
+        float ss = 0.0f, gh = 0.0f;
+        for (int64_t c = threadIdx.x; c < p.cols; c += RN_THREADS) {
+            const float v = at<DT>(h, c);
+            ss += v * v;
+            gh += at<DT>(dy, c) * weight_at<DT>(p.w, p.w32, c) * v;
+        }
+        ss = block_all<SumOp>(ss);
+        gh = block_all<SumOp>(gh);
+        const float inv = 1.0f / sqrtf(ss / (float)p.cols + p.eps);
+        const float mean = gh * inv / (float)p.cols;   // of g * n
+        T* dx = static_cast<T*>(p.dx) + row * p.sdx;
+        for (int64_t c = threadIdx.x; c < p.cols; c += RN_THREADS) {
+            const float g = at<DT>(dy, c) * weight_at<DT>(p.w, p.w32, c);
+            float v = inv * (g - at<DT>(h, c) * inv * mean);
+            if (dh) v += at<DT>(dh, c);
+            put<DT>(dx, c, v);
+        }
     }
 }
 
@@ -574,7 +580,7 @@ void forward(const NormArgs& p, hipStream_t s) {
         if (p.out8) hipLaunchKernelGGL((rms_norm_kernel<DT, true, NC, TPR>), grid, block, 0, s, p);
         else hipLaunchKernelGGL((rms_norm_kernel<DT, false, NC, TPR>), grid, block, 0, s, p);
     });
-    if (!done) hipLaunchKernelGGL((rms_norm_any_kernel<DT>), dim3((unsigned)p.rows), dim3(RN_THREADS), 0, s, p);
+    if (!done) hipLaunchKernelGGL((rms_norm_any_kernel<DT>), rows_grid(p.rows), dim3(RN_THREADS), 0, s, p);
 }
 
 template <int DT>
@@ -602,11 +608,11 @@ tvk_status backward(NormBwdArgs p, void* dw, hipStream_t s) {
         if (have && dw) {
             p.inv = part;
             part += p.rows;
-            if (p.rows > 0) hipLaunchKernelGGL((rms_norm_inv_kernel<DT>), dim3((unsigned)p.rows), dim3(RN_THREADS), 0, s, p);
+            if (p.rows > 0) hipLaunchKernelGGL((rms_norm_inv_kernel<DT>), rows_grid(p.rows), dim3(RN_THREADS), 0, s, p);
             hipLaunchKernelGGL((rms_norm_dweight_kernel<DT>), dim3((unsigned)((p.cols + 63) / 64), (unsigned)parts),
                                dim3(RN_THREADS), 0, s, p, part);
         }
-        if (have && p.rows > 0) hipLaunchKernelGGL((rms_norm_bwd_any_kernel<DT>), dim3((unsigned)p.rows), dim3(RN_THREADS), 0, s, p);
+        if (have && p.rows > 0) hipLaunchKernelGGL((rms_norm_bwd_any_kernel<DT>), rows_grid(p.rows), dim3(RN_THREADS), 0, s, p);
     }
     if (!have) return fail(TVK_ERR_OOM, "tvk_rms_norm_bwd: workspace allocation failed");
     if (dw && !p.dw)
