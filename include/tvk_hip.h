@@ -22,8 +22,9 @@
  *     scratch (split-K partials, repacked operands, convolution partials, the
  *     attention delta, partial sums of rows and of split keys) from a per-device
  *     pool for the kernels they queue on their `stream`. A buffer is leased
- *     again only for the stream its first lease named, so stream order puts
- *     each call's kernels after the previous holder's; concurrent calls (other
+ *     again only for the stream its first lease named (on hipStreamPerThread
+ *     for that thread's), so stream order puts each call's kernels after the
+ *     previous holder's; concurrent calls (other
  *     threads, other streams) get other buffers; buffers are freed only after
  *     the device has drained (on growth, allocation failure or
  *     tvk_empty_cache). Calls may therefore come from any thread and any
@@ -555,15 +556,18 @@ tvk_status tvk_paged_append(const tvk_paged_append_desc* desc);
 /* out[b,t,h,:] = sum_j softmax_j(scale * q[b,t,h,:] . k[j, h / group, :]) v[j, h / group, :]
  * over positions j of sequence b with j <= p and, when window > 0, j > p - window,
  * p = seq_lens[b] - new_tokens + t the token's own position. A token without
- * keys gives out = 0 and lse = +inf; lse (NULL: not wanted) otherwise as
- * tvk_attention_fwd's. Scores and the softmax are float32; in the MFMA kernel
+ * keys (padding, or one whose every score is -inf) gives out = 0 and lse = +inf;
+ * lse (NULL: not wanted) otherwise as tvk_attention_fwd's. Scores and the softmax are float32; in the MFMA kernel
  * the probabilities are rounded to the dtype before the product with v.
  * max_len: a bound on seq_lens the host knows (it sizes the launch: how the
- * keys are split over workgroups), longer sequences are cut to it; 0: the
- * table's reach. Slots past a sequence's length are never read into a result.
+ * keys are split over workgroups), longer sequences are cut to it, as if they
+ * ended there, so a call that is captured and replayed for growing sequences
+ * needs one for all of its replays; 0: the table's reach. Slots past a
+ * sequence's length are never read into a result.
  * dtype F32, F16 or BF16, head_dim up to 512. Head dims in 16s up to 256 with
  * 16-byte aligned rows, caches below 64 GiB and any cache type but F8E4M3FN
- * beside F32 run the MFMA kernel, other cases a general one. Table entries past a
+ * beside F32 run the MFMA kernel, up to 2^24 blocks of rows (of a sequence and a
+ * key/value head), other cases a general one. Table entries past a
  * sequence's pages may be read, and what they name, but not into a result. Partial
  * sums of split keys use library scratch and are joined in an order that depends
  * on sizes and lengths alone (the same bits every run). */

@@ -18,7 +18,7 @@
 //      the product for value e is column EV * m + e of the output. float32
 //      values and probabilities are operands of the 16x16x4 product as they are.
 //
-// Work is dealt by every workgroup itself, from the lengths on the device: a
+// Work is dealt by every workgroup itself (paged_deal.h), from the lengths on the device: a
 // batch's lengths are not on the host, and a launch sized by the longest would
 // leave the others' workgroups idle. A segment is a row block of a sequence and a
 // key/value head. Short ones take a wave or a workgroup each, as max_len tells the
@@ -43,9 +43,11 @@
 // that order, which spreads long sequences better: 65 us, 69 for 110 x 1149 keys of 128).
 //
 // Measured: one sequence of 100001 keys (32/8 heads of 128, bfloat16) 82 us, 5.0
-// TB/s; 32 of up to 8000 keys 111 us, 4.9 TB/s; 24 of up to 6001 in 8 bits with 4
-// tokens each 52 us, 3.4 TB/s, where stretches that cross segments end late; 16 with
-// windows of 1000 keys, 12 heads of 80 in float16 16.5 us, 3.1 TB/s.
+// TB/s; 32 of up to 8000 keys 110 us, 4.9 TB/s; 24 of up to 6001 in 8 bits with 4
+// tokens each 53-57 us, 3.4-3.1 TB/s: 592 chunks of 32 to 58 tiles, 37 on average, and
+// the call ends with the longest; 16 with windows of 1000 keys, 12 heads of 80 in
+// float16 16.5 us, 3.1 TB/s. Prompts are far from the products' rate: a tile feeds 32
+// rows only (bfloat16 32/8 heads of 128, one prompt of 8192 tokens 3.9 ms, 140 TFLOP/s).
 #pragma once
 
 #include "attention_kernels.h"
@@ -88,8 +90,11 @@ struct PagedTile {
     static constexpr int EV = D == 96 ? 8 : D / 16;             // V values a lane holds of a row
     static constexpr int DV = 16 * EV;
     static constexpr int VW = EV * ES / 4;                      // the same in 32-bit words
-    // Workgroups a CU by the registers: K and V tiles, Q, O and S, and 90 beside them. Three of bfloat16 and 128 columns
-    // would fit their loop, but 12 waves with a tile each on its way read slower than 8 (32 x 8000 keys: 124 us, 112).
+    // Workgroups a CU that calls are dealt for: an estimate by the registers, K and V tiles, Q, O and S, and 90 beside them.
+    // It is what the kernels for pages of any size get; those for whole pages of 8 bits up to 128 columns and one row block,
+    // of 64 and two, of 256 and one, and of bfloat16 with 128 and two take fewer, and one workgroup more fits.
+    // Three of bfloat16 and 128 columns would fit their loop, but 12 waves with a tile each on its way read slower than 8
+    // (32 x 8000 keys: 124 us, 112).
     static constexpr int regs(int ct) { return 4 * NB * (KL + VW) + ct * (4 * QS + 4 * EV + 4 * NB) + 90; }
     static constexpr int occ(int ct) { return regs(ct) <= 128 ? 4 : regs(ct) <= 168 ? 3 : regs(ct) <= 256 ? 2 : 1; }
 };
