@@ -142,3 +142,34 @@ def test_norm_of_rows_without_values(calls):
         y, scale, _ = decoder.rms_norm_fp8(x, w)
         assert y.shape == x.shape and scale.shape == x.shape[:-1]
     assert [(d.rows, d.cols) for _, d in calls[::2]] == [(15, 0), (0, 0), (0, 8), (1, 0)]
+
+
+@pytest.mark.parametrize("devices,current,want", [(1, 1, []), (2, 0, []), (2, 1, [0, 1])])
+def test_calls_are_made_on_their_tensors_device(monkeypatch, devices, current, want):
+    made, set_to = [], []
+
+    class Library:
+        def tvk_get_device(self, d):
+            d._obj.value = set_to[-1] if set_to else current
+            return 0
+
+        def tvk_set_device(self, d):
+            set_to.append(d)
+            return 0
+
+        def __getattr__(self, name):
+            return lambda d: made.append((name, set_to[-1] if set_to else current)) or 0
+
+    library = Library()
+    monkeypatch.setattr(_abi, "load", lambda: library)
+    monkeypatch.setattr(decoder, "_stream", lambda t: None)
+    monkeypatch.setattr(decoder, "_devices", lambda: devices)
+    cache = decoder.PagedKVCache(2, 40, 4, 1, 8, torch.float32, "cpu")
+    x = torch.zeros((2, 1, 1, 8))
+    cache.extend(1)
+    for name, call in (("tvk_paged_append", lambda: cache.append(x, x, x)), ("tvk_paged_attention", lambda: cache.attend(x)),
+                       ("tvk_rms_norm_fwd", lambda: decoder.rms_norm(x)), ("tvk_rms_norm_fwd", lambda: decoder.rms_norm_fp8(x))):
+        made.clear()
+        set_to.clear()
+        call()
+        assert made == [(name, 0 if devices > 1 else current)] and set_to == want

@@ -6,6 +6,7 @@ these operators from element-wise shaders and keeps dense caches."""
 from __future__ import annotations
 
 import ctypes as C
+import functools
 import math
 
 import torch
@@ -23,6 +24,28 @@ def _stream(t: torch.Tensor):
     s = C.c_void_p()
     _abi.check(_abi.load().tvk_get_stream(t.device.index or 0, C.byref(s)))
     return s.value
+
+
+@functools.lru_cache(maxsize=None)
+def _devices() -> int:
+    return torch.cuda.device_count()
+
+
+def _queue(name: str, desc, t: torch.Tensor) -> None:
+    """Makes the call with t's device current: its kernels and their scratch are that device's."""
+    lib = _abi.load()
+    call = getattr(lib, name)
+    if _devices() <= 1:
+        return _abi.check(call(C.byref(desc)))
+    before, device = C.c_int(), t.device.index or 0
+    _abi.check(lib.tvk_get_device(C.byref(before)))
+    if before.value == device:
+        return _abi.check(call(C.byref(desc)))
+    _abi.check(lib.tvk_set_device(device))
+    try:
+        _abi.check(call(C.byref(desc)))
+    finally:
+        lib.tvk_set_device(before.value)
 
 
 def _capturing(t: torch.Tensor) -> bool:
@@ -72,7 +95,7 @@ class _RmsNorm(torch.autograd.Function):
         y = torch.empty(x2.shape, dtype=x.dtype, device=x.device)
         h = x2 if r2 is None else torch.empty(x2.shape, dtype=x.dtype, device=x.device)
         d = _abi.make_rms_norm_desc(x2, weight, y, r2, None if r2 is None else h, None, eps, _stream(x))
-        _abi.check(_abi.load().tvk_rms_norm_fwd(C.byref(d)))
+        _queue("tvk_rms_norm_fwd", d, x)
         ctx.save_for_backward(h, weight)
         ctx.eps, ctx.shape, ctx.added = eps, shape, r2 is not None
         if r2 is None:
@@ -89,7 +112,7 @@ class _RmsNorm(torch.autograd.Function):
         dw = torch.empty(weight.shape, dtype=weight.dtype, device=weight.device) \
             if weight is not None and ctx.needs_input_grad[1] else None
         d = _abi.make_rms_norm_bwd_desc(dy2, h, weight, dx, dw, dh2, ctx.eps, _stream(h))
-        _abi.check(_abi.load().tvk_rms_norm_bwd(C.byref(d)))
+        _queue("tvk_rms_norm_bwd", d, h)
         dx = dx.view(ctx.shape)
         return dx, dw, dx if ctx.added else None, None
 
@@ -126,7 +149,7 @@ def rms_norm_fp8(x, weight=None, residual=None, eps: float = 1e-5):
     r2 = None if residual is None else _rows(residual.detach())
     h = None if r2 is None else torch.empty(x2.shape, dtype=x.dtype, device=x.device)
     d = _abi.make_rms_norm_desc(x2, weight, y, r2, h, scale, eps, _stream(x))
-    _abi.check(_abi.load().tvk_rms_norm_fwd(C.byref(d)))
+    _queue("tvk_rms_norm_fwd", d, x)
     out = y.view(x.shape), scale.view(x.shape[:-1])
     if h is None:
         return *_without_gradient("rms_norm_fp8", out, x, weight), x
@@ -217,7 +240,7 @@ class PagedKVCache:
         out = torch.empty(q.shape, dtype=q.dtype, device=q.device) if out is None and q is not None else out
         d = _abi.make_paged_append_desc(q, k, v, out, self.k[layer], self.v[layer], self.lens, self.table, rotary, interleaved,
                                         self.k_scale, self.v_scale, _stream(k), self.new)
-        _abi.check(_abi.load().tvk_paged_append(C.byref(d)))
+        _queue("tvk_paged_append", d, k)
         self._appended, self._captured = True, self._captured or _capturing(k)
         if given:
             _written(out)
@@ -234,7 +257,7 @@ class PagedKVCache:
         d = _abi.make_paged_attention_desc(q, self.k[layer], self.v[layer], out, self.lens, self.table,
                                            max_len, scale, window, self.k_scale, self.v_scale, stream=_stream(q),
                                            new_lens=self.new)
-        _abi.check(_abi.load().tvk_paged_attention(C.byref(d)))
+        _queue("tvk_paged_attention", d, q)
         if given:
             _written(out)
         return _without_gradient("PagedKVCache.attend", out, q)
