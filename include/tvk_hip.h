@@ -18,7 +18,8 @@
  *   - strides are in ELEMENTS, not bytes, and may be zero (broadcast) or any
  *     positive value; element offsets must fit in int64.
  *   - scratch memory: tvk_gemm, tvk_conv2d_*, tvk_conv_*, tvk_reduce_sum,
- *     tvk_attention_bwd, tvk_rms_norm_bwd and tvk_paged_attention lease library
+ *     tvk_attention_bwd, tvk_rms_norm_bwd, tvk_layer_norm_bwd and
+ *     tvk_paged_attention lease library
  *     scratch (split-K partials, repacked operands, convolution partials, the
  *     attention delta, partial sums of rows and of split keys) from a per-device
  *     pool for the kernels they queue on their `stream`. A buffer is leased
@@ -496,6 +497,65 @@ typedef struct {
 } tvk_rms_norm_bwd_desc;
 
 tvk_status tvk_rms_norm_bwd(const tvk_rms_norm_bwd_desc* desc);
+
+/* ------------------------------------------------------------------------- */
+/* Layer norm                                                                 */
+/* ------------------------------------------------------------------------- */
+
+/* For every row of `cols` values, with the sums in float32:
+ *   h = x + residual, rounded to `dtype` (h = x without a residual),
+ *   y = (h - mean(h)) / sqrt(mean((h - mean(h))^2) + eps) * weight + bias
+ * (weight NULL: ones, bias NULL: zeros), y rounded to `out_dtype`: `dtype`
+ * itself, or F8E4M3FN with a scale for each 128 columns of a row,
+ *   scale[row][block] = max|y| / 448 over the block (1 where it is all zero),
+ *   out = y / scale rounded to nearest even (NaN stays NaN),
+ * the form in which tvk_gemm_f8 takes its rows (the last block may be shorter).
+ * h goes to residual_out when that is not NULL. dtype: F32, F16 or BF16;
+ * weight_dtype, the weight's and bias's: `dtype` or F32. Rows are contiguous,
+ * `*_stride` elements apart; any alignment. out may be x or residual, and
+ * residual_out may be x or residual (the same rows, same strides), when the
+ * types agree. No scratch. */
+typedef struct {
+    int32_t dtype, out_dtype, weight_dtype, reserved;
+    int64_t rows, cols;
+    const void* x; int64_t x_stride;
+    const void* residual; int64_t residual_stride;       /* NULL: none */
+    const void* weight;                                  /* [cols] */
+    const void* bias;                                    /* [cols] */
+    void* out; int64_t out_stride;
+    void* residual_out; int64_t residual_out_stride;     /* NULL: not wanted */
+    float* scale; int64_t scale_stride[2];               /* [rows][ceil(cols / 128)], F8E4M3FN only */
+    double eps;
+    void* stream;
+} tvk_layer_norm_desc;
+
+tvk_status tvk_layer_norm_fwd(const tvk_layer_norm_desc* desc);
+
+/* Gradients of tvk_layer_norm_fwd (out_dtype == dtype) from the gradient dy of
+ * out, the forward's h (x without a residual) and, when not NULL, the gradient
+ * dh of residual_out. With inv = 1 / sqrt(variance + eps), n = (h - mean) inv,
+ * recomputed from h, and g = dy * weight, all in float32:
+ *   dx = inv (g - mean(g) - n * mean(g * n)) + dh,
+ *   dweight = sum over rows of dy * n,   dbias = sum over rows of dy.
+ * dx is the gradient of x and of residual alike. dweight, dbias (weight_dtype)
+ * NULL: not wanted. The sums over rows run in an order that depends on the
+ * sizes alone: the same bits every run. dx may be dy, h or dh (same strides).
+ * May use library scratch when dweight or dbias is wanted. */
+typedef struct {
+    int32_t dtype, weight_dtype;
+    int64_t rows, cols;
+    const void* dy; int64_t dy_stride;
+    const void* h; int64_t h_stride;
+    const void* dh; int64_t dh_stride;                   /* NULL: none */
+    const void* weight;                                  /* [cols], NULL: ones */
+    void* dx; int64_t dx_stride;
+    void* dweight;                                       /* [cols] */
+    void* dbias;                                         /* [cols] */
+    double eps;
+    void* stream;
+} tvk_layer_norm_bwd_desc;
+
+tvk_status tvk_layer_norm_bwd(const tvk_layer_norm_bwd_desc* desc);
 
 /* ------------------------------------------------------------------------- */
 /* Paged key/value cache: append with rotation, attention                     */

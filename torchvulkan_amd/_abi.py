@@ -157,6 +157,7 @@ class BinaryDesc(C.Structure):
     ]
 
 
+I64x2 = C.c_int64 * 2
 I64x4 = C.c_int64 * 4
 
 
@@ -213,6 +214,36 @@ class RmsNormBwdDesc(C.Structure):
         ("weight", C.c_void_p),
         ("dx", C.c_void_p), ("dx_stride", C.c_int64),
         ("dweight", C.c_void_p),
+        ("eps", C.c_double),
+        ("stream", C.c_void_p),
+    ]
+
+
+class LayerNormDesc(C.Structure):
+    _fields_ = [
+        ("dtype", C.c_int32), ("out_dtype", C.c_int32), ("weight_dtype", C.c_int32), ("reserved", C.c_int32),
+        ("rows", C.c_int64), ("cols", C.c_int64),
+        ("x", C.c_void_p), ("x_stride", C.c_int64),
+        ("residual", C.c_void_p), ("residual_stride", C.c_int64),
+        ("weight", C.c_void_p), ("bias", C.c_void_p),
+        ("out", C.c_void_p), ("out_stride", C.c_int64),
+        ("residual_out", C.c_void_p), ("residual_out_stride", C.c_int64),
+        ("scale", C.c_void_p), ("scale_stride", I64x2),
+        ("eps", C.c_double),
+        ("stream", C.c_void_p),
+    ]
+
+
+class LayerNormBwdDesc(C.Structure):
+    _fields_ = [
+        ("dtype", C.c_int32), ("weight_dtype", C.c_int32),
+        ("rows", C.c_int64), ("cols", C.c_int64),
+        ("dy", C.c_void_p), ("dy_stride", C.c_int64),
+        ("h", C.c_void_p), ("h_stride", C.c_int64),
+        ("dh", C.c_void_p), ("dh_stride", C.c_int64),
+        ("weight", C.c_void_p),
+        ("dx", C.c_void_p), ("dx_stride", C.c_int64),
+        ("dweight", C.c_void_p), ("dbias", C.c_void_p),
         ("eps", C.c_double),
         ("stream", C.c_void_p),
     ]
@@ -330,6 +361,8 @@ def load() -> C.CDLL:
         lib.tvk_attention_bwd.argtypes = [C.POINTER(AttentionBwdDesc)]
         lib.tvk_rms_norm_fwd.argtypes = [C.POINTER(RmsNormDesc)]
         lib.tvk_rms_norm_bwd.argtypes = [C.POINTER(RmsNormBwdDesc)]
+        lib.tvk_layer_norm_fwd.argtypes = [C.POINTER(LayerNormDesc)]
+        lib.tvk_layer_norm_bwd.argtypes = [C.POINTER(LayerNormBwdDesc)]
         lib.tvk_paged_append.argtypes = [C.POINTER(PagedAppendDesc)]
         lib.tvk_paged_attention.argtypes = [C.POINTER(PagedAttentionDesc)]
         lib.tvk_calibrate_mfma.argtypes = [C.c_int, C.c_int, C.c_int, C.POINTER(C.c_double), C.POINTER(C.c_double)]
@@ -354,7 +387,8 @@ _ALL_ENTRY_POINTS = (
     "tvk_conv_candidates", "tvk_conv_choose", "tvk_conv_tune",
     "tvk_copy", "tvk_copy_plan",
     "tvk_fill", "tvk_reduce_sum", "tvk_binary", "tvk_attention_fwd",
-    "tvk_attention_bwd", "tvk_rms_norm_fwd", "tvk_rms_norm_bwd", "tvk_paged_append", "tvk_paged_attention",
+    "tvk_attention_bwd", "tvk_rms_norm_fwd", "tvk_rms_norm_bwd", "tvk_layer_norm_fwd", "tvk_layer_norm_bwd",
+    "tvk_paged_append", "tvk_paged_attention",
     "tvk_gemm_noalloc", "tvk_event_create", "tvk_event_destroy", "tvk_event_record",
     "tvk_event_query", "tvk_event_synchronize", "tvk_event_elapsed", "tvk_stream_wait_event", "tvk_stream_query",
     "tvk_calibrate_mfma", "tvk_calibrate_mfma_operands",
@@ -587,7 +621,7 @@ def attention_bwd(q, k, v, out, lse, dout, bias=None, causal=False, scale=None, 
 
 
 # ---------------------------------------------------------------------------
-# root-mean-square norm, paged key/value cache
+# norms, paged key/value cache
 # ---------------------------------------------------------------------------
 
 def _invalid(message: str):
@@ -689,6 +723,106 @@ def rms_norm_bwd(dy, h, weight=None, dh=None, eps=1e-5, stream=None):
     d = make_rms_norm_bwd_desc(dy, h, weight, dx, dweight, dh, eps, _stream_of(h, stream))
     check(load().tvk_rms_norm_bwd(C.byref(d)))
     return dx, dweight
+
+
+F8_BLOCK = 128   # values that share a scale in a row of 8-bit floats
+
+
+def blocks_of(n: int) -> int:
+    return -(-n // F8_BLOCK)
+
+
+def _scales(t, rows: int, cols: int, what: str):
+    """Address and strides of a float32 [rows, cols] array of scales, any strides."""
+    if tuple(t.shape) != (rows, cols) or t.dtype != _torch().float32:
+        raise _invalid(f"{what}: float32 {(rows, cols)} is expected, not {t.dtype} {tuple(t.shape)}")
+    return t.data_ptr(), I64x2(*t.stride())
+
+
+def make_layer_norm_desc(x, weight, bias, out, residual=None, residual_out=None, scale=None, eps=1e-5,
+                         stream=None) -> LayerNormDesc:
+    """Describes tvk_layer_norm_fwd over [rows, cols] device tensors; out of x's dtype, or float8_e4m3fn with the
+    float32 scales [rows, ceil(cols / 128)] in `scale`."""
+    torch = _torch()
+    if x.dim() != 2:
+        raise _invalid(f"x: {x.dim()} dimensions, expected [rows, cols]")
+    rows, cols = x.shape
+    d = LayerNormDesc()
+    d.dtype = _dtype_code(x.dtype)
+    d.rows, d.cols = rows, cols
+    d.x, d.x_stride = x.data_ptr(), _row_stride(x, rows, cols, x.dtype, "x")
+    d.weight_dtype = d.dtype
+    wdtypes = (x.dtype, torch.float32)
+    if weight is not None:
+        d.weight, d.weight_dtype = _vector(weight, cols, wdtypes, "weight"), _dtype_code(weight.dtype)
+        wdtypes = (weight.dtype,)
+    if bias is not None:
+        d.bias, d.weight_dtype = _vector(bias, cols, wdtypes, "bias"), _dtype_code(bias.dtype)
+    if residual is not None:
+        d.residual, d.residual_stride = residual.data_ptr(), _row_stride(residual, rows, cols, x.dtype, "residual")
+    if residual_out is not None:
+        d.residual_out, d.residual_out_stride = residual_out.data_ptr(), _row_stride(residual_out, rows, cols, x.dtype,
+                                                                                     "residual_out")
+    in8 = out.dtype == torch.float8_e4m3fn
+    d.out_dtype = TVK_F8E4M3FN if in8 else d.dtype
+    d.out, d.out_stride = out.data_ptr(), _row_stride(out, rows, cols, out.dtype if in8 else x.dtype, "out")
+    if in8 != (scale is not None):
+        raise _invalid("scale: wanted with a float8_e4m3fn output and only then")
+    if in8:
+        d.scale, d.scale_stride = _scales(scale, rows, blocks_of(cols), "scale")
+    d.eps = float(eps)
+    d.stream = stream
+    return d
+
+
+def layer_norm_fwd(x, weight=None, bias=None, residual=None, eps=1e-5, out_dtype=None, stream=None):
+    """(y, h, scale) of tvk_layer_norm_fwd over a [rows, cols] tensor: h is x where there is no residual; scale is None
+    unless out_dtype is float8_e4m3fn."""
+    torch = _torch()
+    y = torch.empty(x.shape, dtype=out_dtype or x.dtype, device=x.device)
+    h = torch.empty(x.shape, dtype=x.dtype, device=x.device) if residual is not None else None
+    scale = torch.empty((x.shape[0], blocks_of(x.shape[1])), dtype=torch.float32, device=x.device) \
+        if y.dtype == torch.float8_e4m3fn else None
+    d = make_layer_norm_desc(x, weight, bias, y, residual, h, scale, eps, _stream_of(x, stream))
+    check(load().tvk_layer_norm_fwd(C.byref(d)))
+    return y, x if h is None else h, scale
+
+
+def make_layer_norm_bwd_desc(dy, h, weight, dx, dweight=None, dbias=None, dh=None, eps=1e-5, stream=None) -> LayerNormBwdDesc:
+    """Describes tvk_layer_norm_bwd over [rows, cols] device tensors."""
+    torch = _torch()
+    if h.dim() != 2:
+        raise _invalid(f"h: {h.dim()} dimensions, expected [rows, cols]")
+    rows, cols = h.shape
+    d = LayerNormBwdDesc()
+    d.dtype = _dtype_code(h.dtype)
+    d.rows, d.cols = rows, cols
+    d.dy, d.dy_stride = dy.data_ptr(), _row_stride(dy, rows, cols, h.dtype, "dy")
+    d.h, d.h_stride = h.data_ptr(), _row_stride(h, rows, cols, h.dtype, "h")
+    if dh is not None:
+        d.dh, d.dh_stride = dh.data_ptr(), _row_stride(dh, rows, cols, h.dtype, "dh")
+    d.dx, d.dx_stride = dx.data_ptr(), _row_stride(dx, rows, cols, h.dtype, "dx")
+    wdtype = next((t.dtype for t in (weight, dweight, dbias) if t is not None), h.dtype)
+    if weight is not None:
+        d.weight = _vector(weight, cols, (h.dtype, torch.float32), "weight")
+    if dweight is not None:
+        d.dweight = _vector(dweight, cols, (wdtype,), "dweight")
+    if dbias is not None:
+        d.dbias = _vector(dbias, cols, (wdtype,), "dbias")
+    d.weight_dtype = _dtype_code(wdtype)
+    d.eps = float(eps)
+    d.stream = stream
+    return d
+
+
+def layer_norm_bwd(dy, h, weight=None, dh=None, eps=1e-5, stream=None):
+    """(dx, dweight, dbias) of tvk_layer_norm_bwd; the gradients of weight and bias have the weight's dtype, h's without one."""
+    torch = _torch()
+    dx = torch.empty(h.shape, dtype=h.dtype, device=h.device)
+    dweight, dbias = (torch.empty(h.shape[1], dtype=h.dtype if weight is None else weight.dtype, device=h.device) for _ in range(2))
+    d = make_layer_norm_bwd_desc(dy, h, weight, dx, dweight, dbias, dh, eps, _stream_of(h, stream))
+    check(load().tvk_layer_norm_bwd(C.byref(d)))
+    return dx, dweight, dbias
 
 
 def make_paged_cache(k_cache, v_cache, seq_lens, table, k_scale=None, v_scale=None, new_lens=None) -> PagedCache:

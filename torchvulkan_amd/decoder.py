@@ -1,6 +1,6 @@
 """The decoder block's operators as a program uses them: the root-mean-square
-norm with its gradients, and a paged key/value cache that prompts and new tokens
-are appended to and attended over. Tensors of the vulkan device or of "cuda"; the
+norm and layer norm with their gradients, and a paged key/value cache that prompts
+and new tokens are appended to and attended over. Tensors of the vulkan device or of "cuda"; the
 calls are queued on the tensors' device's current stream. The reference composes
 these operators from element-wise shaders and keeps dense caches."""
 from __future__ import annotations
@@ -13,7 +13,7 @@ import torch
 
 from . import _abi
 
-__all__ = ["rms_norm", "rms_norm_fp8", "rotary_table", "PagedKVCache"]
+__all__ = ["rms_norm", "rms_norm_fp8", "layer_norm", "layer_norm_fp8", "rotary_table", "PagedKVCache"]
 
 
 def _stream(t: torch.Tensor):
@@ -124,10 +124,10 @@ def _check_devices(device, *tensors) -> None:
             raise _abi.TvkError(_abi.TVK_ERR_INVALID, f"tensors on {device} and {t.device}")
 
 
-def _check_norm(x, weight, residual) -> None:
+def _check_norm(x, weight, residual, bias=None) -> None:
     if x.dim() == 0 or (residual is not None and (residual.shape != x.shape or residual.dtype != x.dtype)):
         raise _abi.TvkError(_abi.TVK_ERR_INVALID, "x: [..., cols], and a residual of its shape and dtype, are expected")
-    _check_devices(x.device, weight, residual)
+    _check_devices(x.device, weight, residual, bias)
 
 
 def rms_norm(x, weight=None, residual=None, eps: float = 1e-5):
@@ -154,6 +154,63 @@ def rms_norm_fp8(x, weight=None, residual=None, eps: float = 1e-5):
     if h is None:
         return *_without_gradient("rms_norm_fp8", out, x, weight), x
     return _without_gradient("rms_norm_fp8", (*out, h.view(x.shape)), x, weight, residual)
+
+
+class _LayerNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, residual, eps):
+        shape, x2 = x.shape, _rows(x)
+        r2 = None if residual is None else _rows(residual)
+        y = torch.empty(x2.shape, dtype=x.dtype, device=x.device)
+        h = x2 if r2 is None else torch.empty(x2.shape, dtype=x.dtype, device=x.device)
+        d = _abi.make_layer_norm_desc(x2, weight, bias, y, r2, None if r2 is None else h, None, eps, _stream(x))
+        _queue("tvk_layer_norm_fwd", d, x)
+        ctx.save_for_backward(h, weight)
+        ctx.eps, ctx.shape, ctx.added, ctx.bias = eps, shape, r2 is not None, None if bias is None else bias.dtype
+        if r2 is None:
+            return y.view(shape), None
+        return y.view(shape), h.view(shape)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy, dh):
+        h, weight = ctx.saved_tensors
+        dy2 = torch.zeros(h.shape, dtype=h.dtype, device=h.device) if dy is None else _rows(dy)
+        dh2 = None if dh is None else _rows(dh)
+        dx = torch.empty(h.shape, dtype=h.dtype, device=h.device)
+        dw = torch.empty(weight.shape, dtype=weight.dtype, device=weight.device) \
+            if weight is not None and ctx.needs_input_grad[1] else None
+        db = torch.empty(h.shape[1:], dtype=ctx.bias, device=h.device) if ctx.bias and ctx.needs_input_grad[2] else None
+        d = _abi.make_layer_norm_bwd_desc(dy2, h, weight, dx, dw, db, dh2, ctx.eps, _stream(h))
+        _queue("tvk_layer_norm_bwd", d, h)
+        dx = dx.view(ctx.shape)
+        return dx, dw, db, dx if ctx.added else None, None
+
+
+def layer_norm(x, weight=None, bias=None, residual=None, eps: float = 1e-5):
+    """(x - mean(x)) / sqrt(var(x) + eps) * weight + bias over the last dimension; with a residual (y, h) of
+    h = x + residual (tvk_layer_norm_fwd, tvk_layer_norm_bwd). Differentiable in x, weight, bias and residual where rms_norm
+    is. weight and bias have one dtype, x's or float32."""
+    _check_norm(x, weight, residual, bias)
+    y, h = _LayerNorm.apply(x, weight, bias, residual, float(eps))
+    return y if residual is None else (y, h)
+
+
+def layer_norm_fp8(x, weight=None, bias=None, residual=None, eps: float = 1e-5):
+    """(y, scale, h): the norm in float8_e4m3fn with a float32 scale for each 128 columns of a row, scale
+    [..., ceil(cols / 128)]; h is x without a residual. No gradient: a backward pass that reaches the results raises."""
+    _check_norm(x, weight, residual, bias)
+    x2 = _rows(x.detach())
+    y = torch.empty(x2.shape, dtype=torch.float8_e4m3fn, device=x.device)
+    scale = torch.empty((x2.shape[0], _abi.blocks_of(x2.shape[1])), dtype=torch.float32, device=x.device)
+    r2 = None if residual is None else _rows(residual.detach())
+    h = None if r2 is None else torch.empty(x2.shape, dtype=x.dtype, device=x.device)
+    d = _abi.make_layer_norm_desc(x2, weight, bias, y, r2, h, scale, eps, _stream(x))
+    _queue("tvk_layer_norm_fwd", d, x)
+    out = y.view(x.shape), scale.view(*x.shape[:-1], scale.shape[1])
+    if h is None:
+        return *_without_gradient("layer_norm_fp8", out, x, weight, bias), x
+    return _without_gradient("layer_norm_fp8", (*out, h.view(x.shape)), x, weight, bias, residual)
 
 
 def rotary_table(positions: int, rotary_dim: int, base: float = 10000.0, device="cpu") -> torch.Tensor:
