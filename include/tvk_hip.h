@@ -18,8 +18,8 @@
  *   - strides are in ELEMENTS, not bytes, and may be zero (broadcast) or any
  *     positive value; element offsets must fit in int64.
  *   - scratch memory: tvk_gemm, tvk_conv2d_*, tvk_conv_*, tvk_reduce_sum,
- *     tvk_attention_bwd, tvk_rms_norm_bwd, tvk_layer_norm_bwd and
- *     tvk_paged_attention lease library
+ *     tvk_attention_bwd, tvk_rms_norm_bwd, tvk_layer_norm_bwd, tvk_distill_fwd
+ *     and tvk_paged_attention lease library
  *     scratch (split-K partials, repacked operands, convolution partials, the
  *     attention delta, partial sums of rows and of split keys) from a per-device
  *     pool for the kernels they queue on their `stream`. A buffer is leased
@@ -556,6 +556,63 @@ typedef struct {
 } tvk_layer_norm_bwd_desc;
 
 tvk_status tvk_layer_norm_bwd(const tvk_layer_norm_bwd_desc* desc);
+
+/* ------------------------------------------------------------------------- */
+/* Distillation from a teacher's top logits                                   */
+/* ------------------------------------------------------------------------- */
+
+/* For every row, from the student's `cols` logits x and a list of `top` entries
+ * (index, teacher's logit t), with a temperature T and all sums in float32:
+ *   q_j = softmax over the row's entries of t_j / T,
+ *   log p = log softmax over the row's logits of x / T,
+ *   loss = T^2 * sum_j q_j (log q_j - log p[index_j]).
+ * An entry whose index is outside [0, cols) is none (shorter lists are padded
+ * with -1); an index that stands in a row twice counts with both. A row whose
+ * entries are none, or weigh nothing (t all -inf), has loss 0 and a gradient of
+ * zeros, whatever its logits are. Infinite or NaN logits and t otherwise give
+ * what the formulas give.
+ * lse: log of the sum of exp(x / T), +inf for a row without entries; target: q,
+ * an index that stands there twice having it all at its first entry. Both are
+ * for tvk_distill_bwd, and may be NULL where that is not called.
+ * dtype: F32, F16 or BF16; teacher_dtype: `dtype` or F32; index_dtype: I32 or
+ * I64. Rows are contiguous, `*_stride` elements apart (0: one for all, of what
+ * is read); any alignment. top up to 2048. Few rows use library scratch. */
+typedef struct {
+    int32_t dtype, teacher_dtype, index_dtype, reserved;
+    int64_t rows, cols, top;
+    const void* logits; int64_t logits_stride;
+    const void* index; int64_t index_stride;
+    const void* teacher; int64_t teacher_stride;
+    float* loss;                                         /* [rows] */
+    float* lse;                                          /* [rows] */
+    float* target; int64_t target_stride;                /* [rows][top] */
+    double temperature;
+    void* stream;
+} tvk_distill_desc;
+
+tvk_status tvk_distill_fwd(const tvk_distill_desc* desc);
+
+/* Gradient of tvk_distill_fwd's losses with respect to the logits, from the
+ * forward's lse and target and the losses' gradients dloss (float32):
+ *   dlogits[i] = dloss * T * (exp(x_i / T - lse) - sum of q over the entries of index i),
+ * rounded once, probabilities below 2^-126 being taken as zero. dloss_stride 0:
+ * one gradient for all rows. dlogits (`dtype`) may
+ * be logits (the same strides). Every place is written by one workgroup, in an
+ * order of its own: the same bits every run. No scratch. */
+typedef struct {
+    int32_t dtype, index_dtype;
+    int64_t rows, cols, top;
+    const void* logits; int64_t logits_stride;
+    const void* index; int64_t index_stride;
+    const float* lse;
+    const float* target; int64_t target_stride;
+    const float* dloss; int64_t dloss_stride;
+    void* dlogits; int64_t dlogits_stride;
+    double temperature;
+    void* stream;
+} tvk_distill_bwd_desc;
+
+tvk_status tvk_distill_bwd(const tvk_distill_bwd_desc* desc);
 
 /* ------------------------------------------------------------------------- */
 /* Paged key/value cache: append with rotation, attention                     */

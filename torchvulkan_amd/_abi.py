@@ -249,6 +249,35 @@ class LayerNormBwdDesc(C.Structure):
     ]
 
 
+class DistillDesc(C.Structure):
+    _fields_ = [
+        ("dtype", C.c_int32), ("teacher_dtype", C.c_int32), ("index_dtype", C.c_int32), ("reserved", C.c_int32),
+        ("rows", C.c_int64), ("cols", C.c_int64), ("top", C.c_int64),
+        ("logits", C.c_void_p), ("logits_stride", C.c_int64),
+        ("index", C.c_void_p), ("index_stride", C.c_int64),
+        ("teacher", C.c_void_p), ("teacher_stride", C.c_int64),
+        ("loss", C.c_void_p), ("lse", C.c_void_p),
+        ("target", C.c_void_p), ("target_stride", C.c_int64),
+        ("temperature", C.c_double),
+        ("stream", C.c_void_p),
+    ]
+
+
+class DistillBwdDesc(C.Structure):
+    _fields_ = [
+        ("dtype", C.c_int32), ("index_dtype", C.c_int32),
+        ("rows", C.c_int64), ("cols", C.c_int64), ("top", C.c_int64),
+        ("logits", C.c_void_p), ("logits_stride", C.c_int64),
+        ("index", C.c_void_p), ("index_stride", C.c_int64),
+        ("lse", C.c_void_p),
+        ("target", C.c_void_p), ("target_stride", C.c_int64),
+        ("dloss", C.c_void_p), ("dloss_stride", C.c_int64),
+        ("dlogits", C.c_void_p), ("dlogits_stride", C.c_int64),
+        ("temperature", C.c_double),
+        ("stream", C.c_void_p),
+    ]
+
+
 class PagedCache(C.Structure):
     _fields_ = [
         ("dtype", C.c_int32), ("reserved", C.c_int32),
@@ -363,6 +392,8 @@ def load() -> C.CDLL:
         lib.tvk_rms_norm_bwd.argtypes = [C.POINTER(RmsNormBwdDesc)]
         lib.tvk_layer_norm_fwd.argtypes = [C.POINTER(LayerNormDesc)]
         lib.tvk_layer_norm_bwd.argtypes = [C.POINTER(LayerNormBwdDesc)]
+        lib.tvk_distill_fwd.argtypes = [C.POINTER(DistillDesc)]
+        lib.tvk_distill_bwd.argtypes = [C.POINTER(DistillBwdDesc)]
         lib.tvk_paged_append.argtypes = [C.POINTER(PagedAppendDesc)]
         lib.tvk_paged_attention.argtypes = [C.POINTER(PagedAttentionDesc)]
         lib.tvk_calibrate_mfma.argtypes = [C.c_int, C.c_int, C.c_int, C.POINTER(C.c_double), C.POINTER(C.c_double)]
@@ -388,6 +419,7 @@ _ALL_ENTRY_POINTS = (
     "tvk_copy", "tvk_copy_plan",
     "tvk_fill", "tvk_reduce_sum", "tvk_binary", "tvk_attention_fwd",
     "tvk_attention_bwd", "tvk_rms_norm_fwd", "tvk_rms_norm_bwd", "tvk_layer_norm_fwd", "tvk_layer_norm_bwd",
+    "tvk_distill_fwd", "tvk_distill_bwd",
     "tvk_paged_append", "tvk_paged_attention",
     "tvk_gemm_noalloc", "tvk_event_create", "tvk_event_destroy", "tvk_event_record",
     "tvk_event_query", "tvk_event_synchronize", "tvk_event_elapsed", "tvk_stream_wait_event", "tvk_stream_query",
@@ -621,7 +653,7 @@ def attention_bwd(q, k, v, out, lse, dout, bias=None, causal=False, scale=None, 
 
 
 # ---------------------------------------------------------------------------
-# norms, paged key/value cache
+# norms, distillation loss, paged key/value cache
 # ---------------------------------------------------------------------------
 
 def _invalid(message: str):
@@ -823,6 +855,76 @@ def layer_norm_bwd(dy, h, weight=None, dh=None, eps=1e-5, stream=None):
     d = make_layer_norm_bwd_desc(dy, h, weight, dx, dweight, dbias, dh, eps, _stream_of(h, stream))
     check(load().tvk_layer_norm_bwd(C.byref(d)))
     return dx, dweight, dbias
+
+
+def _logits_and_entries(d, logits, index) -> None:
+    """Logits [rows, cols] and the indexes [rows, top] of a row's entries, in d."""
+    torch = _torch()
+    if logits.dim() != 2 or index.dim() != 2:
+        raise _invalid("logits: [rows, cols] and index: [rows, top] are expected")
+    if index.dtype not in (torch.int32, torch.int64):
+        raise TvkUnsupported(TVK_ERR_UNSUPPORTED, f"index: dtype {index.dtype}, expected int32 or int64")
+    d.dtype = _dtype_code(logits.dtype)
+    d.index_dtype = TVK_I64 if index.dtype == torch.int64 else TVK_I32
+    d.rows, d.cols = logits.shape
+    d.top = index.shape[1]
+    d.logits, d.logits_stride = logits.data_ptr(), _row_stride(logits, d.rows, d.cols, logits.dtype, "logits")
+    d.index, d.index_stride = index.data_ptr(), _row_stride(index, d.rows, d.top, index.dtype, "index")
+
+
+def make_distill_desc(logits, index, teacher, loss, lse=None, target=None, temperature=1.0, stream=None) -> DistillDesc:
+    """Describes tvk_distill_fwd over device tensors: logits [rows, cols], index and teacher [rows, top]; float32 loss [rows]
+    and, for the gradient, lse [rows] and target [rows, top]."""
+    torch = _torch()
+    d = DistillDesc()
+    _logits_and_entries(d, logits, index)
+    if teacher.dtype not in (logits.dtype, torch.float32):
+        raise _invalid(f"teacher: dtype {teacher.dtype}, expected {logits.dtype} or float32")
+    d.teacher_dtype = _dtype_code(teacher.dtype)
+    d.teacher, d.teacher_stride = teacher.data_ptr(), _row_stride(teacher, d.rows, d.top, teacher.dtype, "teacher")
+    d.loss = _vector(loss, d.rows, (torch.float32,), "loss")
+    if lse is not None:
+        d.lse = _vector(lse, d.rows, (torch.float32,), "lse")
+    if target is not None:
+        d.target, d.target_stride = target.data_ptr(), _row_stride(target, d.rows, d.top, torch.float32, "target")
+    d.temperature = float(temperature)
+    d.stream = stream
+    return d
+
+
+def distill_fwd(logits, index, teacher, temperature=1.0, stream=None):
+    """(loss, lse, target) of tvk_distill_fwd, new float32 tensors."""
+    torch = _torch()
+    loss, lse = (torch.empty(logits.shape[0], dtype=torch.float32, device=logits.device) for _ in range(2))
+    target = torch.empty(index.shape, dtype=torch.float32, device=logits.device)
+    d = make_distill_desc(logits, index, teacher, loss, lse, target, temperature, _stream_of(logits, stream))
+    check(load().tvk_distill_fwd(C.byref(d)))
+    return loss, lse, target
+
+
+def make_distill_bwd_desc(logits, index, lse, target, dloss, dlogits, temperature=1.0, stream=None) -> DistillBwdDesc:
+    """Describes tvk_distill_bwd; dloss is [rows], of any stride."""
+    torch = _torch()
+    d = DistillBwdDesc()
+    _logits_and_entries(d, logits, index)
+    d.lse = _vector(lse, d.rows, (torch.float32,), "lse")
+    d.target, d.target_stride = target.data_ptr(), _row_stride(target, d.rows, d.top, torch.float32, "target")
+    if tuple(dloss.shape) != (d.rows,) or dloss.dtype != torch.float32:
+        raise _invalid("dloss: float32 [rows] is expected")
+    d.dloss, d.dloss_stride = dloss.data_ptr(), dloss.stride(0)
+    d.dlogits, d.dlogits_stride = dlogits.data_ptr(), _row_stride(dlogits, d.rows, d.cols, logits.dtype, "dlogits")
+    d.temperature = float(temperature)
+    d.stream = stream
+    return d
+
+
+def distill_bwd(logits, index, lse, target, dloss, temperature=1.0, stream=None):
+    """dlogits of tvk_distill_bwd, a new tensor of the logits' dtype."""
+    torch = _torch()
+    dlogits = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+    d = make_distill_bwd_desc(logits, index, lse, target, dloss, dlogits, temperature, _stream_of(logits, stream))
+    check(load().tvk_distill_bwd(C.byref(d)))
+    return dlogits
 
 
 def make_paged_cache(k_cache, v_cache, seq_lens, table, k_scale=None, v_scale=None, new_lens=None) -> PagedCache:

@@ -13,7 +13,7 @@ import torch
 
 from . import _abi
 
-__all__ = ["rms_norm", "rms_norm_fp8", "layer_norm", "layer_norm_fp8", "rotary_table", "PagedKVCache"]
+__all__ = ["rms_norm", "rms_norm_fp8", "layer_norm", "layer_norm_fp8", "distill_loss", "rotary_table", "PagedKVCache"]
 
 
 def _stream(t: torch.Tensor):
@@ -211,6 +211,38 @@ def layer_norm_fp8(x, weight=None, bias=None, residual=None, eps: float = 1e-5):
     if h is None:
         return *_without_gradient("layer_norm_fp8", out, x, weight, bias), x
     return _without_gradient("layer_norm_fp8", (*out, h.view(x.shape)), x, weight, bias, residual)
+
+
+class _Distill(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, index, teacher, temperature):
+        x, i, t = _rows(logits), _rows(index), _rows(teacher)
+        loss, lse = (torch.empty(x.shape[0], dtype=torch.float32, device=x.device) for _ in range(2))
+        target = torch.empty(i.shape, dtype=torch.float32, device=x.device)
+        d = _abi.make_distill_desc(x, i, t, loss, lse, target, temperature, _stream(x))
+        _queue("tvk_distill_fwd", d, x)
+        ctx.save_for_backward(x, i, lse, target)
+        ctx.temperature, ctx.shape = temperature, logits.shape
+        return loss.view(logits.shape[:-1])
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dloss):
+        x, i, lse, target = ctx.saved_tensors
+        dlogits = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        d = _abi.make_distill_bwd_desc(x, i, lse, target, dloss.reshape(-1), dlogits, ctx.temperature, _stream(x))
+        _queue("tvk_distill_bwd", d, x)
+        return dlogits.view(ctx.shape), None, None, None
+
+
+def distill_loss(logits, index, teacher, temperature: float = 1.0):
+    """The loss of every row of logits [..., cols] against a teacher's top logits: index and teacher [..., top], an index
+    outside the columns being no entry (tvk_distill_fwd). float32 [...]; differentiable in logits where rms_norm is, the
+    teacher's logits being constants."""
+    if logits.dim() == 0 or index.shape != teacher.shape or index.dim() != logits.dim() or index.shape[:-1] != logits.shape[:-1]:
+        raise _abi.TvkError(_abi.TVK_ERR_INVALID, "logits: [..., cols], index and teacher: [..., top] are expected")
+    _check_devices(logits.device, index, teacher)
+    return _Distill.apply(logits, index, teacher.detach(), float(temperature))
 
 
 def rotary_table(positions: int, rotary_dim: int, base: float = 10000.0, device="cpu") -> torch.Tensor:
