@@ -18,8 +18,8 @@
  *   - strides are in ELEMENTS, not bytes, and may be zero (broadcast) or any
  *     positive value; element offsets must fit in int64.
  *   - scratch memory: tvk_gemm, tvk_conv2d_*, tvk_conv_*, tvk_reduce_sum,
- *     tvk_attention_bwd, tvk_rms_norm_bwd, tvk_layer_norm_bwd, tvk_distill_fwd
- *     and tvk_paged_attention lease library
+ *     tvk_attention_bwd, tvk_rms_norm_bwd, tvk_layer_norm_bwd, tvk_distill_fwd,
+ *     tvk_gemm_f8 and tvk_paged_attention lease library
  *     scratch (split-K partials, repacked operands, convolution partials, the
  *     attention delta, partial sums of rows and of split keys) from a per-device
  *     pool for the kernels they queue on their `stream`. A buffer is leased
@@ -556,6 +556,58 @@ typedef struct {
 } tvk_layer_norm_bwd_desc;
 
 tvk_status tvk_layer_norm_bwd(const tvk_layer_norm_bwd_desc* desc);
+
+/* ------------------------------------------------------------------------- */
+/* 8-bit floats in blocks of 128                                              */
+/* ------------------------------------------------------------------------- */
+
+/* x [rows, cols] (F32, F16 or BF16) in F8E4M3FN, in blocks of 128 columns and
+ * block_rows rows, 1 (activations) or 128 (weights), the last ones shorter:
+ *   scale[block] = max|x| / 448 over the block (NaN aside; 1 where it is all zero),
+ *   out = x / scale rounded to nearest even (by way of the scale's reciprocal;
+ *   NaN stays NaN, a block with an infinity becomes zeros and NaN).
+ * Rows are contiguous, `*_stride` elements apart; any alignment. out and scale
+ * must not lie over x. No scratch. */
+typedef struct {
+    int32_t dtype, block_rows;
+    int64_t rows, cols;
+    const void* x; int64_t x_stride;
+    void* out; int64_t out_stride;
+    float* scale; int64_t scale_stride[2];   /* [ceil(rows / block_rows)][ceil(cols / 128)] */
+    void* stream;
+} tvk_quantize_f8_desc;
+
+tvk_status tvk_quantize_f8(const tvk_quantize_f8_desc* desc);
+
+/* out[m][n] = sum over blocks b of 128 values of k of
+ *     a_scale[m][b] * b_scale[n / 128][b] * sum over k in b of a[m][k] * b[n][k]
+ *   + bias[n],
+ * a and b F8E4M3FN with float32 scales; the sums of blocks are float32, the
+ * result is rounded once to out_dtype (F32, F16 or BF16). A block's sum over k is
+ * float32 for an F32 output; for the 16-bit ones it is the matrix unit's of 8-bit
+ * floats, which cuts the products of eight neighbouring values of k off 2^-13
+ * below the largest of them. a_dtype F32, F16 or BF16: a is first brought
+ * into 8 bits as by tvk_quantize_f8 with block_rows 1, with the same bits, and
+ * a_scale is not read. bias (NULL: none) has out_dtype or F32. Rows are
+ * contiguous, `*_stride` elements apart, scales at any strides (0: one for all);
+ * any alignment: rows that 16-byte loads do not meet are copied to library
+ * scratch for more than 64 rows of a, and 16- and 32-bit a's 8 bits go there for
+ * more than 16. The sums run in an order that depends on the sizes alone: the
+ * same bits every run. out must not lie over an input. K up to 2^22, or with up to
+ * 64 rows 2^31 - 65536. */
+typedef struct {
+    int32_t a_dtype, out_dtype, bias_dtype, reserved;
+    int64_t M, N, K;
+    const void* a; int64_t a_stride;                        /* [M][K] */
+    const float* a_scale; int64_t a_scale_stride[2];        /* [M][ceil(K / 128)] */
+    const void* b; int64_t b_stride;                        /* [N][K] */
+    const float* b_scale; int64_t b_scale_stride[2];        /* [ceil(N / 128)][ceil(K / 128)] */
+    const void* bias;                                       /* [N] */
+    void* out; int64_t out_stride;
+    void* stream;
+} tvk_gemm_f8_desc;
+
+tvk_status tvk_gemm_f8(const tvk_gemm_f8_desc* desc);
 
 /* ------------------------------------------------------------------------- */
 /* Distillation from a teacher's top logits                                   */

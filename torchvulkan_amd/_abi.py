@@ -278,6 +278,31 @@ class DistillBwdDesc(C.Structure):
     ]
 
 
+class QuantizeF8Desc(C.Structure):
+    _fields_ = [
+        ("dtype", C.c_int32), ("block_rows", C.c_int32),
+        ("rows", C.c_int64), ("cols", C.c_int64),
+        ("x", C.c_void_p), ("x_stride", C.c_int64),
+        ("out", C.c_void_p), ("out_stride", C.c_int64),
+        ("scale", C.c_void_p), ("scale_stride", I64x2),
+        ("stream", C.c_void_p),
+    ]
+
+
+class GemmF8Desc(C.Structure):
+    _fields_ = [
+        ("a_dtype", C.c_int32), ("out_dtype", C.c_int32), ("bias_dtype", C.c_int32), ("reserved", C.c_int32),
+        ("M", C.c_int64), ("N", C.c_int64), ("K", C.c_int64),
+        ("a", C.c_void_p), ("a_stride", C.c_int64),
+        ("a_scale", C.c_void_p), ("a_scale_stride", I64x2),
+        ("b", C.c_void_p), ("b_stride", C.c_int64),
+        ("b_scale", C.c_void_p), ("b_scale_stride", I64x2),
+        ("bias", C.c_void_p),
+        ("out", C.c_void_p), ("out_stride", C.c_int64),
+        ("stream", C.c_void_p),
+    ]
+
+
 class PagedCache(C.Structure):
     _fields_ = [
         ("dtype", C.c_int32), ("reserved", C.c_int32),
@@ -394,6 +419,8 @@ def load() -> C.CDLL:
         lib.tvk_layer_norm_bwd.argtypes = [C.POINTER(LayerNormBwdDesc)]
         lib.tvk_distill_fwd.argtypes = [C.POINTER(DistillDesc)]
         lib.tvk_distill_bwd.argtypes = [C.POINTER(DistillBwdDesc)]
+        lib.tvk_quantize_f8.argtypes = [C.POINTER(QuantizeF8Desc)]
+        lib.tvk_gemm_f8.argtypes = [C.POINTER(GemmF8Desc)]
         lib.tvk_paged_append.argtypes = [C.POINTER(PagedAppendDesc)]
         lib.tvk_paged_attention.argtypes = [C.POINTER(PagedAttentionDesc)]
         lib.tvk_calibrate_mfma.argtypes = [C.c_int, C.c_int, C.c_int, C.POINTER(C.c_double), C.POINTER(C.c_double)]
@@ -419,7 +446,7 @@ _ALL_ENTRY_POINTS = (
     "tvk_copy", "tvk_copy_plan",
     "tvk_fill", "tvk_reduce_sum", "tvk_binary", "tvk_attention_fwd",
     "tvk_attention_bwd", "tvk_rms_norm_fwd", "tvk_rms_norm_bwd", "tvk_layer_norm_fwd", "tvk_layer_norm_bwd",
-    "tvk_distill_fwd", "tvk_distill_bwd",
+    "tvk_distill_fwd", "tvk_distill_bwd", "tvk_quantize_f8", "tvk_gemm_f8",
     "tvk_paged_append", "tvk_paged_attention",
     "tvk_gemm_noalloc", "tvk_event_create", "tvk_event_destroy", "tvk_event_record",
     "tvk_event_query", "tvk_event_synchronize", "tvk_event_elapsed", "tvk_stream_wait_event", "tvk_stream_query",
@@ -855,6 +882,67 @@ def layer_norm_bwd(dy, h, weight=None, dh=None, eps=1e-5, stream=None):
     d = make_layer_norm_bwd_desc(dy, h, weight, dx, dweight, dbias, dh, eps, _stream_of(h, stream))
     check(load().tvk_layer_norm_bwd(C.byref(d)))
     return dx, dweight, dbias
+
+
+def make_quantize_f8_desc(x, out, scale, block_rows=1, stream=None) -> QuantizeF8Desc:
+    """Describes tvk_quantize_f8 of a [rows, cols] device tensor: float8_e4m3fn out, float32 scale
+    [ceil(rows / block_rows), ceil(cols / 128)]."""
+    torch = _torch()
+    if x.dim() != 2:
+        raise _invalid(f"x: {x.dim()} dimensions, expected [rows, cols]")
+    if block_rows not in (1, F8_BLOCK):
+        raise TvkUnsupported(TVK_ERR_UNSUPPORTED, f"blocks of {block_rows} rows, expected 1 or {F8_BLOCK}")
+    d = QuantizeF8Desc()
+    d.dtype, d.block_rows = _dtype_code(x.dtype), block_rows
+    d.rows, d.cols = x.shape
+    d.x, d.x_stride = x.data_ptr(), _row_stride(x, d.rows, d.cols, x.dtype, "x")
+    d.out, d.out_stride = out.data_ptr(), _row_stride(out, d.rows, d.cols, torch.float8_e4m3fn, "out")
+    d.scale, d.scale_stride = _scales(scale, -(-d.rows // block_rows), blocks_of(d.cols), "scale")
+    d.stream = stream
+    return d
+
+
+def quantize_f8(x, block_rows=1, stream=None):
+    """(out, scale) of tvk_quantize_f8, new tensors."""
+    torch = _torch()
+    out = torch.empty(x.shape, dtype=torch.float8_e4m3fn, device=x.device)
+    scale = torch.empty((-(-x.shape[0] // block_rows), blocks_of(x.shape[1])), dtype=torch.float32, device=x.device)
+    check(load().tvk_quantize_f8(C.byref(make_quantize_f8_desc(x, out, scale, block_rows, _stream_of(x, stream)))))
+    return out, scale
+
+
+def make_gemm_f8_desc(a, a_scale, b, b_scale, out, bias=None, stream=None) -> GemmF8Desc:
+    """Describes tvk_gemm_f8 over device tensors: a [M, K] in float8_e4m3fn with a_scale [M, ceil(K / 128)], or in another
+    type without; b [N, K] in float8_e4m3fn with b_scale [ceil(N / 128), ceil(K / 128)]; out [M, N]."""
+    torch = _torch()
+    if a.dim() != 2 or b.dim() != 2 or out.dim() != 2:
+        raise _invalid("a: [M, K], b: [N, K] and out: [M, N] are expected")
+    d = GemmF8Desc()
+    (d.M, d.K), d.N = a.shape, b.shape[0]
+    in8 = a.dtype == torch.float8_e4m3fn
+    d.a_dtype = TVK_F8E4M3FN if in8 else _dtype_code(a.dtype)
+    d.a, d.a_stride = a.data_ptr(), _row_stride(a, d.M, d.K, a.dtype, "a")
+    if in8 != (a_scale is not None):
+        raise _invalid("a_scale: wanted with a float8_e4m3fn a and only then")
+    if in8:
+        d.a_scale, d.a_scale_stride = _scales(a_scale, d.M, blocks_of(d.K), "a_scale")
+    d.b, d.b_stride = b.data_ptr(), _row_stride(b, d.N, d.K, torch.float8_e4m3fn, "b")
+    d.b_scale, d.b_scale_stride = _scales(b_scale, blocks_of(d.N), blocks_of(d.K), "b_scale")
+    d.out_dtype = d.bias_dtype = _dtype_code(out.dtype)
+    d.out, d.out_stride = out.data_ptr(), _row_stride(out, d.M, d.N, out.dtype, "out")
+    if bias is not None:
+        d.bias, d.bias_dtype = _vector(bias, d.N, (out.dtype, torch.float32), "bias"), _dtype_code(bias.dtype)
+    d.stream = stream
+    return d
+
+
+def gemm_f8(a, a_scale, b, b_scale, bias=None, out_dtype=None, stream=None):
+    """out of tvk_gemm_f8, a new tensor of out_dtype (a's, where that is not 8-bit; bfloat16)."""
+    torch = _torch()
+    out_dtype = out_dtype or (torch.bfloat16 if a.dtype == torch.float8_e4m3fn else a.dtype)
+    out = torch.empty((a.shape[0], b.shape[0]), dtype=out_dtype, device=a.device)
+    check(load().tvk_gemm_f8(C.byref(make_gemm_f8_desc(a, a_scale, b, b_scale, out, bias, _stream_of(a, stream)))))
+    return out
 
 
 def _logits_and_entries(d, logits, index) -> None:

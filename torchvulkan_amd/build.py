@@ -72,6 +72,8 @@ FILE_FLAGS = {
     "gemm_dma128.hip": VGPR_FORM,
     "gemm_seq_ring.hip": VGPR_FORM,
     "gemm_skinny.hip": VGPR_FORM,
+    "gemm_f8.hip": VGPR_FORM,
+    "gemm_f8_ring.hip": VGPR_FORM,
     "conv.hip": VGPR_FORM,
     "conv_nhwc.hip": VGPR_FORM,
     "conv_stem.hip": VGPR_FORM,

@@ -1,0 +1,231 @@
+// Products of 8-bit floats with a scale for each block of 128 (tvk_gemm_f8):
+//   out[m][n] = sum over blocks b of sa[m][b] sb[n / 128][b] sum over k in b of A[m][k] W[n][k]  (+ bias[n]).
+// A matrix instruction takes 128 values of k, a block, into a sum of its own,
+// which is added to the running one times the two scales: four multiply-adds a
+// lane beside 32 cycles of the matrix unit.
+//
+// Up to 64 rows are bound by the bytes of W (this file): a workgroup takes 16 rows
+// of W, its waves the blocks in turn, W and the rows of A straight from memory into
+// the instruction's operands, several blocks on their way at once; the waves' sums
+// meet in LDS. Up to 16 rows of A in 16 or 32 bits are brought into 8 bits on the
+// way, by each workgroup for itself; more rows in a launch of their own. More than
+// 64 rows run gemm_f8_ring.hip.
+#include "gemm_f8.h"
+
+using namespace tvk;
+
+namespace {
+
+constexpr int FR_WAVES = 8;
+constexpr int FR_ROWS = 16;     // of W a workgroup
+
+// 32 bytes of a row, of which `valid` are there (zeros behind them), at any alignment.
+__device__ __forceinline__ i32x8 load32(const uint8_t* p, int valid) {
+    union { Words<16> h[2]; i32x8 v; } u;
+    u.v = i32x8{0, 0, 0, 0, 0, 0, 0, 0};
+    if (valid >= 32) {
+        u.h[0] = load_words<16, 1>(p);
+        u.h[1] = load_words<16, 1>(p + 16);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 32; ++i)
+            if (i < valid) u.v[i / 4] |= (int)((uint32_t)p[i] << i % 4 * 8);
+    }
+    return u.v;
+}
+
+// The same of a row in DT, with the scale of the block that the lanes of one row share out.
+template <int DT>
+__device__ __forceinline__ i32x8 quantize32(const typename elem<DT>::T* p, int valid, float& scale) {
+    typedef typename elem<DT>::T T;
+    constexpr int VEC = 16 / (int)sizeof(T);
+    float v[32];
+    if (valid >= 32) {
+#pragma unroll
+        for (int i = 0; i < 32; i += VEC) {
+            const Words<16> w = load_words<16, sizeof(T)>(p + i);
+#pragma unroll
+            for (int k = 0; k < VEC; ++k) v[i + k] = word_at<DT>(w, k);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 32; ++i) v[i] = i < valid ? elem<DT>::to_f32(p[i]) : 0.0f;
+    }
+    float top = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 32; ++i) top = fmaxf(top, fabsf(v[i]));
+    top = fmaxf(top, __shfl_xor(top, 16));
+    const F8Scale s(fmaxf(top, __shfl_xor(top, 32)));
+    scale = s.s;
+    i32x8 r;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) r[i] = (int)s.pack4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+    return r;
+}
+
+// ADT: the type of A, TVK_F8E4M3FN with scales. MT: blocks of 16 rows of A.
+template <int ADT, int MT, bool WIDE>
+__global__ __launch_bounds__(64 * FR_WAVES) void gemm_f8_rows_kernel(GemmF8Args p) {
+    constexpr bool IN8 = ADT == TVK_F8E4M3FN;
+    constexpr int U = MT == 1 ? 4 : 2;   // blocks on their way
+    const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+    const int r = lane % 16, g = lane / 16, n0 = blockIdx.x * FR_ROWS;
+    const uint8_t* w = p.b + (int64_t)min(n0 + r, p.N - 1) * p.ldb + 32 * g;   // rows past N compute what is not stored
+    const float* sb = p.sb + (int64_t)(n0 / F8_BLOCK) * p.sb_n;
+    f32x4 acc[MT];
+#pragma unroll
+    for (int j = 0; j < MT; ++j) acc[j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    for (int b0 = wave; b0 < p.blocks; b0 += FR_WAVES * U) {
+        i32x8 fw[U], fx[U][MT];
+        float s[U][MT];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int b = b0 + FR_WAVES * u, valid = b < p.blocks ? p.K - b * F8_BLOCK - 32 * g : 0;
+            fw[u] = load32(w + (int64_t)b * F8_BLOCK, valid);
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int b = b0 + FR_WAVES * u, bc = min(b, p.blocks - 1), valid = b < p.blocks ? p.K - b * F8_BLOCK - 32 * g : 0;
+            const float scale = sb[(int64_t)bc * p.sb_b];
+#pragma unroll
+            for (int j = 0; j < MT; ++j) {
+                const int m = 16 * j + r, mc = min(m, p.M - 1), there = m < p.M ? valid : 0;
+                if constexpr (IN8) {
+                    fx[u][j] = load32(static_cast<const uint8_t*>(p.a) + (int64_t)mc * p.lda + (int64_t)b * F8_BLOCK + 32 * g, there);
+                    s[u][j] = p.sa[(int64_t)mc * p.sa_m + (int64_t)bc * p.sa_b] * scale;
+                } else {
+                    typedef typename elem<IN8 ? TVK_F32 : ADT>::T T;
+                    fx[u][j] = quantize32<IN8 ? TVK_F32 : ADT>(static_cast<const T*>(p.a) + (int64_t)mc * p.lda + (int64_t)b * F8_BLOCK + 32 * g,
+                                                               there, s[u][j]);
+                    s[u][j] *= scale;
+                }
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            if (b0 + FR_WAVES * u < p.blocks)   // (a block past the end must not weigh in: its scale may be infinite)
+#pragma unroll
+                for (int j = 0; j < MT; ++j) {
+                    const f32x4 d = f8_mfma<WIDE>(fw[u], fx[u][j]);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) acc[j][i] = fmaf(d[i], s[u][j], acc[j][i]);
+                }
+    }
+    // [wave][m][n]: the waves' sums added in order
+    __shared__ __attribute__((aligned(16))) float sum[FR_WAVES][MT * 16][FR_ROWS + 4];
+#pragma unroll
+    for (int j = 0; j < MT; ++j) *reinterpret_cast<f32x4*>(&sum[wave][16 * j + r][4 * g]) = acc[j];
+    __syncthreads();
+    for (int i = threadIdx.x; i < MT * 16 * FR_ROWS; i += 64 * FR_WAVES) {
+        const int m = i / FR_ROWS, n = n0 + i % FR_ROWS;
+        if (m >= p.M || n >= p.N) continue;
+        float v = sum[0][m][i % FR_ROWS];
+#pragma unroll
+        for (int k = 1; k < FR_WAVES; ++k) v += sum[k][m][i % FR_ROWS];
+        const int64_t o = m * p.ldo + n;
+        if (p.out_dtype == TVK_F32) static_cast<float*>(p.out)[o] = f8_finish<TVK_F32>(p, n, v);
+        else if (p.out_dtype == TVK_F16) static_cast<half_t*>(p.out)[o] = f8_finish<TVK_F16>(p, n, v);
+        else static_cast<uint16_t*>(p.out)[o] = f8_finish<TVK_BF16>(p, n, v);
+    }
+}
+
+template <int ADT, bool WIDE>
+void few_rows(const GemmF8Args& p, hipStream_t s) {
+    const dim3 grid((unsigned)((p.N + FR_ROWS - 1) / FR_ROWS)), block(64 * FR_WAVES);
+    if (p.M <= 16) hipLaunchKernelGGL((gemm_f8_rows_kernel<ADT, 1, WIDE>), grid, block, 0, s, p);
+    else if constexpr (ADT == TVK_F8E4M3FN) {
+        if (p.M <= 32) hipLaunchKernelGGL((gemm_f8_rows_kernel<ADT, 2, WIDE>), grid, block, 0, s, p);
+        else hipLaunchKernelGGL((gemm_f8_rows_kernel<ADT, 4, WIDE>), grid, block, 0, s, p);
+    }
+}
+
+template <int ADT>
+void few_rows(const GemmF8Args& p, hipStream_t s) {
+    if (p.out_dtype == TVK_F32) few_rows<ADT, true>(p, s);
+    else few_rows<ADT, false>(p, s);
+}
+
+constexpr int64_t RING_MOST = 1 << 22;   // bytes from row to row: a tile's offsets stay within 31 bits
+
+// Rows that the tiled kernel's loads of 16 bytes meet.
+bool ring_rows(const void* p, int64_t stride, int K) {
+    return reinterpret_cast<uintptr_t>(p) % 16 == 0 && stride % 16 == 0 && stride <= RING_MOST && K % 16 == 0;
+}
+
+}  // namespace
+
+extern "C" tvk_status tvk_gemm_f8(const tvk_gemm_f8_desc* d) {
+    auto bad = [](tvk_status st, const char* m) { return fail(st, std::string("tvk_gemm_f8: ") + m); };
+    if (!d) return bad(TVK_ERR_INVALID, "desc is NULL");
+    const bool in8 = d->a_dtype == TVK_F8E4M3FN;
+    if (!in8 && !norm_dtype(d->a_dtype)) return bad(TVK_ERR_UNSUPPORTED, "a's dtype must be float8_e4m3fn, float32, float16 or bfloat16");
+    if (!norm_dtype(d->out_dtype)) return bad(TVK_ERR_UNSUPPORTED, "the output's dtype must be float32, float16 or bfloat16");
+    if (d->bias_dtype != d->out_dtype && d->bias_dtype != TVK_F32)
+        return bad(TVK_ERR_UNSUPPORTED, "the bias's dtype must be the output's or float32");
+    if (d->M < 0 || d->N < 0 || d->K < 0) return bad(TVK_ERR_INVALID, "negative size");
+    if (d->M > 0x7fffffff || d->N > 0x7fffffff || d->K > 0x7fff0000) return bad(TVK_ERR_UNSUPPORTED, "sizes below 2^31 only");
+    if (d->M == 0 || d->N == 0) return TVK_OK;
+    if ((d->K > 0 && (!d->a || !d->b || !d->b_scale || (in8 && !d->a_scale))) || !d->out) return bad(TVK_ERR_INVALID, "NULL tensor");
+    if (d->a_stride < 0 || d->b_stride < 0 || d->a_scale_stride[0] < 0 || d->a_scale_stride[1] < 0 || d->b_scale_stride[0] < 0 ||
+        d->b_scale_stride[1] < 0 || !rows_apart(d->out_stride, d->M, d->N))
+        return bad(TVK_ERR_INVALID, "negative strides, or output rows that overlap");
+    if (d->M > 64 && d->K > RING_MOST) return bad(TVK_ERR_UNSUPPORTED, "K up to 2^22 only for more than 64 rows");
+    if (((d->M + 127) / 128) * ((d->N + 127) / 128) > (1 << 22)) return bad(TVK_ERR_UNSUPPORTED, "more than 2^22 tiles of 128 x 128");
+    GemmF8Args p{};
+    p.a = d->a;
+    p.b = static_cast<const uint8_t*>(d->b);
+    p.sa = d->a_scale;
+    p.sb = d->b_scale;
+    p.bias = d->bias;
+    p.out = d->out;
+    p.lda = d->a_stride;
+    p.ldb = d->b_stride;
+    p.ldo = d->out_stride;
+    p.sa_m = d->a_scale_stride[0];
+    p.sa_b = d->a_scale_stride[1];
+    p.sb_n = d->b_scale_stride[0];
+    p.sb_b = d->b_scale_stride[1];
+    p.M = (int)d->M;
+    p.N = (int)d->N;
+    p.K = (int)d->K;
+    p.blocks = (p.K + F8_BLOCK - 1) / F8_BLOCK;
+    p.out_dtype = d->out_dtype;
+    p.bias32 = d->bias_dtype == TVK_F32;
+    const hipStream_t s = resolve_stream(d->stream);
+    const int64_t wide = (int64_t)p.blocks * F8_BLOCK;
+    const bool ring = p.M > 64;
+    // what has to be laid out first: rows of A in 16 or 32 bits, and for the tiled kernel rows that 16-byte loads do not meet
+    const bool make_a = !in8 && p.M > 16, pad_a = ring && in8 && !ring_rows(d->a, d->a_stride, p.K);
+    const bool pad_b = ring && !ring_rows(d->b, d->b_stride, p.K);
+    Scratch scratch;
+    if (p.K > 0 && (make_a || pad_a || pad_b)) {
+        const int64_t bytes_a = make_a || pad_a ? p.M * wide : 0, bytes_b = pad_b ? p.N * wide : 0;
+        const int64_t bytes_s = make_a ? (int64_t)p.blocks * p.M * 4 : 0;
+        uint8_t* at = static_cast<uint8_t*>(scratch.get((size_t)(bytes_a + bytes_b + bytes_s) + 16, s));
+        if (!at) return bad(TVK_ERR_OOM, "workspace allocation failed");
+        if (make_a) {
+            float* scale = reinterpret_cast<float*>(at + bytes_a + bytes_b);
+            f8_quantize_rows(d->a_dtype, d->a, d->a_stride, at, scale, p.M, p.K, s);
+            p.sa = scale;
+            p.sa_m = 1;
+            p.sa_b = p.M;
+        } else if (pad_a) {
+            f8_pad_rows(static_cast<const uint8_t*>(d->a), d->a_stride, at, p.M, p.K, s);
+        }
+        if (bytes_a) p.a = at, p.lda = wide;
+        if (pad_b) {
+            f8_pad_rows(p.b, p.ldb, at + bytes_a, p.N, p.K, s);
+            p.b = at + bytes_a;
+            p.ldb = wide;
+        }
+    }
+    if (ring && p.K % 16) p.K = (int)wide;   // both are copies then, with zeros up to there
+    if (ring) f8_ring(p, s);
+    else if (in8 || make_a) few_rows<TVK_F8E4M3FN>(p, s);
+    else if (d->a_dtype == TVK_F32) few_rows<TVK_F32>(p, s);
+    else if (d->a_dtype == TVK_F16) few_rows<TVK_F16>(p, s);
+    else few_rows<TVK_BF16>(p, s);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return fail(TVK_ERR_DEVICE, std::string("tvk_gemm_f8: launch failed: ") + hipGetErrorString(e));
+    return TVK_OK;
+}

@@ -13,7 +13,8 @@ import torch
 
 from . import _abi
 
-__all__ = ["rms_norm", "rms_norm_fp8", "layer_norm", "layer_norm_fp8", "distill_loss", "rotary_table", "PagedKVCache"]
+__all__ = ["rms_norm", "rms_norm_fp8", "layer_norm", "layer_norm_fp8", "quantize_fp8", "linear_fp8", "distill_loss",
+            "rotary_table", "PagedKVCache"]
 
 
 def _stream(t: torch.Tensor):
@@ -211,6 +212,35 @@ def layer_norm_fp8(x, weight=None, bias=None, residual=None, eps: float = 1e-5):
     if h is None:
         return *_without_gradient("layer_norm_fp8", out, x, weight, bias), x
     return _without_gradient("layer_norm_fp8", (*out, h.view(x.shape)), x, weight, bias, residual)
+
+
+def quantize_fp8(x, block_rows: int = 1):
+    """(values, scale): x [..., cols] in float8_e4m3fn with a float32 scale for each 128 columns of a row, scale
+    [..., ceil(cols / 128)]; with block_rows 128, for a weight [rows, cols], a scale for each 128 x 128 of it
+    (tvk_quantize_f8). No gradient: a backward pass that reaches the results raises."""
+    if x.dim() == 0 or (block_rows != 1 and x.dim() != 2):
+        raise _abi.TvkError(_abi.TVK_ERR_INVALID, "x: [..., cols] is expected, [rows, cols] with blocks of 128 rows")
+    x2 = _rows(x.detach())
+    out = torch.empty(x2.shape, dtype=torch.float8_e4m3fn, device=x.device)
+    scale = torch.empty((-(-x2.shape[0] // max(1, block_rows)), _abi.blocks_of(x2.shape[1])), dtype=torch.float32, device=x.device)
+    _queue("tvk_quantize_f8", _abi.make_quantize_f8_desc(x2, out, scale, block_rows, _stream(x)), x)
+    results = (out.view(x.shape), scale if block_rows != 1 else scale.view(*x.shape[:-1], scale.shape[1]))
+    return _without_gradient("quantize_fp8", results, x)
+
+
+def linear_fp8(x, weight, weight_scale, bias=None, x_scale=None, out_dtype=None):
+    """x [..., k] times an 8-bit weight [n, k], as quantize_fp8(w, 128) gives it: [..., n] in out_dtype (x's; bfloat16 for an
+    8-bit x). x is 8-bit with x_scale [..., ceil(k / 128)], as layer_norm_fp8 gives it, or in 16 or 32 bits, brought
+    into that form by the call (tvk_gemm_f8). No gradient: a backward pass that reaches the result raises."""
+    if x.dim() == 0 or (x_scale is not None and x_scale.shape[:-1] != x.shape[:-1]):
+        raise _abi.TvkError(_abi.TVK_ERR_INVALID, "x: [..., k], and x_scale: [..., ceil(k / 128)], are expected")
+    _check_devices(x.device, weight, weight_scale, bias, x_scale)
+    x2 = _rows(x.detach())
+    s2 = None if x_scale is None else x_scale.detach().reshape(x2.shape[0], x_scale.shape[-1])
+    out = torch.empty((x2.shape[0], weight.shape[0]), device=x.device,
+                      dtype=out_dtype or (torch.bfloat16 if x.dtype == torch.float8_e4m3fn else x.dtype))
+    _queue("tvk_gemm_f8", _abi.make_gemm_f8_desc(x2, s2, weight.detach(), weight_scale.detach(), out, bias, _stream(x)), x)
+    return _without_gradient("linear_fp8", out.view(*x.shape[:-1], weight.shape[0]), x, weight, weight_scale, bias, x_scale)
 
 
 class _Distill(torch.autograd.Function):
