@@ -667,6 +667,44 @@ typedef struct {
 tvk_status tvk_distill_bwd(const tvk_distill_bwd_desc* desc);
 
 /* ------------------------------------------------------------------------- */
+/* Sampling                                                                   */
+/* ------------------------------------------------------------------------- */
+
+/* The next token of every row of logits, drawn with the row's number `random`
+ * in [0, 1). A token weighs w = exp((x - max x) / T), in 64 bits; in the order
+ * from the largest logit down, of equal ones the lowest index first, are kept
+ *   the first top_k (0 or less: all), of those
+ *   the shortest prefix that weighs at least top_p of their sum (1 and above, or
+ *     NaN: all; 0 and less: the first), and of that
+ *   those with w >= min_p (0 and less, or NaN: all; above 1 is taken as 1);
+ * token = the lowest index at which the sum of the kept tokens' weights up to it
+ * is above random times their total; logprob = log of its share of the total.
+ * T 0, below or NaN: the largest logit's token, the lowest index of equal ones,
+ * and logprob 0. Weights below 2^-45 count as zero. NaN logits count as -inf,
+ * beside +inf the others weigh nothing; a row without any logit above -inf gives
+ * token -1 and logprob NaN. random below 0, or NaN, counts as 0, 1 and above as
+ * the last of the kept.
+ * temperature, top_k, top_p, min_p: a value for each row, on the device (NULL: 1,
+ * and no filter), so that a captured call follows them. dtype F32, F16 or BF16;
+ * rows are contiguous, logits_stride elements apart (0: one for all), of any
+ * alignment and at most 2^19 values. The same bits every run. */
+typedef struct {
+    int32_t dtype, reserved;
+    int64_t rows, cols;
+    const void* logits; int64_t logits_stride;
+    const float* random;                                 /* [rows] */
+    const float* temperature;                            /* [rows] */
+    const int32_t* top_k;                                /* [rows] */
+    const float* top_p;                                  /* [rows] */
+    const float* min_p;                                  /* [rows] */
+    int64_t* token;                                      /* [rows] */
+    float* logprob;                                      /* [rows], NULL: not wanted */
+    void* stream;
+} tvk_sample_desc;
+
+tvk_status tvk_sample(const tvk_sample_desc* desc);
+
+/* ------------------------------------------------------------------------- */
 /* Paged key/value cache: append with rotation, attention                     */
 /* ------------------------------------------------------------------------- */
 

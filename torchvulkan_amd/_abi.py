@@ -303,6 +303,18 @@ class GemmF8Desc(C.Structure):
     ]
 
 
+class SampleDesc(C.Structure):
+    _fields_ = [
+        ("dtype", C.c_int32), ("reserved", C.c_int32),
+        ("rows", C.c_int64), ("cols", C.c_int64),
+        ("logits", C.c_void_p), ("logits_stride", C.c_int64),
+        ("random", C.c_void_p),
+        ("temperature", C.c_void_p), ("top_k", C.c_void_p), ("top_p", C.c_void_p), ("min_p", C.c_void_p),
+        ("token", C.c_void_p), ("logprob", C.c_void_p),
+        ("stream", C.c_void_p),
+    ]
+
+
 class PagedCache(C.Structure):
     _fields_ = [
         ("dtype", C.c_int32), ("reserved", C.c_int32),
@@ -421,6 +433,7 @@ def load() -> C.CDLL:
         lib.tvk_distill_bwd.argtypes = [C.POINTER(DistillBwdDesc)]
         lib.tvk_quantize_f8.argtypes = [C.POINTER(QuantizeF8Desc)]
         lib.tvk_gemm_f8.argtypes = [C.POINTER(GemmF8Desc)]
+        lib.tvk_sample.argtypes = [C.POINTER(SampleDesc)]
         lib.tvk_paged_append.argtypes = [C.POINTER(PagedAppendDesc)]
         lib.tvk_paged_attention.argtypes = [C.POINTER(PagedAttentionDesc)]
         lib.tvk_calibrate_mfma.argtypes = [C.c_int, C.c_int, C.c_int, C.POINTER(C.c_double), C.POINTER(C.c_double)]
@@ -446,7 +459,7 @@ _ALL_ENTRY_POINTS = (
     "tvk_copy", "tvk_copy_plan",
     "tvk_fill", "tvk_reduce_sum", "tvk_binary", "tvk_attention_fwd",
     "tvk_attention_bwd", "tvk_rms_norm_fwd", "tvk_rms_norm_bwd", "tvk_layer_norm_fwd", "tvk_layer_norm_bwd",
-    "tvk_distill_fwd", "tvk_distill_bwd", "tvk_quantize_f8", "tvk_gemm_f8",
+    "tvk_distill_fwd", "tvk_distill_bwd", "tvk_quantize_f8", "tvk_gemm_f8", "tvk_sample",
     "tvk_paged_append", "tvk_paged_attention",
     "tvk_gemm_noalloc", "tvk_event_create", "tvk_event_destroy", "tvk_event_record",
     "tvk_event_query", "tvk_event_synchronize", "tvk_event_elapsed", "tvk_stream_wait_event", "tvk_stream_query",
@@ -680,7 +693,7 @@ def attention_bwd(q, k, v, out, lse, dout, bias=None, causal=False, scale=None, 
 
 
 # ---------------------------------------------------------------------------
-# norms, distillation loss, paged key/value cache
+# norms, 8-bit block products, distillation loss, sampling, paged key/value cache
 # ---------------------------------------------------------------------------
 
 def _invalid(message: str):
@@ -1013,6 +1026,38 @@ def distill_bwd(logits, index, lse, target, dloss, temperature=1.0, stream=None)
     d = make_distill_bwd_desc(logits, index, lse, target, dloss, dlogits, temperature, _stream_of(logits, stream))
     check(load().tvk_distill_bwd(C.byref(d)))
     return dlogits
+
+
+def make_sample_desc(logits, random, token, logprob=None, temperature=None, top_k=None, top_p=None, min_p=None,
+                     stream=None) -> SampleDesc:
+    """Describes tvk_sample over device tensors: logits [rows, cols], random [rows] in [0, 1), int64 token [rows], and for
+    each row temperature, top_p, min_p (float32) and top_k (int32)."""
+    torch = _torch()
+    if logits.dim() != 2:
+        raise _invalid(f"logits: {logits.dim()} dimensions, expected [rows, cols]")
+    d = SampleDesc()
+    d.dtype = _dtype_code(logits.dtype)
+    d.rows, d.cols = logits.shape
+    d.logits, d.logits_stride = logits.data_ptr(), _row_stride(logits, d.rows, d.cols, logits.dtype, "logits")
+    d.random = _vector(random, d.rows, (torch.float32,), "random")
+    for name, t in (("temperature", temperature), ("top_p", top_p), ("min_p", min_p), ("logprob", logprob)):
+        if t is not None:
+            setattr(d, name, _vector(t, d.rows, (torch.float32,), name))
+    if top_k is not None:
+        d.top_k = _vector(top_k, d.rows, (torch.int32,), "top_k")
+    d.token = _vector(token, d.rows, (torch.int64,), "token")
+    d.stream = stream
+    return d
+
+
+def sample(logits, random, temperature=None, top_k=None, top_p=None, min_p=None, stream=None):
+    """(token, logprob) of tvk_sample, new tensors."""
+    torch = _torch()
+    token = torch.empty(logits.shape[0], dtype=torch.int64, device=logits.device)
+    logprob = torch.empty(logits.shape[0], dtype=torch.float32, device=logits.device)
+    d = make_sample_desc(logits, random, token, logprob, temperature, top_k, top_p, min_p, _stream_of(logits, stream))
+    check(load().tvk_sample(C.byref(d)))
+    return token, logprob
 
 
 def make_paged_cache(k_cache, v_cache, seq_lens, table, k_scale=None, v_scale=None, new_lens=None) -> PagedCache:

@@ -14,7 +14,7 @@ import torch
 from . import _abi
 
 __all__ = ["rms_norm", "rms_norm_fp8", "layer_norm", "layer_norm_fp8", "quantize_fp8", "linear_fp8", "distill_loss",
-            "rotary_table", "PagedKVCache"]
+           "sample", "rotary_table", "PagedKVCache"]
 
 
 def _stream(t: torch.Tensor):
@@ -273,6 +273,33 @@ def distill_loss(logits, index, teacher, temperature: float = 1.0):
         raise _abi.TvkError(_abi.TVK_ERR_INVALID, "logits: [..., cols], index and teacher: [..., top] are expected")
     _check_devices(logits.device, index, teacher)
     return _Distill.apply(logits, index, teacher.detach(), float(temperature))
+
+
+def sample(logits, random, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
+    """(token, logprob): the next token of every row of logits [..., cols], int64 [...], drawn with the numbers random [...]
+    in [0, 1), and the logarithm of the probability that it was drawn with (tvk_sample). temperature, top_k, top_p and min_p
+    are numbers, or tensors [...] (float32, top_k int32) of the logits' device that a captured call follows. No gradient: a
+    backward pass that reaches the results raises."""
+    shape = logits.shape[:-1]
+    if logits.dim() == 0 or random.shape != shape:
+        raise _abi.TvkError(_abi.TVK_ERR_INVALID, "logits: [..., cols] and random: [...] are expected")
+
+    def of_rows(value, dtype, off, name):
+        if not isinstance(value, torch.Tensor):
+            return None if value == off else torch.full((math.prod(shape),), value, dtype=dtype, device=logits.device)
+        if value.shape != shape or value.dtype != dtype:
+            raise _abi.TvkError(_abi.TVK_ERR_INVALID, f"{name}: {dtype} {tuple(shape)} is expected, not {value.dtype} {tuple(value.shape)}")
+        return value.detach().reshape(-1)
+
+    filters = [of_rows(temperature, torch.float32, 1.0, "temperature"), of_rows(top_k, torch.int32, 0, "top_k"),
+               of_rows(top_p, torch.float32, 1.0, "top_p"), of_rows(min_p, torch.float32, 0.0, "min_p")]
+    _check_devices(logits.device, random, *filters)
+    x = _rows(logits.detach())
+    token = torch.empty(x.shape[0], dtype=torch.int64, device=x.device)
+    logprob = torch.empty(x.shape[0], dtype=torch.float32, device=x.device)
+    _queue("tvk_sample", _abi.make_sample_desc(x, random.detach().reshape(-1), token, logprob, *filters, _stream(x)), x)
+    token, logprob = token.view(shape), logprob.view(shape)
+    return token, _without_gradient("sample", logprob, logits, random)
 
 
 def rotary_table(positions: int, rotary_dim: int, base: float = 10000.0, device="cpu") -> torch.Tensor:
