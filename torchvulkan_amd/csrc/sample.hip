@@ -3,19 +3,30 @@
 // With s = x / T a token weighs exp(s - max s); what the filters leave is a prefix
 // of the tokens in the order of their logits, equal ones in that of their indexes:
 // those above a border value and the first few that equal it. So nothing is
-// sorted. A histogram over the logits' distance from the largest, counts and sums
-// of weights, says which bin the border of a filter falls into; the bin's own
-// values, a few, are compared with each other in LDS, or spread over a histogram
-// of their own until they are few or all equal. The token is then the first in the
+// sorted. A histogram over the logits' distance from the largest, of counts or of
+// weights, says which bin the border of a filter falls into; the bin's own values,
+// a few, are compared with each other in LDS, or spread over a histogram of their
+// own until they are few or all equal. The token is then the first in the
 // vocabulary's order at which the sum of kept weights passes the random number's
-// share of their total, found by halving ranges 16 ways.
+// share of their total: sums over stretches of the row say in which it lies.
 //
 // Weights are integers: 2^44 exp(s - max s) from float64, rounded. Their sums are
 // exact in 64 bits whatever the order (2^44 times at most 2^19 tokens), so that the
-// atomics of a histogram and the split of a row over threads leave no trace in the
-// result, and the borders fall where the formulas in 64 bits put them: float32
-// weights would put one in 10^4 draws from a flat distribution elsewhere.
+// atomics of a histogram and the split of a row over threads and workgroups leave
+// no trace in the result, and the borders fall where the formulas in 64 bits put
+// them: float32 weights would put one in 10^4 draws from a flat distribution
+// elsewhere.
+//
+// The row stays in the registers of 1024 threads, 64 K values in 16 bits, and is
+// read again for every pass past that. Most of a small call is latency, and much of
+// that the code's own: a line of 64 bytes that no cache holds takes as long as a
+// load. So passes are loops over a thread's words, not unrolled, helpers are called,
+// not inlined, and nothing is read in a chain that can be read at once. Few rows are
+// cut among workgroups, in four launches: the largest, the histogram, what lies in
+// and above the border's bin, the token.
 #include "norm_rows.h"
+
+#include <cfloat>
 
 using namespace tvk;
 
@@ -26,7 +37,16 @@ typedef unsigned long long u64;
 constexpr int SA_THREADS = 1024, SA_WAVES = SA_THREADS / 64;
 constexpr int SA_BINS = 2 * SA_THREADS;
 constexpr int SA_LIST = 256;       // values of a bin that are compared with each other
+constexpr int SA_FEW = 512;        // tokens that are
+constexpr int SA_PIECES = 32;      // of a row, at most
 constexpr int64_t SA_MOST_COLS = 1 << 19;
+
+// Where a row that is cut among workgroups goes on.
+enum { SA_FIRST, SA_ALL, SA_TOKENS, SA_SUMS, SA_WHOLE };
+struct RowState {
+    int mode, bin;
+    u64 above, need;
+};
 
 struct SampleArgs {
     const void* x;
@@ -39,383 +59,820 @@ struct SampleArgs {
     float* logprob;
     int64_t rows, stride;
     int cols;
+    // of rows cut into pieces
+    int pieces, piece;     // chunks of a piece
+    RowState* state;       // [rows]
+    u64* bins;             // [rows][pieces][SA_BINS]
+    u64* places;           // [rows][SA_BINS]
+    float* tops;           // [rows][pieces]
+    unsigned* listed;      // [rows][pieces]
+    float* list_v;         // [rows][pieces][SA_FEW]
+    int* list_at;
 };
 
-// A row's weights.
+constexpr int SA_STEPS = 64;   // of a power of two in a table
+
+// 2^(44 + j / 64), from the exponential's series.
+struct StepTable {
+    double v[SA_STEPS];
+    constexpr StepTable() : v{} {
+        for (int j = 0; j < SA_STEPS; ++j) {
+            double term = 0x1p44, sum = 0x1p44;
+            for (int n = 1; n < 24; ++n) sum += term *= 0.693147180559945309 * j / SA_STEPS / n;
+            v[j] = sum;
+        }
+    }
+};
+__constant__ StepTable kSteps = StepTable();
+
+// A row's weights: exp((x - top) / T) = 2^(n / 64) 2^r, n whole and |r| <= 1 / 128.
 struct Heat {
-    float top;   // the largest logit
-    double c;    // log2(e) / T
-    // exp((x - top) / T), within 2^-46 of itself; below 2^-50 zero
-    __device__ double weight(float x) const {
-        if (x == top) return 1.0;   // infinities too
-        const double t = ((double)x - (double)top) * c;
-        if (!(t > -50.0)) return 0.0;
-        const double n = rint(t), f = (t - n) * 0.693147180559945309;
-        // the exponential's series up to f^11 / 11!: |f| <= 0.3466, so what follows is below 7e-15
-        double p = 1.0 / 39916800;
-        p = fma(p, f, 1.0 / 3628800);
-        p = fma(p, f, 1.0 / 362880);
-        p = fma(p, f, 1.0 / 40320);
-        p = fma(p, f, 1.0 / 5040);
-        p = fma(p, f, 1.0 / 720);
-        p = fma(p, f, 1.0 / 120);
-        p = fma(p, f, 1.0 / 24);
-        p = fma(p, f, 1.0 / 6);
-        p = fma(p, f, 0.5);
-        p = fma(p, f, 1.0);
-        p = fma(p, f, 1.0);
-        return ldexp(p, (int)n);
+    float top;             // the largest logit
+    double c;              // 64 log2(e) / T
+    const double* table;   // 2^(44 + j / 64), in LDS
+
+    // 2^44 times the weight, within 2^-44 of it; next to nothing below 2^-60. Beside an infinite logit the others weigh nothing.
+    __device__ __forceinline__ double large_weight(float x) const {
+        if (top == INFINITY) return x == top ? 0x1p44 : 0.0;
+        const double y = fmax(((double)x - (double)top) * c, -60.0 * SA_STEPS);
+        const double shifted = y + 0x1.8p52;   // n in its low bits
+        const int n = (int)(uint32_t)__builtin_bit_cast(u64, shifted);
+        const double f = y - (shifted - 0x1.8p52), ln = 0.0108304246962491454;   // ln 2 / 64; f ln at most 0.0054 in magnitude
+        // its exponential: (f ln)^5 / 120 is left, 4e-14
+        const double p = fma(fma(fma(fma(f, ln * ln * ln * ln / 24, ln * ln * ln / 6), f, ln * ln / 2), f, ln), f, 1.0);
+        return __builtin_bit_cast(double, __builtin_bit_cast(u64, table[n & (SA_STEPS - 1)] * p) + ((u64)(uint32_t)(n >> 6) << 52));
     }
-    __device__ static u64 whole(double w) {   // 2^44 w rounded: the low bits of a sum whose last place is 1
-        return __builtin_bit_cast(u64, fma(w, 0x1p44, 0x1p52)) & ((1ull << 52) - 1);
+    __device__ static u64 whole(double w) {   // rounded: the low bits of a sum whose last place is 1
+        return __builtin_bit_cast(u64, w + 0x1p52) & ((1ull << 52) - 1);
     }
-    __device__ u64 whole_weight(float x) const { return whole(weight(x)); }
+    __device__ __forceinline__ u64 whole_weight(float x) const { return whole(large_weight(x)); }
 };
 
-// A row in chunks of 16 bytes; -inf past its end and for NaN, and zeros of one sign.
+// Chunks [first, end) of 16 bytes of a row, thread t those at first + t + 1024 j, eight of them in registers.
 template <int DT>
-struct Logits {
+struct Row8 {
     typedef typename elem<DT>::T T;
-    static constexpr int VEC = 16 / (int)sizeof(T);
+    typedef uint32_t W32 __attribute__((ext_vector_type(32)));
+    static constexpr int VEC = 16 / (int)sizeof(T), HELD = 8 * SA_THREADS;   // chunks that are held
+    static constexpr int N = 2, STEP = DT == TVK_F32 ? 2 : 1;                // values handled together, their words
     const T* row;
-    int cols, chunks;
-    __device__ static float cleaned(float v) { return v == v ? v + 0.0f : -INFINITY; }
-    __device__ void load(int c, float (&v)[VEC]) const {
-        if ((c + 1) * VEC <= cols) {
-            const Words<16> w = load_words<16, sizeof(T)>(row + c * VEC);
+    int cols, first, end, at, words;   // at: the first of the held; words of a thread
+    W32 w;
+
+    __device__ __forceinline__ Row8(const SampleArgs& p, int64_t r, int first, int last)
+        : row(static_cast<const T*>(p.x) + r * p.stride), cols(p.cols), first(first), end(min(last, (p.cols + VEC - 1) / VEC)) {
+        load(first);
+    }
+    __device__ __forceinline__ void load(int from) {
+        at = from;
+        words = min(8, (end - from + SA_THREADS - 1) / SA_THREADS) * 4;
+        const int whole = min(end, cols / VEC), mine = from + (int)threadIdx.x;   // past `whole` lies at most a piece of a chunk
+        const T* p = row + (int64_t)mine * VEC;
+        Words<16> c[8];
 #pragma unroll
-            for (int k = 0; k < VEC; ++k) v[k] = cleaned(word_at<DT>(w, k));
-        } else {
+        for (int j = 0; j < 8; ++j) {
+            c[j] = {};
+            if (mine + j * SA_THREADS < whole) c[j] = load_words<16, sizeof(T)>(p + j * SA_THREADS * VEC);
+        }
 #pragma unroll
-            for (int k = 0; k < VEC; ++k) v[k] = c * VEC + k < cols ? cleaned(elem<DT>::to_f32(row[c * VEC + k])) : -INFINITY;
+        for (int j = 0; j < 32; ++j) w[j] = c[j / 4].w[j % 4];
+        if (from + words / 4 * SA_THREADS <= whole) return;
+        constexpr uint32_t LOWEST = DT == TVK_F32 ? 0xff800000u : DT == TVK_F16 ? 0xfc00fc00u : 0xff80ff80u;   // -inf
+#pragma unroll 1
+        for (int k = words - 4; k < words; ++k) {   // of a thread's last chunk
+            uint32_t v = w[k];
+            const int i = mine + k / 4 * SA_THREADS;
+            if (i >= whole) {
+                v = LOWEST;
+                const int e = i * VEC + k % 4 * (VEC / 4);   // the word's first value
+                if (i < end && e < cols) {
+                    if constexpr (DT == TVK_F32) v = __builtin_bit_cast(uint32_t, row[e]);
+                    else {
+                        v = (LOWEST & 0xffff0000u) | __builtin_bit_cast(uint16_t, row[e]);
+                        if (e + 1 < cols) v = (v & 0xffffu) | (uint32_t)__builtin_bit_cast(uint16_t, row[e + 1]) << 16;
+                    }
+                }
+            }
+            w[k] = v;
         }
     }
-    // f(chunk, values) over the row
+    // f(index of the first, two values) over the chunks; NaN as -inf. A chunk's last call is where (index + 2) % VEC is 0.
     template <class F>
-    __device__ void each(F&& f) const {
-        for (int c = threadIdx.x; c < chunks; c += SA_THREADS) {
-            float v[VEC];
-            load(c, v);
-            f(c, v);
+    __device__ __forceinline__ void each(F&& f) {
+#pragma unroll 1
+        for (int from = first; from < end; from += HELD) {
+            if (at != from) load(from);
+#pragma unroll 1
+            for (int k = 0; k < words; k += STEP) {
+                const Words<8> two{{w[k], w[k + STEP - 1]}};
+                const float v[N] = {fmaxf(word_at<DT>(two, 0), -INFINITY), fmaxf(word_at<DT>(two, 1), -INFINITY)};
+                f((from + (int)threadIdx.x + k / 4 * SA_THREADS) * VEC + k % 4 * (VEC / 4), v);
+            }
         }
+    }
+    __device__ float value(int i) const {
+        const float v = elem<DT>::to_f32(row[i]);
+        return v == v ? v : -INFINITY;
     }
 };
 
-// A sum or a maximum over the workgroup, the same bits in every thread.
-template <class V, class F>
-__device__ V all_threads(V v, V* part, F&& f) {
+struct AddOp { template <class V> __device__ static V of(V a, V b) { return a + b; } };
+struct LeastOp { template <class V> __device__ static V of(V a, V b) { return a < b ? a : b; } };
+struct MostOp { template <class V> __device__ static V of(V a, V b) { return a > b ? a : b; } };
+
+// A value from another lane, by CTRL; lanes without a source, or outside ROWS (bits of groups of 16), get `none`.
+template <int CTRL, int ROWS = 0xf, class V>
+__device__ __forceinline__ V from_lane(V v, V none) {
+    if constexpr (sizeof(V) == 8) {
+        const u64 u = __builtin_bit_cast(u64, v), n = __builtin_bit_cast(u64, none);
+        const uint32_t lo = __builtin_amdgcn_update_dpp((int)n, (int)u, CTRL, ROWS, 0xf, false);
+        const uint32_t hi = __builtin_amdgcn_update_dpp((int)(n >> 32), (int)(u >> 32), CTRL, ROWS, 0xf, false);
+        return __builtin_bit_cast(V, (u64)hi << 32 | lo);
+    } else {
+        return __builtin_bit_cast(V, __builtin_amdgcn_update_dpp(__builtin_bit_cast(int, none), __builtin_bit_cast(int, v), CTRL, ROWS, 0xf, false));
+    }
+}
+
+// Over 16 lanes, in each of them.
+template <class Op, class V>
+__device__ __forceinline__ V lanes16(V v) {
+    v = Op::of(v, from_lane<0xB1>(v, v));    // lane ^ 1
+    v = Op::of(v, from_lane<0x4E>(v, v));    // lane ^ 2
+    v = Op::of(v, from_lane<0x141>(v, v));   // mirrored in 8
+    return Op::of(v, from_lane<0x140>(v, v));   // mirrored in 16
+}
+
+// Over the workgroup, the same bits in every thread: waves first, then the waves' results.
+template <class Op, class V>
+__device__ __forceinline__ V all_threads(V v) {
+    __shared__ V part[SA_WAVES * 4];
+    v = lanes16<Op>(v);
+    __syncthreads();
+    if (threadIdx.x % 16 == 0) part[threadIdx.x / 16] = v;
+    __syncthreads();
+    v = part[threadIdx.x % 16];
 #pragma unroll
-    for (int m = 1; m < 64; m <<= 1) v = f(v, __shfl_xor(v, m));
-    __syncthreads();
-    if (threadIdx.x % 64 == 0) part[threadIdx.x / 64] = v;
-    __syncthreads();
-    v = part[0];
-    for (int w = 1; w < SA_WAVES; ++w) v = f(v, part[w]);
+    for (int i = 1; i < 4; ++i) v = Op::of(v, part[threadIdx.x % 16 + 16 * i]);
+    return lanes16<Op>(v);
+}
+
+// Sum of the lanes up to this one.
+__device__ __forceinline__ u64 lanes_up_to(u64 v) {
+    v += from_lane<0x111>(v, (u64)0);         // from the lane before, and 2, 4, 8 before, in groups of 16
+    v += from_lane<0x112>(v, (u64)0);
+    v += from_lane<0x114>(v, (u64)0);
+    v += from_lane<0x118>(v, (u64)0);
+    v += from_lane<0x142, 0xa>(v, (u64)0);    // the first group's last to the second, the third's to the fourth
+    v += from_lane<0x143, 0xc>(v, (u64)0);    // the first half's last to the second half
     return v;
 }
 
-// Sum of the lanes before this one.
-template <class V>
-__device__ V lanes_before(V v) {
-    const V own = v;
-#pragma unroll
-    for (int m = 1; m < 64; m <<= 1) {
-        const V o = __shfl_up(v, m);
-        if ((int)(threadIdx.x % 64) >= m) v += o;
-    }
-    return v - own;
-}
-
-struct Bins {
+// Sums by bin: of weights, or counts in the same words.
+union Bins {
     u64 w[SA_BINS];
-    unsigned n[SA_BINS];
+    unsigned n[2 * SA_BINS];
 };
 
 struct Shared {
-    Bins all, part;        // of the whole row, of a bin
-    float list[SA_LIST];
-    u64 list_w[SA_LIST];
+    Bins all, part;
+    double table[SA_STEPS];
+    float list[SA_FEW + 4];   // (loops over a list run in fours)
+    int list_at[SA_FEW + 4];
+    u64 list_w[SA_FEW + 4];
     u64 sums[SA_WAVES];
-    unsigned counts[SA_WAVES];
-    float values[SA_WAVES];
+    unsigned counts[SA_PIECES];
     // what one thread finds for all
-    u64 found_w;
+    u64 found_w, found_own;
     unsigned found_n, found_count, listed;
-    int found;
+    int found, last;
     float border;
-    int64_t token;
 };
 
-// Values between lo and hi in bins of equal width, the largest first.
+// Values between lo and hi in bins of equal width, the largest first. Rounding moves no value past another, so what is in a
+// bin is settled by the same expression wherever it is asked. FINE: in float64, which tells any two values apart, so that
+// lo and hi never share a bin.
+template <bool FINE>
 struct Range {
+    typedef std::conditional_t<FINE, double, float> F;
     float lo, hi;
-    double scale;
-    __device__ bool has(float x) const { return x >= lo && x <= hi; }
-    __device__ int bin(float x) const { return (int)fmin(((double)hi - (double)x) * scale, (double)(SA_BINS - 1)); }
+    F scale;
+    __device__ __forceinline__ bool has(float x) const { return x >= lo && x <= hi; }
+    __device__ __forceinline__ int bin(float x) const {
+        const F b = ((F)hi - (F)x) * scale;
+        return (int)(b < (F)(SA_BINS - 1) ? b : (F)(SA_BINS - 1));   // infinities and NaN: the last
+    }
 };
 
-// The values that a filter keeps: above t, and the first `ties` that equal it. w: weight of those above.
+// Weights from 1 to 2^-40, the rest in the last bin.
+__device__ inline Range<false> first_range(float top, float heat) {
+    return {top == INFINITY ? top : -FLT_MAX, top, (float)(SA_BINS / (28.0 * heat))};
+}
+
+// The values that a filter keeps: above t, and the first `ties` of the `equal` that equal it.
 struct Border {
     float t;
-    unsigned ties;
-    u64 w;
+    unsigned ties, equal;
 };
 
-template <int DT>
-__device__ void fill_bins(const Logits<DT>& x, const Heat& h, const Range& r, Bins& b) {
-    for (int i = threadIdx.x; i < SA_BINS; i += SA_THREADS) b.w[i] = 0, b.n[i] = 0;
-    __syncthreads();
-    x.each([&](int, const float (&v)[Logits<DT>::VEC]) {
-#pragma unroll
-        for (int k = 0; k < Logits<DT>::VEC; ++k)
-            if (r.has(v[k])) {
-                const int i = r.bin(v[k]);
-                atomicAdd(&b.n[i], 1u);
-                const u64 w = h.whole_weight(v[k]);
-                if (w) atomicAdd(&b.w[i], w);
-            }
-    });
+// A row's filters.
+struct Filters {
+    float heat, top_p, least, random;
+    int top_k;
+    bool by_k, by_p;
+    __device__ Filters(const SampleArgs& p, int64_t row) {
+        heat = p.temperature ? p.temperature[row] : 1.0f;
+        top_p = p.top_p ? p.top_p[row] : 1.0f;
+        least = p.min_p ? p.min_p[row] : 0.0f;
+        top_k = p.top_k ? p.top_k[row] : 0;
+        random = p.random[row];
+        by_k = top_k > 0 && top_k < p.cols;
+        by_p = top_p < 1.0f;
+    }
+    __device__ bool first_only(float top) const { return top == -INFINITY || !(heat > 0.0f) || top_k == 1 || top_p <= 0.0f; }
+    __device__ Heat weights(float top, const Shared& s) const { return {top, SA_STEPS * 1.4426950408889634 / heat, s.table}; }
+    // the weight that reaches top_p's share
+    __device__ u64 share(u64 total) const { return min(total, max((u64)1, (u64)ceil((double)top_p * (double)total))); }
+    // what the sum of weights up to the token is to pass
+    __device__ u64 goal(u64 total) const {
+        const double share = random > 0.0f ? (double)random * (double)total : 0.0;
+        return min(share < (double)total ? (u64)share : total - 1, total - 1);
+    }
+    // 2^44 v's weight, zero where min_p drops it
+    __device__ __forceinline__ u64 weigh(const Heat& h, float v) const {
+        const double w = h.large_weight(v);
+        return least > 0.0f && w < fmin((double)least, 1.0) * 0x1p44 ? (u64)0 : Heat::whole(w);
+    }
+};
+
+__device__ inline void make_table(Shared& s) {
+    if (threadIdx.x < SA_STEPS) s.table[threadIdx.x] = kSteps.v[threadIdx.x];
     __syncthreads();
 }
 
-// The first bin with which the count, or the weight, reaches `need`: s.found, and what is before it.
-__device__ inline void find_bin(const Bins& b, bool by_count, u64 need, Shared& s) {
+__device__ __forceinline__ void clear(Bins& b) {
+    __syncthreads();
+    b.w[threadIdx.x] = b.w[threadIdx.x + SA_THREADS] = 0;
+    __syncthreads();
+}
+
+__device__ __forceinline__ u64 sum_of(const Bins& b, Shared& s) {
+    return all_threads<AddOp>(b.w[threadIdx.x] + b.w[threadIdx.x + SA_THREADS]);
+}
+
+template <int DT, bool FINE>
+__device__ __forceinline__ void fill_bins(Row8<DT>& x, const Heat& h, const Range<FINE>& r, bool counts, Bins& b) {
+    constexpr int N = Row8<DT>::N;
+    clear(b);
+    if (counts)
+        x.each([&](int, const float (&v)[N]) {
+#pragma unroll
+            for (int k = 0; k < N; ++k)
+                if (r.has(v[k])) atomicAdd(&b.n[r.bin(v[k])], 1u);
+        });
+    else
+        x.each([&](int, const float (&v)[N]) {
+            u64 w[N];
+            int bin[N];
+#pragma unroll
+            for (int k = 0; k < N; ++k) {
+                w[k] = h.whole_weight(v[k]);
+                bin[k] = r.bin(v[k]);
+            }
+#pragma unroll
+            for (int k = 0; k < N; ++k)
+                if (r.has(v[k]) && w[k]) atomicAdd(&b.w[bin[k]], w[k]);
+        });
+    __syncthreads();
+}
+
+// The first bin with which the count, or the weight, reaches `need`: s.found (-1: none), s.found_w before it, s.found_own in it.
+__device__ __forceinline__ void find_bin(bool part, bool counts, u64 need, Shared& s) {
+    const Bins& b = part ? s.part : s.all;
     const int i = 2 * threadIdx.x, wave = threadIdx.x / 64;
-    const u64 w0 = b.w[i], w1 = b.w[i + 1];
-    const unsigned n0 = b.n[i], n1 = b.n[i + 1];
-    u64 w = lanes_before(w0 + w1);
-    unsigned n = lanes_before(n0 + n1);
+    const u64 v0 = counts ? b.n[i] : b.w[i], v1 = counts ? b.n[i + 1] : b.w[i + 1];
+    u64 v = lanes_up_to(v0 + v1);
     __syncthreads();
     if (threadIdx.x == 0) s.found = -1;
-    if (threadIdx.x % 64 == 63) s.sums[wave] = w + w0 + w1, s.counts[wave] = n + n0 + n1;
+    if (threadIdx.x % 64 == 63) s.sums[wave] = v;
     __syncthreads();
-    for (int k = 0; k < wave; ++k) w += s.sums[k], n += s.counts[k];
-    auto reaches = [&](u64 w, unsigned n) { return by_count ? n >= need : w >= need; };
-    const bool first = !reaches(w, n) && reaches(w + w0, n + n0), second = !reaches(w + w0, n + n0) && reaches(w + w0 + w1, n + n0 + n1);
+    const int other = threadIdx.x % SA_WAVES;
+    v += lanes16<AddOp>(other < wave ? s.sums[other] : (u64)0) - (v0 + v1);
+    const bool first = v < need && v + v0 >= need, second = v + v0 < need && v + v0 + v1 >= need;
     if (first || second) {
         s.found = first ? i : i + 1;
-        s.found_w = first ? w : w + w0;
-        s.found_n = first ? n : n + n0;
-        s.found_count = first ? n0 : n1;
+        s.found_w = first ? v : v + v0;
+        s.found_own = first ? v0 : v1;
     }
     __syncthreads();
 }
 
-// Where the first `need` tokens end, or those that weigh `need` together.
-template <int DT>
-__device__ Border find_border(const Logits<DT>& x, const Heat& h, Range r, bool by_count, u64 need, Shared& s) {
-    u64 above_w = 0;
-    unsigned above_n = 0;
-    const Bins* bins = &s.all;
-    for (;;) {   // a bin's values are fewer than its range's or lie closer, until they are equal
-        find_bin(*bins, by_count, need - (by_count ? above_n : above_w), s);
-        const int bin = s.found;
-        if (bin < 0) return {-INFINITY, 0, above_w};   // (sums are exact: they reach what is asked of them)
-        above_w += s.found_w;
-        above_n += s.found_n;
-        const unsigned count = s.found_count;
-        __syncthreads();
-        if (threadIdx.x == 0) s.listed = 0;
-        __syncthreads();
-        float lo = INFINITY, hi = -INFINITY;
-        x.each([&](int, const float (&v)[Logits<DT>::VEC]) {
-#pragma unroll
-            for (int k = 0; k < Logits<DT>::VEC; ++k)
-                if (r.has(v[k]) && r.bin(v[k]) == bin) {
-                    lo = fminf(lo, v[k]);
-                    hi = fmaxf(hi, v[k]);
-                    if (count <= SA_LIST) {
-                        const unsigned i = atomicAdd(&s.listed, 1u);
-                        s.list[i] = v[k];
-                        s.list_w[i] = h.whole_weight(v[k]);
-                    }
-                }
-        });
-        lo = all_threads(lo, s.values, [](float a, float b) { return fminf(a, b); });
-        hi = all_threads(hi, s.values, [](float a, float b) { return fmaxf(a, b); });
-        if (lo == hi) {
-            const u64 left = need - (by_count ? above_n : above_w), w = h.whole_weight(lo);
-            return {lo, by_count ? (unsigned)left : (unsigned)((left + w - 1) / w), above_w};
-        }
-        if (count <= SA_LIST) {
-            if (threadIdx.x < count) {
-                const float own = s.list[threadIdx.x];
-                u64 w = above_w;
-                unsigned n = above_n, equal = 0;
-                for (unsigned i = 0; i < count; ++i) {
-                    const float o = s.list[i];
-                    if (o > own) w += s.list_w[i], ++n;
-                    equal += o == own;
-                }
-                const u64 each = s.list_w[threadIdx.x], before = by_count ? n : w;
-                if (before < need && need <= before + (by_count ? equal : equal * each)) {   // all that equal the border write the same
-                    s.border = own;
-                    s.found_n = by_count ? (unsigned)(need - before) : (unsigned)((need - before + each - 1) / each);
-                    s.found_w = w;
-                }
-            }
-            __syncthreads();
-            return {s.border, s.found_n, s.found_w};
-        }
-        r = {lo, hi, SA_BINS / ((double)hi - (double)lo)};
-        fill_bins(x, h, r, s.part);
-        bins = &s.part;
-    }
-}
+// The border among the values of one bin: those before it count, or weigh, `above`.
+struct InBin {
+    bool done;
+    Border b;
+    float lo, hi;
+};
 
-template <int DT>
-__device__ void sample_row(const SampleArgs& p, int64_t row, Shared& s) {
-    constexpr int VEC = Logits<DT>::VEC;
-    const Logits<DT> x{static_cast<const typename elem<DT>::T*>(p.x) + row * p.stride, p.cols, (p.cols + VEC - 1) / VEC};
-    float top = -INFINITY, low = INFINITY;
-    int at = 0x7fffffff;
-    unsigned count = 0;   // of tokens that weigh anything
-    x.each([&](int c, const float (&v)[VEC]) {
+template <int DT, bool FINE>
+__device__ __forceinline__ InBin border_in_bin(Row8<DT>& x, const Heat& h, const Range<FINE>& r, int bin, bool counts, u64 need, u64 above,
+                                               Shared& s) {
+    constexpr int N = Row8<DT>::N;
+    __syncthreads();
+    if (threadIdx.x == 0) s.listed = 0;
+    __syncthreads();
+    float lo = INFINITY, hi = -INFINITY;
+    x.each([&](int, const float (&v)[N]) {
 #pragma unroll
-        for (int k = 0; k < VEC; ++k) {
-            if (v[k] > top) top = v[k], at = c * VEC + k;
-            if (v[k] != -INFINITY) low = fminf(low, v[k]), ++count;
+        for (int k = 0; k < N; ++k) {
+            if (!r.has(v[k]) || r.bin(v[k]) != bin) continue;
+            lo = fminf(lo, v[k]);
+            hi = fmaxf(hi, v[k]);
+            const unsigned i = atomicAdd(&s.listed, 1u);
+            if (i < SA_LIST) s.list[i] = v[k];
         }
     });
-    const float own = top;
-    top = all_threads(top, s.values, [](float a, float b) { return fmaxf(a, b); });
-    at = (int)all_threads(own == top ? (unsigned)at : 0x7fffffffu, s.counts, [](unsigned a, unsigned b) { return a < b ? a : b; });
-    const float heat = p.temperature ? p.temperature[row] : 1.0f, random = p.random[row];
-    const float top_p = p.top_p ? p.top_p[row] : 1.0f, least = p.min_p ? p.min_p[row] : 0.0f;
-    const int top_k = p.top_k ? p.top_k[row] : 0;
-    if (top == -INFINITY || !(heat > 0.0f) || top_k == 1 || top_p <= 0.0f) {   // nothing, or the largest
-        if (threadIdx.x == 0) {
-            p.token[row] = top == -INFINITY ? -1 : at;
-            if (p.logprob) p.logprob[row] = top == -INFINITY ? NAN : 0.0f;
+    lo = all_threads<LeastOp>(lo);
+    hi = all_threads<MostOp>(hi);
+    const unsigned count = s.listed;
+    if (lo == hi) {
+        const u64 left = need - above, w = h.whole_weight(lo);
+        return {true, {lo, counts ? (unsigned)left : (unsigned)((left + w - 1) / w), count}, lo, hi};
+    }
+    if (count > SA_LIST) return {false, {}, lo, hi};
+    if (threadIdx.x < count) s.list_w[threadIdx.x] = counts ? 1 : h.whole_weight(s.list[threadIdx.x]);
+    if (threadIdx.x < 4) s.list[count + threadIdx.x] = -INFINITY;
+    __syncthreads();
+    if (threadIdx.x < count) {
+        const float own = s.list[threadIdx.x];
+        u64 before = above;
+        unsigned equal = 0;
+#pragma unroll 1
+        for (unsigned i = 0; i < count; i += 4)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const float o = s.list[i + k];
+                if (o > own) before += s.list_w[i + k];
+                equal += o == own;
+            }
+        const u64 each = s.list_w[threadIdx.x];
+        if (before < need && need <= before + equal * each) {   // all that equal the border write the same
+            s.border = own;
+            s.found_n = (unsigned)((need - before + each - 1) / each);
+            s.found_count = equal;
         }
+    }
+    __syncthreads();
+    return {true, {s.border, s.found_n, s.found_count}, lo, hi};
+}
+
+// Where the first `need` tokens end, or those that weigh `need` together, in bin `bin` of r, `above` being before it.
+template <int DT>
+__device__ __forceinline__ Border border_from_bin(Row8<DT>& x, const Heat& h, const Range<false>& r, int bin, bool counts, u64 need, u64 above,
+                                                  Shared& s) {
+    InBin in = border_in_bin(x, h, r, bin, counts, need, above, s);
+    while (!in.done) {   // a bin's values are fewer than its range's or lie closer, until they are equal
+        const Range<true> fine{in.lo, in.hi, SA_BINS / ((double)in.hi - (double)in.lo)};
+        fill_bins(x, h, fine, counts, s.part);
+        find_bin(true, counts, need - above, s);
+        above += s.found_w;
+        in = border_in_bin(x, h, fine, s.found, counts, need, above, s);
+    }
+    return in.b;
+}
+
+// Places in the vocabulary's order in bins of 2^SHIFT: a wave's chunks of one step.
+template <int DT>
+struct Places {
+    static constexpr int SHIFT = DT == TVK_F32 ? 8 : 9, MASK = (1 << SHIFT) - 1;
+    static_assert(1 << SHIFT == 64 * Row8<DT>::VEC && SA_MOST_COLS >> SHIFT <= SA_BINS, "a wave's chunks; bins for all");
+};
+
+// The index of the last of the first b.ties tokens that equal the border.
+template <int DT>
+__device__ __forceinline__ int last_tie(Row8<DT>& x, const Border& b, Shared& s) {
+    typedef Places<DT> At;
+    constexpr int N = Row8<DT>::N;
+    if (b.ties == b.equal) return 0x7fffffff;
+    clear(s.part);
+    x.each([&](int i, const float (&v)[N]) {   // (a chunk is within a bin)
+        unsigned n = 0;
+#pragma unroll
+        for (int k = 0; k < N; ++k) n += v[k] == b.t;
+        if (n) atomicAdd(&s.part.n[i >> At::SHIFT], n);
+    });
+    __syncthreads();
+    find_bin(true, true, b.ties, s);
+    const int bin = s.found, i = (bin << At::SHIFT) + (int)threadIdx.x;
+    const u64 need = b.ties - s.found_w;
+    clear(s.part);
+    if (threadIdx.x <= At::MASK && i >= 0 && i < x.cols) s.part.n[threadIdx.x] = x.value(i) == b.t;
+    __syncthreads();
+    find_bin(true, true, need, s);
+    return (bin << At::SHIFT) + s.found;
+}
+
+// What the filters leave.
+struct Keep {
+    float t;
+    int last;   // the index of the last tie
+    __device__ __forceinline__ bool has(int i, float v) const { return v > t || (v == t && i <= last); }
+};
+
+// The weights of the tokens that `has` keeps, in the places' bins: a wave's step is a bin, and nobody else's.
+template <int DT, class F>
+__device__ __forceinline__ void add_places(Row8<DT>& x, const Heat& h, const Filters& f, u64* places, F&& has) {
+    constexpr int N = Row8<DT>::N, VEC = Row8<DT>::VEC;
+    u64 sum = 0;   // of a chunk, then of a wave's
+    x.each([&](int i, const float (&v)[N]) {
+        bool keep[N], any = false;
+#pragma unroll
+        for (int k = 0; k < N; ++k) any |= keep[k] = has(i + k, v[k]);
+        if (any) {
+            u64 w[N];
+#pragma unroll
+            for (int k = 0; k < N; ++k) w[k] = f.weigh(h, v[k]);
+#pragma unroll
+            for (int k = 0; k < N; ++k) sum += keep[k] ? w[k] : 0;
+        }
+        if (i % VEC == VEC - N) {   // (the same for all) the chunk's end
+            sum = lanes_up_to(sum);
+            if (threadIdx.x % 64 == 63 && i / VEC - 63 < x.end) places[i >> Places<DT>::SHIFT] = sum;
+            sum = 0;
+        }
+    });
+}
+
+__device__ inline void put(const SampleArgs& p, int64_t row, int token, float v, const Heat& h, const Filters& f, u64 total) {
+    p.token[row] = token;
+    if (!p.logprob) return;
+    const double d = v == h.top ? 0.0 : ((double)v - (double)h.top) / f.heat;
+    // log of the total in float32, and one step of Newton's method: e is within 2^-20 of 1
+    const double sum = (double)total * 0x1p-44;
+    const float log32 = __builtin_amdgcn_logf((float)sum) * 0.693147181f;
+    const double e = sum * (Heat{0.0f, SA_STEPS * 1.4426950408889634, h.table}.large_weight(-log32) * 0x1p-44) - 1.0;
+    p.logprob[row] = (float)(d - (log32 + (e - 0.5 * e * e)));
+}
+
+// The token, from the places' sums of weights (s.all): the first at which they pass the random number's share.
+template <int DT>
+__device__ __forceinline__ void draw(const SampleArgs& p, int64_t row, const typename elem<DT>::T* x, const Heat& h, const Filters& f,
+                                     const Keep& k, Shared& s) {
+    typedef Places<DT> At;
+    const u64 total = sum_of(s.all, s), goal = f.goal(total);
+    find_bin(false, false, goal + 1, s);
+    const int bin = s.found, i = (bin << At::SHIFT) + (int)threadIdx.x;
+    const u64 need = goal + 1 - s.found_w;
+    clear(s.part);
+    float v = -INFINITY;
+    if (threadIdx.x <= At::MASK && i >= 0 && i < p.cols) {
+        v = elem<DT>::to_f32(x[i]);
+        if (k.has(i, v)) s.part.w[threadIdx.x] = f.weigh(h, v);   // (NaN is not kept)
+    }
+    __syncthreads();
+    find_bin(true, false, need, s);
+    if ((int)threadIdx.x == s.found) put(p, row, i, v, h, f, total);
+}
+
+__device__ inline void put_first(const SampleArgs& p, int64_t row, float top, unsigned at) {
+    if (threadIdx.x != 0) return;
+    p.token[row] = top == -INFINITY ? -1 : (int64_t)at;
+    if (p.logprob) p.logprob[row] = top == -INFINITY ? NAN : 0.0f;
+}
+
+// The first place of the largest among a thread's values.
+template <int DT>
+__device__ __forceinline__ unsigned first_of(Row8<DT>& x, float top) {
+    constexpr int N = Row8<DT>::N;
+    unsigned at = 0x7fffffff;
+    x.each([&](int i, const float (&v)[N]) {
+#pragma unroll
+        for (int k = 0; k < N; ++k) at = min(at, v[k] == top ? (unsigned)(i + k) : at);
+    });
+    return at;
+}
+
+// All that is left, of n <= SA_FEW tokens (s.list, s.list_at) that hold what the filters can keep: compared with each other, a
+// thread each.
+__device__ __forceinline__ void finish_few(const SampleArgs& p, int64_t row, int n, const Heat& h, const Filters& f, Shared& s) {
+    const int t = threadIdx.x;
+    const bool there = t < n;
+    const float v = there ? s.list[t] : -INFINITY;
+    const int at = there ? s.list_at[t] : 0;
+    const u64 w = there ? h.whole_weight(v) : 0;
+    if (there) s.list_w[t] = w;
+    if (t < 4) s.list[n + t] = -INFINITY, s.list_at[n + t] = 0x7fffffff, s.list_w[n + t] = 0;
+    __syncthreads();
+    u64 above = 0;   // of the tokens in front of this one
+    int rank = 0;
+    if (there)
+#pragma unroll 1
+        for (int i = 0; i < n; i += 4)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const float o = s.list[i + k];
+                const bool front = o > v || (o == v && s.list_at[i + k] < at);
+                rank += front;
+                above += front ? s.list_w[i + k] : 0;
+            }
+    bool keep = there && (!f.by_k || rank < f.top_k);
+    if (f.by_p) {
+        const u64 need = f.share(all_threads<AddOp>(keep ? w : (u64)0));
+        keep = keep && above < need;
+    }
+    const u64 own = keep ? f.weigh(h, v) : 0;
+    const u64 total = all_threads<AddOp>(own), goal = f.goal(total);
+    if (there) s.list_w[t] = own;
+    __syncthreads();
+    u64 before = 0;
+    if (there)
+#pragma unroll 1
+        for (int i = 0; i < n; i += 4)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) before += s.list_at[i + k] < at ? s.list_w[i + k] : 0;
+    if (before <= goal && goal < before + own) put(p, row, at, v, h, f, total);
+}
+
+// The values down to bin `bin`, with their places: s.listed of them, at most SA_FEW kept.
+template <int DT, class F>
+__device__ __forceinline__ void list_tokens(Row8<DT>& x, float* v_out, int* at_out, Shared& s, F&& has) {
+    constexpr int N = Row8<DT>::N;
+    __syncthreads();
+    if (threadIdx.x == 0) s.listed = 0;
+    __syncthreads();
+    x.each([&](int i, const float (&v)[N]) {
+#pragma unroll
+        for (int k = 0; k < N; ++k)
+            if (has(v[k])) {
+                const unsigned o = atomicAdd(&s.listed, 1u);
+                if (o < SA_FEW) {
+                    v_out[o] = v[k];
+                    at_out[o] = i + k;
+                }
+            }
+    });
+    __syncthreads();
+}
+
+// A row by one workgroup, with its largest logit known.
+template <int DT>
+__device__ void whole_row(const SampleArgs& p, int64_t row, Row8<DT>& x, float top, const Filters& f, Shared& s) {
+    if (f.first_only(top)) {
+        put_first(p, row, top, all_threads<LeastOp>(first_of(x, top)));
         return;
     }
-    low = all_threads(low, s.values, [](float a, float b) { return fminf(a, b); });
-    count = all_threads(count, s.counts, [](unsigned a, unsigned b) { return a + b; });
-    const Heat h{top, 1.4426950408889634 / heat};
-    if (top == INFINITY) low = top;   // beside an infinite logit the others weigh nothing
-    const bool by_k = top_k > 0 && (unsigned)top_k < count, by_p = top_p < 1.0f;
+    const Heat h = f.weights(top, s);
     Border b{-INFINITY, 0, 0};
-    if (by_k || by_p) {
-        if (low == top) {   // all equal
-            unsigned n = 0;
-            x.each([&](int, const float (&v)[VEC]) {
-#pragma unroll
-                for (int k = 0; k < VEC; ++k) n += v[k] == top;
-            });
-            n = all_threads(n, s.counts, [](unsigned a, unsigned b) { return a + b; });
-            if (by_k) n = min(n, (unsigned)top_k);
-            b = {top, by_p ? max(1u, (unsigned)ceil((double)top_p * n)) : n, 0};
-        } else {
-            const double span = fmin((double)top - (double)low, 28.0 * heat);   // weights from 1 to 2^-40; the rest in the last bin
-            const Range r{low, top, SA_BINS / span};
-            fill_bins(x, h, r, s.all);
-            u64 total = 0;
-            if (by_k) {
-                b = find_border(x, h, r, true, (u64)top_k, s);
-                total = b.w + b.ties * h.whole_weight(b.t);
-            } else {
-                u64 w = 0;
-                for (int i = threadIdx.x; i < SA_BINS; i += SA_THREADS) w += s.all.w[i];
-                total = all_threads(w, s.sums, [](u64 a, u64 b) { return a + b; });
+    Range<false> r = first_range(top, f.heat);
+    if (f.by_k) {   // no weights are needed
+        fill_bins(x, h, r, true, s.all);
+        find_bin(false, true, (u64)f.top_k, s);
+        const int bin = s.found;
+        if (bin >= 0) {   // else there are fewer
+            const u64 above = s.found_w;
+            if (above + s.found_own <= SA_FEW) {
+                list_tokens(x, s.list, s.list_at, s, [&](float v) { return r.has(v) && r.bin(v) <= bin; });
+                finish_few(p, row, (int)s.listed, h, f, s);
+                return;
             }
-            if (by_p) {
-                const u64 need = min(total, max((u64)1, (u64)ceil((double)top_p * (double)total)));
-                b = find_border(x, h, r, false, need, s);
-            }
+            b = border_from_bin(x, h, r, bin, true, (u64)f.top_k, above, s);
         }
     }
-    // Kept: v > b.t, the first b.ties that equal it, and of those what weighs `least` of the largest.
-    const bool by_least = least > 0.0f;
-    const double floor_w = fmin((double)least, 1.0);
-    auto weigh = [&](float v) {
-        const double w = h.weight(v);
-        return by_least && w < floor_w ? (u64)0 : Heat::whole(w);
-    };
-    const u64 tie_w = b.ties ? weigh(b.t) : 0;
-    // chunks [first, end) hold the token; before them lie `ties` equal to the border and the weight `base`
-    int first = 0, end = x.chunks;
-    unsigned ties = 0;
-    u64 base = 0, goal = 0, total = 0;
-    for (bool whole_row = true; whole_row || end - first > 64; whole_row = false) {
-        const int each = ((end - first + SA_WAVES - 1) / SA_WAVES + 63) / 64 * 64, wave = threadIdx.x / 64;
-        u64 w = 0;
-        unsigned n = 0;
-        for (int c = first + wave * each + threadIdx.x % 64; c < min(first + (wave + 1) * each, end); c += 64) {
-            float v[VEC];
-            x.load(c, v);
-#pragma unroll
-            for (int k = 0; k < VEC; ++k) {
-                if (v[k] > b.t) w += weigh(v[k]);
-                n += v[k] == b.t;
-            }
-        }
-#pragma unroll
-        for (int m = 1; m < 64; m <<= 1) w += __shfl_xor(w, m), n += __shfl_xor(n, m);
-        __syncthreads();
-        if (threadIdx.x % 64 == 0) s.sums[wave] = w, s.counts[wave] = n;
-        __syncthreads();
-        auto kept_ties = [&](unsigned before, unsigned n) { return min(before + n, max(b.ties, before)) - before; };
-        if (whole_row) {
-            unsigned t = 0;
-            for (int k = 0; k < SA_WAVES; ++k) total += s.sums[k] + kept_ties(t, s.counts[k]) * tie_w, t += s.counts[k];
-            const double share = random > 0.0f ? (double)random * (double)total : 0.0;
-            goal = share < (double)total ? (u64)share : total - 1;
-            goal = min(goal, total - 1);
-        }
-        for (int k = 0;; ++k) {   // the first wave whose chunks pass the goal
-            const u64 sum = s.sums[k] + kept_ties(ties, s.counts[k]) * tie_w;
-            if (base + sum > goal || k == SA_WAVES - 1) {
-                first = min(first + k * each, end);
-                end = min(first + each, end);
-                break;
-            }
-            base += sum;
-            ties += s.counts[k];
-        }
+    if (f.by_p) {
+        r.lo = fmaxf(r.lo, b.t);
+        fill_bins(x, h, r, false, s.all);
+        u64 total = sum_of(s.all, s);
+        if (b.equal > b.ties) total -= (b.equal - b.ties) * h.whole_weight(b.t);
+        const u64 need = f.share(total);
+        find_bin(false, false, need, s);
+        b = border_from_bin(x, h, r, s.found, false, need, s.found_w, s);
     }
-    if (threadIdx.x < 64) {
-        float v[VEC];
-        const int c = first + threadIdx.x;
-        if (c < end) x.load(c, v);
-        else
-#pragma unroll
-            for (int k = 0; k < VEC; ++k) v[k] = -INFINITY;
-        unsigned n = 0;
-#pragma unroll
-        for (int k = 0; k < VEC; ++k) n += b.ties && v[k] == b.t;
-        ties += lanes_before(n);
-        u64 w[VEC], sum = 0;
-#pragma unroll
-        for (int k = 0; k < VEC; ++k) {
-            w[k] = v[k] > b.t ? weigh(v[k]) : v[k] == b.t && b.ties && ties++ < b.ties ? tie_w : 0;
-            sum += w[k];
-        }
-        base += lanes_before(sum);
-        if (base <= goal && base + sum > goal) {   // one lane's
-            int k = 0;
-#pragma unroll
-            for (int i = 0; i < VEC; ++i)
-                if (base <= goal) base += w[i], k = i;
-            p.token[row] = c * VEC + k;
-            if (p.logprob) {
-                float picked = v[0];
-#pragma unroll
-                for (int i = 1; i < VEC; ++i) picked = k == i ? v[i] : picked;
-                const double d = picked == top ? 0.0 : ((double)picked - (double)top) / heat;
-                p.logprob[row] = (float)(d - log((double)total * 0x1p-44));
-            }
-        }
-    }
+    const Keep k{b.t, last_tie(x, b, s)};
+    clear(s.all);
+    add_places(x, h, f, s.all.w, [&](int i, float v) { return k.has(i, v); });
+    __syncthreads();
+    draw<DT>(p, row, x.row, h, f, k, s);
 }
 
 template <int DT>
-__global__ __launch_bounds__(SA_THREADS) void sample_kernel(SampleArgs p) {
+__device__ __forceinline__ float largest(Row8<DT>& x, Shared& s) {
+    constexpr int N = Row8<DT>::N;
+    float top = -INFINITY;
+    x.each([&](int, const float (&v)[N]) {
+#pragma unroll
+        for (int k = 0; k < N; ++k) top = fmaxf(top, v[k]);
+    });
+    return all_threads<MostOp>(top);
+}
+
+template <int DT>
+__global__ __launch_bounds__(SA_THREADS) void sample_rows_kernel(SampleArgs p) {
     __shared__ Shared s;
+    make_table(s);
     for (int64_t row = blockIdx.x; row < p.rows; row += gridDim.x) {
-        sample_row<DT>(p, row, s);
+        Row8<DT> x(p, row, 0, 0x7fffffff);
+        whole_row(p, row, x, largest(x, s), Filters(p, row), s);
         __syncthreads();
     }
+}
+
+// ---------------------------------------------------------------------------
+// rows cut among workgroups
+// ---------------------------------------------------------------------------
+
+template <int DT>
+__global__ __launch_bounds__(SA_THREADS) void sample_top_kernel(SampleArgs p) {
+    __shared__ Shared s;
+    const int64_t row = blockIdx.x / (unsigned)p.pieces;
+    const int piece = blockIdx.x % (unsigned)p.pieces;
+    Row8<DT> x(p, row, piece * p.piece, (piece + 1) * p.piece);
+    const float top = largest(x, s);
+    if (threadIdx.x == 0) p.tops[blockIdx.x] = top;
+}
+
+__device__ __forceinline__ float top_of(const SampleArgs& p, int64_t row) {
+    const int lane = threadIdx.x % 64;
+    return lanes64_all<MaxOp>(lane < p.pieces ? p.tops[row * p.pieces + lane] : -INFINITY);
+}
+
+// A piece's histogram; or where no border is wanted what the token is found from.
+template <int DT>
+__global__ __launch_bounds__(SA_THREADS) void sample_bins_kernel(SampleArgs p) {
+    __shared__ Shared s;
+    make_table(s);
+    const int64_t row = blockIdx.x / (unsigned)p.pieces;
+    const int piece = blockIdx.x % (unsigned)p.pieces;
+    Row8<DT> x(p, row, piece * p.piece, (piece + 1) * p.piece);
+    const float top = top_of(p, row);
+    const Filters f(p, row);
+    if (f.first_only(top)) {
+        const unsigned at = all_threads<LeastOp>(first_of(x, top));
+        if (threadIdx.x == 0) p.listed[blockIdx.x] = at;
+        return;
+    }
+    const Heat h = f.weights(top, s);
+    if (!f.by_k && !f.by_p) {
+        add_places(x, h, f, p.places + row * SA_BINS, [](int, float) { return true; });
+        return;
+    }
+    fill_bins(x, h, first_range(top, f.heat), f.by_k, s.all);
+    u64* out = p.bins + (int64_t)blockIdx.x * SA_BINS;
+    out[threadIdx.x] = s.all.w[threadIdx.x];
+    out[threadIdx.x + SA_THREADS] = s.all.w[threadIdx.x + SA_THREADS];
+}
+
+// The border's bin, from all pieces' histograms, and what of a piece lies in it and above.
+template <int DT>
+__global__ __launch_bounds__(SA_THREADS) void sample_border_kernel(SampleArgs p) {
+    __shared__ Shared s;
+    make_table(s);
+    const int64_t row = blockIdx.x / (unsigned)p.pieces;
+    const int piece = blockIdx.x % (unsigned)p.pieces;
+    const float top = top_of(p, row);
+    const Filters f(p, row);
+    auto state = [&](int mode, int bin, u64 above, u64 need) {
+        if (piece == 0 && threadIdx.x == 0) p.state[row] = {mode, bin, above, need};
+    };
+    if (f.first_only(top)) return state(SA_FIRST, 0, 0, 0);
+    if (!f.by_k && !f.by_p) return state(SA_ALL, 0, 0, 0);
+    Row8<DT> x(p, row, piece * p.piece, (piece + 1) * p.piece);
+    const Heat h = f.weights(top, s);
+    const u64* in = p.bins + row * p.pieces * SA_BINS + threadIdx.x;
+    u64 a = 0, b = 0;   // counts are two to a word, and do not carry: there are at most 2^19
+#pragma unroll 8
+    for (int i = 0; i < p.pieces; ++i) {
+        a += in[(int64_t)i * SA_BINS];
+        b += in[(int64_t)i * SA_BINS + SA_THREADS];
+    }
+    s.all.w[threadIdx.x] = a;
+    s.all.w[threadIdx.x + SA_THREADS] = b;
+    __syncthreads();
+    const u64 need = f.by_k ? (u64)f.top_k : f.share(sum_of(s.all, s));
+    find_bin(false, f.by_k, need, s);
+    const int bin = s.found;
+    const u64 above = s.found_w, own = s.found_own;
+    u64* places = p.places + row * SA_BINS;
+    if (bin < 0) {   // fewer tokens than top_k
+        if (f.by_p) return state(SA_WHOLE, 0, 0, 0);
+        add_places(x, h, f, places, [](int, float) { return true; });
+        return state(SA_ALL, 0, 0, 0);
+    }
+    const Range<false> r = first_range(top, f.heat);
+    const bool few = f.by_k && above + own <= SA_FEW;
+    if (f.by_k && f.by_p && !few) return state(SA_WHOLE, 0, 0, 0);
+    const int64_t list = (int64_t)blockIdx.x * SA_FEW;
+    list_tokens(x, p.list_v + list, p.list_at + list, s, [&](float v) {
+        return r.has(v) && (few ? r.bin(v) <= bin : r.bin(v) == bin);
+    });
+    if (threadIdx.x == 0) p.listed[blockIdx.x] = s.listed;
+    if (!few) add_places(x, h, f, places, [&](int, float v) { return r.has(v) && r.bin(v) < bin; });
+    state(few ? SA_TOKENS : SA_SUMS, bin, above, need);
+}
+
+template <int DT>
+__global__ __launch_bounds__(SA_THREADS) void sample_token_kernel(SampleArgs p) {
+    __shared__ Shared s;
+    make_table(s);
+    const int64_t row = blockIdx.x;
+    const float top = top_of(p, row);
+    const Filters f(p, row);
+    const RowState st = p.state[row];
+    const int lane = threadIdx.x % 64;
+    const unsigned listed = lane < p.pieces ? p.listed[row * p.pieces + lane] : st.mode == SA_FIRST ? 0x7fffffffu : 0u;
+    if (st.mode == SA_FIRST) return put_first(p, row, top, all_threads<LeastOp>(listed));
+    const Heat h = f.weights(top, s);
+    const typename elem<DT>::T* x = static_cast<const typename elem<DT>::T*>(p.x) + row * p.stride;
+    int n = 0;
+    bool whole = st.mode == SA_WHOLE;
+    if (st.mode == SA_TOKENS || st.mode == SA_SUMS) {   // the pieces' lists, one behind the other: a thread an entry
+        const u64 up_to = lanes_up_to(listed);
+        n = (int)__builtin_amdgcn_readlane((int)up_to, 63);   // (at most 2^19)
+        if (threadIdx.x < SA_PIECES) s.counts[threadIdx.x] = (unsigned)up_to;
+        __syncthreads();
+        whole = n > SA_FEW;
+        if (!whole && (int)threadIdx.x < n) {
+            int i = 0;   // the first piece whose entries reach past this thread's
+            for (int half = SA_PIECES / 2; half > 0; half /= 2)
+                if (s.counts[i + half - 1] <= threadIdx.x) i += half;
+            const int64_t from = (row * p.pieces + i) * SA_FEW + threadIdx.x - (i ? s.counts[i - 1] : 0);
+            s.list[threadIdx.x] = p.list_v[from];
+            s.list_at[threadIdx.x] = p.list_at[from];
+        }
+        __syncthreads();
+    }
+    if (whole) {   // too many of them: from the start
+        Row8<DT> all(p, row, 0, 0x7fffffff);
+        return whole_row(p, row, all, top, f, s);
+    }
+    if (st.mode == SA_TOKENS) return finish_few(p, row, n, h, f, s);
+    clear(s.all);
+    const int places = (p.cols >> Places<DT>::SHIFT) + 1;
+    for (int i = threadIdx.x; i < places && i < SA_BINS; i += SA_THREADS)
+        if (i << Places<DT>::SHIFT < p.cols) s.all.w[i] = p.places[row * SA_BINS + i];
+    Keep k{-INFINITY, 0x7fffffff};
+    if (st.mode == SA_SUMS) {   // the bin's tokens, compared with each other
+        const int t = threadIdx.x;
+        const bool there = t < n;
+        const float v = there ? s.list[t] : 0.0f;
+        const int at = there ? s.list_at[t] : 0;
+        if (there) s.list_w[t] = f.by_k ? 1 : h.whole_weight(v);
+        if (t < 4) s.list[n + t] = -INFINITY, s.list_at[n + t] = 0x7fffffff, s.list_w[n + t] = 0;
+        __syncthreads();
+        u64 before = st.above;
+        if (there)
+#pragma unroll 1
+            for (int i = 0; i < n; i += 4)
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    const float o = s.list[i + k];
+                    before += o > v || (o == v && s.list_at[i + k] < at) ? s.list_w[i + k] : 0;
+                }
+        if (there && before < st.need) {
+            const u64 w = f.weigh(h, v);
+            if (w) atomicAdd(&s.all.w[at >> Places<DT>::SHIFT], w);
+            if (before + s.list_w[t] >= st.need) {   // the last of them
+                s.border = v;
+                s.last = at;
+            }
+        }
+        __syncthreads();
+        k = {s.border, s.last};
+    }
+    __syncthreads();
+    draw<DT>(p, row, x, h, f, k, s);
+}
+
+template <int DT>
+tvk_status launch(SampleArgs p, hipStream_t s) {
+    // A workgroup a CU is wanted; pieces of 256 chunks or more
+    const int chunks = (p.cols + Row8<DT>::VEC - 1) / Row8<DT>::VEC;
+    const int64_t pieces = std::min<int64_t>({SA_PIECES, 256 / p.rows, chunks / 256});
+    const dim3 block(SA_THREADS);
+    if (pieces < 2) {
+        hipLaunchKernelGGL((sample_rows_kernel<DT>), dim3((unsigned)std::min<int64_t>(p.rows, 1 << 20)), block, 0, s, p);
+        return TVK_OK;
+    }
+    p.piece = (int)((chunks + pieces - 1) / pieces + 63) / 64 * 64;   // whole places
+    p.pieces = (chunks + p.piece - 1) / p.piece;
+    const int64_t all = p.rows * p.pieces;
+    Scratch scratch;
+    char* at = static_cast<char*>(scratch.get((size_t)(all * (SA_BINS * 8 + SA_FEW * 8 + 8) + p.rows * (SA_BINS * 8 + (int64_t)sizeof(RowState))), s));
+    if (!at) return fail(TVK_ERR_OOM, "tvk_sample: workspace allocation failed");
+    auto take = [&](auto*& to, int64_t n) {
+        to = reinterpret_cast<std::remove_reference_t<decltype(to)>>(at);
+        at += n * sizeof(*to);
+    };
+    take(p.bins, all * SA_BINS);
+    take(p.places, p.rows * SA_BINS);
+    take(p.state, p.rows);
+    take(p.list_v, all * SA_FEW);
+    take(p.list_at, all * SA_FEW);
+    take(p.tops, all);
+    take(p.listed, all);
+    hipLaunchKernelGGL((sample_top_kernel<DT>), dim3((unsigned)all), block, 0, s, p);
+    hipLaunchKernelGGL((sample_bins_kernel<DT>), dim3((unsigned)all), block, 0, s, p);
+    hipLaunchKernelGGL((sample_border_kernel<DT>), dim3((unsigned)all), block, 0, s, p);
+    hipLaunchKernelGGL((sample_token_kernel<DT>), dim3((unsigned)p.rows), block, 0, s, p);
+    return TVK_OK;
 }
 
 }  // namespace
@@ -430,13 +887,21 @@ extern "C" tvk_status tvk_sample(const tvk_sample_desc* d) {
     if (d->rows == 0) return TVK_OK;
     if ((d->cols > 0 && !d->logits) || !d->random || !d->token) return bad(TVK_ERR_INVALID, "NULL tensor");
     if (d->logits_stride < 0) return bad(TVK_ERR_INVALID, "negative strides");
-    const SampleArgs p{d->logits, d->temperature, d->top_k, d->top_p, d->min_p, d->random, d->token, d->logprob,
-                       d->rows, d->logits_stride, (int)d->cols};
+    SampleArgs p{};
+    p.x = d->logits;
+    p.temperature = d->temperature;
+    p.top_k = d->top_k;
+    p.top_p = d->top_p;
+    p.min_p = d->min_p;
+    p.random = d->random;
+    p.token = d->token;
+    p.logprob = d->logprob;
+    p.rows = d->rows;
+    p.stride = d->logits_stride;
+    p.cols = (int)d->cols;
     const hipStream_t s = resolve_stream(d->stream);
-    const dim3 grid((unsigned)std::min<int64_t>(d->rows, 1 << 20)), block(SA_THREADS);
-    if (d->dtype == TVK_F32) hipLaunchKernelGGL((sample_kernel<TVK_F32>), grid, block, 0, s, p);
-    else if (d->dtype == TVK_F16) hipLaunchKernelGGL((sample_kernel<TVK_F16>), grid, block, 0, s, p);
-    else hipLaunchKernelGGL((sample_kernel<TVK_BF16>), grid, block, 0, s, p);
+    const tvk_status st = d->dtype == TVK_F32 ? launch<TVK_F32>(p, s) : d->dtype == TVK_F16 ? launch<TVK_F16>(p, s) : launch<TVK_BF16>(p, s);
+    if (st != TVK_OK) return st;
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return bad(TVK_ERR_DEVICE, (std::string("launch failed: ") + hipGetErrorString(e)).c_str());
     return TVK_OK;
