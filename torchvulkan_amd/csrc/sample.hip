@@ -17,7 +17,7 @@
 // them: float32 weights would put one in 10^4 draws from a flat distribution
 // elsewhere.
 //
-// The row stays in the registers of 1024 threads, 64 K values in 16 bits, and is
+// The row stays in the registers of 1024 threads, 32 K values in 16 bits, and is
 // read again for every pass past that. Most of a small call is latency, and much of
 // that the code's own: a line of 64 bytes that no cache holds takes as long as a
 // load. So passes are loops over a thread's words, not unrolled, helpers are called,
@@ -36,8 +36,10 @@ typedef unsigned long long u64;
 
 constexpr int SA_THREADS = 1024, SA_WAVES = SA_THREADS / 64;
 constexpr int SA_BINS = 2 * SA_THREADS;
+constexpr int SA_CHUNKS = 4;       // of 16 bytes, that a thread holds
 constexpr int SA_LIST = 256;       // values of a bin that are compared with each other
 constexpr int SA_FEW = 512;        // tokens that are
+constexpr int SA_KEPT = 8192;      // tokens that are weighed from a list
 constexpr int SA_PIECES = 32;      // of a row, at most
 constexpr int64_t SA_MOST_COLS = 1 << 19;
 
@@ -57,7 +59,7 @@ struct SampleArgs {
     const float* random;
     int64_t* token;
     float* logprob;
-    int64_t rows, stride;
+    int64_t rows, stride, row0;   // row0: of a launch
     int cols;
     // of rows cut into pieces
     int pieces, piece;     // chunks of a piece
@@ -108,34 +110,35 @@ struct Heat {
     __device__ __forceinline__ u64 whole_weight(float x) const { return whole(large_weight(x)); }
 };
 
-// Chunks [first, end) of 16 bytes of a row, thread t those at first + t + 1024 j, eight of them in registers.
+// Chunks [first, end) of 16 bytes of a row, thread t those at first + t + 1024 j, SA_CHUNKS of them in registers.
 template <int DT>
-struct Row8 {
+struct RowIn {
     typedef typename elem<DT>::T T;
-    typedef uint32_t W32 __attribute__((ext_vector_type(32)));
-    static constexpr int VEC = 16 / (int)sizeof(T), HELD = 8 * SA_THREADS;   // chunks that are held
+    typedef uint32_t W __attribute__((ext_vector_type(4 * SA_CHUNKS)));
+    static constexpr int VEC = 16 / (int)sizeof(T), HELD = SA_CHUNKS * SA_THREADS;   // chunks that are held
     static constexpr int N = 2, STEP = DT == TVK_F32 ? 2 : 1;                // values handled together, their words
     const T* row;
     int cols, first, end, at, words;   // at: the first of the held; words of a thread
-    W32 w;
+    const int* places = nullptr;       // of a list
+    W w;
 
-    __device__ __forceinline__ Row8(const SampleArgs& p, int64_t r, int first, int last)
+    __device__ __forceinline__ RowIn(const SampleArgs& p, int64_t r, int first, int last)
         : row(static_cast<const T*>(p.x) + r * p.stride), cols(p.cols), first(first), end(min(last, (p.cols + VEC - 1) / VEC)) {
         load(first);
     }
     __device__ __forceinline__ void load(int from) {
         at = from;
-        words = min(8, (end - from + SA_THREADS - 1) / SA_THREADS) * 4;
+        words = min(SA_CHUNKS, (end - from + SA_THREADS - 1) / SA_THREADS) * 4;
         const int whole = min(end, cols / VEC), mine = from + (int)threadIdx.x;   // past `whole` lies at most a piece of a chunk
         const T* p = row + (int64_t)mine * VEC;
-        Words<16> c[8];
+        Words<16> c[SA_CHUNKS];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
+        for (int j = 0; j < SA_CHUNKS; ++j) {
             c[j] = {};
             if (mine + j * SA_THREADS < whole) c[j] = load_words<16, sizeof(T)>(p + j * SA_THREADS * VEC);
         }
 #pragma unroll
-        for (int j = 0; j < 32; ++j) w[j] = c[j / 4].w[j % 4];
+        for (int j = 0; j < 4 * SA_CHUNKS; ++j) w[j] = c[j / 4].w[j % 4];
         if (from + words / 4 * SA_THREADS <= whole) return;
         constexpr uint32_t LOWEST = DT == TVK_F32 ? 0xff800000u : DT == TVK_F16 ? 0xfc00fc00u : 0xff80ff80u;   // -inf
 #pragma unroll 1
@@ -156,7 +159,26 @@ struct Row8 {
             w[k] = v;
         }
     }
-    // f(index of the first, two values) over the chunks; NaN as -inf. A chunk's last call is where (index + 2) % VEC is 0.
+    // From here on the n tokens of a list instead (at most as many as are held), whose places are in LDS.
+    __device__ __forceinline__ void take(const float* v, const int* v_places, int n) {
+        static_assert(SA_KEPT <= 4 * SA_CHUNKS / STEP * N * SA_THREADS, "a list is held");
+        first = at = 0;
+        end = 1;
+        words = (n + N * SA_THREADS - 1) / (N * SA_THREADS) * STEP;
+        places = v_places;
+        auto value = [&](int i) { return elem<DT>::from_f32(i < n ? v[i] : -INFINITY); };
+#pragma unroll 1
+        for (int k = 0; k < words; k += STEP) {
+            const int i = threadIdx.x + k / STEP * N * SA_THREADS;
+            if constexpr (DT == TVK_F32) {
+                w[k] = __builtin_bit_cast(uint32_t, value(i));
+                w[k + 1] = __builtin_bit_cast(uint32_t, value(i + SA_THREADS));
+            } else {
+                w[k] = __builtin_bit_cast(uint16_t, value(i)) | (uint32_t)__builtin_bit_cast(uint16_t, value(i + SA_THREADS)) << 16;
+            }
+        }
+    }
+    // f(indexes, two values) over the chunks; NaN as -inf. A chunk's last call is where (the second index + 1) % VEC is 0.
     template <class F>
     __device__ __forceinline__ void each(F&& f) {
 #pragma unroll 1
@@ -166,7 +188,13 @@ struct Row8 {
             for (int k = 0; k < words; k += STEP) {
                 const Words<8> two{{w[k], w[k + STEP - 1]}};
                 const float v[N] = {fmaxf(word_at<DT>(two, 0), -INFINITY), fmaxf(word_at<DT>(two, 1), -INFINITY)};
-                f((from + (int)threadIdx.x + k / 4 * SA_THREADS) * VEC + k % 4 * (VEC / 4), v);
+                const int e = (from + (int)threadIdx.x + k / 4 * SA_THREADS) * VEC + k % 4 * (VEC / 4);
+                int i[N] = {e, e + 1};
+                if (places) {
+                    i[0] = places[threadIdx.x + k / STEP * N * SA_THREADS];
+                    i[1] = places[threadIdx.x + (k / STEP * N + 1) * SA_THREADS];
+                }
+                f(i, v);
             }
         }
     }
@@ -236,9 +264,10 @@ union Bins {
 struct Shared {
     Bins all, part;
     double table[SA_STEPS];
-    float list[SA_FEW + 4];   // (loops over a list run in fours)
-    int list_at[SA_FEW + 4];
-    u64 list_w[SA_FEW + 4];
+    float list[SA_KEPT];
+    int list_at[SA_KEPT], kept_at[SA_KEPT];
+    u64 list_w[SA_FEW], before[SA_FEW];
+    unsigned rank[SA_FEW];
     u64 sums[SA_WAVES];
     unsigned counts[SA_PIECES];
     // what one thread finds for all
@@ -248,12 +277,40 @@ struct Shared {
     float border;
 };
 
+// For each of the n <= SA_FEW entries of s.list (list_at, list_w) the weight, s.before, and the number, s.rank, of those that
+// `front(v, at, other v, other at)` puts in front of it. Waves share the comparisons out: 64 entries each with a part of all.
+template <class F>
+__device__ __forceinline__ void compare_all(int n, Shared& s, F&& front) {
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), lane = threadIdx.x % 64;
+    if (threadIdx.x < SA_FEW) s.before[threadIdx.x] = 0, s.rank[threadIdx.x] = 0;
+    __syncthreads();
+    const int groups = (n + 63) / 64, parts = SA_WAVES / groups;   // (no groups: nothing to do)
+    const int each = (n + parts - 1) / parts, i = wave % groups * 64 + lane, first = wave / groups * each;
+    if (i < n && wave / groups < parts) {
+        const float v = s.list[i];
+        const int at = s.list_at[i];
+        u64 before = 0;
+        unsigned rank = 0;
+#pragma unroll 4
+        for (int k = first; k < min(first + each, n); ++k) {
+            const bool f = front(v, at, s.list[k], s.list_at[k]);
+            rank += f;
+            before += f ? s.list_w[k] : 0;
+        }
+        if (rank) {
+            atomicAdd(&s.rank[i], rank);
+            atomicAdd(&s.before[i], before);
+        }
+    }
+    __syncthreads();
+}
+__device__ __forceinline__ bool in_front(float v, int at, float o, int o_at) { return o > v || (o == v && o_at < at); }
+
 // Values between lo and hi in bins of equal width, the largest first. Rounding moves no value past another, so what is in a
-// bin is settled by the same expression wherever it is asked. FINE: in float64, which tells any two values apart, so that
-// lo and hi never share a bin.
-template <bool FINE>
+// bin is settled by the same expression wherever it is asked; and float64 tells any two values apart, so that lo and hi share
+// no bin where the scale is that of their distance. float32 is enough, and faster, where only the first range is asked for.
+template <class F>
 struct Range {
-    typedef std::conditional_t<FINE, double, float> F;
     float lo, hi;
     F scale;
     __device__ __forceinline__ bool has(float x) const { return x >= lo && x <= hi; }
@@ -264,8 +321,9 @@ struct Range {
 };
 
 // Weights from 1 to 2^-40, the rest in the last bin.
-__device__ inline Range<false> first_range(float top, float heat) {
-    return {top == INFINITY ? top : -FLT_MAX, top, (float)(SA_BINS / (28.0 * heat))};
+template <class F>
+__device__ inline Range<F> first_range(float top, float heat) {
+    return {top == INFINITY ? top : -FLT_MAX, top, (F)(SA_BINS / (28.0 * heat))};
 }
 
 // The values that a filter keeps: above t, and the first `ties` of the `equal` that equal it.
@@ -319,18 +377,18 @@ __device__ __forceinline__ u64 sum_of(const Bins& b, Shared& s) {
     return all_threads<AddOp>(b.w[threadIdx.x] + b.w[threadIdx.x + SA_THREADS]);
 }
 
-template <int DT, bool FINE>
-__device__ __forceinline__ void fill_bins(Row8<DT>& x, const Heat& h, const Range<FINE>& r, bool counts, Bins& b) {
-    constexpr int N = Row8<DT>::N;
+template <int DT, class F>
+__device__ __forceinline__ void fill_bins(RowIn<DT>& x, const Heat& h, const Range<F>& r, bool counts, Bins& b) {
+    constexpr int N = RowIn<DT>::N;
     clear(b);
     if (counts)
-        x.each([&](int, const float (&v)[N]) {
+        x.each([&](const int (&)[N], const float (&v)[N]) {
 #pragma unroll
             for (int k = 0; k < N; ++k)
                 if (r.has(v[k])) atomicAdd(&b.n[r.bin(v[k])], 1u);
         });
     else
-        x.each([&](int, const float (&v)[N]) {
+        x.each([&](const int (&)[N], const float (&v)[N]) {
             u64 w[N];
             int bin[N];
 #pragma unroll
@@ -373,15 +431,15 @@ struct InBin {
     float lo, hi;
 };
 
-template <int DT, bool FINE>
-__device__ __forceinline__ InBin border_in_bin(Row8<DT>& x, const Heat& h, const Range<FINE>& r, int bin, bool counts, u64 need, u64 above,
+template <int DT>
+__device__ __forceinline__ InBin border_in_bin(RowIn<DT>& x, const Heat& h, const Range<double>& r, int bin, bool counts, u64 need, u64 above,
                                                Shared& s) {
-    constexpr int N = Row8<DT>::N;
+    constexpr int N = RowIn<DT>::N;
     __syncthreads();
     if (threadIdx.x == 0) s.listed = 0;
     __syncthreads();
     float lo = INFINITY, hi = -INFINITY;
-    x.each([&](int, const float (&v)[N]) {
+    x.each([&](const int (&)[N], const float (&v)[N]) {
 #pragma unroll
         for (int k = 0; k < N; ++k) {
             if (!r.has(v[k]) || r.bin(v[k]) != bin) continue;
@@ -398,67 +456,43 @@ __device__ __forceinline__ InBin border_in_bin(Row8<DT>& x, const Heat& h, const
         const u64 left = need - above, w = h.whole_weight(lo);
         return {true, {lo, counts ? (unsigned)left : (unsigned)((left + w - 1) / w), count}, lo, hi};
     }
-    if (count > SA_LIST) return {false, {}, lo, hi};
-    if (threadIdx.x < count) s.list_w[threadIdx.x] = counts ? 1 : h.whole_weight(s.list[threadIdx.x]);
-    if (threadIdx.x < 4) s.list[count + threadIdx.x] = -INFINITY;
-    __syncthreads();
-    if (threadIdx.x < count) {
-        const float own = s.list[threadIdx.x];
-        u64 before = above;
-        unsigned equal = 0;
-#pragma unroll 1
-        for (unsigned i = 0; i < count; i += 4)
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                const float o = s.list[i + k];
-                if (o > own) before += s.list_w[i + k];
-                equal += o == own;
-            }
-        const u64 each = s.list_w[threadIdx.x];
-        if (before < need && need <= before + equal * each) {   // all that equal the border write the same
-            s.border = own;
-            s.found_n = (unsigned)((need - before + each - 1) / each);
-            s.found_count = equal;
-        }
+    if (count > SA_LIST) return {false, {-INFINITY, 0, 0}, lo, hi};
+    const bool there = threadIdx.x < count;
+    const float own = there ? s.list[threadIdx.x] : 0.0f;
+    const u64 each = there ? counts ? 1 : h.whole_weight(own) : 0;
+    if (there) s.list_w[threadIdx.x] = each, s.list_at[threadIdx.x] = (int)threadIdx.x;
+    compare_all((int)count, s, [](float v, int, float o, int) { return o > v; });
+    const u64 before = there ? above + s.before[threadIdx.x] : 0;
+    const unsigned larger = there ? s.rank[threadIdx.x] : 0;
+    compare_all((int)count, s, [](float v, int, float o, int) { return o >= v; });
+    const unsigned equal = there ? s.rank[threadIdx.x] - larger : 0;
+    if (there && before < need && need <= before + equal * each) {   // all that equal the border write the same
+        s.border = own;
+        s.found_n = (unsigned)((need - before + each - 1) / each);
+        s.found_count = equal;
     }
     __syncthreads();
     return {true, {s.border, s.found_n, s.found_count}, lo, hi};
-}
-
-// Where the first `need` tokens end, or those that weigh `need` together, in bin `bin` of r, `above` being before it.
-template <int DT>
-__device__ __forceinline__ Border border_from_bin(Row8<DT>& x, const Heat& h, const Range<false>& r, int bin, bool counts, u64 need, u64 above,
-                                                  Shared& s) {
-    InBin in = border_in_bin(x, h, r, bin, counts, need, above, s);
-    while (!in.done) {   // a bin's values are fewer than its range's or lie closer, until they are equal
-        const Range<true> fine{in.lo, in.hi, SA_BINS / ((double)in.hi - (double)in.lo)};
-        fill_bins(x, h, fine, counts, s.part);
-        find_bin(true, counts, need - above, s);
-        above += s.found_w;
-        in = border_in_bin(x, h, fine, s.found, counts, need, above, s);
-    }
-    return in.b;
 }
 
 // Places in the vocabulary's order in bins of 2^SHIFT: a wave's chunks of one step.
 template <int DT>
 struct Places {
     static constexpr int SHIFT = DT == TVK_F32 ? 8 : 9, MASK = (1 << SHIFT) - 1;
-    static_assert(1 << SHIFT == 64 * Row8<DT>::VEC && SA_MOST_COLS >> SHIFT <= SA_BINS, "a wave's chunks; bins for all");
+    static_assert(1 << SHIFT == 64 * RowIn<DT>::VEC && SA_MOST_COLS >> SHIFT <= SA_BINS, "a wave's chunks; bins for all");
 };
 
 // The index of the last of the first b.ties tokens that equal the border.
 template <int DT>
-__device__ __forceinline__ int last_tie(Row8<DT>& x, const Border& b, Shared& s) {
+__device__ __forceinline__ int last_tie(RowIn<DT>& x, const Border& b, Shared& s) {
     typedef Places<DT> At;
-    constexpr int N = Row8<DT>::N;
+    constexpr int N = RowIn<DT>::N;
     if (b.ties == b.equal) return 0x7fffffff;
     clear(s.part);
-    x.each([&](int i, const float (&v)[N]) {   // (a chunk is within a bin)
-        unsigned n = 0;
+    x.each([&](const int (&i)[N], const float (&v)[N]) {
 #pragma unroll
-        for (int k = 0; k < N; ++k) n += v[k] == b.t;
-        if (n) atomicAdd(&s.part.n[i >> At::SHIFT], n);
+        for (int k = 0; k < N; ++k)
+            if (v[k] == b.t) atomicAdd(&s.part.n[i[k] >> At::SHIFT], 1u);
     });
     __syncthreads();
     find_bin(true, true, b.ties, s);
@@ -478,15 +512,36 @@ struct Keep {
     __device__ __forceinline__ bool has(int i, float v) const { return v > t || (v == t && i <= last); }
 };
 
+// The tokens that `has` names, with their places: s.listed of them, at most MOST kept.
+template <int MOST, int DT, class F>
+__device__ __forceinline__ void list_tokens(RowIn<DT>& x, float* v_out, int* at_out, Shared& s, F&& has) {
+    constexpr int N = RowIn<DT>::N;
+    __syncthreads();
+    if (threadIdx.x == 0) s.listed = 0;
+    __syncthreads();
+    x.each([&](const int (&i)[N], const float (&v)[N]) {
+#pragma unroll
+        for (int k = 0; k < N; ++k)
+            if (has(i[k], v[k])) {
+                const unsigned o = atomicAdd(&s.listed, 1u);
+                if (o < MOST) {
+                    v_out[o] = v[k];
+                    at_out[o] = i[k];
+                }
+            }
+    });
+    __syncthreads();
+}
+
 // The weights of the tokens that `has` keeps, in the places' bins: a wave's step is a bin, and nobody else's.
 template <int DT, class F>
-__device__ __forceinline__ void add_places(Row8<DT>& x, const Heat& h, const Filters& f, u64* places, F&& has) {
-    constexpr int N = Row8<DT>::N, VEC = Row8<DT>::VEC;
+__device__ __forceinline__ void add_all_places(RowIn<DT>& x, const Heat& h, const Filters& f, u64* places, F&& has) {
+    constexpr int N = RowIn<DT>::N, VEC = RowIn<DT>::VEC;
     u64 sum = 0;   // of a chunk, then of a wave's
-    x.each([&](int i, const float (&v)[N]) {
+    x.each([&](const int (&i)[N], const float (&v)[N]) {
         bool keep[N], any = false;
 #pragma unroll
-        for (int k = 0; k < N; ++k) any |= keep[k] = has(i + k, v[k]);
+        for (int k = 0; k < N; ++k) any |= keep[k] = has(i[k], v[k]);
         if (any) {
             u64 w[N];
 #pragma unroll
@@ -494,12 +549,34 @@ __device__ __forceinline__ void add_places(Row8<DT>& x, const Heat& h, const Fil
 #pragma unroll
             for (int k = 0; k < N; ++k) sum += keep[k] ? w[k] : 0;
         }
-        if (i % VEC == VEC - N) {   // (the same for all) the chunk's end
+        if (i[0] % VEC == VEC - N) {   // (the same for all) the chunk's end
             sum = lanes_up_to(sum);
-            if (threadIdx.x % 64 == 63 && i / VEC - 63 < x.end) places[i >> Places<DT>::SHIFT] = sum;
+            if (threadIdx.x % 64 == 63 && i[0] / VEC - 63 < x.end) places[i[0] >> Places<DT>::SHIFT] = sum;
             sum = 0;
         }
     });
+}
+
+// The same where few may be kept: those are listed first, and weighed by as many threads. s.part is used.
+template <int DT, class F>
+__device__ __forceinline__ void add_listed_places(RowIn<DT>& x, const Heat& h, const Filters& f, u64* places, Shared& s, F&& has) {
+    const unsigned n = s.listed;
+    if (n > SA_KEPT) return add_all_places(x, h, f, places, has);   // (not of a list)
+    clear(s.part);
+    for (unsigned t = threadIdx.x; t < n; t += SA_THREADS) {
+        const u64 w = f.weigh(h, s.list[t]);
+        if (w) atomicAdd(&s.part.w[s.list_at[t] >> Places<DT>::SHIFT], w);
+    }
+    __syncthreads();
+    constexpr int PER = 64;   // chunks of a place
+    const int from = x.places ? 0 : x.first / PER, to = x.places ? SA_BINS : (x.end + PER - 1) / PER;
+    for (int i = from + (int)threadIdx.x; i < to; i += SA_THREADS) places[i] = s.part.w[i];
+}
+
+template <int DT, class F>
+__device__ __forceinline__ void add_places(RowIn<DT>& x, const Heat& h, const Filters& f, u64* places, Shared& s, F&& has) {
+    list_tokens<SA_KEPT>(x, s.list, s.list_at, s, has);
+    add_listed_places(x, h, f, places, s, has);
 }
 
 __device__ inline void put(const SampleArgs& p, int64_t row, int token, float v, const Heat& h, const Filters& f, u64 total) {
@@ -541,12 +618,12 @@ __device__ inline void put_first(const SampleArgs& p, int64_t row, float top, un
 
 // The first place of the largest among a thread's values.
 template <int DT>
-__device__ __forceinline__ unsigned first_of(Row8<DT>& x, float top) {
-    constexpr int N = Row8<DT>::N;
+__device__ __forceinline__ unsigned first_of(RowIn<DT>& x, float top) {
+    constexpr int N = RowIn<DT>::N;
     unsigned at = 0x7fffffff;
-    x.each([&](int i, const float (&v)[N]) {
+    x.each([&](const int (&i)[N], const float (&v)[N]) {
 #pragma unroll
-        for (int k = 0; k < N; ++k) at = min(at, v[k] == top ? (unsigned)(i + k) : at);
+        for (int k = 0; k < N; ++k) at = min(at, v[k] == top ? (unsigned)i[k] : at);
     });
     return at;
 }
@@ -560,20 +637,9 @@ __device__ __forceinline__ void finish_few(const SampleArgs& p, int64_t row, int
     const int at = there ? s.list_at[t] : 0;
     const u64 w = there ? h.whole_weight(v) : 0;
     if (there) s.list_w[t] = w;
-    if (t < 4) s.list[n + t] = -INFINITY, s.list_at[n + t] = 0x7fffffff, s.list_w[n + t] = 0;
-    __syncthreads();
-    u64 above = 0;   // of the tokens in front of this one
-    int rank = 0;
-    if (there)
-#pragma unroll 1
-        for (int i = 0; i < n; i += 4)
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                const float o = s.list[i + k];
-                const bool front = o > v || (o == v && s.list_at[i + k] < at);
-                rank += front;
-                above += front ? s.list_w[i + k] : 0;
-            }
+    compare_all(n, s, in_front);
+    const u64 above = there ? s.before[t] : 0;   // of the tokens in front of this one
+    const int rank = there ? (int)s.rank[t] : 0;
     bool keep = there && (!f.by_k || rank < f.top_k);
     if (f.by_p) {
         const u64 need = f.share(all_threads<AddOp>(keep ? w : (u64)0));
@@ -582,97 +648,88 @@ __device__ __forceinline__ void finish_few(const SampleArgs& p, int64_t row, int
     const u64 own = keep ? f.weigh(h, v) : 0;
     const u64 total = all_threads<AddOp>(own), goal = f.goal(total);
     if (there) s.list_w[t] = own;
-    __syncthreads();
-    u64 before = 0;
-    if (there)
-#pragma unroll 1
-        for (int i = 0; i < n; i += 4)
-#pragma unroll
-            for (int k = 0; k < 4; ++k) before += s.list_at[i + k] < at ? s.list_w[i + k] : 0;
+    compare_all(n, s, [](float, int at, float, int o) { return o < at; });
+    const u64 before = there ? s.before[t] : 0;
     if (before <= goal && goal < before + own) put(p, row, at, v, h, f, total);
-}
-
-// The values down to bin `bin`, with their places: s.listed of them, at most SA_FEW kept.
-template <int DT, class F>
-__device__ __forceinline__ void list_tokens(Row8<DT>& x, float* v_out, int* at_out, Shared& s, F&& has) {
-    constexpr int N = Row8<DT>::N;
-    __syncthreads();
-    if (threadIdx.x == 0) s.listed = 0;
-    __syncthreads();
-    x.each([&](int i, const float (&v)[N]) {
-#pragma unroll
-        for (int k = 0; k < N; ++k)
-            if (has(v[k])) {
-                const unsigned o = atomicAdd(&s.listed, 1u);
-                if (o < SA_FEW) {
-                    v_out[o] = v[k];
-                    at_out[o] = i + k;
-                }
-            }
-    });
-    __syncthreads();
 }
 
 // A row by one workgroup, with its largest logit known.
 template <int DT>
-__device__ void whole_row(const SampleArgs& p, int64_t row, Row8<DT>& x, float top, const Filters& f, Shared& s) {
+__device__ __forceinline__ void whole_row(const SampleArgs& p, int64_t row, RowIn<DT>& x, float top, const Filters& f, Shared& s) {
     if (f.first_only(top)) {
         put_first(p, row, top, all_threads<LeastOp>(first_of(x, top)));
         return;
     }
     const Heat h = f.weights(top, s);
     Border b{-INFINITY, 0, 0};
-    Range<false> r = first_range(top, f.heat);
-    if (f.by_k) {   // no weights are needed
-        fill_bins(x, h, r, true, s.all);
-        find_bin(false, true, (u64)f.top_k, s);
-        const int bin = s.found;
-        if (bin >= 0) {   // else there are fewer
-            const u64 above = s.found_w;
-            if (above + s.found_own <= SA_FEW) {
-                list_tokens(x, s.list, s.list_at, s, [&](float v) { return r.has(v) && r.bin(v) <= bin; });
-                finish_few(p, row, (int)s.listed, h, f, s);
-                return;
-            }
-            b = border_from_bin(x, h, r, bin, true, (u64)f.top_k, above, s);
+    const Range<double> whole = first_range<double>(top, f.heat);
+#pragma unroll 1
+    for (int filter = 0; filter < 2; ++filter) {
+        const bool counts = filter == 0;   // top_k needs no weights; top_p's are of what that leaves
+        if (!(counts ? f.by_k : f.by_p)) continue;
+        if (!counts && f.by_k && b.t != -INFINITY) {   // from here on the tokens that top_k leaves, where a list holds them
+            list_tokens<SA_KEPT>(x, s.list, s.kept_at, s, [&](int, float v) { return v >= b.t; });
+            if (s.listed <= SA_KEPT) x.take(s.list, s.kept_at, (int)s.listed);
+            __syncthreads();
         }
-    }
-    if (f.by_p) {
+        Range<double> r = whole;
         r.lo = fmaxf(r.lo, b.t);
-        fill_bins(x, h, r, false, s.all);
-        u64 total = sum_of(s.all, s);
-        if (b.equal > b.ties) total -= (b.equal - b.ties) * h.whole_weight(b.t);
-        const u64 need = f.share(total);
-        find_bin(false, false, need, s);
-        b = border_from_bin(x, h, r, s.found, false, need, s.found_w, s);
+        u64 need = 0, above = 0;
+#pragma unroll 1
+        for (bool first = true;; first = false) {
+            fill_bins(x, h, r, counts, s.all);
+            if (first) {
+                u64 total = sum_of(s.all, s);   // (of weights)
+                if (b.equal > b.ties) total -= (b.equal - b.ties) * h.whole_weight(b.t);
+                need = counts ? (u64)f.top_k : f.share(total);
+            }
+            find_bin(false, counts, need - above, s);
+            const int bin = s.found;
+            if (bin < 0) break;   // fewer tokens than top_k (other sums are exact: they reach what is asked of them)
+            above += s.found_w;
+            if (first && counts && above + s.found_own <= SA_FEW) {
+                list_tokens<SA_FEW>(x, s.list, s.list_at, s, [&](int, float v) { return r.has(v) && r.bin(v) <= bin; });
+                return finish_few(p, row, (int)s.listed, h, f, s);
+            }
+            const InBin in = border_in_bin(x, h, r, bin, counts, need, above, s);
+            b = in.b;
+            if (in.done) break;
+            // a bin's values are fewer than its range's or lie closer, until they are equal
+            r = {in.lo, in.hi, SA_BINS / ((double)in.hi - (double)in.lo)};
+        }
     }
     const Keep k{b.t, last_tie(x, b, s)};
     clear(s.all);
-    add_places(x, h, f, s.all.w, [&](int i, float v) { return k.has(i, v); });
+    auto has = [&](int i, float v) { return k.has(i, v); };
+    if (f.by_k || f.by_p) {
+        add_places(x, h, f, s.all.w, s, has);
+    } else {
+        add_all_places(x, h, f, s.all.w, has);
+    }
     __syncthreads();
     draw<DT>(p, row, x.row, h, f, k, s);
 }
 
 template <int DT>
-__device__ __forceinline__ float largest(Row8<DT>& x, Shared& s) {
-    constexpr int N = Row8<DT>::N;
+__device__ __forceinline__ float largest(RowIn<DT>& x, Shared& s) {
+    constexpr int N = RowIn<DT>::N;
     float top = -INFINITY;
-    x.each([&](int, const float (&v)[N]) {
+    x.each([&](const int (&)[N], const float (&v)[N]) {
 #pragma unroll
         for (int k = 0; k < N; ++k) top = fmaxf(top, v[k]);
     });
     return all_threads<MostOp>(top);
 }
 
+// (No loop over rows: what it would keep from one to the next does not fit the registers, and scratch memory costs a launch
+// 7 us.)
 template <int DT>
 __global__ __launch_bounds__(SA_THREADS) void sample_rows_kernel(SampleArgs p) {
     __shared__ Shared s;
     make_table(s);
-    for (int64_t row = blockIdx.x; row < p.rows; row += gridDim.x) {
-        Row8<DT> x(p, row, 0, 0x7fffffff);
-        whole_row(p, row, x, largest(x, s), Filters(p, row), s);
-        __syncthreads();
-    }
+    const int64_t row = p.row0 + blockIdx.x;
+    RowIn<DT> x(p, row, 0, 0x7fffffff);
+    whole_row(p, row, x, largest(x, s), Filters(p, row), s);
 }
 
 // ---------------------------------------------------------------------------
@@ -684,7 +741,7 @@ __global__ __launch_bounds__(SA_THREADS) void sample_top_kernel(SampleArgs p) {
     __shared__ Shared s;
     const int64_t row = blockIdx.x / (unsigned)p.pieces;
     const int piece = blockIdx.x % (unsigned)p.pieces;
-    Row8<DT> x(p, row, piece * p.piece, (piece + 1) * p.piece);
+    RowIn<DT> x(p, row, piece * p.piece, (piece + 1) * p.piece);
     const float top = largest(x, s);
     if (threadIdx.x == 0) p.tops[blockIdx.x] = top;
 }
@@ -701,7 +758,7 @@ __global__ __launch_bounds__(SA_THREADS) void sample_bins_kernel(SampleArgs p) {
     make_table(s);
     const int64_t row = blockIdx.x / (unsigned)p.pieces;
     const int piece = blockIdx.x % (unsigned)p.pieces;
-    Row8<DT> x(p, row, piece * p.piece, (piece + 1) * p.piece);
+    RowIn<DT> x(p, row, piece * p.piece, (piece + 1) * p.piece);
     const float top = top_of(p, row);
     const Filters f(p, row);
     if (f.first_only(top)) {
@@ -711,10 +768,10 @@ __global__ __launch_bounds__(SA_THREADS) void sample_bins_kernel(SampleArgs p) {
     }
     const Heat h = f.weights(top, s);
     if (!f.by_k && !f.by_p) {
-        add_places(x, h, f, p.places + row * SA_BINS, [](int, float) { return true; });
+        add_all_places(x, h, f, p.places + row * SA_BINS, [](int, float) { return true; });
         return;
     }
-    fill_bins(x, h, first_range(top, f.heat), f.by_k, s.all);
+    fill_bins(x, h, first_range<float>(top, f.heat), f.by_k, s.all);
     u64* out = p.bins + (int64_t)blockIdx.x * SA_BINS;
     out[threadIdx.x] = s.all.w[threadIdx.x];
     out[threadIdx.x + SA_THREADS] = s.all.w[threadIdx.x + SA_THREADS];
@@ -727,6 +784,7 @@ __global__ __launch_bounds__(SA_THREADS) void sample_border_kernel(SampleArgs p)
     make_table(s);
     const int64_t row = blockIdx.x / (unsigned)p.pieces;
     const int piece = blockIdx.x % (unsigned)p.pieces;
+    RowIn<DT> x(p, row, piece * p.piece, (piece + 1) * p.piece);
     const float top = top_of(p, row);
     const Filters f(p, row);
     auto state = [&](int mode, int bin, u64 above, u64 need) {
@@ -734,7 +792,6 @@ __global__ __launch_bounds__(SA_THREADS) void sample_border_kernel(SampleArgs p)
     };
     if (f.first_only(top)) return state(SA_FIRST, 0, 0, 0);
     if (!f.by_k && !f.by_p) return state(SA_ALL, 0, 0, 0);
-    Row8<DT> x(p, row, piece * p.piece, (piece + 1) * p.piece);
     const Heat h = f.weights(top, s);
     const u64* in = p.bins + row * p.pieces * SA_BINS + threadIdx.x;
     u64 a = 0, b = 0;   // counts are two to a word, and do not carry: there are at most 2^19
@@ -753,18 +810,39 @@ __global__ __launch_bounds__(SA_THREADS) void sample_border_kernel(SampleArgs p)
     u64* places = p.places + row * SA_BINS;
     if (bin < 0) {   // fewer tokens than top_k
         if (f.by_p) return state(SA_WHOLE, 0, 0, 0);
-        add_places(x, h, f, places, [](int, float) { return true; });
+        add_all_places(x, h, f, places, [](int, float) { return true; });
         return state(SA_ALL, 0, 0, 0);
     }
-    const Range<false> r = first_range(top, f.heat);
+    const Range<float> r = first_range<float>(top, f.heat);
     const bool few = f.by_k && above + own <= SA_FEW;
     if (f.by_k && f.by_p && !few) return state(SA_WHOLE, 0, 0, 0);
+    // the bin's tokens, or all down to it, are listed; those above it weighed
     const int64_t list = (int64_t)blockIdx.x * SA_FEW;
-    list_tokens(x, p.list_v + list, p.list_at + list, s, [&](float v) {
-        return r.has(v) && (few ? r.bin(v) <= bin : r.bin(v) == bin);
-    });
-    if (threadIdx.x == 0) p.listed[blockIdx.x] = s.listed;
-    if (!few) add_places(x, h, f, places, [&](int, float v) { return r.has(v) && r.bin(v) < bin; });
+    if (threadIdx.x == 0) s.found_n = 0;
+    constexpr int N = RowIn<DT>::N;
+    auto above_it = [&](int i, float v) {
+        const int o = r.has(v) ? r.bin(v) : SA_BINS;
+        if (o == bin || (few && o < bin)) {
+            const unsigned at = atomicAdd(&s.found_n, 1u);
+            if (at < SA_FEW) {
+                p.list_v[list + at] = v;
+                p.list_at[list + at] = i;
+            }
+        }
+        return o < bin;
+    };
+    if (few) {
+        __syncthreads();
+        x.each([&](const int (&i)[N], const float (&v)[N]) {
+#pragma unroll
+            for (int k = 0; k < N; ++k) above_it(i[k], v[k]);
+        });
+        __syncthreads();
+    } else {
+        list_tokens<SA_KEPT>(x, s.list, s.list_at, s, above_it);
+        add_listed_places(x, h, f, places, s, [&](int, float v) { return r.has(v) && r.bin(v) < bin; });
+    }
+    if (threadIdx.x == 0) p.listed[blockIdx.x] = s.found_n;
     state(few ? SA_TOKENS : SA_SUMS, bin, above, need);
 }
 
@@ -800,7 +878,7 @@ __global__ __launch_bounds__(SA_THREADS) void sample_token_kernel(SampleArgs p) 
         __syncthreads();
     }
     if (whole) {   // too many of them: from the start
-        Row8<DT> all(p, row, 0, 0x7fffffff);
+        RowIn<DT> all(p, row, 0, 0x7fffffff);
         return whole_row(p, row, all, top, f, s);
     }
     if (st.mode == SA_TOKENS) return finish_few(p, row, n, h, f, s);
@@ -814,22 +892,14 @@ __global__ __launch_bounds__(SA_THREADS) void sample_token_kernel(SampleArgs p) 
         const bool there = t < n;
         const float v = there ? s.list[t] : 0.0f;
         const int at = there ? s.list_at[t] : 0;
-        if (there) s.list_w[t] = f.by_k ? 1 : h.whole_weight(v);
-        if (t < 4) s.list[n + t] = -INFINITY, s.list_at[n + t] = 0x7fffffff, s.list_w[n + t] = 0;
-        __syncthreads();
-        u64 before = st.above;
-        if (there)
-#pragma unroll 1
-            for (int i = 0; i < n; i += 4)
-#pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    const float o = s.list[i + k];
-                    before += o > v || (o == v && s.list_at[i + k] < at) ? s.list_w[i + k] : 0;
-                }
+        const u64 each = there ? f.by_k ? 1 : h.whole_weight(v) : 0;
+        if (there) s.list_w[t] = each;
+        compare_all(n, s, in_front);
+        const u64 before = there ? st.above + s.before[t] : 0;
         if (there && before < st.need) {
             const u64 w = f.weigh(h, v);
             if (w) atomicAdd(&s.all.w[at >> Places<DT>::SHIFT], w);
-            if (before + s.list_w[t] >= st.need) {   // the last of them
+            if (before + each >= st.need) {   // the last of them
                 s.border = v;
                 s.last = at;
             }
@@ -844,11 +914,13 @@ __global__ __launch_bounds__(SA_THREADS) void sample_token_kernel(SampleArgs p) 
 template <int DT>
 tvk_status launch(SampleArgs p, hipStream_t s) {
     // A workgroup a CU is wanted; pieces of 256 chunks or more
-    const int chunks = (p.cols + Row8<DT>::VEC - 1) / Row8<DT>::VEC;
+    const int chunks = (p.cols + RowIn<DT>::VEC - 1) / RowIn<DT>::VEC;
     const int64_t pieces = std::min<int64_t>({SA_PIECES, 256 / p.rows, chunks / 256});
     const dim3 block(SA_THREADS);
     if (pieces < 2) {
-        hipLaunchKernelGGL((sample_rows_kernel<DT>), dim3((unsigned)std::min<int64_t>(p.rows, 1 << 20)), block, 0, s, p);
+        constexpr int64_t MOST = 1 << 21;   // rows of a launch: 2^32 threads are too many
+        for (p.row0 = 0; p.row0 < p.rows; p.row0 += MOST)
+            hipLaunchKernelGGL((sample_rows_kernel<DT>), dim3((unsigned)std::min(p.rows - p.row0, MOST)), block, 0, s, p);
         return TVK_OK;
     }
     p.piece = (int)((chunks + pieces - 1) / pieces + 63) / 64 * 64;   // whole places
