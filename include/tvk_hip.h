@@ -589,8 +589,8 @@ tvk_status tvk_quantize_f8(const tvk_quantize_f8_desc* desc);
  * below the largest of them. a_dtype F32, F16 or BF16: a is first brought
  * into 8 bits as by tvk_quantize_f8 with block_rows 1, with the same bits, and
  * a_scale is not read. bias (NULL: none) has out_dtype or F32. Rows are
- * contiguous, `*_stride` elements apart, scales at any strides (0: one for all);
- * any alignment: rows that 16-byte loads do not meet are copied to library
+ * contiguous, `*_stride` elements apart, scales at any strides (0: one for all;
+ * for more than 64 rows of a at most 2^20 from row to row); any alignment: rows that 16-byte loads do not meet are copied to library
  * scratch for more than 64 rows of a, and 16- and 32-bit a's 8 bits go there for
  * more than 16. The sums run in an order that depends on the sizes alone: the
  * same bits every run. out must not lie over an input. K up to 2^22, or with up to

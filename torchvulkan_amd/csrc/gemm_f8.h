@@ -19,6 +19,9 @@ struct GemmF8Args {
     int M, N, K, blocks;    // blocks: ceil(K / 128)
     int tiles_m, tiles_n;
     int out_dtype, bias32;
+    // of the tiled kernel
+    float* part;            // [splits][M][part_n], the sums of a split K, or NULL
+    int part_n, split_blocks;
 };
 
 namespace {
@@ -50,11 +53,21 @@ __device__ __forceinline__ f32x4 f8_mfma(i32x8 w, i32x8 x) {
     return d;
 }
 
-// One output from its float32 sum.
 template <int DT>
-__device__ inline typename elem<DT>::T f8_finish(const GemmF8Args& p, int n, float v) {
-    if (p.bias) v += p.bias32 ? static_cast<const float*>(p.bias)[n] : at<DT>(p.bias, n);
-    return elem<DT>::from_f32(v);
+__device__ __forceinline__ float f8_bias(const GemmF8Args& p, int n) {
+    return p.bias32 ? static_cast<const float*>(p.bias)[n] : at<DT>(p.bias, n);
+}
+
+// Stores one output from its float32 sum.
+__device__ __forceinline__ void f8_put(const GemmF8Args& p, int64_t m, int n, float v) {
+    const int64_t o = m * p.ldo + n;
+    if (p.out_dtype == TVK_F32) {
+        static_cast<float*>(p.out)[o] = p.bias ? v + f8_bias<TVK_F32>(p, n) : v;
+    } else if (p.out_dtype == TVK_F16) {
+        put<TVK_F16>(p.out, o, p.bias ? v + f8_bias<TVK_F16>(p, n) : v);
+    } else {
+        put<TVK_BF16>(p.out, o, p.bias ? v + f8_bias<TVK_BF16>(p, n) : v);
+    }
 }
 
 }  // namespace
@@ -64,7 +77,9 @@ void f8_quantize_rows(int dtype, const void* x, int64_t x_stride, uint8_t* out, 
 // 8-bit rows copied to rows of whole blocks, zeros behind them.
 void f8_pad_rows(const uint8_t* x, int64_t x_stride, uint8_t* out, int64_t rows, int64_t cols, hipStream_t s);
 
-// Queues the tiled kernel: 16-byte aligned 8-bit rows, K a multiple of 16.
-void f8_ring(const GemmF8Args& p, hipStream_t s);
+// Queues the tiled kernel: 16-byte aligned 8-bit rows, K a multiple of 16. Of `splits` parts of K, which f8_ring_splits
+// suggests, the sums go to p.part and are joined by a second launch.
+int f8_ring_splits(const GemmF8Args& p);
+void f8_ring(const GemmF8Args& p, int splits, hipStream_t s);
 
 }  // namespace tvk

@@ -80,30 +80,31 @@ __global__ __launch_bounds__(64 * FR_WAVES) void gemm_f8_rows_kernel(GemmF8Args 
         float s[U][MT];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            const int b = b0 + FR_WAVES * u, valid = b < p.blocks ? p.K - b * F8_BLOCK - 32 * g : 0;
-            fw[u] = load32(w + (int64_t)b * F8_BLOCK, valid);
+            const int b = b0 + FR_WAVES * u;
+            if (b < p.blocks) fw[u] = load32(w + (int64_t)b * F8_BLOCK, p.K - b * F8_BLOCK - 32 * g);
         }
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            const int b = b0 + FR_WAVES * u, bc = min(b, p.blocks - 1), valid = b < p.blocks ? p.K - b * F8_BLOCK - 32 * g : 0;
-            const float scale = sb[(int64_t)bc * p.sb_b];
+            const int b = b0 + FR_WAVES * u, valid = p.K - b * F8_BLOCK - 32 * g;
+            if (b >= p.blocks) continue;
+            const float scale = sb[(int64_t)b * p.sb_b];
 #pragma unroll
             for (int j = 0; j < MT; ++j) {
-                const int m = 16 * j + r, mc = min(m, p.M - 1), there = m < p.M ? valid : 0;
+                const int m = min(16 * j + r, p.M - 1);   // rows past M compute what is not stored
                 if constexpr (IN8) {
-                    fx[u][j] = load32(static_cast<const uint8_t*>(p.a) + (int64_t)mc * p.lda + (int64_t)b * F8_BLOCK + 32 * g, there);
-                    s[u][j] = p.sa[(int64_t)mc * p.sa_m + (int64_t)bc * p.sa_b] * scale;
+                    fx[u][j] = load32(static_cast<const uint8_t*>(p.a) + m * p.lda + (int64_t)b * F8_BLOCK + 32 * g, valid);
+                    s[u][j] = p.sa[m * p.sa_m + b * p.sa_b] * scale;
                 } else {
                     typedef typename elem<IN8 ? TVK_F32 : ADT>::T T;
-                    fx[u][j] = quantize32<IN8 ? TVK_F32 : ADT>(static_cast<const T*>(p.a) + (int64_t)mc * p.lda + (int64_t)b * F8_BLOCK + 32 * g,
-                                                               there, s[u][j]);
+                    fx[u][j] = quantize32<IN8 ? TVK_F32 : ADT>(static_cast<const T*>(p.a) + m * p.lda + (int64_t)b * F8_BLOCK + 32 * g,
+                                                               valid, s[u][j]);
                     s[u][j] *= scale;
                 }
             }
         }
 #pragma unroll
         for (int u = 0; u < U; ++u)
-            if (b0 + FR_WAVES * u < p.blocks)   // (a block past the end must not weigh in: its scale may be infinite)
+            if (b0 + FR_WAVES * u < p.blocks)
 #pragma unroll
                 for (int j = 0; j < MT; ++j) {
                     const f32x4 d = f8_mfma<WIDE>(fw[u], fx[u][j]);
@@ -122,10 +123,7 @@ __global__ __launch_bounds__(64 * FR_WAVES) void gemm_f8_rows_kernel(GemmF8Args 
         float v = sum[0][m][i % FR_ROWS];
 #pragma unroll
         for (int k = 1; k < FR_WAVES; ++k) v += sum[k][m][i % FR_ROWS];
-        const int64_t o = m * p.ldo + n;
-        if (p.out_dtype == TVK_F32) static_cast<float*>(p.out)[o] = f8_finish<TVK_F32>(p, n, v);
-        else if (p.out_dtype == TVK_F16) static_cast<half_t*>(p.out)[o] = f8_finish<TVK_F16>(p, n, v);
-        else static_cast<uint16_t*>(p.out)[o] = f8_finish<TVK_BF16>(p, n, v);
+        f8_put(p, m, n, v);
     }
 }
 
@@ -145,7 +143,8 @@ void few_rows(const GemmF8Args& p, hipStream_t s) {
     else few_rows<ADT, false>(p, s);
 }
 
-constexpr int64_t RING_MOST = 1 << 22;   // bytes from row to row: a tile's offsets stay within 31 bits
+constexpr int64_t RING_MOST = 1 << 22;     // bytes from row to row, and
+constexpr int64_t SCALES_MOST = 1 << 20;   // scales: a tile's offsets stay within 31 bits
 
 // Rows that the tiled kernel's loads of 16 bytes meet.
 bool ring_rows(const void* p, int64_t stride, int K) {
@@ -169,6 +168,8 @@ extern "C" tvk_status tvk_gemm_f8(const tvk_gemm_f8_desc* d) {
     if (d->a_stride < 0 || d->b_stride < 0 || d->a_scale_stride[0] < 0 || d->a_scale_stride[1] < 0 || d->b_scale_stride[0] < 0 ||
         d->b_scale_stride[1] < 0 || !rows_apart(d->out_stride, d->M, d->N))
         return bad(TVK_ERR_INVALID, "negative strides, or output rows that overlap");
+    if (d->M > 64 && (d->a_scale_stride[0] > SCALES_MOST || d->b_scale_stride[0] > SCALES_MOST))
+        return bad(TVK_ERR_UNSUPPORTED, "scales up to 2^20 from row to row only for more than 64 rows");
     if (d->M > 64 && d->K > RING_MOST) return bad(TVK_ERR_UNSUPPORTED, "K up to 2^22 only for more than 64 rows");
     if (((d->M + 127) / 128) * ((d->N + 127) / 128) > (1 << 22)) return bad(TVK_ERR_UNSUPPORTED, "more than 2^22 tiles of 128 x 128");
     GemmF8Args p{};
@@ -197,12 +198,16 @@ extern "C" tvk_status tvk_gemm_f8(const tvk_gemm_f8_desc* d) {
     // what has to be laid out first: rows of A in 16 or 32 bits, and for the tiled kernel rows that 16-byte loads do not meet
     const bool make_a = !in8 && p.M > 16, pad_a = ring && in8 && !ring_rows(d->a, d->a_stride, p.K);
     const bool pad_b = ring && !ring_rows(d->b, d->b_stride, p.K);
+    const int splits = ring ? f8_ring_splits(p) : 1;
     Scratch scratch;
-    if (p.K > 0 && (make_a || pad_a || pad_b)) {
+    if (splits > 1 || (p.K > 0 && (make_a || pad_a || pad_b))) {
         const int64_t bytes_a = make_a || pad_a ? p.M * wide : 0, bytes_b = pad_b ? p.N * wide : 0;
-        const int64_t bytes_s = make_a ? (int64_t)p.blocks * p.M * 4 : 0;
-        uint8_t* at = static_cast<uint8_t*>(scratch.get((size_t)(bytes_a + bytes_b + bytes_s) + 16, s));
+        const int64_t bytes_s = make_a ? ((int64_t)p.blocks * p.M * 4 + 15) / 16 * 16 : 0;
+        p.part_n = (p.N + 3) / 4 * 4;
+        const int64_t bytes_p = splits > 1 ? (int64_t)splits * p.M * p.part_n * 4 : 0;
+        uint8_t* at = static_cast<uint8_t*>(scratch.get((size_t)(bytes_a + bytes_b + bytes_s + bytes_p) + 16, s));
         if (!at) return bad(TVK_ERR_OOM, "workspace allocation failed");
+        if (splits > 1) p.part = reinterpret_cast<float*>(at + bytes_a + bytes_b + bytes_s);
         if (make_a) {
             float* scale = reinterpret_cast<float*>(at + bytes_a + bytes_b);
             f8_quantize_rows(d->a_dtype, d->a, d->a_stride, at, scale, p.M, p.K, s);
@@ -220,7 +225,7 @@ extern "C" tvk_status tvk_gemm_f8(const tvk_gemm_f8_desc* d) {
         }
     }
     if (ring && p.K % 16) p.K = (int)wide;   // both are copies then, with zeros up to there
-    if (ring) f8_ring(p, s);
+    if (ring) f8_ring(p, splits, s);
     else if (in8 || make_a) few_rows<TVK_F8E4M3FN>(p, s);
     else if (d->a_dtype == TVK_F32) few_rows<TVK_F32>(p, s);
     else if (d->a_dtype == TVK_F16) few_rows<TVK_F16>(p, s);
