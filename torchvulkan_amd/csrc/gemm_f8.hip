@@ -17,7 +17,7 @@ using namespace tvk;
 namespace {
 
 constexpr int FR_WAVES = 8;
-constexpr int FR_ROWS = 16;     // of W a workgroup
+constexpr int NT4 = 12288, NT2 = 6144;   // columns
 
 // 32 bytes of a row, of which `valid` are there (zeros behind them), at any alignment.
 __device__ __forceinline__ i32x8 load32(const uint8_t* p, int valid) {
@@ -63,25 +63,31 @@ __device__ __forceinline__ i32x8 quantize32(const typename elem<DT>::T* p, int v
     return r;
 }
 
-// ADT: the type of A, TVK_F8E4M3FN with scales. MT: blocks of 16 rows of A.
-template <int ADT, int MT, bool WIDE>
+// ADT: the type of A, TVK_F8E4M3FN with scales. MT, NT: blocks of 16 rows of A and of W; U: blocks of k on their way.
+template <int ADT, int MT, int NT, int U, bool WIDE>
 __global__ __launch_bounds__(64 * FR_WAVES) void gemm_f8_rows_kernel(GemmF8Args p) {
     constexpr bool IN8 = ADT == TVK_F8E4M3FN;
-    constexpr int U = MT == 1 ? 4 : 2;   // blocks on their way
+    static_assert(F8_BLOCK % (16 * NT) == 0, "one scale of W a workgroup and block");
     const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
-    const int r = lane % 16, g = lane / 16, n0 = blockIdx.x * FR_ROWS;
-    const uint8_t* w = p.b + (int64_t)min(n0 + r, p.N - 1) * p.ldb + 32 * g;   // rows past N compute what is not stored
-    const float* sb = p.sb + (int64_t)(n0 / F8_BLOCK) * p.sb_n;
-    f32x4 acc[MT];
+    const int r = lane % 16, g = lane / 16, n0 = blockIdx.x * 16 * NT;
+    const uint8_t* w[NT];
 #pragma unroll
-    for (int j = 0; j < MT; ++j) acc[j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    for (int i = 0; i < NT; ++i) w[i] = p.b + (int64_t)min(n0 + 16 * i + r, p.N - 1) * p.ldb + 32 * g;   // rows past N compute what is not stored
+    const float* sb = p.sb + (int64_t)(n0 / F8_BLOCK) * p.sb_n;
+    f32x4 acc[NT][MT];
+#pragma unroll
+    for (int i = 0; i < NT; ++i)
+#pragma unroll
+        for (int j = 0; j < MT; ++j) acc[i][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
     for (int b0 = wave; b0 < p.blocks; b0 += FR_WAVES * U) {
-        i32x8 fw[U], fx[U][MT];
+        i32x8 fw[U][NT], fx[U][MT];
         float s[U][MT];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             const int b = b0 + FR_WAVES * u;
-            if (b < p.blocks) fw[u] = load32(w + (int64_t)b * F8_BLOCK, p.K - b * F8_BLOCK - 32 * g);
+            if (b >= p.blocks) continue;
+#pragma unroll
+            for (int i = 0; i < NT; ++i) fw[u][i] = load32(w[i] + (int64_t)b * F8_BLOCK, p.K - b * F8_BLOCK - 32 * g);
         }
 #pragma unroll
         for (int u = 0; u < U; ++u) {
@@ -106,34 +112,50 @@ __global__ __launch_bounds__(64 * FR_WAVES) void gemm_f8_rows_kernel(GemmF8Args 
         for (int u = 0; u < U; ++u)
             if (b0 + FR_WAVES * u < p.blocks)
 #pragma unroll
-                for (int j = 0; j < MT; ++j) {
-                    const f32x4 d = f8_mfma<WIDE>(fw[u], fx[u][j]);
+                for (int i = 0; i < NT; ++i)
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) acc[j][i] = fmaf(d[i], s[u][j], acc[j][i]);
-                }
+                    for (int j = 0; j < MT; ++j) {
+                        const f32x4 d = f8_mfma<WIDE>(fw[u][i], fx[u][j]);
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) acc[i][j][e] = fmaf(d[e], s[u][j], acc[i][j][e]);
+                    }
     }
     // [wave][m][n]: the waves' sums added in order
-    __shared__ __attribute__((aligned(16))) float sum[FR_WAVES][MT * 16][FR_ROWS + 4];
+    __shared__ __attribute__((aligned(16))) float sum[FR_WAVES][MT * 16][NT * 16 + 4];
 #pragma unroll
-    for (int j = 0; j < MT; ++j) *reinterpret_cast<f32x4*>(&sum[wave][16 * j + r][4 * g]) = acc[j];
+    for (int i = 0; i < NT; ++i)
+#pragma unroll
+        for (int j = 0; j < MT; ++j) *reinterpret_cast<f32x4*>(&sum[wave][16 * j + r][16 * i + 4 * g]) = acc[i][j];
     __syncthreads();
-    for (int i = threadIdx.x; i < MT * 16 * FR_ROWS; i += 64 * FR_WAVES) {
-        const int m = i / FR_ROWS, n = n0 + i % FR_ROWS;
-        if (m >= p.M || n >= p.N) continue;
-        float v = sum[0][m][i % FR_ROWS];
+    for (int q = threadIdx.x; q < MT * 16 * NT * 16; q += 64 * FR_WAVES) {
+        const int m = q / (NT * 16), c = q % (NT * 16);
+        if (m >= p.M || n0 + c >= p.N) continue;
+        float v = sum[0][m][c];
 #pragma unroll
-        for (int k = 1; k < FR_WAVES; ++k) v += sum[k][m][i % FR_ROWS];
-        f8_put(p, m, n, v);
+        for (int k = 1; k < FR_WAVES; ++k) v += sum[k][m][c];
+        f8_put(p, m, n0 + c, v);
     }
+}
+
+template <int ADT, int MT, int NT, int U, bool WIDE>
+void launch_rows(const GemmF8Args& p, hipStream_t s) {
+    hipLaunchKernelGGL((gemm_f8_rows_kernel<ADT, MT, NT, U, WIDE>), dim3((unsigned)((p.N + 16 * NT - 1) / (16 * NT))), dim3(64 * FR_WAVES), 0, s, p);
 }
 
 template <int ADT, bool WIDE>
 void few_rows(const GemmF8Args& p, hipStream_t s) {
-    const dim3 grid((unsigned)((p.N + FR_ROWS - 1) / FR_ROWS)), block(64 * FR_WAVES);
-    if (p.M <= 16) hipLaunchKernelGGL((gemm_f8_rows_kernel<ADT, 1, WIDE>), grid, block, 0, s, p);
-    else if constexpr (ADT == TVK_F8E4M3FN) {
-        if (p.M <= 32) hipLaunchKernelGGL((gemm_f8_rows_kernel<ADT, 2, WIDE>), grid, block, 0, s, p);
-        else hipLaunchKernelGGL((gemm_f8_rows_kernel<ADT, 4, WIDE>), grid, block, 0, s, p);
+    if (p.M <= 16) {
+        if (p.N >= NT4) launch_rows<ADT, 1, 4, 2, WIDE>(p, s);
+        else if (p.N >= NT2) launch_rows<ADT, 1, 2, 4, WIDE>(p, s);
+        else launch_rows<ADT, 1, 1, 4, WIDE>(p, s);
+    } else if constexpr (ADT == TVK_F8E4M3FN) {
+        if (p.M <= 32) {
+            if (p.N >= NT2) launch_rows<ADT, 2, 2, 2, WIDE>(p, s);
+            else launch_rows<ADT, 2, 1, 2, WIDE>(p, s);
+        } else {
+            if (p.N >= NT2) launch_rows<ADT, 4, 2, 1, WIDE>(p, s);
+            else launch_rows<ADT, 4, 1, 2, WIDE>(p, s);
+        }
     }
 }
 
