@@ -34,40 +34,98 @@ __device__ __forceinline__ i32x8 load32(const uint8_t* p, int valid) {
     return u.v;
 }
 
-// The same of a row in DT, with the scale of the block that the lanes of one row share out.
-template <int DT>
-__device__ __forceinline__ i32x8 quantize32(const typename elem<DT>::T* p, int valid, float& scale) {
-    typedef typename elem<DT>::T T;
-    constexpr int VEC = 16 / (int)sizeof(T);
-    float v[32];
-    if (valid >= 32) {
-#pragma unroll
-        for (int i = 0; i < 32; i += VEC) {
-            const Words<16> w = load_words<16, sizeof(T)>(p + i);
-#pragma unroll
-            for (int k = 0; k < VEC; ++k) v[i + k] = word_at<DT>(w, k);
-        }
-    } else {
-#pragma unroll
-        for (int i = 0; i < 32; ++i) v[i] = i < valid ? elem<DT>::to_f32(p[i]) : 0.0f;
-    }
-    float top = 0.0f;
-#pragma unroll
-    for (int i = 0; i < 32; ++i) top = fmaxf(top, fabsf(v[i]));
-    top = fmaxf(top, __shfl_xor(top, 16));
-    const F8Scale s(fmaxf(top, __shfl_xor(top, 32)));
-    scale = s.s;
-    i32x8 r;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) r[i] = (int)s.pack4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
-    return r;
-}
+// How a wave has its rows of A: in 8 bits with scales; in wider types, 32 values a lane, each lane those of its
+// operand; the same for up to 4 rows, 8 values a lane, handed round afterwards (a quarter of the arithmetic, which is
+// what bounds one row of them: 1 x 4096 x 14336 from bf16 TBD).
+enum { X_F8, X_OWN, X_SHARED };
 
-// ADT: the type of A, TVK_F8E4M3FN with scales. MT, NT: blocks of 16 rows of A and of W; U: blocks of k on their way.
-template <int ADT, int MT, int NT, int U, bool WIDE>
+// What a lane loads of one block of A, and the operands that become of it.
+template <int ADT, int FORM, int MT>
+struct XBlock {
+    typedef typename elem<FORM == X_F8 ? TVK_F32 : ADT>::T T;
+    static constexpr int DT = FORM == X_F8 ? TVK_F32 : ADT, VALUES = FORM == X_OWN ? 32 : 8, VEC = 16 / (int)sizeof(T);
+    i32x8 x[FORM == X_F8 ? MT : 1];
+    float s[MT];
+    Words<16> raw[VALUES / VEC];
+
+    // Block b, all 128 values of it; rows past M compute what is not stored.
+    __device__ __forceinline__ void load(const GemmF8Args& p, int lane, int b) {
+        if constexpr (FORM == X_F8) {
+#pragma unroll
+            for (int j = 0; j < MT; ++j) {
+                const int m = min(16 * j + lane % 16, p.M - 1);
+                x[j] = load32(static_cast<const uint8_t*>(p.a) + m * p.lda + (int64_t)b * F8_BLOCK + lane / 16 * 32, 32);
+                s[j] = p.sa[m * p.sa_m + b * p.sa_b];
+            }
+        } else {
+            const int m = min(FORM == X_OWN ? lane % 16 : lane / 16, p.M - 1), k = FORM == X_OWN ? lane / 16 * 32 : lane % 16 * 8;
+            const T* at = static_cast<const T*>(p.a) + m * p.lda + (int64_t)b * F8_BLOCK + k;
+#pragma unroll
+            for (int i = 0; i < VALUES / VEC; ++i) raw[i] = load_words<16, sizeof(T)>(at + i * VEC);
+        }
+    }
+
+    // The same of a block of which `valid` values of this lane's 32 are there.
+    __device__ __forceinline__ void load_part(const GemmF8Args& p, int lane, int b, int valid) {
+#pragma unroll
+        for (int j = 0; j < MT; ++j) {
+            const int m = min(16 * j + lane % 16, p.M - 1);
+            const int64_t at = m * p.lda + (int64_t)b * F8_BLOCK + lane / 16 * 32;
+            if constexpr (FORM == X_F8) {
+                x[j] = load32(static_cast<const uint8_t*>(p.a) + at, valid);
+                s[j] = p.sa[m * p.sa_m + b * p.sa_b];
+            } else {
+                float v[32];
+#pragma unroll
+                for (int i = 0; i < 32; ++i) v[i] = i < valid ? elem<DT>::to_f32(static_cast<const T*>(p.a)[at + i]) : 0.0f;
+                quantize(v);
+            }
+        }
+    }
+
+    // 32 values a lane, with the scale of the block that the four lanes of one row share out.
+    __device__ __forceinline__ void quantize(const float (&v)[32]) {
+        float top = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 32; ++i) top = fmaxf(top, fabsf(v[i]));
+        top = fmaxf(top, __shfl_xor(top, 16));
+        const F8Scale to(fmaxf(top, __shfl_xor(top, 32)));
+        s[0] = to.s;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[0][i] = (int)to.pack4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+    }
+
+    // Makes x and s of what load() brought.
+    __device__ __forceinline__ void make(int lane) {
+        if constexpr (FORM == X_OWN) {
+            float v[32];
+#pragma unroll
+            for (int i = 0; i < 32; ++i) v[i] = word_at<DT>(raw[i / VEC], i % VEC);
+            quantize(v);
+        } else if constexpr (FORM == X_SHARED) {
+            float v[8], top = 0.0f;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] = word_at<DT>(raw[i / VEC], i % VEC), top = fmaxf(top, fabsf(v[i]));
+#pragma unroll
+            for (int i = 1; i < 16; i *= 2) top = fmaxf(top, __shfl_xor(top, i));
+            const F8Scale to(top);
+            const int lo = (int)to.pack4(v[0], v[1], v[2], v[3]), hi = (int)to.pack4(v[4], v[5], v[6], v[7]);
+            const int from = lane % 4 * 16;   // lanes of the row that this lane's operand holds; its copies past 4 rows are not stored
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                x[0][2 * i] = __shfl(lo, from + lane / 16 * 4 + i);
+                x[0][2 * i + 1] = __shfl(hi, from + lane / 16 * 4 + i);
+            }
+            s[0] = __shfl(to.s, from);
+        }
+    }
+};
+
+// ADT: the type of A. MT, NT: blocks of 16 rows of A and of W; U: blocks of k on their way.
+template <int ADT, int FORM, int MT, int NT, int U, bool WIDE>
 __global__ __launch_bounds__(64 * FR_WAVES) void gemm_f8_rows_kernel(GemmF8Args p) {
-    constexpr bool IN8 = ADT == TVK_F8E4M3FN;
     static_assert(F8_BLOCK % (16 * NT) == 0, "one scale of W a workgroup and block");
+    static_assert(FORM == X_F8 || MT == 1, "16 rows of A in wider types");
     const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
     const int r = lane % 16, g = lane / 16, n0 = blockIdx.x * 16 * NT;
     const uint8_t* w[NT];
@@ -79,46 +137,49 @@ __global__ __launch_bounds__(64 * FR_WAVES) void gemm_f8_rows_kernel(GemmF8Args 
     for (int i = 0; i < NT; ++i)
 #pragma unroll
         for (int j = 0; j < MT; ++j) acc[i][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-    for (int b0 = wave; b0 < p.blocks; b0 += FR_WAVES * U) {
-        i32x8 fw[U][NT], fx[U][MT];
-        float s[U][MT];
+    struct Block {
+        i32x8 w[NT];
+        XBlock<ADT, FORM, MT> x;
+        float s;
+    };
+    auto add = [&](const Block& k) {
+#pragma unroll
+        for (int i = 0; i < NT; ++i)
+#pragma unroll
+            for (int j = 0; j < MT; ++j) {
+                const f32x4 d = f8_mfma<WIDE>(k.w[i], k.x.x[j]);
+                const float scale = k.x.s[j] * k.s;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) acc[i][j][e] = fmaf(d[e], scale, acc[i][j][e]);
+            }
+    };
+    const int full = p.K / F8_BLOCK;
+    for (int b0 = wave; b0 < full; b0 += FR_WAVES * U) {
+        Block on[U];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             const int b = b0 + FR_WAVES * u;
-            if (b >= p.blocks) continue;
+            if (b >= full) continue;
 #pragma unroll
-            for (int i = 0; i < NT; ++i) fw[u][i] = load32(w[i] + (int64_t)b * F8_BLOCK, p.K - b * F8_BLOCK - 32 * g);
+            for (int i = 0; i < NT; ++i) on[u].w[i] = load32(w[i] + (int64_t)b * F8_BLOCK, 32);
+            on[u].x.load(p, lane, b);
+            on[u].s = sb[(int64_t)b * p.sb_b];
         }
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            const int b = b0 + FR_WAVES * u, valid = p.K - b * F8_BLOCK - 32 * g;
-            if (b >= p.blocks) continue;
-            const float scale = sb[(int64_t)b * p.sb_b];
-#pragma unroll
-            for (int j = 0; j < MT; ++j) {
-                const int m = min(16 * j + r, p.M - 1);   // rows past M compute what is not stored
-                if constexpr (IN8) {
-                    fx[u][j] = load32(static_cast<const uint8_t*>(p.a) + m * p.lda + (int64_t)b * F8_BLOCK + 32 * g, valid);
-                    s[u][j] = p.sa[m * p.sa_m + b * p.sa_b] * scale;
-                } else {
-                    typedef typename elem<IN8 ? TVK_F32 : ADT>::T T;
-                    fx[u][j] = quantize32<IN8 ? TVK_F32 : ADT>(static_cast<const T*>(p.a) + m * p.lda + (int64_t)b * F8_BLOCK + 32 * g,
-                                                               valid, s[u][j]);
-                    s[u][j] *= scale;
-                }
-            }
+            if (b0 + FR_WAVES * u >= full) continue;
+            on[u].x.make(lane);
+            add(on[u]);
         }
+    }
+    if (full < p.blocks && wave == full % FR_WAVES) {
+        Block k;
+        const int valid = p.K - full * F8_BLOCK - 32 * g;
 #pragma unroll
-        for (int u = 0; u < U; ++u)
-            if (b0 + FR_WAVES * u < p.blocks)
-#pragma unroll
-                for (int i = 0; i < NT; ++i)
-#pragma unroll
-                    for (int j = 0; j < MT; ++j) {
-                        const f32x4 d = f8_mfma<WIDE>(fw[u][i], fx[u][j]);
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) acc[i][j][e] = fmaf(d[e], s[u][j], acc[i][j][e]);
-                    }
+        for (int i = 0; i < NT; ++i) k.w[i] = load32(w[i] + (int64_t)full * F8_BLOCK, valid);
+        k.x.load_part(p, lane, full, valid);
+        k.s = sb[(int64_t)full * p.sb_b];
+        add(k);
     }
     // [wave][m][n]: the waves' sums added in order
     __shared__ __attribute__((aligned(16))) float sum[FR_WAVES][MT * 16][NT * 16 + 4];
@@ -137,25 +198,32 @@ __global__ __launch_bounds__(64 * FR_WAVES) void gemm_f8_rows_kernel(GemmF8Args 
     }
 }
 
-template <int ADT, int MT, int NT, int U, bool WIDE>
+template <int ADT, int FORM, int MT, int NT, int U, bool WIDE>
 void launch_rows(const GemmF8Args& p, hipStream_t s) {
-    hipLaunchKernelGGL((gemm_f8_rows_kernel<ADT, MT, NT, U, WIDE>), dim3((unsigned)((p.N + 16 * NT - 1) / (16 * NT))), dim3(64 * FR_WAVES), 0, s, p);
+    hipLaunchKernelGGL((gemm_f8_rows_kernel<ADT, FORM, MT, NT, U, WIDE>), dim3((unsigned)((p.N + 16 * NT - 1) / (16 * NT))),
+                       dim3(64 * FR_WAVES), 0, s, p);
+}
+
+template <int ADT, int FORM, bool WIDE>
+void rows_16(const GemmF8Args& p, hipStream_t s) {
+    if (p.N >= NT4) launch_rows<ADT, FORM, 1, 4, 2, WIDE>(p, s);
+    else if (p.N >= NT2) launch_rows<ADT, FORM, 1, 2, 4, WIDE>(p, s);
+    else launch_rows<ADT, FORM, 1, 1, 4, WIDE>(p, s);
 }
 
 template <int ADT, bool WIDE>
 void few_rows(const GemmF8Args& p, hipStream_t s) {
-    if (p.M <= 16) {
-        if (p.N >= NT4) launch_rows<ADT, 1, 4, 2, WIDE>(p, s);
-        else if (p.N >= NT2) launch_rows<ADT, 1, 2, 4, WIDE>(p, s);
-        else launch_rows<ADT, 1, 1, 4, WIDE>(p, s);
-    } else if constexpr (ADT == TVK_F8E4M3FN) {
-        if (p.M <= 32) {
-            if (p.N >= NT2) launch_rows<ADT, 2, 2, 2, WIDE>(p, s);
-            else launch_rows<ADT, 2, 1, 2, WIDE>(p, s);
-        } else {
-            if (p.N >= NT2) launch_rows<ADT, 4, 2, 1, WIDE>(p, s);
-            else launch_rows<ADT, 4, 1, 2, WIDE>(p, s);
-        }
+    if constexpr (ADT != TVK_F8E4M3FN) {
+        if (p.M <= 4) rows_16<ADT, X_SHARED, WIDE>(p, s);
+        else rows_16<ADT, X_OWN, WIDE>(p, s);
+    } else if (p.M <= 16) {
+        rows_16<ADT, X_F8, WIDE>(p, s);
+    } else if (p.M <= 32) {
+        if (p.N >= NT2) launch_rows<ADT, X_F8, 2, 2, 2, WIDE>(p, s);
+        else launch_rows<ADT, X_F8, 2, 1, 2, WIDE>(p, s);
+    } else {
+        if (p.N >= NT2) launch_rows<ADT, X_F8, 4, 2, 1, WIDE>(p, s);
+        else launch_rows<ADT, X_F8, 4, 1, 2, WIDE>(p, s);
     }
 }
 
@@ -171,6 +239,16 @@ constexpr int64_t SCALES_MOST = 1 << 20;   // scales: a tile's offsets stay with
 // Rows that the tiled kernel's loads of 16 bytes meet.
 bool ring_rows(const void* p, int64_t stride, int K) {
     return reinterpret_cast<uintptr_t>(p) % 16 == 0 && stride % 16 == 0 && stride <= RING_MOST && K % 16 == 0;
+}
+
+// Where up to 64 rows run the tiled kernel too, rows that it can load as they lie: it reads A once for 128 rows of W
+// and not once for 16 or 32, and in exchange splits K and joins the sums in a launch of its own. Tiled against rows:
+// 64 x 2048 x 4096 13.0 and 15.8 us, 64 x 14336 x 4096 23.7 and 33.1, 32 x 14336 x 4096 21.1 and 24.2;
+// 64 x 1024 x 1024 10.5 and 6.0, 32 x 8192 x 4096 14.9 and 13.9.
+bool tiles_pay(const GemmF8Args& p, const tvk_gemm_f8_desc* d) {
+    return p.M > 16 && (int64_t)p.N * p.K >= (p.M > 32 ? 1 << 23 : 3 << 24) && p.K % 16 == 0 && p.K <= RING_MOST &&
+           p.sa_m <= SCALES_MOST && p.sb_n <= SCALES_MOST && ring_rows(p.b, p.ldb, p.K) &&
+           (d->a_dtype != TVK_F8E4M3FN || ring_rows(d->a, d->a_stride, p.K));
 }
 
 }  // namespace
@@ -216,7 +294,7 @@ extern "C" tvk_status tvk_gemm_f8(const tvk_gemm_f8_desc* d) {
     p.bias32 = d->bias_dtype == TVK_F32;
     const hipStream_t s = resolve_stream(d->stream);
     const int64_t wide = (int64_t)p.blocks * F8_BLOCK;
-    const bool ring = p.M > 64;
+    const bool ring = p.M > 64 || tiles_pay(p, d);
     // what has to be laid out first: rows of A in 16 or 32 bits, and for the tiled kernel rows that 16-byte loads do not meet
     const bool make_a = !in8 && p.M > 16, pad_a = ring && in8 && !ring_rows(d->a, d->a_stride, p.K);
     const bool pad_b = ring && !ring_rows(d->b, d->b_stride, p.K);
