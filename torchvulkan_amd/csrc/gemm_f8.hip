@@ -19,19 +19,44 @@ namespace {
 constexpr int FR_WAVES = 8;
 constexpr int NT4 = 12288, NT2 = 6144;   // columns
 
-// 32 bytes of a row, of which `valid` are there (zeros behind them), at any alignment.
-__device__ __forceinline__ i32x8 load32(const uint8_t* p, int valid) {
+// A lane's 32 values of a block of k, of A and of W alike, whose order does not matter to the sum: 16 of the first
+// half and 16 of the second, so that the four lanes of a row load 64 bytes side by side.
+__device__ __forceinline__ int half_at(int g, int half) { return 64 * half + 16 * g; }
+
+// They of a row of bytes at any alignment, of a whole block.
+__device__ __forceinline__ i32x8 load32(const uint8_t* block, int g) {
     union { Words<16> h[2]; i32x8 v; } u;
-    u.v = i32x8{0, 0, 0, 0, 0, 0, 0, 0};
-    if (valid >= 32) {
-        u.h[0] = load_words<16, 1>(p);
-        u.h[1] = load_words<16, 1>(p + 16);
-    } else {
 #pragma unroll
-        for (int i = 0; i < 32; ++i)
-            if (i < valid) u.v[i / 4] |= (int)((uint32_t)p[i] << i % 4 * 8);
-    }
+    for (int h = 0; h < 2; ++h) u.h[h] = load_words<16, 1>(block + half_at(g, h));
     return u.v;
+}
+
+// The same from `at` on in a row of K bytes, with zeros behind its end: the last 16 of the row, moved down, or where it
+// has fewer, one after the other.
+__device__ __forceinline__ i32x8 load_rest(const uint8_t* row, int at, int g, int K) {
+    i32x8 v = {0, 0, 0, 0, 0, 0, 0, 0};
+    if (K >= 16) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const int k = at + half_at(g, h), from = min(k, K - 16), by = k - from;
+            Words<16> w = load_words<16, 1>(row + from);
+#pragma unroll
+            for (int step = 2; step >= 1; step /= 2)   // words, then the bytes of one
+#pragma unroll
+                for (int i = 0; i < 4; ++i) w.w[i] = by & 4 * step ? (i + step < 4 ? w.w[i + step] : 0u) : w.w[i];
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                v[4 * h + i] = by < 16 ? (int)__builtin_amdgcn_alignbyte(i < 3 ? w.w[i + 1] : 0u, w.w[i], (uint32_t)by % 4) : 0;
+        }
+    } else {
+#pragma unroll 1
+        for (int i = 0; i < 16; ++i) {
+            const int k = half_at(g, 0) + i, byte = k < K ? row[k] : 0;
+#pragma unroll
+            for (int q = 0; q < 4; ++q) v[q] |= i / 4 == q ? byte << i % 4 * 8 : 0;
+        }
+    }
+    return v;
 }
 
 // How a wave has its rows of A: in 8 bits with scales; in wider types, 32 values a lane, each lane those of its
@@ -54,30 +79,34 @@ struct XBlock {
 #pragma unroll
             for (int j = 0; j < MT; ++j) {
                 const int m = min(16 * j + lane % 16, p.M - 1);
-                x[j] = load32(static_cast<const uint8_t*>(p.a) + m * p.lda + (int64_t)b * F8_BLOCK + lane / 16 * 32, 32);
+                x[j] = load32(static_cast<const uint8_t*>(p.a) + m * p.lda + (int64_t)b * F8_BLOCK, lane / 16);
                 s[j] = p.sa[m * p.sa_m + b * p.sa_b];
             }
         } else {
-            const int m = min(FORM == X_OWN ? lane % 16 : lane / 16, p.M - 1), k = FORM == X_OWN ? lane / 16 * 32 : lane % 16 * 8;
-            const T* at = static_cast<const T*>(p.a) + m * p.lda + (int64_t)b * F8_BLOCK + k;
+            const int m = min(FORM == X_OWN ? lane % 16 : lane / 16, p.M - 1);
+            const T* block = static_cast<const T*>(p.a) + m * p.lda + (int64_t)b * F8_BLOCK;
 #pragma unroll
-            for (int i = 0; i < VALUES / VEC; ++i) raw[i] = load_words<16, sizeof(T)>(at + i * VEC);
+            for (int i = 0; i < VALUES; i += VEC)
+                raw[i / VEC] = load_words<16, sizeof(T)>(block + (FORM == X_OWN ? half_at(lane / 16, i / 16) + i % 16 : lane % 16 * 8 + i));
         }
     }
 
-    // The same of a block of which `valid` values of this lane's 32 are there.
-    __device__ __forceinline__ void load_part(const GemmF8Args& p, int lane, int b, int valid) {
+    // The same of a last block that is not whole.
+    __device__ __forceinline__ void load_rest(const GemmF8Args& p, int lane, int b) {
 #pragma unroll
         for (int j = 0; j < MT; ++j) {
             const int m = min(16 * j + lane % 16, p.M - 1);
-            const int64_t at = m * p.lda + (int64_t)b * F8_BLOCK + lane / 16 * 32;
             if constexpr (FORM == X_F8) {
-                x[j] = load32(static_cast<const uint8_t*>(p.a) + at, valid);
+                x[j] = ::load_rest(static_cast<const uint8_t*>(p.a) + m * p.lda, b * F8_BLOCK, lane / 16, p.K);
                 s[j] = p.sa[m * p.sa_m + b * p.sa_b];
             } else {
                 float v[32];
 #pragma unroll
-                for (int i = 0; i < 32; ++i) v[i] = i < valid ? elem<DT>::to_f32(static_cast<const T*>(p.a)[at + i]) : 0.0f;
+                for (int i = 0; i < 32; ++i) {
+                    const int k = b * F8_BLOCK + half_at(lane / 16, i / 16) + i % 16;
+                    v[i] = elem<DT>::to_f32(static_cast<const T*>(p.a)[m * p.lda + min(k, p.K - 1)]);
+                    v[i] = k < p.K ? v[i] : 0.0f;
+                }
                 quantize(v);
             }
         }
@@ -113,8 +142,9 @@ struct XBlock {
             const int from = lane % 4 * 16;   // lanes of the row that this lane's operand holds; its copies past 4 rows are not stored
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                x[0][2 * i] = __shfl(lo, from + lane / 16 * 4 + i);
-                x[0][2 * i + 1] = __shfl(hi, from + lane / 16 * 4 + i);
+                const int lane_of = from + (half_at(lane / 16, i / 2) + 8 * (i % 2)) / 8;
+                x[0][2 * i] = __shfl(lo, lane_of);
+                x[0][2 * i + 1] = __shfl(hi, lane_of);
             }
             s[0] = __shfl(to.s, from);
         }
@@ -123,14 +153,14 @@ struct XBlock {
 
 // ADT: the type of A. MT, NT: blocks of 16 rows of A and of W; U: blocks of k on their way.
 template <int ADT, int FORM, int MT, int NT, int U, bool WIDE>
-__global__ __launch_bounds__(64 * FR_WAVES) void gemm_f8_rows_kernel(GemmF8Args p) {
+__global__ __launch_bounds__(64 * FR_WAVES, MT == 4 ? 4 : 1) void gemm_f8_rows_kernel(GemmF8Args p) {
     static_assert(F8_BLOCK % (16 * NT) == 0, "one scale of W a workgroup and block");
     static_assert(FORM == X_F8 || MT == 1, "16 rows of A in wider types");
     const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
     const int r = lane % 16, g = lane / 16, n0 = blockIdx.x * 16 * NT;
     const uint8_t* w[NT];
 #pragma unroll
-    for (int i = 0; i < NT; ++i) w[i] = p.b + (int64_t)min(n0 + 16 * i + r, p.N - 1) * p.ldb + 32 * g;   // rows past N compute what is not stored
+    for (int i = 0; i < NT; ++i) w[i] = p.b + (int64_t)min(n0 + 16 * i + r, p.N - 1) * p.ldb;   // rows past N compute what is not stored
     const float* sb = p.sb + (int64_t)(n0 / F8_BLOCK) * p.sb_n;
     f32x4 acc[NT][MT];
 #pragma unroll
@@ -161,7 +191,7 @@ __global__ __launch_bounds__(64 * FR_WAVES) void gemm_f8_rows_kernel(GemmF8Args 
             const int b = b0 + FR_WAVES * u;
             if (b >= full) continue;
 #pragma unroll
-            for (int i = 0; i < NT; ++i) on[u].w[i] = load32(w[i] + (int64_t)b * F8_BLOCK, 32);
+            for (int i = 0; i < NT; ++i) on[u].w[i] = load32(w[i] + (int64_t)b * F8_BLOCK, g);
             on[u].x.load(p, lane, b);
             on[u].s = sb[(int64_t)b * p.sb_b];
         }
@@ -174,10 +204,9 @@ __global__ __launch_bounds__(64 * FR_WAVES) void gemm_f8_rows_kernel(GemmF8Args 
     }
     if (full < p.blocks && wave == full % FR_WAVES) {
         Block k;
-        const int valid = p.K - full * F8_BLOCK - 32 * g;
 #pragma unroll
-        for (int i = 0; i < NT; ++i) k.w[i] = load32(w[i] + (int64_t)full * F8_BLOCK, valid);
-        k.x.load_part(p, lane, full, valid);
+        for (int i = 0; i < NT; ++i) k.w[i] = load_rest(w[i], full * F8_BLOCK, g, p.K);
+        k.x.load_rest(p, lane, full);
         k.s = sb[(int64_t)full * p.sb_b];
         add(k);
     }
@@ -223,7 +252,7 @@ void few_rows(const GemmF8Args& p, hipStream_t s) {
         else launch_rows<ADT, X_F8, 2, 1, 2, WIDE>(p, s);
     } else {
         if (p.N >= NT2) launch_rows<ADT, X_F8, 4, 2, 1, WIDE>(p, s);
-        else launch_rows<ADT, X_F8, 4, 1, 2, WIDE>(p, s);
+        else launch_rows<ADT, X_F8, 4, 1, 1, WIDE>(p, s);
     }
 }
 
