@@ -242,7 +242,7 @@ __global__ __launch_bounds__(DI_THREADS) void distill_bwd_kernel(DistillArgs p) 
     extern __shared__ float entry[];
     typedef typename elem<DT>::T T;
     constexpr int VEC = 16 / (int)sizeof(T), GROUP = 4;
-    for (int64_t work = blockIdx.x; work < p.rows * p.pieces; work += gridDim.x) {
+    for (int64_t work = p.rows * p.pieces - 1 - blockIdx.x; work >= 0; work -= gridDim.x) {   // the rows that forward read last come first
         const int64_t row = work / p.pieces, begin = work % p.pieces * p.piece, end = min(begin + p.piece, p.cols);
         const T* x = static_cast<const T*>(p.x) + row * p.sx;
         T* o = static_cast<T*>(p.dx) + row * p.sdx;
