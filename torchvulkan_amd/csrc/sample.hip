@@ -39,6 +39,7 @@ constexpr int SA_BINS = 2 * SA_THREADS;
 constexpr int SA_CHUNKS = 4;       // of 16 bytes, that a thread holds
 constexpr int SA_LIST = 256;       // values of a bin that are compared with each other
 constexpr int SA_FEW = 512;        // tokens that are
+constexpr int SA_SOME = 128;       // more of them than this are first spread over bins
 constexpr int SA_KEPT = 8192;      // tokens that are weighed from a list
 constexpr int SA_PIECES = 32;      // of a row, at most
 constexpr int64_t SA_MOST_COLS = 1 << 19;
@@ -110,12 +111,12 @@ struct Heat {
     __device__ __forceinline__ u64 whole_weight(float x) const { return whole(large_weight(x)); }
 };
 
-// Chunks [first, end) of 16 bytes of a row, thread t those at first + t + 1024 j, SA_CHUNKS of them in registers.
-template <int DT>
+// Chunks [first, end) of 16 bytes of a row, thread t those at first + t + 1024 j, C of them in registers.
+template <int DT, int C = SA_CHUNKS>
 struct RowIn {
     typedef typename elem<DT>::T T;
-    typedef uint32_t W __attribute__((ext_vector_type(4 * SA_CHUNKS)));
-    static constexpr int VEC = 16 / (int)sizeof(T), HELD = SA_CHUNKS * SA_THREADS;   // chunks that are held
+    typedef uint32_t W __attribute__((ext_vector_type(4 * C)));
+    static constexpr int VEC = 16 / (int)sizeof(T), HELD = C * SA_THREADS;   // chunks that are held
     static constexpr int N = 2, STEP = DT == TVK_F32 ? 2 : 1;                // values handled together, their words
     const T* row;
     int cols, first, end, at, words;   // at: the first of the held; words of a thread
@@ -128,17 +129,17 @@ struct RowIn {
     }
     __device__ __forceinline__ void load(int from) {
         at = from;
-        words = min(SA_CHUNKS, (end - from + SA_THREADS - 1) / SA_THREADS) * 4;
+        words = min(C, (end - from + SA_THREADS - 1) / SA_THREADS) * 4;
         const int whole = min(end, cols / VEC), mine = from + (int)threadIdx.x;   // past `whole` lies at most a piece of a chunk
         const T* p = row + (int64_t)mine * VEC;
-        Words<16> c[SA_CHUNKS];
+        Words<16> c[C];
 #pragma unroll
-        for (int j = 0; j < SA_CHUNKS; ++j) {
+        for (int j = 0; j < C; ++j) {
             c[j] = {};
             if (mine + j * SA_THREADS < whole) c[j] = load_words<16, sizeof(T)>(p + j * SA_THREADS * VEC);
         }
 #pragma unroll
-        for (int j = 0; j < 4 * SA_CHUNKS; ++j) w[j] = c[j / 4].w[j % 4];
+        for (int j = 0; j < 4 * C; ++j) w[j] = c[j / 4].w[j % 4];
         if (from + words / 4 * SA_THREADS <= whole) return;
         constexpr uint32_t LOWEST = DT == TVK_F32 ? 0xff800000u : DT == TVK_F16 ? 0xfc00fc00u : 0xff80ff80u;   // -inf
 #pragma unroll 1
@@ -161,7 +162,7 @@ struct RowIn {
     }
     // From here on the n tokens of a list instead (at most as many as are held), whose places are in LDS.
     __device__ __forceinline__ void take(const float* v, const int* v_places, int n) {
-        static_assert(SA_KEPT <= 4 * SA_CHUNKS / STEP * N * SA_THREADS, "a list is held");
+        static_assert(SA_KEPT <= 4 * C / STEP * N * SA_THREADS, "a list is held");
         first = at = 0;
         end = 1;
         words = (n + N * SA_THREADS - 1) / (N * SA_THREADS) * STEP;
@@ -230,6 +231,18 @@ __device__ __forceinline__ V lanes16(V v) {
     return Op::of(v, from_lane<0x140>(v, v));   // mirrored in 16
 }
 
+// What is the same in every lane, in a scalar register: vector registers are what the kernels run out of.
+template <class V>
+__device__ __forceinline__ V of_all(V v) {
+    if constexpr (sizeof(V) == 8) {
+        const u64 u = __builtin_bit_cast(u64, v);
+        return __builtin_bit_cast(V, (u64)(uint32_t)__builtin_amdgcn_readfirstlane((int)(u >> 32)) << 32 |
+                                         (uint32_t)__builtin_amdgcn_readfirstlane((int)u));
+    } else {
+        return __builtin_bit_cast(V, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, v)));
+    }
+}
+
 // Over the workgroup, the same bits in every thread: waves first, then the waves' results.
 template <class Op, class V>
 __device__ __forceinline__ V all_threads(V v) {
@@ -245,13 +258,14 @@ __device__ __forceinline__ V all_threads(V v) {
 }
 
 // Sum of the lanes up to this one.
-__device__ __forceinline__ u64 lanes_up_to(u64 v) {
-    v += from_lane<0x111>(v, (u64)0);         // from the lane before, and 2, 4, 8 before, in groups of 16
-    v += from_lane<0x112>(v, (u64)0);
-    v += from_lane<0x114>(v, (u64)0);
-    v += from_lane<0x118>(v, (u64)0);
-    v += from_lane<0x142, 0xa>(v, (u64)0);    // the first group's last to the second, the third's to the fourth
-    v += from_lane<0x143, 0xc>(v, (u64)0);    // the first half's last to the second half
+template <class V>
+__device__ __forceinline__ V lanes_up_to(V v) {
+    v += from_lane<0x111>(v, (V)0);         // from the lane before, and 2, 4, 8 before, in groups of 16
+    v += from_lane<0x112>(v, (V)0);
+    v += from_lane<0x114>(v, (V)0);
+    v += from_lane<0x118>(v, (V)0);
+    v += from_lane<0x142, 0xa>(v, (V)0);    // the first group's last to the second, the third's to the fourth
+    v += from_lane<0x143, 0xc>(v, (V)0);    // the first half's last to the second half
     return v;
 }
 
@@ -263,9 +277,9 @@ union Bins {
 
 struct Shared {
     Bins all, part;
-    double table[SA_STEPS];
     float list[SA_KEPT];
     int list_at[SA_KEPT], kept_at[SA_KEPT];
+    double table[SA_STEPS];
     u64 list_w[SA_FEW], before[SA_FEW];
     unsigned rank[SA_FEW];
     u64 sums[SA_WAVES];
@@ -317,6 +331,11 @@ struct Range {
     __device__ __forceinline__ int bin(float x) const {
         const F b = ((F)hi - (F)x) * scale;
         return (int)(b < (F)(SA_BINS - 1) ? b : (F)(SA_BINS - 1));   // infinities and NaN: the last
+    }
+    // the bin within a bin
+    __device__ __forceinline__ int part(float x, int bin) const {
+        const double b = ((double)((F)hi - (F)x) * (double)scale - bin) * SA_BINS;
+        return b > 0.0 ? (int)fmin(b, (double)(SA_BINS - 1)) : 0;
     }
 };
 
@@ -377,8 +396,8 @@ __device__ __forceinline__ u64 sum_of(const Bins& b, Shared& s) {
     return all_threads<AddOp>(b.w[threadIdx.x] + b.w[threadIdx.x + SA_THREADS]);
 }
 
-template <int DT, class F>
-__device__ __forceinline__ void fill_bins(RowIn<DT>& x, const Heat& h, const Range<F>& r, bool counts, Bins& b) {
+template <int DT, int C, class F>
+__device__ __forceinline__ void fill_bins(RowIn<DT, C>& x, const Heat& h, const Range<F>& r, bool counts, Bins& b) {
     constexpr int N = RowIn<DT>::N;
     clear(b);
     if (counts)
@@ -431,8 +450,8 @@ struct InBin {
     float lo, hi;
 };
 
-template <int DT>
-__device__ __forceinline__ InBin border_in_bin(RowIn<DT>& x, const Heat& h, const Range<double>& r, int bin, bool counts, u64 need, u64 above,
+template <int DT, int C>
+__device__ __forceinline__ InBin border_in_bin(RowIn<DT, C>& x, const Heat& h, const Range<double>& r, int bin, bool counts, u64 need, u64 above,
                                                Shared& s) {
     constexpr int N = RowIn<DT>::N;
     __syncthreads();
@@ -483,8 +502,8 @@ struct Places {
 };
 
 // The index of the last of the first b.ties tokens that equal the border.
-template <int DT>
-__device__ __forceinline__ int last_tie(RowIn<DT>& x, const Border& b, Shared& s) {
+template <int DT, int C>
+__device__ __forceinline__ int last_tie(RowIn<DT, C>& x, const Border& b, Shared& s) {
     typedef Places<DT> At;
     constexpr int N = RowIn<DT>::N;
     if (b.ties == b.equal) return 0x7fffffff;
@@ -513,8 +532,8 @@ struct Keep {
 };
 
 // The tokens that `has` names, with their places: s.listed of them, at most MOST kept.
-template <int MOST, int DT, class F>
-__device__ __forceinline__ void list_tokens(RowIn<DT>& x, float* v_out, int* at_out, Shared& s, F&& has) {
+template <int MOST, int DT, int C, class F>
+__device__ __forceinline__ void list_tokens(RowIn<DT, C>& x, float* v_out, int* at_out, Shared& s, F&& has) {
     constexpr int N = RowIn<DT>::N;
     __syncthreads();
     if (threadIdx.x == 0) s.listed = 0;
@@ -533,9 +552,40 @@ __device__ __forceinline__ void list_tokens(RowIn<DT>& x, float* v_out, int* at_
     __syncthreads();
 }
 
+// The same, none kept where they are more, in two passes: `count` (which may do more) first, so that a wave asks for its
+// share of the list once and not for each word. Many tokens of a piece are faster listed so, 64 x 128000 with flat
+// distributions 60 us and 66; rows that one workgroup takes, with what they do besides, are not: 256 x 128000 148 and 134.
+template <int MOST, int DT, int C, class G, class F>
+__device__ __forceinline__ void list_counted(RowIn<DT, C>& x, float* v_out, int* at_out, Shared& s, G&& count, F&& has) {
+    constexpr int N = RowIn<DT>::N;
+    __syncthreads();
+    if (threadIdx.x == 0) s.listed = 0;
+    __syncthreads();
+    unsigned n = 0;
+    x.each([&](const int (&i)[N], const float (&v)[N]) {
+#pragma unroll
+        for (int k = 0; k < N; ++k) n += count(i[k], v[k]);
+    });
+    const unsigned up_to = lanes_up_to(n);
+    unsigned o = 0;
+    if (threadIdx.x % 64 == 63) o = atomicAdd(&s.listed, up_to);
+    o = (unsigned)__builtin_amdgcn_readlane((int)o, 63) + up_to - n;
+    __syncthreads();
+    if (s.listed <= MOST && __any(n))
+        x.each([&](const int (&i)[N], const float (&v)[N]) {
+#pragma unroll
+            for (int k = 0; k < N; ++k)
+                if (has(i[k], v[k])) {
+                    v_out[o] = v[k];
+                    at_out[o++] = i[k];
+                }
+        });
+    __syncthreads();
+}
+
 // The weights of the tokens that `has` keeps, in the places' bins: a wave's step is a bin, and nobody else's.
-template <int DT, class F>
-__device__ __forceinline__ void add_all_places(RowIn<DT>& x, const Heat& h, const Filters& f, u64* places, F&& has) {
+template <int DT, int C, class F>
+__device__ __forceinline__ void add_all_places(RowIn<DT, C>& x, const Heat& h, const Filters& f, u64* places, F&& has) {
     constexpr int N = RowIn<DT>::N, VEC = RowIn<DT>::VEC;
     u64 sum = 0;   // of a chunk, then of a wave's
     x.each([&](const int (&i)[N], const float (&v)[N]) {
@@ -557,9 +607,10 @@ __device__ __forceinline__ void add_all_places(RowIn<DT>& x, const Heat& h, cons
     });
 }
 
-// The same where few may be kept: those are listed first, and weighed by as many threads. s.part is used.
-template <int DT, class F>
-__device__ __forceinline__ void add_listed_places(RowIn<DT>& x, const Heat& h, const Filters& f, u64* places, Shared& s, F&& has) {
+// The same where some may be left out: those that are kept were listed (s.list), where the list holds them, and are weighed
+// by as many threads. s.part is used.
+template <int DT, int C, class F>
+__device__ __forceinline__ void add_listed_places(RowIn<DT, C>& x, const Heat& h, const Filters& f, u64* places, Shared& s, F&& has) {
     const unsigned n = s.listed;
     if (n > SA_KEPT) return add_all_places(x, h, f, places, has);   // (not of a list)
     clear(s.part);
@@ -573,8 +624,8 @@ __device__ __forceinline__ void add_listed_places(RowIn<DT>& x, const Heat& h, c
     for (int i = from + (int)threadIdx.x; i < to; i += SA_THREADS) places[i] = s.part.w[i];
 }
 
-template <int DT, class F>
-__device__ __forceinline__ void add_places(RowIn<DT>& x, const Heat& h, const Filters& f, u64* places, Shared& s, F&& has) {
+template <int DT, int C, class F>
+__device__ __forceinline__ void add_places(RowIn<DT, C>& x, const Heat& h, const Filters& f, u64* places, Shared& s, F&& has) {
     list_tokens<SA_KEPT>(x, s.list, s.list_at, s, has);
     add_listed_places(x, h, f, places, s, has);
 }
@@ -617,8 +668,8 @@ __device__ inline void put_first(const SampleArgs& p, int64_t row, float top, un
 }
 
 // The first place of the largest among a thread's values.
-template <int DT>
-__device__ __forceinline__ unsigned first_of(RowIn<DT>& x, float top) {
+template <int DT, int C>
+__device__ __forceinline__ unsigned first_of(RowIn<DT, C>& x, float top) {
     constexpr int N = RowIn<DT>::N;
     unsigned at = 0x7fffffff;
     x.each([&](const int (&i)[N], const float (&v)[N]) {
@@ -654,8 +705,8 @@ __device__ __forceinline__ void finish_few(const SampleArgs& p, int64_t row, int
 }
 
 // A row by one workgroup, with its largest logit known.
-template <int DT>
-__device__ __forceinline__ void whole_row(const SampleArgs& p, int64_t row, RowIn<DT>& x, float top, const Filters& f, Shared& s) {
+template <int DT, int C>
+__device__ __forceinline__ void whole_row(const SampleArgs& p, int64_t row, RowIn<DT, C>& x, float top, const Filters& f, Shared& s) {
     if (f.first_only(top)) {
         put_first(p, row, top, all_threads<LeastOp>(first_of(x, top)));
         return;
@@ -710,8 +761,8 @@ __device__ __forceinline__ void whole_row(const SampleArgs& p, int64_t row, RowI
     draw<DT>(p, row, x.row, h, f, k, s);
 }
 
-template <int DT>
-__device__ __forceinline__ float largest(RowIn<DT>& x, Shared& s) {
+template <int DT, int C>
+__device__ __forceinline__ float largest(RowIn<DT, C>& x, Shared& s) {
     constexpr int N = RowIn<DT>::N;
     float top = -INFINITY;
     x.each([&](const int (&)[N], const float (&v)[N]) {
@@ -748,7 +799,7 @@ __global__ __launch_bounds__(SA_THREADS) void sample_top_kernel(SampleArgs p) {
 
 __device__ __forceinline__ float top_of(const SampleArgs& p, int64_t row) {
     const int lane = threadIdx.x % 64;
-    return lanes64_all<MaxOp>(lane < p.pieces ? p.tops[row * p.pieces + lane] : -INFINITY);
+    return of_all(lanes64_all<MaxOp>(lane < p.pieces ? p.tops[row * p.pieces + lane] : -INFINITY));
 }
 
 // A piece's histogram; or where no border is wanted what the token is found from.
@@ -839,8 +890,9 @@ __global__ __launch_bounds__(SA_THREADS) void sample_border_kernel(SampleArgs p)
         });
         __syncthreads();
     } else {
-        list_tokens<SA_KEPT>(x, s.list, s.list_at, s, above_it);
-        add_listed_places(x, h, f, places, s, [&](int, float v) { return r.has(v) && r.bin(v) < bin; });
+        auto has = [&](int, float v) { return r.has(v) && r.bin(v) < bin; };
+        list_counted<SA_KEPT>(x, s.list, s.list_at, s, above_it, has);
+        add_listed_places(x, h, f, places, s, has);
     }
     if (threadIdx.x == 0) p.listed[blockIdx.x] = s.found_n;
     state(few ? SA_TOKENS : SA_SUMS, bin, above, need);
@@ -859,33 +911,65 @@ __global__ __launch_bounds__(SA_THREADS) void sample_token_kernel(SampleArgs p) 
     if (st.mode == SA_FIRST) return put_first(p, row, top, all_threads<LeastOp>(listed));
     const Heat h = f.weights(top, s);
     const typename elem<DT>::T* x = static_cast<const typename elem<DT>::T*>(p.x) + row * p.stride;
-    int n = 0;
+    int n = 0, base = 0;   // entries, and where they lie in s.list
     bool whole = st.mode == SA_WHOLE;
     if (st.mode == SA_TOKENS || st.mode == SA_SUMS) {   // the pieces' lists, one behind the other: a thread an entry
-        const u64 up_to = lanes_up_to(listed);
+        const unsigned up_to = lanes_up_to(listed);
         n = (int)__builtin_amdgcn_readlane((int)up_to, 63);   // (at most 2^19)
-        if (threadIdx.x < SA_PIECES) s.counts[threadIdx.x] = (unsigned)up_to;
+        if (threadIdx.x < SA_PIECES) s.counts[threadIdx.x] = up_to;
         __syncthreads();
-        whole = n > SA_FEW;
-        if (!whole && (int)threadIdx.x < n) {
-            int i = 0;   // the first piece whose entries reach past this thread's
-            for (int half = SA_PIECES / 2; half > 0; half /= 2)
-                if (s.counts[i + half - 1] <= threadIdx.x) i += half;
-            const int64_t from = (row * p.pieces + i) * SA_FEW + threadIdx.x - (i ? s.counts[i - 1] : 0);
-            s.list[threadIdx.x] = p.list_v[from];
-            s.list_at[threadIdx.x] = p.list_at[from];
+        whole = n > (st.mode == SA_TOKENS ? SA_FEW : SA_KEPT / 2) || (lane < p.pieces && listed > SA_FEW);
+        whole = __any(whole);
+        base = st.mode == SA_SUMS && n > SA_SOME ? SA_KEPT / 2 : 0;
+        if (!whole)
+            for (int t = threadIdx.x; t < n; t += SA_THREADS) {
+                int i = 0;   // the first piece whose entries reach past this one
+                for (int half = SA_PIECES / 2; half > 0; half /= 2)
+                    if (s.counts[i + half - 1] <= t) i += half;
+                const int64_t from = (row * p.pieces + i) * SA_FEW + t - (i ? s.counts[i - 1] : 0);
+                s.list[base + t] = p.list_v[from];
+                s.list_at[base + t] = p.list_at[from];
+            }
+        __syncthreads();
+    }
+    clear(s.all);
+    const int places = (p.cols >> Places<DT>::SHIFT) + 1;
+    if (st.mode == SA_ALL || st.mode == SA_SUMS)
+        for (int i = threadIdx.x; i < places && i < SA_BINS; i += SA_THREADS)
+            if (i << Places<DT>::SHIFT < p.cols) s.all.w[i] = p.places[row * SA_BINS + i];
+    u64 before_list = st.above;
+    if (base && !whole) {   // of many, those are weighed that lie above the border's bin within the bin
+        const Range<float> r = first_range<float>(top, f.heat);
+        clear(s.part);
+        for (int t = threadIdx.x; t < n; t += SA_THREADS)
+            atomicAdd(&s.part.w[r.part(s.list[base + t], st.bin)], f.by_k ? (u64)1 : h.whole_weight(s.list[base + t]));
+        __syncthreads();
+        find_bin(true, false, st.need - st.above, s);
+        const int part = s.found;
+        before_list += s.found_w;
+        if (threadIdx.x == 0) s.listed = 0;
+        __syncthreads();
+        for (int t = threadIdx.x; t < n; t += SA_THREADS) {
+            const float v = s.list[base + t];
+            const int at = s.list_at[base + t], bin = r.part(v, st.bin);
+            if (bin < part) {
+                const u64 w = f.weigh(h, v);
+                if (w) atomicAdd(&s.all.w[at >> Places<DT>::SHIFT], w);
+            } else if (bin == part) {
+                const unsigned o = atomicAdd(&s.listed, 1u);
+                if (o < SA_FEW) s.list[o] = v, s.list_at[o] = at;
+            }
         }
+        __syncthreads();
+        n = (int)s.listed;
+        whole = n > SA_FEW;
         __syncthreads();
     }
     if (whole) {   // too many of them: from the start
-        RowIn<DT> all(p, row, 0, 0x7fffffff);
+        RowIn<DT, SA_CHUNKS / 2> all(p, row, 0, 0x7fffffff);   // (the others' registers are in use here)
         return whole_row(p, row, all, top, f, s);
     }
     if (st.mode == SA_TOKENS) return finish_few(p, row, n, h, f, s);
-    clear(s.all);
-    const int places = (p.cols >> Places<DT>::SHIFT) + 1;
-    for (int i = threadIdx.x; i < places && i < SA_BINS; i += SA_THREADS)
-        if (i << Places<DT>::SHIFT < p.cols) s.all.w[i] = p.places[row * SA_BINS + i];
     Keep k{-INFINITY, 0x7fffffff};
     if (st.mode == SA_SUMS) {   // the bin's tokens, compared with each other
         const int t = threadIdx.x;
@@ -895,7 +979,7 @@ __global__ __launch_bounds__(SA_THREADS) void sample_token_kernel(SampleArgs p) 
         const u64 each = there ? f.by_k ? 1 : h.whole_weight(v) : 0;
         if (there) s.list_w[t] = each;
         compare_all(n, s, in_front);
-        const u64 before = there ? st.above + s.before[t] : 0;
+        const u64 before = there ? before_list + s.before[t] : 0;
         if (there && before < st.need) {
             const u64 w = f.weigh(h, v);
             if (w) atomicAdd(&s.all.w[at >> Places<DT>::SHIFT], w);
