@@ -146,6 +146,19 @@ def test_unlike_scales(gpu):
             check(x, u, f"{heat} {kw}", temperature=[heat] * 8, **kw)
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,cols", [(2, 128000), (12, 70001)])
+def test_borders_among_many(gpu, dtype, rows, cols):
+    """Flat distributions: the border lies among hundreds or thousands of tokens of nearly one weight, much is above it."""
+    for std in (0.01, 0.2, 1.0, 3.0):
+        x, u = rand(rows, cols, dtype, 11, std)
+        heat = torch.linspace(0.6, 2.5, rows)
+        for p in (0.05, 0.5, 0.95):
+            check(x, u, f"{std} {p}", top_p=[p] * rows, temperature=heat)
+        check(x, u, f"{std} top_k", top_k=[cols // 3] * rows, temperature=heat)
+        check(x, u, f"{std} min_p", top_p=[0.9] * rows, min_p=[0.2] * rows)
+
+
 def test_masks_and_not_numbers(gpu):
     x, u = rand(9, 2000, torch.float32, 6)
     x[0] = -math.inf                       # nothing
