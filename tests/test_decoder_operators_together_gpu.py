@@ -1,0 +1,110 @@
+"""Layer norms in 8 bits, products of 8-bit blocks, the loss against a teacher and the drawing of tokens, one behind the
+other as examples/decode.py uses them.
+
+The run of a block against 64 bits: each 8-bit rounding is off by at most half a step, 2^-4 of the value (of the block's
+largest / 448 times 2^-10 for the smallest). As a vector of many values whose errors are unlike, what is left of two
+operands is below sqrt(2) 2^-4 = 0.089 of the product, of two products in a row below 0.13; the bfloat16 roundings between
+them add 2^-8 each. Both bounds are of the relative distance of whole tensors."""
+from __future__ import annotations
+
+import importlib.util
+from pathlib import Path
+
+import pytest
+import torch
+
+from torchvulkan_amd import decoder
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def example():
+    spec = importlib.util.spec_from_file_location("decode_example", Path(__file__).resolve().parent.parent / "examples" / "decode.py")
+    module = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(module)
+    return module
+
+
+def apart(a, b):
+    a, b = a.double().cpu(), b.double().cpu()
+    return float((a - b).norm() / b.norm())
+
+
+@pytest.mark.parametrize("rows", [1, 3, 17, 200])
+def test_norm_product_norm_product(gpu, rows):
+    gen = torch.Generator().manual_seed(rows)
+    x, r = (torch.randn((rows, 520), generator=gen).bfloat16() for _ in range(2))
+    w, b = torch.rand(520, generator=gen) + 0.5, torch.randn(520, generator=gen) / 4
+    up, down = torch.randn((1032, 520), generator=gen).bfloat16() / 16, torch.randn((520, 1032), generator=gen).bfloat16() / 16
+    dev = [t.cuda() for t in (x, r, w, b, up, down)]
+    eights = [decoder.quantize_fp8(t, 128) for t in dev[4:]]
+
+    def block(x, r, w, b):
+        y, scale, h = decoder.layer_norm_fp8(x, w, b, r)
+        u = decoder.linear_fp8(y, *eights[0], x_scale=scale)
+        return u, decoder.linear_fp8(u.relu(), *eights[1]), h
+
+    u, out, h = block(*dev[:4])
+    hd = x.double() + r.double()
+    y = torch.nn.functional.layer_norm(hd, (520,), w.double(), b.double(), 1e-5)
+    ud = y @ up.double().t()
+    assert apart(h, hd) < 2.0 ** -8
+    assert apart(u, ud) < 0.09 + 2.0 ** -8
+    assert apart(out, ud.relu() @ down.double().t()) < 0.13 + 2.0 ** -6
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        again = block(*dev[:4])
+    for _ in range(3):
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(p, q) for p, q in zip(again, (u, out, h)))
+        eager = block(*dev[:4])
+        assert all(torch.equal(p, q) for p, q in zip(eager, (u, out, h)))
+
+
+@pytest.mark.parametrize("draw", [None, dict(temperature=0.9, top_k=40, top_p=0.9), dict(temperature=1.3, min_p=0.02)])
+def test_captured_tokens_are_the_eager_ones(gpu, example, draw):
+    model = example.Decoder(layers=2, dim=256, heads=4, heads_kv=2, hidden=520, vocab=500, block=example.Block8)
+    prompts = torch.randint(0, 500, (3, 70), generator=torch.Generator().manual_seed(0)).cuda()
+    captured = example.generate(model, prompts, 12, draw=draw, seed=3)[0]
+    assert captured.shape == (3, 12) and captured.min() >= 0 and captured.max() < 500
+    numbers = torch.rand((12, 3), generator=torch.Generator().manual_seed(3)).cuda()
+    cache = model.cache(3, 82)
+    cache.extend(70)
+    token, eager = prompts, []
+    for step in range(12):
+        if step:
+            cache.extend(1)
+        logits = model(token, cache, max_len=82 if step else None)
+        token = logits.argmax(-1, keepdim=True) if draw is None else decoder.sample(logits, numbers[step], **draw)[0][:, None]
+        eager.append(token)
+    assert torch.equal(captured, torch.cat(eager, 1))
+
+
+def test_gradients_of_a_step(gpu, example):
+    """Against autograd in 64 bits. What bfloat16 leaves: the norm's rounding, 2^-8 of a value at most, is 2^-8 sum |y w| / T <=
+    2^-8 * 11 / 2 = 0.021 in an exponent, the logits' 2^-8 * 5 / 2 = 0.01; so p is off by at most 0.032 of itself, p being
+    the smaller part of p - q; that is rounded once, 2^-8, and so are the product's gradient and the norm's incoming one."""
+    rows, dim, vocab, top = 300, 256, 1000, 16
+    gen = torch.Generator().manual_seed(1)
+    x = torch.randn((rows, dim), generator=gen).bfloat16()
+    index = torch.stack([torch.randperm(vocab, generator=gen)[:top] for _ in range(rows)])
+    teacher = torch.randn((rows, top), generator=gen) * 2
+    head = example.Head(dim, vocab)
+    leaves = [t.detach().cpu().double().requires_grad_() for t in (head.product, head.weight, head.bias)]
+    logits = torch.nn.functional.layer_norm(x.double(), (dim,), leaves[1], leaves[2], 1e-5) @ leaves[0].t()
+    q = torch.softmax(teacher.double() / 2, -1)
+    lp = torch.log_softmax(logits / 2, -1).gather(1, index)
+    loss = ((q * (q.log() - lp)).sum(-1) * 4).mean()
+    loss.backward()
+    got, grads = head.step(x.to("vulkan"), index.to("vulkan"), teacher.to("vulkan"))
+    assert abs(got - float(loss.detach())) < 0.032 * 4
+    for g, leaf in zip(grads, leaves):
+        assert apart(g, leaf.grad) < 0.032 + 3 * 2.0 ** -8
+    assert not torch.equal(head.bias.detach().cpu(), torch.zeros(dim))
+
+
+def test_the_example_s_steps_run(gpu, example):
+    losses = example.distill_steps(300, 128, 500, 16, 2)
+    assert len(losses) == 2 and all(x == x and x > 0 for x in losses)
