@@ -19,9 +19,10 @@
  *     positive value; element offsets must fit in int64.
  *   - scratch memory: tvk_gemm, tvk_conv2d_*, tvk_conv_*, tvk_reduce_sum,
  *     tvk_attention_bwd, tvk_rms_norm_bwd, tvk_layer_norm_bwd, tvk_distill_fwd,
- *     tvk_gemm_f8 and tvk_paged_attention lease library
+ *     tvk_gemm_f8, tvk_sample and tvk_paged_attention lease library
  *     scratch (split-K partials, repacked operands, convolution partials, the
- *     attention delta, partial sums of rows and of split keys) from a per-device
+ *     attention delta, partial sums of rows and of split keys, histograms of
+ *     rows cut among workgroups) from a per-device
  *     pool for the kernels they queue on their `stream`. A buffer is leased
  *     again only for the stream its first lease named (on hipStreamPerThread
  *     for that thread's), so stream order puts each call's kernels after the
@@ -590,9 +591,11 @@ tvk_status tvk_quantize_f8(const tvk_quantize_f8_desc* desc);
  * into 8 bits as by tvk_quantize_f8 with block_rows 1, with the same bits, and
  * a_scale is not read. bias (NULL: none) has out_dtype or F32. Rows are
  * contiguous, `*_stride` elements apart, scales at any strides (0: one for all;
- * for more than 64 rows of a at most 2^20 from row to row); any alignment: rows that 16-byte loads do not meet are copied to library
- * scratch for more than 64 rows of a, and 16- and 32-bit a's 8 bits go there for
- * more than 16. The sums run in an order that depends on the sizes alone: the
+ * for more than 64 rows of a at most 2^20 from row to row); any alignment: for
+ * more than 64 rows of a, rows that 16-byte loads do not meet are copied to
+ * library scratch, where the 8 bits of more than 16 rows of a 16- or 32-bit a go
+ * too, and the sums of a K that is split. The sums run in an order that depends on
+ * the sizes, and for 17 to 64 rows on whether 16-byte loads meet the rows: the
  * same bits every run. out must not lie over an input. K up to 2^22, or with up to
  * 64 rows 2^31 - 65536. */
 typedef struct {
@@ -687,7 +690,8 @@ tvk_status tvk_distill_bwd(const tvk_distill_bwd_desc* desc);
  * temperature, top_k, top_p, min_p: a value for each row, on the device (NULL: 1,
  * and no filter), so that a captured call follows them. dtype F32, F16 or BF16;
  * rows are contiguous, logits_stride elements apart (0: one for all), of any
- * alignment and at most 2^19 values. The same bits every run. */
+ * alignment and at most 2^19 values. The same bits every run. Few rows use library
+ * scratch. */
 typedef struct {
     int32_t dtype, reserved;
     int64_t rows, cols;

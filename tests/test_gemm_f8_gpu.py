@@ -136,6 +136,34 @@ def test_types_and_bias(gpu, dtype, m):
     check(a, sa, b, sb, rand((333,), 6).to(dtype), dtype, "bias")
 
 
+@pytest.mark.parametrize("m", [1, 4, 5, 16, 32, 64])
+@pytest.mark.parametrize("n,k", [(40, 5), (40, 15), (40, 17), (40, 31), (40, 143), (6145, 300), (12300, 700)])
+def test_few_rows(gpu, m, n, k):
+    """Ends of rows at every part of 16 bytes, and columns enough for several blocks of W a workgroup; wider rows give the
+    bits of their 8-bit form."""
+    for out_dtype in (torch.float32, torch.bfloat16):
+        check(*operands(m, n, k, m + k), out_dtype=out_dtype, what=f"{m} {n} {k}")
+    _, _, b, sb = operands(1, n, k, k)
+    for dtype in DTYPES:
+        a = (rand((m, k), k) * 3).to(dtype).to(DEV)
+        q, sa = _abi.quantize_f8(a)
+        want = _abi.gemm_f8(q, sa, b.to(DEV), sb.to(DEV), out_dtype=dtype)
+        assert torch.equal(_abi.gemm_f8(a, None, b.to(DEV), sb.to(DEV)), want)
+
+
+@pytest.mark.parametrize("m,n,k", [(17, 12290, 4096), (32, 4100, 12288), (33, 2100, 4096), (64, 4096, 2064)])
+def test_few_rows_of_large_weights(gpu, m, n, k):
+    a, sa, b, sb = operands(m, n, k, m)
+    for out_dtype in (torch.float32, torch.float16):
+        check(a, sa, b, sb, out_dtype=out_dtype, what="aligned")
+    wide = torch.zeros((n, k + 16), dtype=torch.uint8, device=DEV).view(F8)   # rows that 16-byte loads do not meet
+    wide[:, 3:k + 3] = b.to(DEV)
+    check(a, sa, b, sb, out_dtype=torch.float16, what="unaligned", dev=[a.to(DEV), sa.to(DEV), wide[:, 3:k + 3], sb.to(DEV)])
+    x = (a.float() * 3).bfloat16().to(DEV)
+    q, sx = _abi.quantize_f8(x)
+    assert torch.equal(_abi.gemm_f8(x, None, b.to(DEV), sb.to(DEV)), _abi.gemm_f8(q, sx, b.to(DEV), sb.to(DEV)))
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("m,n,k", [(1, 100, 300), (7, 33, 4100), (16, 512, 128), (17, 130, 700), (64, 64, 1), (70, 200, 333), (300, 300, 512)])
 def test_rows_in_more_bits(gpu, dtype, m, n, k):

@@ -5,11 +5,19 @@
 // lane beside 32 cycles of the matrix unit.
 //
 // Up to 64 rows are bound by the bytes of W (this file): a workgroup takes 16 rows
-// of W, its waves the blocks in turn, W and the rows of A straight from memory into
-// the instruction's operands, several blocks on their way at once; the waves' sums
-// meet in LDS. Up to 16 rows of A in 16 or 32 bits are brought into 8 bits on the
-// way, by each workgroup for itself; more rows in a launch of their own. More than
-// 64 rows run gemm_f8_ring.hip.
+// of W, or up to 64, its waves the blocks in turn, W and the rows of A straight from
+// memory into the instruction's operands, several blocks on their way at once; the
+// waves' sums meet in LDS. Up to 16 rows of A in 16 or 32 bits are brought into 8
+// bits on the way, by each workgroup for itself; more rows in a launch of their
+// own. More than 64 rows, and from 17 on those of large weights, run
+// gemm_f8_ring.hip.
+//
+// Measured, W read from memory at 5.2 TB/s if nothing else took time: 1 x 14336 x
+// 4096 13.7 us in 8 bits and 15.9 from bfloat16 (11.3 for W's bytes, 3 for a launch);
+// 16 x 14336 x 4096 16.1 and 17.3; 1 x 8192 x 8192 13.9 and 17.6; 50 x 5000 x 4100,
+// no row on 16 bytes, 24 from float16 with the launch that brings it into 8 bits.
+// Loads on their way over the end of a loop's turn, with a next set of registers,
+// were slower, 16.9 us for 15.1: a wave has four blocks of 4096 values in all.
 #include "gemm_f8.h"
 
 using namespace tvk;
@@ -17,7 +25,11 @@ using namespace tvk;
 namespace {
 
 constexpr int FR_WAVES = 8;
-constexpr int NT4 = 12288, NT2 = 6144;   // columns
+// From so many columns on a workgroup takes 4 and 2 blocks of 16 rows of W, so that 5 rows of A and more are read, and brought
+// into 8 bits, less often; workgroups for all CUs are left. 16 rows from bfloat16 by 14336 x 4096, 1, 2 and 4 blocks: 34.1, 23.6
+// and 17.3 us; by 8192 x 4096 18.4, 12.1 and 15.3; by 4096 x 4096 10.3, 11.7 and 14.7. One row: 15.6, 15.0 and 15.9; 9.4, 9.9
+// and 10.8; 1 x 8192 x 8192 17.6, 21.9 and 19.7.
+constexpr int NT4 = 12288, NT2 = 6144;
 
 // A lane's 32 values of a block of k, of A and of W alike, whose order does not matter to the sum: 16 of the first
 // half and 16 of the second, so that the four lanes of a row load 64 bytes side by side.
@@ -60,8 +72,8 @@ __device__ __forceinline__ i32x8 load_rest(const uint8_t* row, int at, int g, in
 }
 
 // How a wave has its rows of A: in 8 bits with scales; in wider types, 32 values a lane, each lane those of its
-// operand; the same for up to 4 rows, 8 values a lane, handed round afterwards (a quarter of the arithmetic, which is
-// what bounds one row of them: 1 x 4096 x 14336 from bf16 TBD).
+// operand; the same for up to 4 rows, 8 values a lane, handed round afterwards (a quarter of the arithmetic, which
+// bounds few columns of a long k: 1 x 4096 x 14336 from bfloat16 15.8 us, each lane its own 24.4).
 enum { X_F8, X_OWN, X_SHARED };
 
 // What a lane loads of one block of A, and the operands that become of it.
@@ -153,7 +165,7 @@ struct XBlock {
 
 // ADT: the type of A. MT, NT: blocks of 16 rows of A and of W; U: blocks of k on their way.
 template <int ADT, int FORM, int MT, int NT, int U, bool WIDE>
-__global__ __launch_bounds__(64 * FR_WAVES, MT == 4 ? 4 : 1) void gemm_f8_rows_kernel(GemmF8Args p) {
+__global__ __launch_bounds__(64 * FR_WAVES, MT == 4 && NT == 1 ? 4 : 1) void gemm_f8_rows_kernel(GemmF8Args p) {
     static_assert(F8_BLOCK % (16 * NT) == 0, "one scale of W a workgroup and block");
     static_assert(FORM == X_F8 || MT == 1, "16 rows of A in wider types");
     const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
@@ -242,11 +254,17 @@ void rows_16(const GemmF8Args& p, hipStream_t s) {
 
 template <int ADT, bool WIDE>
 void few_rows(const GemmF8Args& p, hipStream_t s) {
-    if constexpr (ADT != TVK_F8E4M3FN) {
-        if (p.M <= 4) rows_16<ADT, X_SHARED, WIDE>(p, s);
-        else rows_16<ADT, X_OWN, WIDE>(p, s);
+    constexpr bool IN8 = ADT == TVK_F8E4M3FN;
+    if (p.M <= 4) {
+        // from wider types 4 blocks of W a workgroup where those make one round on the CUs: 1 x 14336 x 4096 11.4 us, W in
+        // the memory's cache, and 15.9, it isn't, where one block takes 14.4 and 15.6; 1 x 28672 x 4096, two rounds, 29.8 and 25.8
+        const int groups = (p.N + 63) / 64;
+        if (!IN8 && groups > 192 && groups <= 256) launch_rows<ADT, IN8 ? X_F8 : X_SHARED, 1, IN8 ? 1 : 4, IN8 ? 4 : 2, WIDE>(p, s);
+        else launch_rows<ADT, IN8 ? X_F8 : X_SHARED, 1, 1, 4, WIDE>(p, s);
     } else if (p.M <= 16) {
-        rows_16<ADT, X_F8, WIDE>(p, s);
+        rows_16<ADT, IN8 ? X_F8 : X_OWN, WIDE>(p, s);
+    } else if constexpr (!IN8) {
+        return;   // (8 bits by now)
     } else if (p.M <= 32) {
         if (p.N >= NT2) launch_rows<ADT, X_F8, 2, 2, 2, WIDE>(p, s);
         else launch_rows<ADT, X_F8, 2, 1, 2, WIDE>(p, s);
@@ -300,7 +318,7 @@ extern "C" tvk_status tvk_gemm_f8(const tvk_gemm_f8_desc* d) {
     if (d->M > 64 && (d->a_scale_stride[0] > SCALES_MOST || d->b_scale_stride[0] > SCALES_MOST))
         return bad(TVK_ERR_UNSUPPORTED, "scales up to 2^20 from row to row only for more than 64 rows");
     if (d->M > 64 && d->K > RING_MOST) return bad(TVK_ERR_UNSUPPORTED, "K up to 2^22 only for more than 64 rows");
-    if (((d->M + 127) / 128) * ((d->N + 127) / 128) > (1 << 22)) return bad(TVK_ERR_UNSUPPORTED, "more than 2^22 tiles of 128 x 128");
+    if (((d->M + 127) / 128) * ((d->N + 127) / 128) >= (1 << 22)) return bad(TVK_ERR_UNSUPPORTED, "2^22 tiles of 128 x 128 or more");
     GemmF8Args p{};
     p.a = d->a;
     p.b = static_cast<const uint8_t*>(d->b);
