@@ -825,7 +825,7 @@ __global__ __launch_bounds__(SA_THREADS) void sample_bins_kernel(SampleArgs p) {
     fill_bins(x, h, first_range<float>(top, f.heat), f.by_k, s.all);
     u64* out = p.bins + (int64_t)blockIdx.x * SA_BINS;
     out[threadIdx.x] = s.all.w[threadIdx.x];
-    out[threadIdx.x + SA_THREADS] = s.all.w[threadIdx.x + SA_THREADS];
+    if (!f.by_k) out[threadIdx.x + SA_THREADS] = s.all.w[threadIdx.x + SA_THREADS];   // (counts are in the first half)
 }
 
 // The border's bin, from all pieces' histograms, and what of a piece lies in it and above.
@@ -845,14 +845,20 @@ __global__ __launch_bounds__(SA_THREADS) void sample_border_kernel(SampleArgs p)
     if (!f.by_k && !f.by_p) return state(SA_ALL, 0, 0, 0);
     const Heat h = f.weights(top, s);
     const u64* in = p.bins + row * p.pieces * SA_BINS + threadIdx.x;
-    u64 a = 0, b = 0;   // counts are two to a word, and do not carry: there are at most 2^19
-#pragma unroll 8
-    for (int i = 0; i < p.pieces; ++i) {
-        a += in[(int64_t)i * SA_BINS];
-        b += in[(int64_t)i * SA_BINS + SA_THREADS];
-    }
-    s.all.w[threadIdx.x] = a;
-    s.all.w[threadIdx.x + SA_THREADS] = b;
+    auto sum = [&](const u64* first) {
+        u64 v = 0;   // counts are two to a word, and do not carry: there are at most 2^19
+#pragma unroll 1
+        for (int i = 0; i < p.pieces; i += 8) {
+            u64 w[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) w[k] = first[(int64_t)min(i + k, p.pieces - 1) * SA_BINS];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) v += i + k < p.pieces ? w[k] : 0;
+        }
+        return v;
+    };
+    s.all.w[threadIdx.x] = sum(in);
+    s.all.w[threadIdx.x + SA_THREADS] = f.by_k ? 0 : sum(in + SA_THREADS);
     __syncthreads();
     const u64 need = f.by_k ? (u64)f.top_k : f.share(sum_of(s.all, s));
     find_bin(false, f.by_k, need, s);
@@ -997,9 +1003,11 @@ __global__ __launch_bounds__(SA_THREADS) void sample_token_kernel(SampleArgs p) 
 
 template <int DT>
 tvk_status launch(SampleArgs p, hipStream_t s) {
-    // A workgroup a CU is wanted; pieces of 256 chunks or more
+    // A workgroup a CU is wanted, for pieces of 512 chunks or more, and the three launches more that they take: one row of
+    // bfloat16, top_k 50 and top_p 0.9, in pieces and not, 16000 values 21.6 and 14.6 us, 32000 22.3 and 19.4, 128000 24 and 51;
+    // top_p alone 27.6 and 25.8, 27.7 and 38.7, 39 and 121.
     const int chunks = (p.cols + RowIn<DT>::VEC - 1) / RowIn<DT>::VEC;
-    const int64_t pieces = std::min<int64_t>({SA_PIECES, 256 / p.rows, chunks / 256});
+    const int64_t pieces = chunks <= 2048 ? 1 : std::min<int64_t>({SA_PIECES, 256 / p.rows, chunks / 512});
     const dim3 block(SA_THREADS);
     if (pieces < 2) {
         constexpr int64_t MOST = 1 << 21;   // rows of a launch: 2^32 threads are too many
