@@ -54,6 +54,16 @@ __device__ inline Soft join(Soft a, Soft b, float c) {
     return {m, a.s * exp2_of((a.m - f) * c) + b.s * exp2_of((b.m - f) * c)};
 }
 
+// Over a wave's lanes in their order, the same bits in each.
+__device__ inline Soft join_lanes(Soft r, float c) {
+#pragma unroll
+    for (int m = 1; m < 64; m <<= 1) {
+        const Soft o{__shfl_xor(r.m, m), __shfl_xor(r.s, m)};
+        r = threadIdx.x & m ? join(o, r, c) : join(r, o, c);
+    }
+    return r;
+}
+
 template <int VALUES>
 __device__ inline void add_values(Soft& r, const float (&x)[VALUES], float c) {
     float m = r.m;
@@ -95,11 +105,7 @@ __device__ Soft soft_piece(const typename elem<DT>::T* row, int64_t begin, int64
         const float x[1] = {elem<DT>::to_f32(row[begin + chunks * VEC + threadIdx.x])};
         add_values(r, x, c);
     }
-#pragma unroll
-    for (int m = 1; m < 64; m <<= 1) {
-        const Soft o{__shfl_xor(r.m, m), __shfl_xor(r.s, m)};
-        r = threadIdx.x & m ? join(o, r, c) : join(r, o, c);
-    }
+    r = join_lanes(r, c);
     __shared__ Soft part[DI_THREADS / 64];
     __syncthreads();
     if (threadIdx.x % 64 == 0) part[threadIdx.x / 64] = r;
@@ -114,40 +120,66 @@ __device__ inline int64_t index_at(const DistillArgs& p, int64_t row, int j) {
     return p.index64 ? static_cast<const int64_t*>(p.index)[row * p.si + j] : static_cast<const int32_t*>(p.index)[row * p.si + j];
 }
 
-// The row's loss, log sum of exponentials and the entries' shares, from the sum over its logits. LDS: table, slots x 3 words.
 template <int DT>
-__device__ void distill_row(const DistillArgs& p, int64_t row, Soft soft, int* table) {
+__device__ inline float teacher_at(const DistillArgs& p, int64_t row, int j) {
+    const int64_t i = row * p.st + j;
+    return p.teacher32 ? static_cast<const float*>(p.teacher)[i] : elem<DT>::to_f32(static_cast<const typename elem<DT>::T*>(p.teacher)[i]);
+}
+
+// A thread's first entry, asked for before the row's logits and used after them.
+struct Entry {
+    int64_t at;
+    float t;
+};
+template <int DT>
+__device__ inline Entry first_entry(const DistillArgs& p, int64_t row) {
+    const int j = threadIdx.x;
+    if (j >= p.top) return {-1, 0.0f};
+    return {index_at(p, row, j), teacher_at<DT>(p, row, j)};
+}
+
+// The row's loss, log sum of exponentials and the entries' shares, from the sum over its logits, by the workgroup's first N
+// threads: all, or a wave, which has no barriers to wait at while the others make room for the next workgroup. Forward of 4096 x
+// 32000 in bfloat16 with 64 entries 62 us, all threads 71; 8192 x 8000 58 and 75. More entries take all. LDS: table, slots x 3 words.
+template <int DT, int N>
+__device__ __forceinline__ void distill_row(const DistillArgs& p, int64_t row, const Entry& own, Soft soft, int* table) {
     typedef typename elem<DT>::T T;
+    auto all = [](auto op, float v) {
+        if constexpr (N == 64) {
+            __threadfence_block();   // (LDS, as a barrier would)
+            return lanes64_all<decltype(op)>(v);
+        } else {
+            return block_all<decltype(op)>(v);
+        }
+    };
     const float c = kLog2e * p.inv_t;
     const T* x = static_cast<const T*>(p.x) + row * p.sx;
+    const float own_x = own.at >= 0 && own.at < p.cols ? elem<DT>::to_f32(x[own.at]) : 0.0f;
     int *key = table, *first = table + p.slots, *count = table + 2 * p.slots;
     __shared__ int twice;
-    for (int i = threadIdx.x; i < p.slots; i += DI_THREADS) {
+    for (int i = threadIdx.x; i < p.slots; i += N) {
         key[i] = -1;
         first[i] = 0x7fffffff;
         count[i] = 0;
     }
     if (threadIdx.x == 0) twice = 0;
     auto named = [&](int j, int64_t& at) {
-        at = index_at(p, row, j);
+        at = j == (int)threadIdx.x ? own.at : index_at(p, row, j);
         return at >= 0 && at < p.cols;
     };
-    auto logit = [&](int j) {
-        const int64_t i = row * p.st + j;
-        return p.teacher32 ? static_cast<const float*>(p.teacher)[i] : elem<DT>::to_f32(static_cast<const T*>(p.teacher)[i]);
-    };
+    auto logit = [&](int j) { return j == (int)threadIdx.x ? own.t : teacher_at<DT>(p, row, j); };
     float top = -INFINITY, bad = 0.0f;
     int64_t at;
-    for (int j = threadIdx.x; j < p.top; j += DI_THREADS)
+    for (int j = threadIdx.x; j < p.top; j += N)
         if (named(j, at)) {
             const float v = logit(j);
             top = fmaxf(top, v);
             bad = v != v ? 1.0f : bad;
         }
-    top = block_all<MaxOp>(top);   // (and every thread is past the table's first values)
-    bad = block_all<MaxOp>(bad);
+    top = all(MaxOp(), top);   // (and every thread is past the table's first values)
+    bad = all(MaxOp(), bad);
     if (top == -INFINITY && bad == 0.0f) {   // nothing to learn from: no loss, and a gradient of zeros whatever the logits are
-        for (int j = threadIdx.x; j < p.top && p.target; j += DI_THREADS) p.target[row * p.sq + j] = 0.0f;
+        for (int j = threadIdx.x; j < p.top && p.target; j += N) p.target[row * p.sq + j] = 0.0f;
         if (threadIdx.x == 0) {
             p.loss[row] = 0.0f;
             if (p.lse) p.lse[row] = INFINITY;
@@ -156,7 +188,7 @@ __device__ void distill_row(const DistillArgs& p, int64_t row, Soft soft, int* t
     }
     auto slot_of = [&](int64_t at) { return (uint32_t)at * 2654435769u >> 8 & (uint32_t)(p.slots - 1); };   // multiplicative hash
     float sum = 0.0f;
-    for (int j = threadIdx.x; j < p.top; j += DI_THREADS)
+    for (int j = threadIdx.x; j < p.top; j += N)
         if (named(j, at)) {
             sum += exp2_of((logit(j) - top) * c);
             for (uint32_t h = slot_of(at);; h = (h + 1) & (uint32_t)(p.slots - 1)) {   // fewer entries than slots
@@ -167,17 +199,17 @@ __device__ void distill_row(const DistillArgs& p, int64_t row, Soft soft, int* t
                 break;
             }
         }
-    sum = block_all<SumOp>(sum);   // (and the table is filled)
+    sum = all(SumOp(), sum);   // (and the table is filled)
     const float log_s = logf(soft.s), log_q = logf(sum);
     auto share = [&](int j) { return exp2_of((logit(j) - top) * c) / sum; };
     float loss = 0.0f;
-    for (int j = threadIdx.x; j < p.top; j += DI_THREADS) {
+    for (int j = threadIdx.x; j < p.top; j += N) {
         float q = 0.0f;
         if (named(j, at)) {
             q = share(j);
             if (q != 0.0f) {
                 const float lq = (logit(j) - top) * p.inv_t - log_q;
-                const float lp = (elem<DT>::to_f32(x[at]) - soft.m) * p.inv_t - log_s;
+                const float lp = ((j == (int)threadIdx.x ? own_x : elem<DT>::to_f32(x[at])) - soft.m) * p.inv_t - log_s;
                 loss += q * (lq - lp);
             }
             if (twice && p.target) {
@@ -191,7 +223,7 @@ __device__ void distill_row(const DistillArgs& p, int64_t row, Soft soft, int* t
         }
         if (p.target) p.target[row * p.sq + j] = q;
     }
-    loss = block_all<SumOp>(loss);
+    loss = all(SumOp(), loss);
     if (threadIdx.x == 0) {
         p.loss[row] = loss * p.t * p.t;
         if (p.lse) {
@@ -201,15 +233,16 @@ __device__ void distill_row(const DistillArgs& p, int64_t row, Soft soft, int* t
     }
 }
 
-// A workgroup a row.
-template <int DT>
+// A workgroup a row. N: threads for what follows the logits.
+template <int DT, int N>
 __global__ __launch_bounds__(DI_THREADS) void distill_rows_kernel(DistillArgs p) {
     extern __shared__ int table[];
     typedef typename elem<DT>::T T;
     for (int64_t row = blockIdx.x; row < p.rows; row += gridDim.x) {
+        if (row != blockIdx.x) __syncthreads();   // the table was the last row's
+        const Entry own = first_entry<DT>(p, row);
         const Soft r = soft_piece<DT>(static_cast<const T*>(p.x) + row * p.sx, 0, p.cols, kLog2e * p.inv_t);
-        distill_row<DT>(p, row, r, table);
-        __syncthreads();   // the table is the next row's
+        if (threadIdx.x < N) distill_row<DT, N>(p, row, own, r, table);
     }
 }
 
@@ -226,14 +259,15 @@ __global__ __launch_bounds__(DI_THREADS) void distill_pieces_kernel(DistillArgs 
     }
 }
 
-template <int DT>
-__global__ __launch_bounds__(DI_THREADS) void distill_join_kernel(DistillArgs p) {
+template <int DT, int N>
+__global__ __launch_bounds__(N) void distill_join_kernel(DistillArgs p) {
     extern __shared__ int table[];
     const int64_t row = blockIdx.x;
     const float* part = p.part + 2 * row * p.pieces;
+    const Entry own = first_entry<DT>(p, row);
     Soft r{-INFINITY, 0.0f};
-    for (int i = 0; i < p.pieces; ++i) r = join(r, Soft{part[2 * i], part[2 * i + 1]}, kLog2e * p.inv_t);
-    distill_row<DT>(p, row, r, table);
+    for (int i = threadIdx.x % 64; i < p.pieces; i += 64) r = join(r, Soft{part[2 * i], part[2 * i + 1]}, kLog2e * p.inv_t);
+    distill_row<DT, N>(p, row, own, join_lanes(r, kLog2e * p.inv_t), table);
 }
 
 // LDS: top floats, the entries' gradients.
@@ -284,14 +318,14 @@ __global__ __launch_bounds__(DI_THREADS) void distill_bwd_kernel(DistillArgs p) 
 
 constexpr int64_t kMostGroups = 1 << 20;
 
-template <int DT>
+template <int DT, int N>
 tvk_status forward(DistillArgs& p, hipStream_t s) {
     const size_t lds = (size_t)p.slots * 12;
     // Two workgroups a CU are wanted; rows that do not make them are cut, into pieces of 4 K values or more
     constexpr int64_t WANTED = 512, PIECE = 4096;
     const int64_t pieces = std::min((WANTED + p.rows - 1) / p.rows, p.cols / PIECE);
     if (pieces < 2) {
-        hipLaunchKernelGGL((distill_rows_kernel<DT>), dim3((unsigned)std::min(p.rows, kMostGroups)), dim3(DI_THREADS), lds, s, p);
+        hipLaunchKernelGGL((distill_rows_kernel<DT, N>), dim3((unsigned)std::min(p.rows, kMostGroups)), dim3(DI_THREADS), lds, s, p);
         return TVK_OK;
     }
     p.piece = ((p.cols + pieces - 1) / pieces + 7) / 8 * 8;
@@ -300,8 +334,13 @@ tvk_status forward(DistillArgs& p, hipStream_t s) {
     p.part = static_cast<float*>(scratch.get((size_t)(p.rows * p.pieces) * 8, s));
     if (!p.part) return fail(TVK_ERR_OOM, "tvk_distill_fwd: workspace allocation failed");
     hipLaunchKernelGGL((distill_pieces_kernel<DT>), dim3((unsigned)(p.rows * p.pieces)), dim3(DI_THREADS), 0, s, p);
-    hipLaunchKernelGGL((distill_join_kernel<DT>), dim3((unsigned)p.rows), dim3(DI_THREADS), lds, s, p);
+    hipLaunchKernelGGL((distill_join_kernel<DT, N>), dim3((unsigned)p.rows), dim3(N), lds, s, p);
     return TVK_OK;
+}
+
+template <int DT>
+tvk_status forward(DistillArgs& p, hipStream_t s) {
+    return p.top <= 64 ? forward<DT, 64>(p, s) : forward<DT, DI_THREADS>(p, s);
 }
 
 template <int DT>
