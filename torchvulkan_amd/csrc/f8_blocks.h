@@ -1,6 +1,6 @@
 // 8-bit floats (e4m3fn) in blocks with a float32 scale each: how every kernel
-// that makes them takes a block's scale and rounds its values, so that all give
-// the same bits.
+// that makes them takes a block's scale and rounds its values, so that all that
+// are given the same values give the same bits.
 #pragma once
 
 #include "words.h"
@@ -27,6 +27,17 @@ struct F8Scale {
         if (!plain()) a /= div, b /= div, c /= div, d /= div;
         return pack4_f8(a, b, c, d);
     }
+    // The same of quotients that are off by what a division's rounding leaves: where the values are a float32 result's own and
+    // not a tensor's, each rounding on the way to 8 bits sends some to the other neighbour. (The remainder is exact.)
+    __device__ uint32_t divide4(float a, float b, float c, float d) const {
+        if (!plain()) return pack4(a, b, c, d);
+        auto over = [&](float v) {
+            const float q = v * mul;
+            return fmaf(fmaf(-q, s, v), mul, q);
+        };
+        return pack4_f8(over(a), over(b), over(c), over(d));
+    }
+    __device__ uint8_t divide1(float a) const { return (uint8_t)divide4(a, 0.0f, 0.0f, 0.0f); }
     __device__ uint8_t pack1(float a) const { return (uint8_t)pack4(a, 0.0f, 0.0f, 0.0f); }
 };
 

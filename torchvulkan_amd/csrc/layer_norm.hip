@@ -82,6 +82,12 @@ __device__ __forceinline__ float lanes_top(float v) {
     return v;
 }
 
+// 1 / sqrt(ss * rcols + eps): the instruction's, a step of 2^-23 or so off, once by Newton's method.
+__device__ __forceinline__ float inv_std(float ss, float rcols, float eps) {
+    const float x = fmaf(ss, rcols, eps), r = inv_rms(ss, rcols, eps);
+    return x > 1e-30f && x < 1e30f ? fmaf(0.5f * r, fmaf(-x * r, r, 1.0f), r) : r;
+}
+
 template <int DT, bool OUT8, int NC, int TPR>
 __global__ __launch_bounds__(row_threads(TPR)) void layer_norm_kernel(LayerArgs p) {
     typedef Row<DT, NC, TPR> R;
@@ -139,7 +145,7 @@ __global__ __launch_bounds__(row_threads(TPR)) void layer_norm_kernel(LayerArgs 
         }
         row_sums<TPR>(dev, turn ^ 1);
         const float e = dev[1] * p.rcols;
-        const float inv = inv_rms(fmaxf(dev[0] - dev[1] * e, 0.0f), p.rcols, p.eps);
+        const float inv = inv_std(fmaxf(dev[0] - dev[1] * e, 0.0f), p.rcols, p.eps);
         if (p.h) {
             T* o = static_cast<T*>(p.h) + row * p.sh;
 #pragma unroll
@@ -147,14 +153,15 @@ __global__ __launch_bounds__(row_threads(TPR)) void layer_norm_kernel(LayerArgs 
                 if (t + TPR * i < chunks) store_words<16, sizeof(T)>(o + (uint32_t)(VEC * (t + TPR * i)), h.c[i]);
             if (has_last) o[VEC * chunks + tt] = elem<DT>::from_f32(h.last);
         }
-        last = fmaf((last - e) * inv, w.r.last, b.r.last);
+        const float shift = -e * inv;
+        last = fmaf(fmaf(last, inv, shift), w.r.last, b.r.last);
 #pragma unroll
         for (int i = 0; i < NC; ++i) {
             float f[VEC], g[VEC];
             w.chunk(i, t, chunks, f);
             b.chunk(i, t, chunks, g);
 #pragma unroll
-            for (int k = 0; k < VEC; ++k) v[i][k] = fmaf((v[i][k] - e) * inv, f[k], g[k]);
+            for (int k = 0; k < VEC; ++k) v[i][k] = fmaf(fmaf(v[i][k], inv, shift), f[k], g[k]);
         }
         if constexpr (OUT8) {
             uint8_t* o = static_cast<uint8_t*>(p.out) + row * p.so;
@@ -177,18 +184,18 @@ __global__ __launch_bounds__(row_threads(TPR)) void layer_norm_kernel(LayerArgs 
                 if (c < chunks) {
                     Words<VEC> q;
 #pragma unroll
-                    for (int k = 0; k < VEC; k += 4) q.w[k / 4] = s.pack4(v[i][k], v[i][k + 1], v[i][k + 2], v[i][k + 3]);
+                    for (int k = 0; k < VEC; k += 4) q.w[k / 4] = s.divide4(v[i][k], v[i][k + 1], v[i][k + 2], v[i][k + 3]);
                     store_words<VEC, 1>(o + (uint32_t)(VEC * c), q);
                 }
                 const bool ours = tc / TPR == i;
-                if (ours && has_last) o[VEC * chunks + tt] = s.pack1(last);
+                if (ours && has_last) o[VEC * chunks + tt] = s.divide1(last);
                 // the block's first chunk, or its first value past the chunks
                 if (VEC * c % F8_BLOCK == 0 && c < chunks) scale[VEC * c / F8_BLOCK * p.ss[1]] = s.s;
                 if (ours && tc >= chunks && has_last && tt == 0) scale[tb * p.ss[1]] = s.s;
             }
             if (tc / TPR >= NC) {   // registers full of chunks, and the values past them a block of their own
                 const F8Scale s(lanes_top<LANES>(last_top));
-                if (has_last) o[VEC * chunks + tt] = s.pack1(last);
+                if (has_last) o[VEC * chunks + tt] = s.divide1(last);
                 if (has_last && tt == 0) scale[tb * p.ss[1]] = s.s;
             }
         } else {
@@ -275,7 +282,7 @@ __global__ __launch_bounds__(THREADS) void layer_norm_bwd_kernel(LayerBwdArgs p,
         add.packed();
         w.r.packed();
         const float e = two[1] * p.rcols;
-        const float inv = inv_rms(fmaxf(two[0] - two[1] * e, 0.0f), p.rcols, p.eps);
+        const float inv = inv_std(fmaxf(two[0] - two[1] * e, 0.0f), p.rcols, p.eps);
         const float gmean = one[1] * p.rcols;
         const float nmean = (two[2] - e * one[1]) * inv * p.rcols;   // of g * n
         auto centred = [&](float v) { return (v - mean) - e; };
@@ -391,8 +398,8 @@ __global__ __launch_bounds__(RN_THREADS) void layer_norm_any_kernel(LayerArgs p)
                 const int64_t c0 = blk * F8_BLOCK + lane, c1 = c0 + 64;
                 const float a = c0 < p.cols ? norm(c0) : 0.0f, b = c1 < p.cols ? norm(c1) : 0.0f;
                 const F8Scale s(lanes64_all<MaxOp>(fmaxf(fabsf(a), fabsf(b))));
-                if (c0 < p.cols) o[c0] = s.pack1(a);
-                if (c1 < p.cols) o[c1] = s.pack1(b);
+                if (c0 < p.cols) o[c0] = s.divide1(a);
+                if (c1 < p.cols) o[c1] = s.divide1(b);
                 if (lane == 0) p.scale[row * p.ss[0] + blk * p.ss[1]] = s.s;
             }
         } else {
