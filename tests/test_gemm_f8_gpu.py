@@ -128,6 +128,13 @@ def test_large(gpu, m, n, k):
     check(*operands(m, n, k, 1), out_dtype=torch.bfloat16)
 
 
+@pytest.mark.parametrize("m,n,k", [(2048, 4096, 144), (2000, 4000, 640), (1400, 4200, 400)])
+def test_middling(gpu, m, n, k):
+    """Tiles of 128 x 256, whole and cut, of one step and of several."""
+    for dtype in (torch.bfloat16, torch.float16):
+        check(*operands(m, n, k, 2), bias=rand((n,), 3), out_dtype=dtype)
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("m", [2, 50, 200])
 def test_types_and_bias(gpu, dtype, m):

@@ -18,6 +18,10 @@
 // 4-11} and the same two shifted by 32. Each group's rows of one parity are then
 // (for c and c + 1) at the eight slots c ^ {0, 1, 6, 7}, c + 1 ^ {2, 3, 4, 5}: no
 // two units on one bank.
+//
+// Measured: 8192 x 14336 x 4096 482 us, 8192^3 525 us (2.0 and 2.1 PFLOP/s; a library's bfloat16 product of 8192^3 958 us). The
+// matrix unit is busy for half of the cycles there: a step's fragments and what is put into LDS take it three
+// quarters of the time that the products take, and a wave's next step starts behind a barrier.
 #include "gemm_common.h"
 #include "gemm_f8.h"
 
@@ -292,17 +296,25 @@ void launch(GemmF8Args p, int splits, hipStream_t s) {
 
 namespace tvk {
 
+// K is split where there are 128 x 128 tiles for half the CUs or fewer, into stretches of 4 blocks or more: 128 x 4096 x 4096 in
+// 1, 2, 4 and 8 parts 27.4, 21.2, 18.5 and 19.8 us, 1024 x 1024 x 14336 in 1, 2 and 4 85.5, 50.9 and 36.5; 512 x 4096 x 4096 in
+// 1, 2 (a workgroup a CU) and 4 27.9, 25.5 and 36.3.
 int f8_ring_splits(const GemmF8Args& p) {
     const int64_t tiles = (int64_t)((p.M + 127) / 128) * ((p.N + 127) / 128);
     return (int)std::max<int64_t>(1, std::min<int64_t>(256 / tiles, p.blocks / 4));
 }
 
 void f8_ring(const GemmF8Args& p, int splits, hipStream_t s) {
-    // 256 x 256 tiles where they fill the CUs; float32 results need a wave's registers for wider operands
-    const bool big = splits == 1 && (int64_t)((p.M + 255) / 256) * ((p.N + 255) / 256) >= 256;
-    if (p.out_dtype == TVK_F32) launch<Tile<128, 128, 2, 2, 2>, true>(p, splits, s);
-    else if (big) launch<Tile<256, 256, 4, 2, 2>, false>(p, splits, s);
-    else launch<Tile<128, 128, 2, 2, 4>, false>(p, splits, s);
+    // float32 results need a wave's registers for wider operands
+    if (p.out_dtype == TVK_F32) return launch<Tile<128, 128, 2, 2, 2>, true>(p, splits, s);
+    // A round of a tile on every CU takes about 30, 42 and 60 us of 4096 values of k for tiles of 128 x 128, 128 x 256 and
+    // 256 x 256 (that is 1.15, 1.6 and 2 PFLOP/s, the smaller ones waiting for LDS): the size whose rounds take least.
+    // 2048 x 4096 x 4096 59.8, 49.7 and 64.8 us; 1024 x 4096 x 4096 29.9, 40.4 and 57.5; 3000 x 4096 x 4096 83.7, 85.5 and 68.0.
+    auto rounds = [&](int64_t bm, int64_t bn) { return ((p.M + bm - 1) / bm * ((p.N + bn - 1) / bn) + 255) / 256; };
+    const int64_t small = 5 * rounds(128, 128), middle = 7 * rounds(128, 256), large = 10 * rounds(256, 256);
+    if (splits > 1 || small <= std::min(middle, large)) launch<Tile<128, 128, 2, 2, 4>, false>(p, splits, s);
+    else if (middle < large) launch<Tile<128, 256, 2, 4, 3>, false>(p, splits, s);
+    else launch<Tile<256, 256, 4, 2, 2>, false>(p, splits, s);
 }
 
 }  // namespace tvk
