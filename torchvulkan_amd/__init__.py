@@ -12,8 +12,9 @@ device_count, current_device, set_device, synchronize, empty_cache,
 memory_allocated, max_memory_allocated, memory_reserved, mem_get_info,
 reset_peak_memory_stats, memory_stats, get_device_properties, get_device_name,
 manual_seed (torchvulkan/__init__.py:32-166). torchvulkan_amd.decoder has the
-operators of a decoder's block that the reference composes or lacks: the
-root-mean-square norm and a paged key/value cache with its attention.
+operators of a decoder that the reference composes or lacks: norms, 8-bit block
+products, a paged key/value cache with its attention, the loss against a teacher's
+top logits and the drawing of the next token.
 """
 from __future__ import annotations
 
@@ -177,4 +178,4 @@ torch.Tensor.vulkan = _tensor_to_vulkan
 torch.Tensor.is_vulkan = property(lambda self: self.device.type == "vulkan")
 torch.utils.generate_methods_for_privateuse1_backend(for_tensor=False)
 
-from . import decoder  # noqa: E402,F401  (the norm and the paged key/value cache)
+from . import decoder  # noqa: E402,F401  (a decoder's operators)

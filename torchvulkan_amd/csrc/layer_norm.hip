@@ -12,6 +12,13 @@
 // (dy) in registers; a second launch adds the workgroups' up in a fixed order.
 // 8-bit output has a scale for each 128 columns: 16 or 32 neighbouring lanes,
 // whose largest value is one reduction among them.
+//
+// Measured, where a copy reaches 5.2 TB/s: 16384 x 4096 of bfloat16 with a residual
+// to 8 bits 92 us (472 MB, 5.1 TB/s); backward of 16384 x 2048 63 us, 5 of them the
+// second launch (268 MB); 5 x 1024 3.3 us, a launch; backward of 1000 x 777 of float32
+// 10 us, two launches. A row of 512 chunks by 512 threads with one chunk each was slower,
+// 101 us and 92, and so was one kept packed between the sums, which fits five
+// workgroups a CU for four, 97 us.
 #include "f8_blocks.h"
 #include "norm_rows.h"
 

@@ -24,6 +24,14 @@
 // not inlined, and nothing is read in a chain that can be read at once. Few rows are
 // cut among workgroups, in four launches: the largest, the histogram, what lies in
 // and above the border's bin, the token.
+//
+// Measured: 1 x 50001 of bfloat16 with top_k and top_p 22 us (launches of 3.7, 4.9, 7.5
+// and 6.7), 64 x 128000 with top_p at temperatures from 0.5 to 1.5 61 us (4.9, 16, 24
+// and 17), 200 x 32003 of float32 with every filter 47 us. The weights of a row, some
+// 210 cycles for 64 of them, and their atomics in LDS bound the larger; a series without
+// the table of fractions was slower (18.9 us for 16.5 in the histogram's launch), and
+// neither comparisons with a bin's ends in place of its number nor sums over runs of
+// one place before the atomics changed the third.
 #include "norm_rows.h"
 
 #include <cfloat>

@@ -1,8 +1,11 @@
-"""The decoder block's operators as a program uses them: the root-mean-square
-norm and layer norm with their gradients, and a paged key/value cache that prompts
-and new tokens are appended to and attended over. Tensors of the vulkan device or of "cuda"; the
-calls are queued on the tensors' device's current stream. The reference composes
-these operators from element-wise shaders and keeps dense caches."""
+"""A decoder's operators as a program uses them: the root-mean-square norm and
+layer norm with their gradients, both in 8 bits too; products of 8-bit floats with
+a scale for each block of 128; a paged key/value cache that prompts and new tokens
+are appended to and attended over; the loss against a teacher's top logits with
+its gradient; and the drawing of the next token. Tensors of the vulkan device or
+of "cuda"; the calls are queued on the tensors' device's current stream. The
+reference composes the norms and the loss from element-wise shaders, keeps dense
+caches, and has no 8-bit blocks."""
 from __future__ import annotations
 
 import ctypes as C
