@@ -63,6 +63,62 @@ def test_norm_product_norm_product(gpu, rows):
         assert all(torch.equal(p, q) for p, q in zip(eager, (u, out, h)))
 
 
+def calls(seed):
+    """Inputs of calls that take the library's scratch, and the calls: sums of a split K, rows cut among workgroups, pieces."""
+    gen = torch.Generator().manual_seed(seed)
+    x = torch.randn((130, 2100), generator=gen).bfloat16().cuda()
+    w = decoder.quantize_fp8(torch.randn((400, 2100), generator=gen).bfloat16().cuda(), 128)
+    logits, number = torch.randn((3, 70000), generator=gen).cuda(), torch.rand(3, generator=gen).cuda()
+    index, teacher = torch.randint(0, 70000, (3, 20), generator=gen).cuda(), torch.randn((3, 20), generator=gen).cuda()
+    inputs = x, logits, number, teacher
+
+    def run():
+        return (decoder.linear_fp8(x, *w), *decoder.sample(logits, number, top_p=0.9), *decoder.sample(logits, number, 0.7, 50, 0.9),
+                decoder.distill_loss(logits, index, teacher, 2.0))
+    return inputs, run
+
+
+def test_streams_at_once(gpu):
+    """The same calls on two streams: each has scratch of its own."""
+    many = [calls(seed)[1] for seed in (1, 2)]
+    want = [run() for run in many]
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream() for _ in range(2)], [[], []]
+    for _ in range(10):
+        for k in range(2):
+            with torch.cuda.stream(streams[k]):
+                got[k].append(many[k]())
+    torch.cuda.synchronize()
+    for k in range(2):
+        for results in got[k]:
+            assert all(torch.equal(a, b) for a, b in zip(results, want[k]))
+
+
+def test_two_graphs(gpu):
+    """Captured one after the other, replayed in turn and beside each other with inputs that change, eager calls between them."""
+    made = [calls(seed) for seed in (3, 4)]
+    graphs, outs = [], []
+    for _, run in made:
+        run()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs.append(run())
+        graphs.append(graph)
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    for turn in range(3):
+        for inputs, _ in made:
+            for t in inputs:
+                t.copy_(t.roll(1, -1))
+        want = [run() for _, run in made]
+        torch.cuda.synchronize()
+        for k in range(2):
+            with torch.cuda.stream(streams[k]):
+                graphs[k].replay()
+        torch.cuda.synchronize()
+        for k in range(2):
+            assert all(torch.equal(a, b) for a, b in zip(outs[k], want[k]))
+
+
 @pytest.mark.parametrize("draw", [None, dict(temperature=0.9, top_k=40, top_p=0.9), dict(temperature=1.3, min_p=0.02)])
 def test_captured_tokens_are_the_eager_ones(gpu, example, draw):
     model = example.Decoder(layers=2, dim=256, heads=4, heads_kv=2, hidden=520, vocab=500, block=example.Block8)

@@ -91,6 +91,16 @@ def test_sizes(gpu, dtype, rows, cols, top):
     check(x, index.to(torch.int32), teacher.to(dtype), heat=2.5, what="int32")
 
 
+@pytest.mark.parametrize("top", [63, 64, 65, 257])
+@pytest.mark.parametrize("rows,cols", [(3, 9000), (700, 90)])
+def test_lists_about_a_wave_s(gpu, rows, cols, top):
+    """Rows that one workgroup takes and rows in pieces, with lists that one wave takes and more."""
+    x, index, teacher = inputs(rows, cols, top, torch.bfloat16, top)
+    index[0, 3:] = -1
+    index[-1, top // 2:] = index[-1, 0]
+    check(x, index, teacher, 1.25)
+
+
 def test_padding_and_twice(gpu):
     x, index, teacher = inputs(6, 3000, 16, torch.float32, 3)
     index[0, 5:] = -1                     # a shorter list
