@@ -153,6 +153,15 @@ def test_many_rows(gpu, dtype, rows, cols):
     check_bwd(rand((rows, cols), dtype, 3), x, w, what="backward")
 
 
+@pytest.mark.parametrize("rows,cols,dtype", [(600, 2100, torch.bfloat16), (700, 4500, torch.float16), (300, 8704, torch.bfloat16),
+                                             (600, 5001, torch.float32), (1, 9000, torch.bfloat16)])
+def test_many_long_rows(gpu, rows, cols, dtype):
+    """Several rows to a workgroup at every length, and one row, whose sums are the gradients themselves."""
+    x, w = rand((rows, cols), dtype, rows, 2.0), rand(cols, dtype, 1)
+    check_bwd(rand((rows, cols), dtype, 3), x, w, rand((rows, cols), dtype, 4), what="backward")
+    check_bwd(rand((rows, cols), dtype, 3), x, w.float(), what="float32 weights")
+
+
 def test_rows_far_from_zero(gpu):
     """A mean a thousand times the deviation: its rounding is taken off again."""
     for cols in (100, 1000, 5000, 9000):

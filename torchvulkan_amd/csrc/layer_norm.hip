@@ -14,7 +14,7 @@
 // whose largest value is one reduction among them.
 //
 // Measured, where a copy reaches 5.2 TB/s: 16384 x 4096 of bfloat16 with a residual
-// to 8 bits 92 us (472 MB, 5.1 TB/s); backward of 16384 x 2048 63 us, 5 of them the
+// to 8 bits 92 us (472 MB, 5.1 TB/s); backward of 16384 x 2048 62 us, 5 of them the
 // second launch (268 MB); 5 x 1024 3.3 us, a launch; backward of 1000 x 777 of float32
 // 10 us, two launches. A row of 512 chunks by 512 threads with one chunk each was slower,
 // 101 us and 92, and so was one kept packed between the sums, which fits five
@@ -68,10 +68,11 @@ __device__ __forceinline__ void row_sums(float (&v)[N], int turn) {
 #pragma unroll
             for (int i = 0; i < N; ++i) part[turn][wave][i] = v[i];
         __syncthreads();
+        constexpr int AT_ONCE = TPR > 512 && N > 2 ? 3 : TPR / 64;   // (three sums of 16 waves take too many registers)
 #pragma unroll
         for (int i = 0; i < N; ++i) {
             v[i] = part[turn][w0][i];
-#pragma unroll
+#pragma unroll AT_ONCE
             for (int w = 1; w < TPR / 64; ++w) v[i] += part[turn][w0 + w][i];
         }
     }
@@ -224,11 +225,18 @@ __global__ __launch_bounds__(THREADS) void layer_norm_bwd_kernel(LayerBwdArgs p,
     const int t = threadIdx.x % TPR, sub = row_of_thread<TPR>(), chunks = (int)p.cols / VEC, tail = (int)p.cols % VEC;
     Weights<DT, NC, TPR> w;
     w.load(p.w, p.w32, t, chunks, tail);
+    // The longest rows leave no registers for the sums of dweight and dbias, nor for the next row: each thread has its sums in
+    // LDS (4096 x 16384 of bfloat16 182 us, in registers with spills 380, and 640 with the next row too).
+    constexpr bool LONG = NC * TPR >= 2048;
+    __shared__ f32x4 acc_lds[LONG ? 2 : 1][LONG ? NC * VEC / 4 : 1][LONG ? TPR : 1];
     float acc[2][NC][VEC], acc_last[2] = {0.0f, 0.0f};
 #pragma unroll
     for (int i = 0; i < NC; ++i)
 #pragma unroll
-        for (int k = 0; k < VEC; ++k) acc[0][i][k] = acc[1][i][k] = 0.0f;
+        for (int k = 0; k < VEC; ++k) {
+            if constexpr (LONG) acc_lds[0][(i * VEC + k) / 4][t] = acc_lds[1][(i * VEC + k) / 4][t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+            else acc[0][i][k] = acc[1][i][k] = 0.0f;
+        }
     int64_t row = (int64_t)blockIdx.x * SUBS + sub;
     const int64_t step = (int64_t)gridDim.x * SUBS;
     R dy, h, dh;   // of the next row, on their way while one is computed
@@ -237,14 +245,15 @@ __global__ __launch_bounds__(THREADS) void layer_norm_bwd_kernel(LayerBwdArgs p,
         h.load(static_cast<const T*>(p.h) + row * p.sh, t, chunks, tail);
         if (p.dh) dh.load(static_cast<const T*>(p.dh) + row * p.sdh, t, chunks, tail);
     };
-    if (row < p.rows) load();
+    if (!LONG && row < p.rows) load();
     // a workgroup's rows keep step: their sums meet at barriers
     for (int64_t first = (int64_t)blockIdx.x * SUBS; first < p.rows; first += step) {
+        if (LONG && row < p.rows) load();
         R gy = dy, x = h, add = dh;
         const bool live = row < p.rows;
         T* dx = static_cast<T*>(p.dx) + row * p.sdx;
         row += step;
-        if (row < p.rows) load();
+        if (!LONG && row < p.rows) load();
         const bool has_last = t < tail;
         float one[2] = {has_last ? x.last : 0.0f, has_last ? gy.last * w.r.last : 0.0f};   // sums of h and of g
 #pragma unroll
@@ -260,9 +269,11 @@ __global__ __launch_bounds__(THREADS) void layer_norm_bwd_kernel(LayerBwdArgs p,
             one[1] += pg;
         }
         row_sums<TPR>(one, 0);
-        gy.packed();
-        x.packed();
-        w.r.packed();
+        if constexpr (NC > 1) {   // (one chunk's floats have room)
+            gy.packed();
+            x.packed();
+            w.r.packed();
+        }
         const float mean = one[0] * p.rcols;
         const float d_last = has_last ? x.last - mean : 0.0f;
         float two[3] = {d_last * d_last, d_last, gy.last * w.r.last * d_last};   // of d^2, d and g d
@@ -284,10 +295,12 @@ __global__ __launch_bounds__(THREADS) void layer_norm_bwd_kernel(LayerBwdArgs p,
         }
         row_sums<TPR>(two, 1);
         if (!live) continue;
-        gy.packed();
-        x.packed();
         add.packed();
-        w.r.packed();
+        if constexpr (NC > 1) {
+            gy.packed();
+            x.packed();
+            w.r.packed();
+        }
         const float e = two[1] * p.rcols;
         const float inv = inv_std(fmaxf(two[0] - two[1] * e, 0.0f), p.rcols, p.eps);
         const float gmean = one[1] * p.rcols;
@@ -296,12 +309,21 @@ __global__ __launch_bounds__(THREADS) void layer_norm_bwd_kernel(LayerBwdArgs p,
 #pragma unroll
         for (int i = 0; i < NC; ++i) {
             float f[VEC], o[VEC];
+            f32x4 grads[2];   // of four columns, LONG
             w.chunk(i, t, chunks, f);
 #pragma unroll
             for (int k = 0; k < VEC; ++k) {
                 const float n = centred(x.at(i, k)) * inv, d = gy.at(i, k);
-                acc[0][i][k] = fmaf(d, n, acc[0][i][k]);
-                acc[1][i][k] += d;
+                if constexpr (LONG)
+                    if (k % 4 == 0) grads[0] = acc_lds[0][(i * VEC + k) / 4][t], grads[1] = acc_lds[1][(i * VEC + k) / 4][t];
+                if constexpr (LONG) {
+                    grads[0][k % 4] = fmaf(d, n, grads[0][k % 4]);
+                    grads[1][k % 4] += d;
+                    if (k % 4 == 3) acc_lds[0][(i * VEC + k) / 4][t] = grads[0], acc_lds[1][(i * VEC + k) / 4][t] = grads[1];
+                } else {
+                    acc[0][i][k] = fmaf(d, n, acc[0][i][k]);
+                    acc[1][i][k] += d;
+                }
                 o[k] = inv * (fmaf(d, f[k], -gmean) - n * nmean);
                 if (p.dh) o[k] += add.at(i, k);
             }
@@ -317,7 +339,27 @@ __global__ __launch_bounds__(THREADS) void layer_norm_bwd_kernel(LayerBwdArgs p,
         }
     }
     if (!part && !p.dw && !p.db) return;
-    __shared__ __attribute__((aligned(16))) float sum[SUBS][VEC * (NC * TPR + 1)];
+    if constexpr (LONG) {   // a workgroup a row at a time: every thread stores its own sums
+        for (int what = 0; what < 2; ++what) {
+            if (!(p.want >> what & 1)) continue;
+            float* out = part + ((int64_t)what * gridDim.x + blockIdx.x) * p.cols;
+            void* grad = what ? p.db : p.dw;
+            auto store = [&](int c, float v) {
+                if (part) out[c] = v;
+                else if (p.w32) static_cast<float*>(grad)[c] = v;
+                else put<DT>(grad, c, v);
+            };
+            for (int q = 0; q < NC * VEC / 4; ++q) {
+                const int i = q / (VEC / 4), c = VEC * (t + TPR * i) + 4 * (q % (VEC / 4));
+                if (t + TPR * i < chunks)
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) store(c + k, acc_lds[what][q][t][k]);
+            }
+            if (t < tail) store(VEC * chunks + t, acc_last[what]);
+        }
+        return;
+    }
+    __shared__ __attribute__((aligned(16))) float sum[LONG ? 1 : SUBS][LONG ? 1 : VEC * (NC * TPR + 1)];
 #pragma unroll
     for (int what = 0; what < 2; ++what) {
         if (!(p.want >> what & 1)) continue;
@@ -504,7 +546,11 @@ tvk_status backward(LayerBwdArgs p, void* dw, void* db, hipStream_t s) {
     };
     bool have = true, single = false;
     const bool done = row_shape(p.rows, 256, p.cols * (int64_t)dtype_size(DT) / 16, [&](auto nc, auto tpr) {
-        constexpr int NC = decltype(nc)::value, TPR = decltype(tpr)::value, THREADS = bwd_threads(TPR), SUBS = THREADS / TPR;
+        // one chunk a thread where two leave no registers for a second workgroup a CU: bfloat16 8192 x 4096 65 us, with two
+        // 80, 4096 x 8192 79 and 103
+        constexpr bool TWICE = decltype(nc)::value == 2 && (decltype(tpr)::value == 256 || decltype(tpr)::value == 512);
+        constexpr int NC = TWICE ? 1 : decltype(nc)::value, TPR = decltype(tpr)::value * (TWICE ? 2 : 1);
+        constexpr int THREADS = bwd_threads(TPR), SUBS = THREADS / TPR;
         const int64_t groups = std::min<int64_t>((p.rows + SUBS - 1) / SUBS, RN_BWD_THREADS / THREADS);
         single = groups == 1;
         if (single) p.dw = dw, p.db = db;
