@@ -144,7 +144,7 @@ def test_types_and_bias(gpu, dtype, m):
 
 
 @pytest.mark.parametrize("m", [1, 4, 5, 16, 32, 64])
-@pytest.mark.parametrize("n,k", [(40, 5), (40, 15), (40, 17), (40, 31), (40, 143), (6145, 300), (12300, 700)])
+@pytest.mark.parametrize("n,k", [(40, 5), (40, 15), (40, 17), (40, 31), (40, 143), (4097, 300), (6145, 300), (8200, 400), (12300, 700)])
 def test_few_rows(gpu, m, n, k):
     """Ends of rows at every part of 16 bytes, and columns enough for several blocks of W a workgroup; wider rows give the
     bits of their 8-bit form."""
@@ -158,7 +158,7 @@ def test_few_rows(gpu, m, n, k):
         assert torch.equal(_abi.gemm_f8(a, None, b.to(DEV), sb.to(DEV)), want)
 
 
-@pytest.mark.parametrize("m,n,k", [(17, 12290, 4096), (32, 4100, 12288), (33, 2100, 4096), (64, 4096, 2064)])
+@pytest.mark.parametrize("m,n,k", [(17, 12290, 4096), (17, 2100, 15440), (32, 4100, 12288), (33, 2100, 4096), (33, 300, 8192), (64, 4096, 2064), (64, 4096, 4112)])
 def test_few_rows_of_large_weights(gpu, m, n, k):
     a, sa, b, sb = operands(m, n, k, m)
     for out_dtype in (torch.float32, torch.float16):

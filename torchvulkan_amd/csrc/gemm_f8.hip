@@ -9,13 +9,13 @@
 // memory into the instruction's operands, several blocks on their way at once; the
 // waves' sums meet in LDS. Up to 16 rows of A in 16 or 32 bits are brought into 8
 // bits on the way, by each workgroup for itself; more rows in a launch of their
-// own. More than 64 rows, and from 17 on those of large weights, run
-// gemm_f8_ring.hip.
+// own. More than 64 rows, and from 17 on those of long k, run gemm_f8_ring.hip.
 //
 // Measured, W read from memory at 5.2 TB/s if nothing else took time: 1 x 14336 x
 // 4096 13.7 us in 8 bits and 15.9 from bfloat16 (11.3 for W's bytes, 3 for a launch);
-// 16 x 14336 x 4096 16.1 and 17.3; 1 x 8192 x 8192 13.9 and 17.6; 50 x 5000 x 4100,
-// no row on 16 bytes, 24 from float16 with the launch that brings it into 8 bits.
+// 16 x 14336 x 4096 16.1 and 17.3; 1 x 8192 x 8192 13.9 and 17.6; 64 x 14336 x 4096
+// 24.5; 50 x 5000 x 4100, no row on 16 bytes, 14.8, and 17.9 from float16 with the
+// launch that brings it into 8 bits.
 // Loads on their way over the end of a loop's turn, with a next set of registers,
 // were slower, 16.9 us for 15.1: a wave has four blocks of 4096 values in all.
 #include "gemm_f8.h"
@@ -25,11 +25,11 @@ using namespace tvk;
 namespace {
 
 constexpr int FR_WAVES = 8;
-// From so many columns on a workgroup takes 4 and 2 blocks of 16 rows of W, so that 5 rows of A and more are read, and brought
-// into 8 bits, less often; workgroups for all CUs are left. 16 rows from bfloat16 by 14336 x 4096, 1, 2 and 4 blocks: 34.1, 23.6
-// and 17.3 us; by 8192 x 4096 18.4, 12.1 and 15.3; by 4096 x 4096 10.3, 11.7 and 14.7. One row: 15.6, 15.0 and 15.9; 9.4, 9.9
-// and 10.8; 1 x 8192 x 8192 17.6, 21.9 and 19.7.
-constexpr int NT4 = 12288, NT2 = 6144;
+// Past so many columns a workgroup takes 2 blocks of 16 rows of W, and 4, so that all workgroups make one round on the CUs, and
+// the rows of A are read, and brought into 8 bits, less often. 16 rows from bfloat16 by 14336 x 4096, 1, 2 and 4 blocks: 34.1,
+// 23.6 and 17.3 us; by 8192 x 4096 18.4, 12.1 and 15.3; by 4096 x 4096 10.3, 11.7 and 14.7. 50 rows by 5000 x 4100 21.6 and 14.8
+// of 1 and 2.
+constexpr int NT2 = 4096, NT4 = 8192;
 
 // A lane's 32 values of a block of k, of A and of W alike, whose order does not matter to the sum: 16 of the first
 // half and 16 of the second, so that the four lanes of a row load 64 bytes side by side.
@@ -247,8 +247,8 @@ void launch_rows(const GemmF8Args& p, hipStream_t s) {
 
 template <int ADT, int FORM, bool WIDE>
 void rows_16(const GemmF8Args& p, hipStream_t s) {
-    if (p.N >= NT4) launch_rows<ADT, FORM, 1, 4, 2, WIDE>(p, s);
-    else if (p.N >= NT2) launch_rows<ADT, FORM, 1, 2, 4, WIDE>(p, s);
+    if (p.N > NT4) launch_rows<ADT, FORM, 1, 4, 2, WIDE>(p, s);
+    else if (p.N > NT2) launch_rows<ADT, FORM, 1, 2, 4, WIDE>(p, s);
     else launch_rows<ADT, FORM, 1, 1, 4, WIDE>(p, s);
 }
 
@@ -266,10 +266,12 @@ void few_rows(const GemmF8Args& p, hipStream_t s) {
     } else if constexpr (!IN8) {
         return;   // (8 bits by now)
     } else if (p.M <= 32) {
-        if (p.N >= NT2) launch_rows<ADT, X_F8, 2, 2, 2, WIDE>(p, s);
+        if (p.N > NT4) launch_rows<ADT, X_F8, 2, 4, 1, WIDE>(p, s);
+        else if (p.N > NT2) launch_rows<ADT, X_F8, 2, 2, 2, WIDE>(p, s);
         else launch_rows<ADT, X_F8, 2, 1, 2, WIDE>(p, s);
     } else {
-        if (p.N >= NT2) launch_rows<ADT, X_F8, 4, 2, 1, WIDE>(p, s);
+        if (p.N > NT4) launch_rows<ADT, X_F8, 4, 4, 1, WIDE>(p, s);
+        else if (p.N > NT2) launch_rows<ADT, X_F8, 4, 2, 1, WIDE>(p, s);
         else launch_rows<ADT, X_F8, 4, 1, 1, WIDE>(p, s);
     }
 }
@@ -288,12 +290,12 @@ bool ring_rows(const void* p, int64_t stride, int K) {
     return reinterpret_cast<uintptr_t>(p) % 16 == 0 && stride % 16 == 0 && stride <= RING_MOST && K % 16 == 0;
 }
 
-// Where up to 64 rows run the tiled kernel too, rows that it can load as they lie: it reads A once for 128 rows of W
-// and not once for 16 or 32, and in exchange splits K and joins the sums in a launch of its own. Tiled against rows:
-// 64 x 2048 x 4096 13.0 and 15.8 us, 64 x 14336 x 4096 23.7 and 33.1, 32 x 14336 x 4096 21.1 and 24.2;
-// 64 x 1024 x 1024 10.5 and 6.0, 32 x 8192 x 4096 14.9 and 13.9.
+// Where up to 64 rows run the tiled kernel too, rows that it can load as they lie: a workgroup of the other takes all of k for
+// its rows of A, this splits k, and joins the sums in a launch of its own. Tiled against rows: 64 x 4096 x 4096 16.2 and 15.9 us,
+// 64 x 4096 x 14336 23.8 and 46.1, 20 x 4096 x 14336 19.8 and 23.5, 48 x 8192 x 6144 20.4 and 22.1; 32 x 8192 x 6144 19.2 and
+// 17.5, 20 x 14336 x 4096 20.7 and 16.2, 64 x 1024 x 1024 10.1 and 5.6.
 bool tiles_pay(const GemmF8Args& p, const tvk_gemm_f8_desc* d) {
-    return p.M > 16 && (int64_t)p.N * p.K >= (p.M > 32 ? 1 << 23 : 3 << 24) && p.K % 16 == 0 && p.K <= RING_MOST &&
+    return p.M > 16 && (int64_t)p.M * p.K >= 1 << 18 && p.K % 16 == 0 && p.K <= RING_MOST &&
            p.sa_m <= SCALES_MOST && p.sb_n <= SCALES_MOST && ring_rows(p.b, p.ldb, p.K) &&
            (d->a_dtype != TVK_F8E4M3FN || ring_rows(d->a, d->a_stride, p.K));
 }
