@@ -7,13 +7,14 @@ operands is below sqrt(2) 2^-4 = 0.089 of the product, of two products in a row 
 them add 2^-8 each. Both bounds are of the relative distance of whole tensors."""
 from __future__ import annotations
 
+import ctypes as C
 import importlib.util
 from pathlib import Path
 
 import pytest
 import torch
 
-from torchvulkan_amd import decoder
+from torchvulkan_amd import _abi, decoder
 
 pytestmark = pytest.mark.gpu
 
@@ -164,3 +165,58 @@ def test_gradients_of_a_step(gpu, example):
 def test_the_example_s_steps_run(gpu, example):
     losses = example.distill_steps(300, 128, 500, 16, 2)
     assert len(losses) == 2 and all(x == x and x > 0 for x in losses)
+
+
+def test_rows_far_apart(gpu):
+    """Rows 2.2 GB from each other, read and written: the bits of rows side by side."""
+    apart, cols = 1_100_000_000, 3000
+    stream = torch.cuda.current_stream().cuda_stream
+    lib = _abi.load()
+    memory = [torch.empty(2 * apart + cols, dtype=torch.bfloat16, device="cuda") for _ in range(2)]
+
+    def far(t, where):
+        out = memory[where].as_strided(t.shape, (apart, 1))
+        out.copy_(t)
+        return out
+
+    gen = torch.Generator().manual_seed(6)
+    x = torch.randn((3, cols), generator=gen).bfloat16().cuda()
+    dy = torch.randn((3, cols), generator=gen).bfloat16().cuda()
+    number = torch.rand(3, generator=gen).cuda()
+    index, teacher = torch.randint(0, cols, (3, 9), generator=gen).cuda(), torch.randn((3, 9), generator=gen).cuda()
+    heat = torch.full((3,), 0.9, device="cuda")
+    want = _abi.sample(x, number, top_p=heat)
+    assert all(torch.equal(a, b) for a, b in zip(_abi.sample(far(x, 0), number, top_p=heat), want))
+
+    loss, lse, target = _abi.distill_fwd(x, index, teacher)
+    want = _abi.distill_bwd(x, index, lse, target, number)
+    xf, out = far(x, 0), far(torch.zeros_like(x), 1)
+    assert all(torch.equal(a, b) for a, b in zip(_abi.distill_fwd(xf, index, teacher), (loss, lse, target)))
+    _abi.check(lib.tvk_distill_bwd(C.byref(_abi.make_distill_bwd_desc(xf, index, lse, target, number, out, 1.0, stream))))
+    assert torch.equal(out, want)
+
+    want = _abi.layer_norm_fwd(x)[0]
+    _abi.check(lib.tvk_layer_norm_fwd(C.byref(_abi.make_layer_norm_desc(xf, None, None, out, stream=stream))))
+    assert torch.equal(out, want)
+    want = _abi.layer_norm_bwd(dy, x)[0]
+    dyf = far(dy, 1)   # and dx over it
+    _abi.check(lib.tvk_layer_norm_bwd(C.byref(_abi.make_layer_norm_bwd_desc(dyf, far(x, 0), None, dyf, stream=stream))))
+    assert torch.equal(dyf, want)
+
+    q, scale = _abi.quantize_f8(x)
+    qf = torch.empty(2 * apart + cols, dtype=torch.uint8, device="cuda").view(torch.float8_e4m3fn).as_strided((3, cols), (apart, 1))
+    sf = torch.empty_like(scale)
+    _abi.check(lib.tvk_quantize_f8(C.byref(_abi.make_quantize_f8_desc(far(x, 0), qf, sf, 1, stream))))
+    assert torch.equal(qf.contiguous().view(torch.uint8), q.view(torch.uint8)) and torch.equal(sf, scale)
+    w, w_scale = _abi.quantize_f8(torch.randn((cols, cols), generator=gen).bfloat16().cuda(), 128)
+    want = _abi.gemm_f8(x, None, w, w_scale)
+    out = far(torch.zeros_like(x), 1)
+    for a, s in ((far(x, 0), None), (qf, scale)):   # (as the rows, and as their 8 bits)
+        out.zero_()
+        _abi.check(lib.tvk_gemm_f8(C.byref(_abi.make_gemm_f8_desc(a, s, w, w_scale, out, stream=stream))))
+        assert torch.equal(out, want)
+    tall = torch.randn((70, 256), generator=gen).bfloat16().cuda()   # the tiled kernel's output
+    wide = memory[0].as_strided((70, 256), (30_000_000, 1))
+    few, few_scale = _abi.quantize_f8(torch.randn((256, 256), generator=gen).bfloat16().cuda(), 128)
+    _abi.check(lib.tvk_gemm_f8(C.byref(_abi.make_gemm_f8_desc(tall, None, few, few_scale, wide, stream=stream))))
+    assert torch.equal(wide, _abi.gemm_f8(tall, None, few, few_scale))
