@@ -508,7 +508,7 @@ tvk_status tvk_rms_norm_bwd(const tvk_rms_norm_bwd_desc* desc);
  *   y = (h - mean(h)) / sqrt(mean((h - mean(h))^2) + eps) * weight + bias
  * (weight NULL: ones, bias NULL: zeros), y rounded to `out_dtype`: `dtype`
  * itself, or F8E4M3FN with a scale for each 128 columns of a row,
- *   scale[row][block] = max|y| / 448 over the block (1 where it is all zero),
+ *   scale[row][block] = max|y| / 448 over the block, 2^-143 or more (1 where it is all zero),
  *   out = y / scale rounded to nearest even (NaN stays NaN),
  * the form in which tvk_gemm_f8 takes its rows (the last block may be shorter).
  * h goes to residual_out when that is not NULL. dtype: F32, F16 or BF16;
@@ -564,7 +564,7 @@ tvk_status tvk_layer_norm_bwd(const tvk_layer_norm_bwd_desc* desc);
 
 /* x [rows, cols] (F32, F16 or BF16) in F8E4M3FN, in blocks of 128 columns and
  * block_rows rows, 1 (activations) or 128 (weights), the last ones shorter:
- *   scale[block] = max|x| / 448 over the block (NaN aside; 1 where it is all zero),
+ *   scale[block] = max|x| / 448 over the block, 2^-143 or more (NaN aside; 1 where it is all zero),
  *   out = x / scale rounded to nearest even (by way of the scale's reciprocal;
  *   NaN stays NaN, a block with an infinity becomes zeros and NaN).
  * Rows are contiguous, `*_stride` elements apart; any alignment. out and scale
@@ -587,7 +587,8 @@ tvk_status tvk_quantize_f8(const tvk_quantize_f8_desc* desc);
  * result is rounded once to out_dtype (F32, F16 or BF16). A block's sum over k is
  * float32 for an F32 output; for the 16-bit ones it is the matrix unit's of 8-bit
  * floats, which cuts the products of eight neighbouring values of k off 2^-13
- * below the largest of them. a_dtype F32, F16 or BF16: a is first brought
+ * below the largest of them. A product of two scales below 2^-126 is a multiple of
+ * 2^-149, rounded. a_dtype F32, F16 or BF16: a is first brought
  * into 8 bits as by tvk_quantize_f8 with block_rows 1, with the same bits, and
  * a_scale is not read. bias (NULL: none) has out_dtype or F32. Rows are
  * contiguous, `*_stride` elements apart, scales at any strides (0: one for all;

@@ -18,6 +18,21 @@ def pytest_configure(config):
     os.environ["TORCHVULKAN_CACHE_DIR"] = tempfile.mkdtemp(prefix="tvk-tuning-")
 
 
+# Tests that hold a value which was found to be wrong. They stay as they are and run; what is right is in the test named beside.
+HOLD_WRONG_VALUES = {
+    "tests/test_gemm_f8_gpu.py::test_quantize_ends_of_the_range":
+        "its row of 1e-44 expects the scale 0 and NaN for finite values, the float32 quotient max / 448 being 0 there; "
+        "tests/test_f8_small_blocks_gpu.py::test_ends_of_the_range has all of its rows",
+}
+
+
+def pytest_collection_modifyitems(items):
+    for item in items:
+        reason = HOLD_WRONG_VALUES.get(item.nodeid)
+        if reason:
+            item.add_marker(pytest.mark.xfail(reason=reason, strict=True))
+
+
 def _gpu_available() -> bool:
     try:
         import torch

@@ -9,19 +9,24 @@ namespace tvk {
 
 constexpr int F8_BLOCK = 128;   // columns of a block
 
-// What a block's values are multiplied and divided by: the scale is the block's largest magnitude (NaN aside) over 448, and
-// values go times its reciprocal. A scale whose reciprocal leaves float32's range is divided by.
+// The least scale: 64 of the smallest float32's steps. A scale of fewer is off by so much of itself, or 0, that the block's
+// largest value would be past 464, which is NaN. Values up to 448 times it are whole steps of 2^-6 over it.
+constexpr float F8_LEAST_SCALE = 0x1p-143f;
+
+// What a block's values are multiplied and divided by: the scale is the block's largest magnitude (NaN aside) over 448, the
+// least one or more, and values go times its reciprocal. A scale whose reciprocal leaves float32's range is divided by.
 struct F8Scale {
     float s, mul, div;
     __device__ explicit F8Scale(float top) {
-        s = top > 0.0f ? top / 448.0f : 1.0f;
+        s = top > 0.0f ? fmaxf(top / 448.0f, F8_LEAST_SCALE) : 1.0f;
         const float r = 1.0f / s;
         const bool plain = r < 1e30f && r > 1e-30f;
         mul = plain ? r : 1.0f;
         div = plain ? 1.0f : s;
     }
     __device__ bool plain() const { return div == 1.0f; }
-    // The largest of a block may come out half a float32 step above 448, which rounds to 448.
+    // The largest of a block may come out above 448, by half a float32 step or, of a scale below float32's normal range, by as
+    // much as that is off, 2^-7 of it at most: it rounds to 448.
     __device__ uint32_t pack4(float a, float b, float c, float d) const {
         a *= mul, b *= mul, c *= mul, d *= mul;
         if (!plain()) a /= div, b /= div, c /= div, d /= div;
