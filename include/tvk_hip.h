@@ -451,7 +451,7 @@ tvk_status tvk_attention_bwd(const tvk_attention_bwd_desc* desc);
  *   h = x + residual, rounded to `dtype` (h = x without a residual),
  *   y = h / sqrt(mean(h^2) + eps) * weight      (weight NULL: ones),
  * y rounded to `out_dtype`: `dtype` itself, or F8E4M3FN with
- *   scale[row] = max|y| / 448 (1 where the row's y is all zero),
+ *   scale[row] = max|y| / 448, 2^-143 or more (1 where the row's y is all zero),
  *   out = y / scale[row] rounded to nearest even (NaN stays NaN),
  * the per-row scales that _scaled_mm multiplies back. h goes to residual_out
  * when that is not NULL. dtype: F32, F16 or BF16; weight_dtype: `dtype` or F32.

@@ -14,6 +14,7 @@
 // Measured (a 2 GiB copy moves 4.9 TB/s): residual, norm and 8 bits of 16384 x 4096 in
 // bfloat16 81 us, 5.8 TB/s; its gradients at 16384 x 2048 56 us, 4.8 TB/s, 5 of them
 // the second launch; 7 x 4096 3.9 us and gradients of 1000 x 777 8.1 us, the launches.
+#include "f8_blocks.h"
 #include "norm_rows.h"
 
 using namespace tvk;
@@ -72,7 +73,7 @@ __global__ __launch_bounds__(RN_THREADS) void rms_norm_any_kernel(NormArgs p) {
             float top = 0.0f;
             for (int64_t c = threadIdx.x; c < p.cols; c += RN_THREADS) top = fmaxf(top, fabsf(norm(c)));
             top = block_all<MaxOp>(top);
-            const float s = top > 0.0f ? top / kF8Max : 1.0f;
+            const float s = top > 0.0f ? fmaxf(top / kF8Max, F8_LEAST_SCALE) : 1.0f;
             if (threadIdx.x == 0) p.scale[row] = s;
             uint8_t* o = static_cast<uint8_t*>(p.out) + row * p.so;
             for (int64_t c = threadIdx.x; c < p.cols; c += RN_THREADS) o[c] = f32_to_f8(norm(c) / s, TVK_F8E4M3FN);
@@ -197,7 +198,7 @@ __global__ __launch_bounds__(row_threads(TPR)) void rms_norm_kernel(NormArgs p) 
             // y = h w inv; its largest magnitude is max|h w| times inv, and y / scale = h w (inv / scale). An inv / scale
             // that leaves float32's range, for rows of values near its ends, is not taken as one factor.
             top *= inv;
-            const float s = top > 0.0f ? top / kF8Max : 1.0f, f8 = inv * __builtin_amdgcn_rcpf(s);
+            const float s = top > 0.0f ? fmaxf(top / kF8Max, F8_LEAST_SCALE) : 1.0f, f8 = inv * __builtin_amdgcn_rcpf(s);
             const bool plain = f8 < 1e30f && f8 > 1e-30f;
             const float a = plain ? f8 : inv, b = plain ? 1.0f : s;
             if (t == 0) p.scale[row] = s;
