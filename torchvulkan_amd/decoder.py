@@ -101,6 +101,7 @@ class _RmsNorm(torch.autograd.Function):
         d = _abi.make_rms_norm_desc(x2, weight, y, r2, None if r2 is None else h, None, eps, _stream(x))
         _queue("tvk_rms_norm_fwd", d, x)
         ctx.save_for_backward(h, weight)
+        ctx.set_materialize_grads(False)   # no zeros for what nothing was made of
         ctx.eps, ctx.shape, ctx.added = eps, shape, r2 is not None
         if r2 is None:
             return y.view(shape), None
@@ -170,6 +171,7 @@ class _LayerNorm(torch.autograd.Function):
         d = _abi.make_layer_norm_desc(x2, weight, bias, y, r2, None if r2 is None else h, None, eps, _stream(x))
         _queue("tvk_layer_norm_fwd", d, x)
         ctx.save_for_backward(h, weight)
+        ctx.set_materialize_grads(False)   # no zeros for what nothing was made of
         ctx.eps, ctx.shape, ctx.added, ctx.bias = eps, shape, r2 is not None, None if bias is None else bias.dtype
         if r2 is None:
             return y.view(shape), None
