@@ -627,9 +627,11 @@ tvk_status tvk_gemm_f8(const tvk_gemm_f8_desc* desc);
  * entries are none, or weigh nothing (t all -inf), has loss 0 and a gradient of
  * zeros, whatever its logits are. Infinite or NaN logits and t otherwise give
  * what the formulas give.
- * lse: log of the sum of exp(x / T), +inf for a row without entries; target: q,
- * an index that stands there twice having it all at its first entry. Both are
- * for tvk_distill_bwd, and may be NULL where that is not called.
+ * softmax: the row's largest logit m and log of the sum of exp((x - m) / T), +inf for
+ * a row without entries; lse: log of the sum of exp(x / T), +inf likewise, m / T and
+ * the other's sum in one float32; target: q, an index that stands there twice
+ * having it all at its first entry. softmax, or lse, and target are for
+ * tvk_distill_bwd, and may be NULL where that is not called.
  * dtype: F32, F16 or BF16; teacher_dtype: `dtype` or F32; index_dtype: I32 or
  * I64. Rows are contiguous, `*_stride` elements apart (0: one for all, of what
  * is read); any alignment. top up to 2048. Few rows use library scratch. */
@@ -644,14 +646,17 @@ typedef struct {
     float* target; int64_t target_stride;                /* [rows][top] */
     double temperature;
     void* stream;
+    float* softmax;                                      /* [rows][2] */
 } tvk_distill_desc;
 
 tvk_status tvk_distill_fwd(const tvk_distill_desc* desc);
 
 /* Gradient of tvk_distill_fwd's losses with respect to the logits, from the
- * forward's lse and target and the losses' gradients dloss (float32):
+ * forward's softmax and target and the losses' gradients dloss (float32):
  *   dlogits[i] = dloss * T * (exp(x_i / T - lse) - sum of q over the entries of index i),
- * rounded once, probabilities below 2^-126 being taken as zero. dloss_stride 0:
+ * rounded once, probabilities below 2^-126 being taken as zero. softmax NULL: lse is
+ * taken in its place, and each probability is then off by lse's rounding, 2^-24
+ * |lse| of itself, which grows with the logits' distance from zero. dloss_stride 0:
  * one gradient for all rows. dlogits (`dtype`) may
  * be logits (the same strides). Every place is written by one workgroup, in an
  * order of its own: the same bits every run. No scratch. */
@@ -666,6 +671,7 @@ typedef struct {
     void* dlogits; int64_t dlogits_stride;
     double temperature;
     void* stream;
+    const float* softmax;                                /* [rows][2] */
 } tvk_distill_bwd_desc;
 
 tvk_status tvk_distill_bwd(const tvk_distill_bwd_desc* desc);

@@ -260,6 +260,7 @@ class DistillDesc(C.Structure):
         ("target", C.c_void_p), ("target_stride", C.c_int64),
         ("temperature", C.c_double),
         ("stream", C.c_void_p),
+        ("softmax", C.c_void_p),
     ]
 
 
@@ -275,6 +276,7 @@ class DistillBwdDesc(C.Structure):
         ("dlogits", C.c_void_p), ("dlogits_stride", C.c_int64),
         ("temperature", C.c_double),
         ("stream", C.c_void_p),
+        ("softmax", C.c_void_p),
     ]
 
 
@@ -973,9 +975,17 @@ def _logits_and_entries(d, logits, index) -> None:
     d.index, d.index_stride = index.data_ptr(), _row_stride(index, d.rows, d.top, index.dtype, "index")
 
 
-def make_distill_desc(logits, index, teacher, loss, lse=None, target=None, temperature=1.0, stream=None) -> DistillDesc:
+def _pairs(t, rows: int, what: str):
+    """Address of a contiguous float32 [rows, 2] tensor."""
+    if tuple(t.shape) != (rows, 2) or t.dtype != _torch().float32 or not t.is_contiguous():
+        raise _invalid(f"{what}: contiguous float32 {(rows, 2)} is expected, not {t.dtype} {tuple(t.shape)}")
+    return t.data_ptr()
+
+
+def make_distill_desc(logits, index, teacher, loss, lse=None, target=None, temperature=1.0, stream=None,
+                      softmax=None) -> DistillDesc:
     """Describes tvk_distill_fwd over device tensors: logits [rows, cols], index and teacher [rows, top]; float32 loss [rows]
-    and, for the gradient, lse [rows] and target [rows, top]."""
+    and, for the gradient, softmax [rows, 2] or lse [rows], and target [rows, top]."""
     torch = _torch()
     d = DistillDesc()
     _logits_and_entries(d, logits, index)
@@ -986,6 +996,8 @@ def make_distill_desc(logits, index, teacher, loss, lse=None, target=None, tempe
     d.loss = _vector(loss, d.rows, (torch.float32,), "loss")
     if lse is not None:
         d.lse = _vector(lse, d.rows, (torch.float32,), "lse")
+    if softmax is not None:
+        d.softmax = _pairs(softmax, d.rows, "softmax")
     if target is not None:
         d.target, d.target_stride = target.data_ptr(), _row_stride(target, d.rows, d.top, torch.float32, "target")
     d.temperature = float(temperature)
@@ -993,22 +1005,25 @@ def make_distill_desc(logits, index, teacher, loss, lse=None, target=None, tempe
     return d
 
 
-def distill_fwd(logits, index, teacher, temperature=1.0, stream=None):
-    """(loss, lse, target) of tvk_distill_fwd, new float32 tensors."""
+def distill_fwd(logits, index, teacher, temperature=1.0, stream=None, softmax=None):
+    """(loss, lse, target) of tvk_distill_fwd, new float32 tensors; softmax, float32 [rows, 2], is written where it is given."""
     torch = _torch()
     loss, lse = (torch.empty(logits.shape[0], dtype=torch.float32, device=logits.device) for _ in range(2))
     target = torch.empty(index.shape, dtype=torch.float32, device=logits.device)
-    d = make_distill_desc(logits, index, teacher, loss, lse, target, temperature, _stream_of(logits, stream))
+    d = make_distill_desc(logits, index, teacher, loss, lse, target, temperature, _stream_of(logits, stream), softmax)
     check(load().tvk_distill_fwd(C.byref(d)))
     return loss, lse, target
 
 
-def make_distill_bwd_desc(logits, index, lse, target, dloss, dlogits, temperature=1.0, stream=None) -> DistillBwdDesc:
-    """Describes tvk_distill_bwd; dloss is [rows], of any stride."""
+def make_distill_bwd_desc(logits, index, lse, target, dloss, dlogits, temperature=1.0, stream=None, softmax=None) -> DistillBwdDesc:
+    """Describes tvk_distill_bwd, which takes softmax [rows, 2], or where there is none lse [rows]; dloss is [rows], of any stride."""
     torch = _torch()
     d = DistillBwdDesc()
     _logits_and_entries(d, logits, index)
-    d.lse = _vector(lse, d.rows, (torch.float32,), "lse")
+    if lse is not None:
+        d.lse = _vector(lse, d.rows, (torch.float32,), "lse")
+    if softmax is not None:
+        d.softmax = _pairs(softmax, d.rows, "softmax")
     d.target, d.target_stride = target.data_ptr(), _row_stride(target, d.rows, d.top, torch.float32, "target")
     if tuple(dloss.shape) != (d.rows,) or dloss.dtype != torch.float32:
         raise _invalid("dloss: float32 [rows] is expected")
@@ -1019,11 +1034,11 @@ def make_distill_bwd_desc(logits, index, lse, target, dloss, dlogits, temperatur
     return d
 
 
-def distill_bwd(logits, index, lse, target, dloss, temperature=1.0, stream=None):
+def distill_bwd(logits, index, lse, target, dloss, temperature=1.0, stream=None, softmax=None):
     """dlogits of tvk_distill_bwd, a new tensor of the logits' dtype."""
     torch = _torch()
     dlogits = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
-    d = make_distill_bwd_desc(logits, index, lse, target, dloss, dlogits, temperature, _stream_of(logits, stream))
+    d = make_distill_bwd_desc(logits, index, lse, target, dloss, dlogits, temperature, _stream_of(logits, stream), softmax)
     check(load().tvk_distill_bwd(C.byref(d)))
     return dlogits
 

@@ -5,8 +5,9 @@
 // brings a larger one; threads and, where a row is cut among workgroups, pieces
 // are joined in a fixed order. What is left is a row's list of `top` entries: a
 // softmax over the teacher's logits and the student's logits at their indexes.
-// Backward reads the logits once more and writes p = exp(x / T - lse) times the
-// row's factor; the entries' places, q less, are written over that after a
+// Backward reads the logits once more and writes p = exp((x - m) / T - log s) times
+// the row's factor (m and log s apart: their sum in one float32 is off by half a step
+// of its own size, and all p with it); the entries' places, q less, are written over that after a
 // barrier, from logits read before it (dlogits may be logits). An index named
 // twice would be two writes to one place, so forward gives the whole of an
 // index's q to its first entry, found in a hash table in LDS.
@@ -33,6 +34,7 @@ struct DistillArgs {
     const void* teacher;
     float* loss;
     float* lse;
+    float* softmax;       // [rows][2]: m and log s, or NULL
     float* target;
     const float* dloss;
     void* dx;
@@ -190,6 +192,7 @@ __device__ __forceinline__ void distill_row(const DistillArgs& p, int64_t row, c
         if (threadIdx.x == 0) {
             p.loss[row] = 0.0f;
             if (p.lse) p.lse[row] = INFINITY;
+            if (p.softmax) p.softmax[2 * row] = 0.0f, p.softmax[2 * row + 1] = INFINITY;
         }
         return;
     }
@@ -237,6 +240,7 @@ __device__ __forceinline__ void distill_row(const DistillArgs& p, int64_t row, c
             const float lse = soft.m * p.inv_t + log_s;
             p.lse[row] = lse == INFINITY ? NAN : lse;   // +inf stands for a row without entries
         }
+        if (p.softmax) p.softmax[2 * row] = soft.m, p.softmax[2 * row + 1] = log_s;   // (s is finite, or NaN)
     }
 }
 
@@ -277,8 +281,8 @@ __global__ __launch_bounds__(N) void distill_join_kernel(DistillArgs p) {
     distill_row<DT, N>(p, row, own, join_lanes(r, kLog2e * p.inv_t), table);
 }
 
-// LDS: top floats, the entries' gradients.
-template <int DT>
+// LDS: top floats, the entries' gradients. APART: from m and log s, else from lse.
+template <int DT, bool APART>
 __global__ __launch_bounds__(DI_THREADS) void distill_bwd_kernel(DistillArgs p) {
     extern __shared__ float entry[];
     typedef typename elem<DT>::T T;
@@ -287,9 +291,14 @@ __global__ __launch_bounds__(DI_THREADS) void distill_bwd_kernel(DistillArgs p) 
         const int64_t row = work / p.pieces, begin = work % p.pieces * p.piece, end = min(begin + p.piece, p.cols);
         const T* x = static_cast<const T*>(p.x) + row * p.sx;
         T* o = static_cast<T*>(p.dx) + row * p.sdx;
-        const float lse = p.lse[row], f = p.dloss[row * p.sd] * p.t;
-        const bool none = lse == INFINITY;
-        auto grad = [&](float v, float q) { return none ? 0.0f : f * (exp2_of(fmaf(v, p.inv_t, -lse) * kLog2e) - q); };
+        const float m = APART ? p.softmax[2 * row] : 0.0f, log_s = APART ? p.softmax[2 * row + 1] : p.lse[row];
+        const bool none = log_s == INFINITY;
+        const float f = p.dloss[row * p.sd] * p.t;
+        auto grad = [&](float v, float q) {
+            float g = f * (exp2_of(fmaf(APART ? v - m : v, p.inv_t, -log_s) * kLog2e) - q);
+            asm("" : "+v"(g));   // a choice below, no branch for every value (33 x 50001 0.8 us)
+            return none ? 0.0f : g;
+        };
         for (int j = threadIdx.x; j < p.top; j += DI_THREADS) {
             const int64_t at = index_at(p, row, j);
             const float q = p.target[row * p.sq + j];
@@ -357,7 +366,8 @@ void backward(DistillArgs& p, hipStream_t s) {
     p.piece = PIECE;
     p.pieces = (int)((p.cols + PIECE - 1) / PIECE);
     const int64_t groups = std::min(p.rows * p.pieces, kMostGroups);
-    hipLaunchKernelGGL((distill_bwd_kernel<DT>), dim3((unsigned)groups), dim3(DI_THREADS), (size_t)p.top * 4, s, p);
+    if (p.softmax) hipLaunchKernelGGL((distill_bwd_kernel<DT, true>), dim3((unsigned)groups), dim3(DI_THREADS), (size_t)p.top * 4, s, p);
+    else hipLaunchKernelGGL((distill_bwd_kernel<DT, false>), dim3((unsigned)groups), dim3(DI_THREADS), (size_t)p.top * 4, s, p);
 }
 
 tvk_status check_distill(const char* who, int32_t dtype, int32_t index_dtype, int64_t rows, int64_t cols, int64_t top, double t) {
@@ -391,6 +401,7 @@ extern "C" tvk_status tvk_distill_fwd(const tvk_distill_desc* d) {
     p.teacher = d->teacher;
     p.loss = d->loss;
     p.lse = d->lse;
+    p.softmax = d->softmax;
     p.target = d->target;
     p.sx = d->logits_stride;
     p.si = d->index_stride;
@@ -419,7 +430,7 @@ extern "C" tvk_status tvk_distill_bwd(const tvk_distill_bwd_desc* d) {
     const tvk_status st = check_distill("tvk_distill_bwd", d->dtype, d->index_dtype, d->rows, d->cols, d->top, d->temperature);
     if (st != TVK_OK) return st;
     if (d->rows == 0 || d->cols == 0) return TVK_OK;
-    if (!d->logits || (d->top > 0 && (!d->index || !d->target)) || !d->lse || !d->dloss || !d->dlogits)
+    if (!d->logits || (d->top > 0 && (!d->index || !d->target)) || (!d->lse && !d->softmax) || !d->dloss || !d->dlogits)
         return fail(TVK_ERR_INVALID, "tvk_distill_bwd: NULL tensor");
     if (d->logits_stride < 0 || d->index_stride < 0 || d->target_stride < 0 || d->dloss_stride < 0 ||
         !rows_apart(d->dlogits_stride, d->rows, d->cols))
@@ -429,6 +440,7 @@ extern "C" tvk_status tvk_distill_bwd(const tvk_distill_bwd_desc* d) {
     p.index = d->index;
     p.target = const_cast<float*>(d->target);
     p.lse = const_cast<float*>(d->lse);
+    p.softmax = const_cast<float*>(d->softmax);
     p.dloss = d->dloss;
     p.dx = d->dlogits;
     p.sx = d->logits_stride;

@@ -252,20 +252,19 @@ class _Distill(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, index, teacher, temperature):
         x, i, t = _rows(logits), _rows(index), _rows(teacher)
-        loss, lse = (torch.empty(x.shape[0], dtype=torch.float32, device=x.device) for _ in range(2))
-        target = torch.empty(i.shape, dtype=torch.float32, device=x.device)
-        d = _abi.make_distill_desc(x, i, t, loss, lse, target, temperature, _stream(x))
+        loss, softmax, target = (torch.empty(s, dtype=torch.float32, device=x.device) for s in (x.shape[0], (x.shape[0], 2), i.shape))
+        d = _abi.make_distill_desc(x, i, t, loss, None, target, temperature, _stream(x), softmax)
         _queue("tvk_distill_fwd", d, x)
-        ctx.save_for_backward(x, i, lse, target)
+        ctx.save_for_backward(x, i, softmax, target)
         ctx.temperature, ctx.shape = temperature, logits.shape
         return loss.view(logits.shape[:-1])
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dloss):
-        x, i, lse, target = ctx.saved_tensors
+        x, i, softmax, target = ctx.saved_tensors
         dlogits = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-        d = _abi.make_distill_bwd_desc(x, i, lse, target, dloss.reshape(-1), dlogits, ctx.temperature, _stream(x))
+        d = _abi.make_distill_bwd_desc(x, i, None, target, dloss.reshape(-1), dlogits, ctx.temperature, _stream(x), softmax)
         _queue("tvk_distill_bwd", d, x)
         return dlogits.view(ctx.shape), None, None, None
 
