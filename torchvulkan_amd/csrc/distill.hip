@@ -375,7 +375,8 @@ tvk_status check_distill(const char* who, int32_t dtype, int32_t index_dtype, in
     if (!norm_dtype(dtype)) return bad(TVK_ERR_UNSUPPORTED, "dtype must be float32, float16 or bfloat16");
     if (index_dtype != TVK_I32 && index_dtype != TVK_I64) return bad(TVK_ERR_UNSUPPORTED, "the indexes must be int32 or int64");
     if (rows < 0 || cols < 0 || top < 0) return bad(TVK_ERR_INVALID, "negative size");
-    if (!(t > 0.0) || !((float)t > 0.0f) || !(1.0f / (float)t > 0.0f) || !((float)t * (float)t < INFINITY) || !(1.0f / (float)t < INFINITY))
+    const float heat = (float)t;   // the kernels' factors are heat, heat * heat, 1 / heat and log2(e) / heat
+    if (!(t > 0.0) || !(heat > 0.0f) || !(1.0f / heat > 0.0f) || !(heat * heat < INFINITY) || !(kLog2e * (1.0f / heat) < INFINITY))
         return bad(TVK_ERR_INVALID, "the temperature must be above zero and finite");
     if (rows > 0x7fffffff || cols > 0x7fffffff) return bad(TVK_ERR_UNSUPPORTED, "rows and columns up to 2^31 - 1 only");
     if (top > DI_MOST_TOP) return bad(TVK_ERR_UNSUPPORTED, "up to 2048 entries a row only");
