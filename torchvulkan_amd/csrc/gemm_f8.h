@@ -19,6 +19,7 @@ struct GemmF8Args {
     int M, N, K, blocks;    // blocks: ceil(K / 128)
     int tiles_m, tiles_n;
     int out_dtype, bias32;
+    int first_n;            // of a launch of the few-row kernel
     // of the tiled kernel
     float* part;            // [splits][M][part_n], the sums of a split K, or NULL
     int part_n, split_blocks;

@@ -169,7 +169,7 @@ __global__ __launch_bounds__(64 * FR_WAVES, MT == 4 && NT == 1 ? 4 : 1) void gem
     static_assert(F8_BLOCK % (16 * NT) == 0, "one scale of W a workgroup and block");
     static_assert(FORM == X_F8 || MT == 1, "16 rows of A in wider types");
     const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
-    const int r = lane % 16, g = lane / 16, n0 = blockIdx.x * 16 * NT;
+    const int r = lane % 16, g = lane / 16, n0 = p.first_n + blockIdx.x * 16 * NT;
     const uint8_t* w[NT];
 #pragma unroll
     for (int i = 0; i < NT; ++i) w[i] = p.b + (int64_t)min(n0 + 16 * i + r, p.N - 1) * p.ldb;   // rows past N compute what is not stored
@@ -240,9 +240,14 @@ __global__ __launch_bounds__(64 * FR_WAVES, MT == 4 && NT == 1 ? 4 : 1) void gem
 }
 
 template <int ADT, int FORM, int MT, int NT, int U, bool WIDE>
-void launch_rows(const GemmF8Args& p, hipStream_t s) {
-    hipLaunchKernelGGL((gemm_f8_rows_kernel<ADT, FORM, MT, NT, U, WIDE>), dim3((unsigned)((p.N + 16 * NT - 1) / (16 * NT))),
-                       dim3(64 * FR_WAVES), 0, s, p);
+void launch_rows(GemmF8Args p, hipStream_t s) {
+    // 2^32 threads in a dimension of a grid are too many; with a second dimension 50 x 5000 x 4100 took 0.7 us more
+    constexpr int64_t MOST = 1 << 20;
+    for (int64_t n = 0; n < p.N; n += MOST * 16 * NT) {
+        p.first_n = (int)n;
+        const int64_t groups = std::min<int64_t>(MOST, (p.N - n + 16 * NT - 1) / (16 * NT));
+        hipLaunchKernelGGL((gemm_f8_rows_kernel<ADT, FORM, MT, NT, U, WIDE>), dim3((unsigned)groups), dim3(64 * FR_WAVES), 0, s, p);
+    }
 }
 
 template <int ADT, int FORM, bool WIDE>
