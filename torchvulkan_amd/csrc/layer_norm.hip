@@ -516,11 +516,11 @@ __global__ __launch_bounds__(RN_THREADS) void layer_norm_bwd_any_kernel(LayerBwd
 
 // The sums over rows: a workgroup takes 64 columns and every gridDim.y-th group of 4 rows; partials [2][gridDim.y][cols].
 template <int DT>
-__global__ __launch_bounds__(RN_THREADS) void layer_norm_sums_kernel(LayerBwdArgs p, float* part) {
+__global__ __launch_bounds__(RN_THREADS) void layer_norm_sums_kernel(LayerBwdArgs p, float* part, int64_t first) {
     __shared__ float sum[2][4][64];
     typedef typename elem<DT>::T T;
     const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
-    const int64_t c = (int64_t)blockIdx.x * 64 + lane;
+    const int64_t c = first + (int64_t)blockIdx.x * 64 + lane;
     float dw = 0.0f, db = 0.0f;
     if (c < p.cols)
         for (int64_t row = (int64_t)blockIdx.y * 4 + wave; row < p.rows; row += (int64_t)gridDim.y * 4) {
@@ -581,15 +581,14 @@ tvk_status backward(LayerBwdArgs p, void* dw, void* db, hipStream_t s) {
             p.stats = part;
             part += 3 * p.rows;
             if (p.rows > 0) hipLaunchKernelGGL((layer_norm_stats_kernel<DT>), rows_grid(p.rows), dim3(RN_THREADS), 0, s, p);
-            hipLaunchKernelGGL((layer_norm_sums_kernel<DT>), dim3((unsigned)((p.cols + 63) / 64), (unsigned)parts),
-                               dim3(RN_THREADS), 0, s, p, part);
+            over_columns<64>(p.cols, [&](int64_t first, unsigned groups) {
+                hipLaunchKernelGGL((layer_norm_sums_kernel<DT>), dim3(groups, (unsigned)parts), dim3(RN_THREADS), 0, s, p, part, first);
+            });
         }
         if (have && p.rows > 0) hipLaunchKernelGGL((layer_norm_bwd_any_kernel<DT>), rows_grid(p.rows), dim3(RN_THREADS), 0, s, p);
     }
     if (!have) return fail(TVK_ERR_OOM, "tvk_layer_norm_bwd: workspace allocation failed");
-    if (p.want && !single)
-        hipLaunchKernelGGL((norm_fold_kernel<DT>), dim3((unsigned)((p.cols + FOLD_COLS - 1) / FOLD_COLS), db ? 2 : 1),
-                           dim3(FOLD_COLS * FOLD_ROWS), 0, s, part, parts, p.cols, dw, db, p.w32);
+    if (p.want && !single) norm_fold<DT>(part, parts, p.cols, dw, db, p.w32, s);
     return TVK_OK;
 }
 

@@ -200,18 +200,26 @@ constexpr int64_t RN_BWD_THREADS = 1024 * 256;
 constexpr int bwd_threads(int tpr) { return tpr < 512 ? 512 : tpr; }
 
 // Adds the partials up: a workgroup FOLD_COLS columns, its threads every FOLD_ROWS-th partial, then those in order. A second
-// row of workgroups does the same for the partials behind those, to db.
+// row of workgroups does the same for the partials behind those, to db. first: of a launch's columns.
 constexpr int FOLD_COLS = 16, FOLD_ROWS = 64;
+
+// Calls launch(first column, workgroups) for all columns, WIDTH to a workgroup: 2^32 threads in a dimension of a grid are too many.
+template <int WIDTH, class F>
+void over_columns(int64_t cols, F&& launch) {
+    constexpr int64_t MOST = 1 << 20;
+    for (int64_t first = 0; first < cols; first += MOST * WIDTH)
+        launch(first, (unsigned)std::min<int64_t>(MOST, (cols - first + WIDTH - 1) / WIDTH));
+}
 
 template <int DT>
 __global__ __launch_bounds__(FOLD_COLS * FOLD_ROWS) void norm_fold_kernel(const float* part, int64_t parts, int64_t cols,
-                                                                         void* dw, void* db, int w32) {
+                                                                         int64_t first, void* dw, void* db, int w32) {
     part += blockIdx.y * parts * cols;
     void* out = blockIdx.y ? db : dw;
     if (!out) return;
     __shared__ float sum[FOLD_ROWS][FOLD_COLS + 1];
     const int x = threadIdx.x % FOLD_COLS, y = threadIdx.x / FOLD_COLS;
-    const int64_t c = (int64_t)blockIdx.x * FOLD_COLS + x;
+    const int64_t c = first + (int64_t)blockIdx.x * FOLD_COLS + x;
     float s = 0.0f;
     if (c < cols) {
         for (int64_t i = y; i < parts; i += 8 * FOLD_ROWS) {   // eight loads on their way together
@@ -231,6 +239,14 @@ __global__ __launch_bounds__(FOLD_COLS * FOLD_ROWS) void norm_fold_kernel(const 
     if (y != 0 || c >= cols) return;
     if (w32) static_cast<float*>(out)[c] = sum[0][x];
     else put<DT>(out, c, sum[0][x]);
+}
+
+template <int DT>
+void norm_fold(const float* part, int64_t parts, int64_t cols, void* dw, void* db, int w32, hipStream_t s) {
+    over_columns<FOLD_COLS>(cols, [&](int64_t first, unsigned groups) {
+        hipLaunchKernelGGL((norm_fold_kernel<DT>), dim3(groups, db ? 2 : 1), dim3(FOLD_COLS * FOLD_ROWS), 0, s, part, parts, cols, first, dw,
+                           db, w32);
+    });
 }
 
 // Calls f(NC, TPR) for rows of `chunks` whole chunks; false past what registers hold. At most two chunks a thread: more

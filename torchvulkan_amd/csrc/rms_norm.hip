@@ -128,11 +128,11 @@ __global__ __launch_bounds__(RN_THREADS) void rms_norm_bwd_any_kernel(NormBwdArg
 
 // dweight's sums: a workgroup takes 64 columns and every gridDim.y-th group of 4 rows; partials [gridDim.y][cols].
 template <int DT>
-__global__ __launch_bounds__(RN_THREADS) void rms_norm_dweight_kernel(NormBwdArgs p, float* part) {
+__global__ __launch_bounds__(RN_THREADS) void rms_norm_dweight_kernel(NormBwdArgs p, float* part, int64_t first) {
     __shared__ float sum[4][64];
     typedef typename elem<DT>::T T;
     const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
-    const int64_t c = (int64_t)blockIdx.x * 64 + lane;
+    const int64_t c = first + (int64_t)blockIdx.x * 64 + lane;
     float s = 0.0f;
     if (c < p.cols)
         for (int64_t row = (int64_t)blockIdx.y * 4 + wave; row < p.rows; row += (int64_t)gridDim.y * 4)
@@ -379,15 +379,14 @@ tvk_status backward(NormBwdArgs p, void* dw, hipStream_t s) {
             p.inv = part;
             part += p.rows;
             if (p.rows > 0) hipLaunchKernelGGL((rms_norm_inv_kernel<DT>), rows_grid(p.rows), dim3(RN_THREADS), 0, s, p);
-            hipLaunchKernelGGL((rms_norm_dweight_kernel<DT>), dim3((unsigned)((p.cols + 63) / 64), (unsigned)parts),
-                               dim3(RN_THREADS), 0, s, p, part);
+            over_columns<64>(p.cols, [&](int64_t first, unsigned groups) {
+                hipLaunchKernelGGL((rms_norm_dweight_kernel<DT>), dim3(groups, (unsigned)parts), dim3(RN_THREADS), 0, s, p, part, first);
+            });
         }
         if (have && p.rows > 0) hipLaunchKernelGGL((rms_norm_bwd_any_kernel<DT>), rows_grid(p.rows), dim3(RN_THREADS), 0, s, p);
     }
     if (!have) return fail(TVK_ERR_OOM, "tvk_rms_norm_bwd: workspace allocation failed");
-    if (dw && !p.dw)
-        hipLaunchKernelGGL((norm_fold_kernel<DT>), dim3((unsigned)((p.cols + FOLD_COLS - 1) / FOLD_COLS)),
-                           dim3(FOLD_COLS * FOLD_ROWS), 0, s, part, parts, p.cols, dw, nullptr, p.w32);
+    if (dw && !p.dw) norm_fold<DT>(part, parts, p.cols, dw, nullptr, p.w32, s);
     return TVK_OK;
 }
 
