@@ -12,7 +12,7 @@
 // own. More than 64 rows, and from 17 on those of long k, run gemm_f8_ring.hip.
 //
 // Measured, W read from memory at 5.2 TB/s if nothing else took time: 1 x 14336 x
-// 4096 13.7 us in 8 bits and 15.9 from bfloat16 (11.3 for W's bytes, 3 for a launch);
+// 4096 13.7 us in 8 bits and 15.8 from bfloat16 (11.3 for W's bytes, 3 for a launch);
 // 16 x 14336 x 4096 16.1 and 17.3; 1 x 8192 x 8192 13.9 and 17.6; 64 x 14336 x 4096
 // 24.5; 50 x 5000 x 4100, no row on 16 bytes, 14.8, and 17.9 from float16 with the
 // launch that brings it into 8 bits.
@@ -261,10 +261,13 @@ template <int ADT, bool WIDE>
 void few_rows(const GemmF8Args& p, hipStream_t s) {
     constexpr bool IN8 = ADT == TVK_F8E4M3FN;
     if (p.M <= 4) {
-        // from wider types 4 blocks of W a workgroup where those make one round on the CUs: 1 x 14336 x 4096 11.4 us, W in
-        // the memory's cache, and 15.9, it isn't, where one block takes 14.4 and 15.6; 1 x 28672 x 4096, two rounds, 29.8 and 25.8
+        // from wider types 4 blocks of W a workgroup for as many columns as with more rows, where those make one round on the CUs.
+        // 1 row of bfloat16, W from memory and, in brackets, from its cache: by 8192 x 4096 10.2 (8.0) us with one block and 11.5
+        // (10.4) with four, by 8704 x 4096 12.4 (10.6) and 11.6 (10.5), by 14336 x 4096 15.6 (14.5) and 15.8 (11.4), by 14336 x
+        // 14336 42.8 (37.3) and 37.7 (31.1), by 16384 x 4096 16.1 (14.7) and 17.5 (12.9), the most that it loses; two rounds, by
+        // 20480 x 4096, 19.8 (18.1) and 25.7 (21.4).
         const int groups = (p.N + 63) / 64;
-        if (!IN8 && groups > 192 && groups <= 256) launch_rows<ADT, IN8 ? X_F8 : X_SHARED, 1, IN8 ? 1 : 4, IN8 ? 4 : 2, WIDE>(p, s);
+        if (!IN8 && p.N > NT4 && groups <= 256) launch_rows<ADT, IN8 ? X_F8 : X_SHARED, 1, IN8 ? 1 : 4, IN8 ? 4 : 2, WIDE>(p, s);
         else launch_rows<ADT, IN8 ? X_F8 : X_SHARED, 1, 1, 4, WIDE>(p, s);
     } else if (p.M <= 16) {
         rows_16<ADT, IN8 ? X_F8 : X_OWN, WIDE>(p, s);
