@@ -43,7 +43,6 @@ struct F8Scale {
         return pack4_f8(over(a), over(b), over(c), over(d));
     }
     __device__ uint8_t divide1(float a) const { return (uint8_t)divide4(a, 0.0f, 0.0f, 0.0f); }
-    __device__ uint8_t pack1(float a) const { return (uint8_t)pack4(a, 0.0f, 0.0f, 0.0f); }
 };
 
 // Whether no two places of a [rows, cols] array with these strides, in elements, are the same.

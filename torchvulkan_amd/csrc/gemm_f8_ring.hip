@@ -22,15 +22,12 @@
 // Measured: 8192 x 14336 x 4096 482 us, 8192^3 525 us (2.0 and 2.1 PFLOP/s; a library's bfloat16 product of 8192^3 958 us). The
 // matrix unit is busy for half of the cycles there: a step's fragments and what is put into LDS take it three
 // quarters of the time that the products take, and a wave's next step starts behind a barrier.
-#include "gemm_common.h"
+#include "gemm_dma.h"
 #include "gemm_f8.h"
 
 using namespace tvk;
 
 namespace {
-
-#define TVK_LDS __attribute__((address_space(3)))
-typedef int i32x4 __attribute__((ext_vector_type(4)));
 
 // Buffer resource over [p, p + bytes): loads past the end return zeros. The same for all lanes of a wave.
 __device__ __forceinline__ i32x4 f8_rsrc(const void* p, int64_t bytes) {
@@ -39,23 +36,11 @@ __device__ __forceinline__ i32x4 f8_rsrc(const void* p, int64_t bytes) {
                  __builtin_amdgcn_readfirstlane((int)min(bytes, (int64_t)0x7fffffff)), 0x00020000};
 }
 
-// 16 bytes per lane from r + voff into LDS at lds_addr + 16 * lane (lds_addr is wave-uniform; it travels in M0). From inline
-// assembly: a compiler-visible load into LDS would make every later LDS read wait for it.
-__device__ __forceinline__ void f8_dma16(i32x4 r, uint32_t lds_addr, uint32_t voff) {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
-                 :: "s"(lds_addr), "v"(voff), "s"(r) : "memory");
-}
-
-// 4 bytes per lane, to lds_addr + 4 * lane.
+// As dma16, 4 bytes per lane, to lds_addr + 4 * lane. (From inline assembly: a compiler-visible load into LDS would make every
+// later LDS read wait for it.)
 __device__ __forceinline__ void f8_dma4(i32x4 r, uint32_t lds_addr, uint32_t voff) {
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dword %1, %2, 0 offen lds"
                  :: "s"(lds_addr), "v"(voff), "s"(r) : "memory");
-}
-
-// Until at most N of the wave's loads are on their way.
-template <int N>
-__device__ __forceinline__ void f8_wait() {
-    asm volatile("s_waitcnt vmcnt(%0)" :: "n"(N) : "memory");
 }
 
 // BM x BN tiles, WM x WN waves, NS steps in LDS.
@@ -120,7 +105,7 @@ __global__ __launch_bounds__(T::THREADS) void gemm_f8_ring_kernel(GemmF8Args p) 
             const uint32_t end = b == p.blocks - 1 ? ~0u : 0u;
             i32x4 r = blk < T::A_LOADS ? ra : rb;
             r[2] = live ? r[2] : 0;
-            f8_dma16(r, slot + (uint32_t)(blk * 1024), (off[q] + (uint32_t)(b * F8_BLOCK)) | (tail[q % 2] & end));
+            dma16(r, slot + (uint32_t)(blk * 1024), (off[q] + (uint32_t)(b * F8_BLOCK)) | (tail[q % 2] & end));
         } else {
             f8_dma4(f8_rsrc(sbase + b * sstep, live ? 0x7fffffff : 0), slot + sat, soff);
         }
@@ -154,7 +139,7 @@ __global__ __launch_bounds__(T::THREADS) void gemm_f8_ring_kernel(GemmF8Args p) 
     if (steps > 0) {
 #pragma unroll
         for (int k = 0; k < NS - 1; ++k) fetch(k);
-        f8_wait<(NS - 2) * (T::LOADS + 1)>();
+        wait_vmcnt<(NS - 2) * (T::LOADS + 1)>();
         __syncthreads();
         fetch(NS - 1);
 #pragma unroll
@@ -177,7 +162,7 @@ __global__ __launch_bounds__(T::THREADS) void gemm_f8_ring_kernel(GemmF8Args p) 
             if (last) {
                 // everything of this step is read and everything of the next has landed, for all waves
                 asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-                f8_wait<(NS - 2) * (T::LOADS + 1)>();
+                wait_vmcnt<(NS - 2) * (T::LOADS + 1)>();
                 __syncthreads();
             }
             fw[(i + 1) % 2] = read(last ? at_w + next : at_w + here + (i + 1) * 16 * F8_BLOCK);
@@ -200,7 +185,7 @@ __global__ __launch_bounds__(T::THREADS) void gemm_f8_ring_kernel(GemmF8Args p) 
             if (last) fetch(step + NS);
         }
     }
-    f8_wait<0>();
+    wait_vmcnt<0>();
     static_assert(FN % 2 == 0, "rows of blocks in turn");
 #pragma unroll
     for (int j = 0; j < FM; ++j)
