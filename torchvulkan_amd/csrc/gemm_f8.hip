@@ -11,11 +11,12 @@
 // bits on the way, by each workgroup for itself; more rows in a launch of their
 // own. More than 64 rows, and from 17 on those of long k, run gemm_f8_ring.hip.
 //
-// Measured, W read from memory at 5.2 TB/s if nothing else took time: 1 x 14336 x
-// 4096 13.7 us in 8 bits and 15.8 from bfloat16 (11.3 for W's bytes, 3 for a launch);
-// 16 x 14336 x 4096 16.1 and 17.3; 1 x 8192 x 8192 13.9 and 17.6; 64 x 14336 x 4096
-// 24.5; 50 x 5000 x 4100, no row on 16 bytes, 14.8, and 17.9 from float16 with the
-// launch that brings it into 8 bits.
+// Measured, W from memory and, in brackets, from its cache: 1 x 14336 x 4096 13.5
+// (12.4) us in 8 bits and 15.8 (11.4) from bfloat16 (11.3 for W's bytes at 5.2 TB/s, 3
+// for a launch); 16 x 14336 x 4096 15.8 (13.3) and 17.2 (15.2); 1 x 8192 x 8192 13.9
+// (12.9) and 17.2 (16.4); 64 x 14336 x 4096 22.3 (21.0) and 25.4 (24.0); 50 x 5000 x
+// 4100, no row on 16 bytes, 16.5 (14.1), and 18.4 (17.2) from float16 with the launch
+// that brings it into 8 bits.
 // Loads on their way over the end of a loop's turn, with a next set of registers,
 // were slower, 16.9 us for 15.1: a wave has four blocks of 4096 values in all.
 #include "gemm_f8.h"

@@ -19,7 +19,7 @@
 // (for c and c + 1) at the eight slots c ^ {0, 1, 6, 7}, c + 1 ^ {2, 3, 4, 5}: no
 // two units on one bank.
 //
-// Measured: 8192 x 14336 x 4096 482 us, 8192^3 525 us (2.0 and 2.1 PFLOP/s; a library's bfloat16 product of 8192^3 958 us). The
+// Measured: 8192 x 14336 x 4096 475 to 492 us, 8192^3 486 us (1.95 to 2.0 and 2.3 PFLOP/s; a library's bfloat16 product of 8192^3 958 us). The
 // matrix unit is busy for half of the cycles there: a step's fragments and what is put into LDS take it three
 // quarters of the time that the products take, and a wave's next step starts behind a barrier.
 #include "gemm_dma.h"

@@ -15,7 +15,7 @@
 // whose largest value is one reduction among them.
 //
 // Measured, where a copy reaches 5.2 TB/s: 16384 x 4096 of bfloat16 with a residual
-// to 8 bits 92 us (472 MB, 5.1 TB/s); backward of 16384 x 2048 62 us, 5 of them the
+// to 8 bits 91 us (472 MB, 5.2 TB/s); backward of 16384 x 2048 62 us, 5 of them the
 // second launch (268 MB); 5 x 1024 3.3 us, a launch; backward of 1000 x 777 of float32
 // 10 us, two launches. A row of 512 chunks by 512 threads with one chunk each was slower,
 // 101 us and 92, and so was one kept packed between the sums, which fits five

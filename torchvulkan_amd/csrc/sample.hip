@@ -17,8 +17,8 @@
 // them: float32 weights would put one in 10^4 draws from a flat distribution
 // elsewhere.
 //
-// The row stays in the registers of 1024 threads, 32 K values in 16 bits, and is
-// read again for every pass past that. Most of a small call is latency, and much of
+// The row stays in the registers of 1024 threads, 32 K values in 16 bits or 16 K in
+// 32, and is read again, stretch by stretch, for every pass past that. Most of a small call is latency, and much of
 // that the code's own: a line of 64 bytes that no cache holds takes as long as a
 // load. So passes are loops over a thread's words, not unrolled, helpers are called,
 // not inlined, and nothing is read in a chain that can be read at once. Few rows are
@@ -27,11 +27,13 @@
 //
 // Measured: 1 x 50001 of bfloat16 with top_k and top_p 22 us (launches of 3.7, 4.9, 7.5
 // and 6.7), 64 x 128000 with top_p at temperatures from 0.5 to 1.5 61 us (4.9, 16, 24
-// and 17), 200 x 32003 of float32 with every filter 47 us. The weights of a row, some
-// 210 cycles for 64 of them, and their atomics in LDS bound the larger; a series without
-// the table of fractions was slower (18.9 us for 16.5 in the histogram's launch), and
-// neither comparisons with a bin's ends in place of its number nor sums over runs of
-// one place before the atomics changed the third.
+// and 17), 200 x 32003 of float32 with every filter 47 us (rows that are read again for
+// every pass); in a replayed graph, whose start is 5 of them, the largest logit alone
+// 18 us of 1 x 50001 and 21 of 64 x 128000, without filters 23 and 30. The weights of a
+// row, some 210 cycles for 64 of them, and their atomics in LDS bound the larger; a
+// series without the table of fractions was slower (18.9 us for 16.5 in the histogram's
+// launch), and neither comparisons with a bin's ends in place of its number nor sums
+// over runs of one place before the atomics changed the third.
 #include "norm_rows.h"
 
 #include <cfloat>
